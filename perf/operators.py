@@ -1,0 +1,545 @@
+"""Operators of a decode or verify step of several conversations, as cases to measure.
+
+Four kinds of call:
+
+  rope     norms of the queries and keys of each head (root of the mean square, a
+           weight per dim), the position rotation in the same pass
+  append   new keys and values into the cells of one or several windows: norm,
+           rotation and Walsh-Hadamard transform of the keys, the window's type
+  shared   attention of a batch of conversations that share a long prefix: every
+           query sees the prefix window's cells and its own conversation's
+  step     what a layer of such a batch does with its new tokens: append (keys,
+           values, queries), then the shared attention
+
+Definitions.  Rotation: pairs (i, i + n_rot / 2) of the first n_rot dims, angle
+fl32(pos theta_i), theta_i = fl32(base^(-2 i / n_rot)): the rounded product is the
+angle that every row of a window is rotated by.  Transform: normalised
+Walsh-Hadamard matrix over chunks of `hadamard` dims.  A cell is visible to a query
+iff 0 <= its position <= the query's; query head h reads kv head h / group.
+
+Sizes are the framework's own (24 query heads on 4 kv heads of 256 dims with 64
+rotated, 8 on 2 of 128, 128-token blocks, windows to 32,768 cells, histories to
+262,144 tokens, prompt chunks of 2,048) and generic ones between them.
+"""
+import math
+import os
+import sys
+
+import numpy as np
+import torch
+
+own = False
+
+BT = 128                                  # tokens per block
+EPS = 1e-6
+BASE = 1e7
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+BLOCK_BYTES = {"q8_0": (34, 18), "q4_0": (18, 18), "f16": (64, 64)}      # bytes of 32 K / V values
+
+
+# ---- the cases -----------------------------------------------------------------
+def _case(name, kind, **kw):
+    c = {"kind": kind, "head_dim": 256, "kv_heads": 4, "group": 6, "n_rot": 64, "type": "bf16", "cache": "q8_0"}
+    c.update(kw)
+    if name:
+        c["name"] = name
+    return c
+
+
+def listed():
+    return [
+        # one token of one conversation: latency
+        _case("rope_1", "rope", tokens=1, pos0=261113, out="bf16", packed=False, hadamard=256),
+        # draft verification on a small model, every dim rotated, fp32
+        _case("rope_33_f32", "rope", head_dim=128, kv_heads=2, group=4, n_rot=128, type="f32", tokens=33, pos0=7001,
+              out="f32", packed=True, hadamard=0),
+        # the benchmark's prompt chunk, out of a joint projection of q, k and v
+        _case("rope_2048", "rope", tokens=2048, pos0=98304, out="bf16", packed=False, hadamard=0),
+        # a decode step of one conversation into an fp16 window
+        _case("append_f16_1", "append", head_dim=128, kv_heads=2, group=4, n_rot=128, cache="f16", lanes=1, tokens=1,
+              ragged=False, window=4608, cell0=4160, hadamard=0),
+        # the verified tokens of sixteen conversations, each its own window
+        _case("append_f16_16x4", "append", n_rot=64, cache="f16", lanes=16, tokens=4, ragged=True, window=1024,
+              cell0=509, hadamard=0),
+        # the benchmark's prompt chunk (a ragged one) into a quantised window
+        _case("append_q8_2047", "append", lanes=1, tokens=2047, ragged=False, window=34816, cell0=32701, hadamard=256),
+        # two conversations that just began, a short prefix on a small model: latency
+        _case("shared_f16_1k_2x1", "shared", head_dim=128, kv_heads=2, group=4, cache="f16", prefix=1000, lanes=2,
+              tokens=1, ragged=False, own_cells=256, fill=130),
+        # eight conversations over a long document, one token each
+        _case("shared_q8_32k_8x1", "shared", prefix=32768, lanes=8, tokens=1, ragged=False, own_cells=2048, fill=1500),
+        # draft verification of sixteen, q4_0 keys, conversations longer than the prefix
+        _case("shared_q4_5k_16x5", "shared", cache="q4_0", type="f32", prefix=5003, lanes=16, tokens=5, ragged=True,
+              own_cells=8192, fill=8000),
+        # draft verification of thirty-two over a long document: the largest
+        _case("shared_q8_32k_32x4", "shared", prefix=32768, lanes=32, tokens=4, ragged=False, own_cells=2048, fill=2000),
+        # a layer of a batch with a shared system prompt on a small model
+        _case("step_f16_8k_12x3", "step", head_dim=128, kv_heads=8, group=4, n_rot=128, cache="f16", prefix=8192,
+              lanes=12, tokens=3, ragged=False, own_cells=1024, fill=777, hadamard=0),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(lo * (hi / lo) ** rng.random()))
+
+
+def draw(rng):
+    kind = rng.choice(["rope", "append", "append", "shared", "shared", "step"])
+    dim, kv, grp, rot = rng.choice([(256, 4, 6, 64), (256, 4, 6, 64), (256, 2, 8, 64), (128, 2, 4, 128), (128, 8, 4, 128),
+                                    (128, 1, 8, 96), (128, 4, 1, 32)])
+    c = _case(None, kind, head_dim=dim, kv_heads=kv, group=grp, n_rot=rot, type=rng.choice(["bf16", "bf16", "f32", "f16"]))
+    if kind == "rope":
+        c.update(tokens=_log(rng, 1, 2048), pos0=_log(rng, 1, 260000), out=rng.choice(["bf16", "f32", "f16"]),
+                 packed=rng.random() < 0.5, hadamard=rng.choice([0, 0, 64, 128]))
+        return c
+    if kind == "append":
+        c["cache"] = rng.choice(["f16", "q8_0", "q4_0"])
+        # several conversations on fp16 windows, long runs of one on any
+        c["lanes"] = rng.randint(2, 24) if c["cache"] == "f16" and rng.random() < 0.6 else 1
+        c["tokens"] = rng.randint(1, 8) if c["lanes"] > 1 else _log(rng, 1, 2048)
+        c["window"] = 128 * (rng.randint(8, 16) if c["lanes"] > 1 else _log(rng, 32, 256))
+        c["cell0"] = rng.randint(0, c["window"] - c["tokens"])
+        c["hadamard"] = 0 if c["cache"] == "f16" else rng.choice([0, dim])
+    else:
+        if c["type"] == "f16":
+            c["type"] = "bf16"
+        c["cache"] = rng.choice(["q8_0", "q8_0", "q4_0", "f16"]) if kind == "shared" else "f16"
+        c["lanes"] = _log(rng, 1, 24)
+        c["tokens"] = rng.randint(1, 4)
+        c["prefix"] = _log(rng, 256, 32768)
+        c["own_cells"] = 128 * _log(rng, 2, 16)
+        c["fill"] = rng.randint(c["tokens"], c["own_cells"])
+        c["hadamard"] = 0
+    c["ragged"] = c["lanes"] > 1 and rng.random() < 0.5
+    return c
+
+
+# ---- inputs --------------------------------------------------------------------
+def _gen(seed, salt):
+    g = torch.Generator(device="cuda")
+    g.manual_seed((int(seed) * 1000003 + salt) & 0x7FFFFFFFFFFFFFFF)
+    return g
+
+
+def _randn(g, *shape):
+    return torch.randn(shape, generator=g, device="cuda")
+
+
+def _counts(case):
+    """Tokens of each conversation in this call."""
+    n, t = case["lanes"], case["tokens"]
+    return [1 + (3 * i + 1) % t for i in range(n)] if case["ragged"] else [t] * n
+
+
+def _theta(n_rot):
+    e = np.float32(-2.0) * np.arange(n_rot // 2, dtype=np.float32) / np.float32(n_rot)
+    return np.power(np.float64(np.float32(BASE)), e.astype(np.float64)).astype(np.float32)
+
+
+def _projections(case, seed, n):
+    """q [n][heads][dim], k and v [n][kv heads][dim]: packed, or the parts of a joint projection's rows."""
+    H, G, D = case["kv_heads"], case["group"], case["head_dim"]
+    x = (_randn(_gen(seed, 3), n, H * (G + 2), D) * 1.7).to(DTYPES[case["type"]])
+    q, k, v = x[:, :H * G], x[:, H * G:H * (G + 1)], x[:, H * (G + 1):]
+    if case.get("packed"):
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    w = 1.0 + 0.2 * _randn(_gen(seed, 4), 2, D)
+    return q, k, v, w[0].contiguous(), w[1].contiguous()
+
+
+def _kinds(case):
+    return ("f16", "f16") if case["cache"] == "f16" else (case["cache"], "q4_0")
+
+
+def _codes(kind, x):
+    """(codes, scales) of the 32-value blocks of fp32 values, as ggml forms q8_0 and q4_0."""
+    x = x.reshape(-1, 32)
+    if kind == "q8_0":
+        d = x.abs().amax(1) / 127.0
+        i = torch.where(d != 0, 1.0 / d, torch.zeros_like(d))
+        y = x * i[:, None]
+        return torch.trunc(y.abs() + 0.5) * torch.sign(y), d.to(torch.float16)
+    top = x.gather(1, x.abs().argmax(1, keepdim=True))[:, 0]
+    d = top * -0.125
+    i = torch.where(d != 0, 1.0 / d, torch.zeros_like(d))
+    return torch.trunc(x * i[:, None] + 8.5).clamp(max=15.0) - 8.0, d.to(torch.float16)
+
+
+def _rows(kind, x):
+    """Cache rows (uint8 [n][bytes]) of fp32 values [n][values]."""
+    if kind == "f16":
+        return x.to(torch.float16).view(torch.uint8).reshape(x.shape[0], -1)
+    q, d = _codes(kind, x)
+    if kind == "q4_0":
+        q = (q + 8).to(torch.uint8)
+        q = q[:, :16] | (q[:, 16:] << 4)
+    else:
+        q = q.to(torch.int8).view(torch.uint8)
+    return torch.cat([d[:, None].view(torch.uint8), q], 1).reshape(x.shape[0], -1)
+
+
+def _window_rows(case, seed, salt, n):
+    e = case["kv_heads"] * case["head_dim"]
+    g, (kk, vk) = _gen(seed, salt), _kinds(case)
+    return _rows(kk, _randn(g, n, e)), _rows(vk, _randn(g, n, e))
+
+
+def _inputs(case, seed):
+    kind, H, G, D = case["kind"], case["kv_heads"], case["group"], case["head_dim"]
+    s = {"case": case, "scale": D ** -0.5}
+    if kind == "rope":
+        n = case["tokens"]
+        s["q"], s["k"], _, s["qw"], s["kw"] = _projections(case, seed, n)
+        s["pos"] = torch.arange(case["pos0"], case["pos0"] + n, dtype=torch.int32, device="cuda")
+        return s
+    cnt = s["counts"] = _counts(case)
+    n, lanes = sum(cnt), case["lanes"]
+    lane, slot = np.repeat(np.arange(lanes), cnt), np.concatenate([np.arange(t) for t in cnt])
+    if kind != "shared":
+        s["q"], s["k"], s["v"], s["qw"], s["kw"] = _projections(case, seed, n)
+    if kind == "append":                  # into windows that hold nothing so far
+        s["first"] = [case["cell0"]] * lanes
+        s["pos"] = torch.from_numpy((case["cell0"] + slot).astype(np.int32)).cuda()
+        s["cells"] = torch.from_numpy(lane * case["window"] + case["cell0"] + slot).cuda()
+        return s
+    if kind == "shared":
+        s["q"] = _randn(_gen(seed, 3), n, H * G, D).to(DTYPES[case["type"]])
+    # a conversation's own cells follow the prefix; those of this call's tokens are its last ones
+    P, C = case["prefix"], case["own_cells"]
+    fill = _fills(case, cnt)
+    s["pos"] = torch.from_numpy((P + np.repeat(fill - np.array(cnt), cnt) + slot).astype(np.int32)).cuda()
+    s["lane"], s["slot"] = torch.from_numpy(lane).cuda(), torch.from_numpy(slot).cuda()
+    s["pk"], s["pv"] = _window_rows(case, seed, 11, P)
+    s["ppos"] = torch.arange(P, dtype=torch.int32, device="cuda")
+    lk, lv = _window_rows(case, seed, 12, lanes * C)
+    s["lk"], s["lv"] = lk.view(lanes, C, -1), lv.view(lanes, C, -1)
+    live = fill - np.array(cnt) if kind == "step" else fill
+    s["first"] = [int(x) for x in live]
+    s["lpos"] = torch.from_numpy(np.where(np.arange(C) < live[:, None], P + np.arange(C), -1).astype(np.int32)).cuda()
+    return s
+
+
+def _fills(case, cnt):
+    """Cells of its own that each conversation has with this call's tokens."""
+    return np.array([max(t, case["fill"] - 7 * i) for i, t in enumerate(cnt)])
+
+
+_kept = {}
+
+
+def _api():
+    """The framework, and the program's execution state: one for the process."""
+    if not _kept:
+        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "kvmem-llama.cpp_amd"))
+        from kvmem_amd import _lib, api
+        _kept.update(api=api, lib=_lib, st=api.State(0))
+    return _kept["api"], _kept["lib"], _kept["st"]
+
+
+def _handles(case, s):
+    """The windows that the program keeps, with what it has written into them, and its step loop's calls."""
+    api, L, st = _api()
+    types = {"q8_0": (L.T_Q8_0, L.T_Q4_0), "q4_0": (L.T_Q4_0, L.T_Q4_0), "f16": (L.T_F16, L.T_F16)}[case["cache"]]
+
+    def window(cells):
+        return api.KVWindow(st, cells, case["kv_heads"], case["head_dim"], BT, *types)
+
+    if case["kind"] == "append":
+        s["windows"] = [window(case["window"]) for _ in range(case["lanes"])]
+    elif case["kind"] != "rope":
+        s["prefix"] = window(-(-case["prefix"] // BT) * BT)
+        s["prefix"].import_rows(0, s.pop("pk"), s.pop("pv"), s["ppos"])
+        s["windows"] = [window(case["own_cells"]) for _ in range(case["lanes"])]
+        for i, w in enumerate(s["windows"]):
+            w.import_rows(0, s["lk"][i], s["lv"][i], s["lpos"][i])
+        del s["lk"], s["lv"]
+    s["calls"] = _calls(case, s)
+    return s
+
+
+def prepare(case, seed):
+    s, H, D = _inputs(case, seed), case["kv_heads"], case["head_dim"]
+    if own:
+        return _handles(case, s)
+    if case["kind"] == "append" and case["cache"] == "f16":
+        s["kc"] = torch.zeros((case["lanes"] * case["window"], H, D), dtype=torch.float16, device="cuda")
+        s["vc"] = torch.zeros_like(s["kc"])
+    return s
+
+
+# ---- one pass: the framework's calls -------------------------------------------
+def _calls(case, s):
+    """The calls of a step loop, their arguments laid out once."""
+    api, L, st = _api()
+    kind, H, G, D = case["kind"], case["kv_heads"], case["group"], case["head_dim"]
+    if kind == "rope":
+        return api.prepare_qk_norm_rope(st, s["q"], s["k"], s["pos"], case["n_rot"], BASE, hadamard_nrot=case["hadamard"],
+                                        q_weight=s["qw"], k_weight=s["kw"], eps=EPS, out_dtype=DTYPES[case["out"]])
+    append = attend = None
+    if kind in ("append", "step"):
+        more = {"q": s["q"], "q_weight": s["qw"]} if kind == "step" else {}
+        append = api.prepare_window_append(st, s["windows"], s["first"], s["counts"], s["k"], s["v"], s["pos"],
+                                           case["n_rot"], BASE, hadamard_nrot=case["hadamard"], k_weight=s["kw"], eps=EPS,
+                                           q_out_dtype=torch.bfloat16, **more)
+    if kind in ("shared", "step"):
+        attend = api.prepare_fa_decode_shared(st, s["prefix"], s["windows"], s["counts"],
+                                              append.q_out if kind == "step" else s["q"], s["pos"], H * G, s["scale"],
+                                              out_dtype=torch.bfloat16)
+    return append, attend
+
+
+def _cells(case, w):
+    """An fp16 window's keys and values, cells first (views of its tiles)."""
+    H, D, n = case["kv_heads"], case["head_dim"], w.n_cells // 64
+    k = w.k.view(torch.float16).view(H, n, 4, D // 32, 4, 16, 8).permute(1, 2, 5, 0, 3, 4, 6)
+    v = w.v.view(torch.float16).view(H, n, D // 16, 4, 16, 2, 8).permute(1, 5, 3, 6, 0, 2, 4)
+    return k, v
+
+
+def _run_own(s):
+    api, L, st = _api()
+    case = s["case"]
+    if case["kind"] == "rope":
+        s["calls"]()
+        return {"q": s["calls"].q_out, "k": s["calls"].k_out}
+    append, attend = s["calls"]
+    res = {}
+    if append is not None:
+        append()
+        if case["cache"] == "f16":
+            res["cells"] = [_cells(case, w) for w in s["windows"]]
+        else:                             # the values that the cells now hold
+            w, n, e = s["windows"][0], s["counts"][0], case["kv_heads"] * case["head_dim"]
+            kr, vr = w.export_rows(case["cell0"], n)
+            res["k"] = api.dequantize_rows(st, w.k_type, kr, e).to(torch.float16)
+            res["v"] = api.dequantize_rows(st, w.v_type, vr, e).to(torch.float16)
+    if attend is not None:
+        attend()
+        res["out"] = attend.out
+        if append is not None:
+            res["q"] = append.q_out
+    return res
+
+
+# ---- one pass: the plain form --------------------------------------------------
+def _norm(x, w):
+    """fp32 rows over the root of their mean square (formed in 64 bits), times the weights."""
+    r = ((x.double() ** 2).mean(-1, keepdim=True) + float(np.float32(EPS))).sqrt().reciprocal().float()
+    return (x * r) * w
+
+
+def _rotate(x, pos, n_rot):
+    """Angles are far from 0, so their cosines and sines are formed in 64 bits."""
+    ang = (pos.float()[:, None] * torch.from_numpy(_theta(n_rot)).to(pos.device)).double()
+    c, s = ang.cos().float()[:, None], ang.sin().float()[:, None]
+    a, b = x[..., :n_rot // 2], x[..., n_rot // 2:n_rot]
+    return torch.cat([a * c - b * s, a * s + b * c, x[..., n_rot:]], -1)
+
+
+def _transform(x, n):
+    """Butterflies: log2 n sums and differences of each value, in the order of the definition."""
+    if not n:
+        return x
+    shape, x, h = x.shape, (x * np.float32(1.0 / math.sqrt(n))).reshape(-1, n), 1
+    while h < n:
+        y = x.view(-1, n // (2 * h), 2, h)
+        x = torch.stack([y[:, :, 0] + y[:, :, 1], y[:, :, 0] - y[:, :, 1]], 2).view(-1, n)
+        h *= 2
+    return x.view(shape)
+
+
+def _held(kind, x):
+    """The values that a window of this type holds for fp32 rows."""
+    if kind == "f16":
+        return x.to(torch.float16)
+    q, d = _codes(kind, x)
+    return (q * d.float()[:, None]).to(torch.float16).view(x.shape)
+
+
+def _values(kind, rows):
+    """fp32 values of cache rows."""
+    if kind == "f16":
+        return rows.contiguous().view(torch.float16).float()
+    b = rows.reshape(-1, 34 if kind == "q8_0" else 18)
+    d = b[:, :2].contiguous().view(torch.float16).float()
+    if kind == "q8_0":
+        q = b[:, 2:].contiguous().view(torch.int8).float()
+    else:
+        q = torch.cat([b[:, 2:] & 15, b[:, 2:] >> 4], 1).float() - 8.0
+    return (q * d).reshape(*rows.shape[:-1], -1)
+
+
+def _attend(s, q, lk, lv, lpos):
+    """Softmax attention of each query over the prefix and its conversation's own cells, fp32."""
+    case = s["case"]
+    H, G, D, n, L, T = case["kv_heads"], case["group"], case["head_dim"], q.shape[0], case["lanes"], case["tokens"]
+    kk, vk = _kinds(case)
+    q = q.float().view(n, H, G, D)
+    pk = _values(kk, s["pk"]).view(-1, H, D).permute(1, 2, 0)                       # [H][D][cells]
+    pv = _values(vk, s["pv"]).view(-1, H, D).permute(1, 0, 2)
+    lk, lv = lk.view(L, -1, H, D).permute(0, 2, 3, 1), lv.view(L, -1, H, D).permute(0, 2, 1, 3)
+    sp = (q.permute(1, 0, 2, 3).reshape(H, n * G, D) @ pk).view(H, n, G, -1).permute(1, 0, 2, 3)
+    # a conversation's rows side by side, the shorter ones filled up
+    pad = torch.zeros((L, T, H, G, D), device=q.device)
+    pad[s["lane"], s["slot"]] = q
+    so = (pad.permute(0, 2, 1, 3, 4).reshape(L, H, T * G, D) @ lk).view(L, H, T, G, -1)
+    so = so.permute(0, 2, 1, 3, 4)[s["lane"], s["slot"]]                            # [n][H][G][cells]
+    seen_p = (s["ppos"][None] >= 0) & (s["ppos"][None] <= s["pos"][:, None])
+    lp = lpos[s["lane"]]
+    seen_o = (lp >= 0) & (lp <= s["pos"][:, None])
+    x = torch.cat([sp, so], -1) * s["scale"]
+    x = torch.where(torch.cat([seen_p, seen_o], -1)[:, None, None], x, torch.full_like(x, -math.inf))
+    top = x.amax(-1, keepdim=True)
+    p = torch.exp(x - torch.where(top == -math.inf, torch.zeros_like(top), top))
+    total = p.sum(-1)
+    C = pv.shape[1]
+    op = (p[..., :C].permute(1, 0, 2, 3).reshape(H, n * G, C) @ pv).view(H, n, G, D).permute(1, 0, 2, 3)
+    pad = torch.zeros((L, T, H, G, p.shape[-1] - C), device=q.device)
+    pad[s["lane"], s["slot"]] = p[..., C:]
+    oo = (pad.permute(0, 2, 1, 3, 4).reshape(L, H, T * G, -1) @ lv).view(L, H, T, G, D).permute(0, 2, 1, 3, 4)
+    o = (op + oo[s["lane"], s["slot"]]) / torch.where(total > 0, total, torch.ones_like(total))[..., None]
+    return o.reshape(n, H * G, D)
+
+
+def run(s):
+    if own:
+        return _run_own(s)
+    case = s["case"]
+    kind, H, D = case["kind"], case["kv_heads"], case["head_dim"]
+    if kind == "rope":
+        q, k = (_transform(_rotate(_norm(x.float(), w), s["pos"], case["n_rot"]), case["hadamard"])
+                for x, w in ((s["q"], s["qw"]), (s["k"], s["kw"])))
+        return {"q": q.to(DTYPES[case["out"]]), "k": k.to(DTYPES[case["out"]])}
+    kk, vk = _kinds(case)
+    if kind in ("append", "step"):
+        k = _held(kk, _transform(_rotate(_norm(s["k"].float(), s["kw"]), s["pos"], case["n_rot"]), case["hadamard"]))
+        v = _held(vk, s["v"].float())
+    if kind == "append":
+        if case["cache"] != "f16":
+            return {"k": k.view(-1, H * D), "v": v.view(-1, H * D)}
+        s["kc"][s["cells"]], s["vc"][s["cells"]] = k, v
+        return {"cells": _per_window(case, s["kc"], s["vc"])}
+    if kind == "shared":
+        lk, lv = _values(kk, s["lk"]), _values(vk, s["lv"])
+        return {"out": _attend(s, s["q"], lk, lv, s["lpos"]).to(torch.bfloat16)}
+    q = _rotate(_norm(s["q"].float(), s["qw"]), s["pos"], case["n_rot"]).to(torch.bfloat16)
+    lk, lv = (s[x].view(torch.float16).view(case["lanes"], -1, H, D) for x in ("lk", "lv"))
+    cell = s["pos"].long() - case["prefix"]
+    lk[s["lane"], cell], lv[s["lane"], cell], s["lpos"][s["lane"], cell] = k, v, s["pos"]
+    out = _attend(s, q, lk.float(), lv.float(), s["lpos"]).to(torch.bfloat16)
+    return {"cells": _per_window(case, lk.reshape(-1, H, D), lv.reshape(-1, H, D)), "out": out, "q": q}
+
+
+def _per_window(case, kc, vc):
+    H, D, n = case["kv_heads"], case["head_dim"], kc.shape[0] // 64 // case["lanes"]
+    k, v = kc.view(-1, n, 4, 16, H, D // 32, 4, 8), vc.view(-1, n, 2, 4, 8, H, D // 16, 16)
+    return list(zip(k.unbind(0), v.unbind(0)))
+
+
+# ---- what a pass cannot do without ---------------------------------------------
+def work(case):
+    kind, H, G, D = case["kind"], case["kv_heads"], case["group"], case["head_dim"]
+    es = 4 if case["type"] == "f32" else 2
+    row = sum(H * D // 32 * b for b in BLOCK_BYTES[case["cache"]])
+    if kind == "rope":
+        n, e = case["tokens"], H * (G + 1) * D
+        eo = 4 if case["out"] == "f32" else 2
+        return {"bytes": n * (e * (es + eo) + 4) + 8 * D, "flops": 10 * n * e}
+    cnt = _counts(case)
+    n = sum(cnt)
+    append = {"bytes": n * (2 * H * D * es + row + 8) + 4 * D, "flops": 12 * n * H * D}
+    if kind == "append":
+        return append
+    P, F = case["prefix"], int(_fills(case, cnt).sum())
+    b = (P + F) * (row + 4) + n * (H * G * D * ((2 if kind == "step" else es) + 2) + 4)
+    f = 4 * H * G * D * n * (P + F // case["lanes"])
+    if kind == "step":
+        b, f = b + append["bytes"] + n * H * G * D * (es + 2) + 4 * D, f + append["flops"] + 10 * n * H * G * D
+    return {"bytes": b, "flops": f}
+
+
+# ---- the same in 64 bits -------------------------------------------------------
+def _exact_head(x, w, pos, n_rot, hadamard):
+    """Norm, rotation and transform of rows [n][heads][dim] in 64 bits."""
+    x = x.double()
+    n, D = x.shape[0], x.shape[-1]
+    x = x / torch.sqrt(torch.linalg.vector_norm(x, dim=-1, keepdim=True) ** 2 / D + float(np.float32(EPS))) * w.double()
+    ang = pos.cpu().numpy().astype(np.float32)[:, None] * _theta(n_rot)[None]
+    turn = torch.from_numpy(np.exp(1j * ang.astype(np.float64))).to(x.device)[:, None]
+    z = torch.complex(x[..., :n_rot // 2].contiguous(), x[..., n_rot // 2:n_rot].contiguous()) * turn
+    x = torch.cat([z.real, z.imag, x[..., n_rot:]], -1)
+    if hadamard:
+        i = np.arange(hadamard)
+        ones = np.array([bin(v).count("1") for v in range(hadamard)])
+        m = torch.from_numpy(np.where(ones[i[:, None] & i[None]] % 2, -1.0, 1.0) / math.sqrt(hadamard)).to(x.device)
+        x = (x.reshape(-1, hadamard) @ m).view(x.shape)
+    return x
+
+
+def _exact_held(kind, x):
+    if kind == "f16":
+        return x
+    b = x.reshape(-1, 32)
+    if kind == "q8_0":
+        step = b.abs().max(1).values / 127
+        code = torch.sign(b) * torch.floor(b.abs() / step[:, None] + 0.5)
+    else:
+        peak = torch.take_along_dim(b, b.abs().max(1, keepdim=True).indices, 1)[:, 0]
+        step = -peak / 8
+        code = torch.clamp(torch.floor(b / step[:, None] + 8.5), max=15) - 8
+    return (code * step.to(torch.float16).double()[:, None]).view(x.shape)
+
+
+def _exact_values(kind, rows):
+    """64-bit values of cache rows."""
+    if kind == "f16":
+        return rows.contiguous().view(torch.float16).double()
+    n = rows.shape[:-1]
+    b = rows.reshape(*n, -1, 34 if kind == "q8_0" else 18)
+    scale = b[..., :2].contiguous().view(torch.float16).double()
+    code = b[..., 2:].to(torch.int64)
+    if kind == "q8_0":
+        code = (code + 128) % 256 - 128
+    else:
+        code = torch.cat([code % 16, code // 16], -1) - 8
+    return (code * scale).reshape(*n, -1)
+
+
+def exact(case, seed):
+    kind, H, G, D = case["kind"], case["kv_heads"], case["group"], case["head_dim"]
+    s = _inputs(case, seed)
+    kk, vk = _kinds(case)
+    if kind == "rope":
+        return {x: _exact_head(s[x], s[x + "w"], s["pos"], case["n_rot"], case["hadamard"]) for x in ("q", "k")}
+    if kind in ("append", "step"):
+        k = _exact_held(kk, _exact_head(s["k"], s["kw"], s["pos"], case["n_rot"], case["hadamard"]))
+        v = _exact_held(vk, s["v"].double())
+    if kind == "append":
+        if case["cache"] != "f16":
+            return {"k": k.reshape(-1, H * D), "v": v.reshape(-1, H * D)}
+        kc = torch.zeros((case["lanes"] * case["window"], H, D), dtype=torch.float64, device="cuda")
+        vc = torch.zeros_like(kc)
+        kc[s["cells"]], vc[s["cells"]] = k, v
+        return {"cells": _per_window(case, kc, vc)}
+    res, q = {}, s["q"].double()
+    pk, pv = (_exact_values(t, s[x]).view(-1, H, D) for t, x in ((kk, "pk"), (vk, "pv")))
+    lk, lv = (_exact_values(t, s[x]).view(case["lanes"], -1, H, D) for t, x in ((kk, "lk"), (vk, "lv")))
+    lpos = s["lpos"].clone()
+    if kind == "step":
+        q = _exact_head(s["q"], s["qw"], s["pos"], case["n_rot"], 0)
+        cell = s["pos"].long() - case["prefix"]
+        lk[s["lane"], cell], lv[s["lane"], cell], lpos[s["lane"], cell] = k, v, s["pos"]
+        res["cells"], res["q"] = _per_window(case, lk.view(-1, H, D), lv.view(-1, H, D)), q
+    out = torch.empty_like(q)
+    for i in range(case["lanes"]):
+        rows = (s["lane"] == i).nonzero()[:, 0]
+        live = lpos[i] >= 0
+        pos = torch.cat([s["ppos"], lpos[i][live]])
+        dead = pos[None] > s["pos"][rows][:, None]
+        for h in range(H):
+            kh, vh = torch.cat([pk[:, h], lk[i, live, h]]), torch.cat([pv[:, h], lv[i, live, h]])
+            x = (q[rows, h * G:(h + 1) * G].reshape(-1, D) @ kh.t().contiguous()) * s["scale"]
+            x = x.view(len(rows), G, -1).masked_fill(dead[:, None], -math.inf)
+            out[rows, h * G:(h + 1) * G] = (torch.softmax(x, -1).view(len(rows) * G, -1) @ vh).view(len(rows), G, D)
+    res["out"] = out
+    return res
