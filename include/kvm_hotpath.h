@@ -526,6 +526,53 @@ int kvm_stagein_enqueue_v(kvm_state *st, const void *packed, size_t nbytes,
 int kvm_stagein_flush(kvm_state *st);
 
 /* ------------------------------------------------------------------------ */
+/* A layer's new tokens: head norms and rotation of Q and K, K / V appended   */
+/* (in the reference, nodes of the graph before build_attn's cpy_k / cpy_v    */
+/* into the cells kvmem_fill_slot_info chose, llama-kvmem-batch.cpp:42-50).   */
+/* ------------------------------------------------------------------------ */
+/* For every head of every token, x its head_dim values (F32, F16 or BF16 of
+ * any strides, read as fp32):
+ *   norm     eps >= 0: y_d = (x_d r) w_d with r = 1 / sqrt(mean of x_d^2 + eps)
+ *            formed in 64 bits and rounded to fp32; weight: device float
+ *            [head_dim] or NULL (ones).  eps < 0: y = x, the weights unused.
+ *   rotation rope != NULL: NeoX pairs (i, i + n_rot / 2) of the first n_rot dims
+ *            (a multiple of 8, 0 = none), angle = the fp32 product pos * theta_i
+ *            with kvm_rope_params' theta: the angles the stage-in's rows have.
+ *   transform hadamard_nrot > 0: the normalised Walsh-Hadamard transform in
+ *            chunks of that many dims (a power of two >= 64 that divides
+ *            head_dim), as the stage-in's.
+ * Each operation is one IEEE fp32 rounding; the result is rounded once to the
+ * output type.  pos: device int32 [tokens].
+ *
+ * kvm_qk_norm_rope writes the rows as [tokens][heads][head_dim] of out_type
+ * (F32, F16, BF16).  q or k may be NULL; both have the same ne0 = head_dim (a
+ * multiple of 8, at most 256) and ne2 = tokens, ne1 is the heads.  The width of
+ * the transform is the caller's (negative is refused: there is no window).  An
+ * output may be its input's own memory where that is packed and of out_type;
+ * otherwise outputs overlap neither inputs nor each other (KVM_EINVAL). */
+int kvm_qk_norm_rope(kvm_state *st, const kvm_view *q, const kvm_view *k, const float *q_weight,
+                     const float *k_weight, float eps, const kvm_rope_params *rope, const int32_t *pos,
+                     int out_type, void *q_out, void *k_out);
+/* kvm_window_append writes new tokens into the cells of one or several windows
+ * (one a conversation, or several runs of one) in one launch: run i takes the
+ * next n_tokens[i] tokens of the views into cells cell0[i] .. of windows[i]
+ * (host arrays of n_runs).  Keys: norm, rotation and transform as above
+ * (hadamard_nrot = -1: the default of the window's K type), then the window's
+ * type (kvm_quantize_rows' formulas); values: the window's type; cell_pos = pos.
+ * The cells end as kvm_window_import_rows of those rows leaves them, shadow_rows
+ * and pending_rows with them, and cells beside them as they were.  Runs are
+ * written in order: where two name the same cell the later one's row stays.
+ * All windows have the same head counts, head_dim and types; the views hold
+ * the runs' tokens exactly.  rope = NULL and eps < 0: the keys as they come.
+ * With q != NULL the tokens' queries are normed, rotated and transformed like
+ * the keys (q_weight; the transform of both leaves the scores as they are) into
+ * q_out, [tokens][heads][head_dim] of q_out_type: what the attention takes. */
+int kvm_window_append(kvm_state *st, const kvm_window *const *windows, const uint32_t *cell0,
+                      const uint32_t *n_tokens, uint32_t n_runs, const kvm_view *k, const kvm_view *v,
+                      const float *k_weight, float eps, const kvm_rope_params *rope, const int32_t *pos,
+                      const kvm_view *q, const float *q_weight, int q_out_type, void *q_out);
+
+/* ------------------------------------------------------------------------ */
 /* Flash attention over the window (ggml_flash_attn_ext as called by          */
 /* build_attn, patches/0002-attn-qk-capture-hook.patch:225,256)              */
 /* ------------------------------------------------------------------------ */

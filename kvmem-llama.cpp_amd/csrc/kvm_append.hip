@@ -1,0 +1,684 @@
+// kvm_append.hip -- what a layer does with its new tokens before it attends: norms of
+// the queries and keys of each head with the position rotation in the same pass
+// (kvm_qk_norm_rope), and the keys and values into the cells of their windows
+// (kvm_window_append).
+//
+// A row is one head of one token.  With x its D values,
+//   r = 1 / sqrt(mean x_d^2 + eps), formed in 64 bits and rounded once,
+//   y_d = (x_d r) w_d,
+//   pairs (i, i + n_rot / 2), angle a = fl32(pos theta_i): y_i' = y_i cos a - y_j sin a,
+//   y_j' = y_i sin a + y_j cos a,
+//   the normalised Walsh-Hadamard transform of chunks of nrot dims: pre-scaled by
+//   1 / sqrt(nrot), butterflies h = 1, 2, ..
+// each operation one fp32 rounding, cos a and sin a the roundings of the 64-bit values.
+// The sum of squares does not depend on the order of its terms then (a 64-bit sum's
+// order changes r in one row of some 1e8), the angles are those of the stage-in's table,
+// and a key row equals the stage-in's for the same values and position.
+#include "kvm_internal.h"
+
+#include <cmath>
+#include <type_traits>
+
+#define KVM_APPEND_RUNS 40u      // runs of one launch: their descriptors are kernel arguments
+
+// ---- device: angles -----------------------------------------------------------
+// cos and sin of an fp32 angle to within an ulp of 64 bits: a - k pi/2 with pi/2 in two
+// doubles (one rounding each, by fma), then the Taylor series, whose first terms left
+// out are below 2^-57 for |r| <= pi/4.
+__device__ inline float2 cos_sin(float angle) {
+    const double a = (double)angle, k = rint(a * 0.63661977236758134308);
+    double r = __builtin_fma(-k, 1.57079632679489661923, a);
+    r = __builtin_fma(-k, 6.123233995736766036e-17, r);
+    const double z = r * r;
+    double c = 1.0 / 20922789888000.0, s = -1.0 / 1307674368000.0;      // 1 / 16!, -1 / 15!
+    c = __builtin_fma(c, z, -1.0 / 87178291200.0);
+    c = __builtin_fma(c, z, 1.0 / 479001600.0);
+    c = __builtin_fma(c, z, -1.0 / 3628800.0);
+    c = __builtin_fma(c, z, 1.0 / 40320.0);
+    c = __builtin_fma(c, z, -1.0 / 720.0);
+    c = __builtin_fma(c, z, 1.0 / 24.0);
+    c = __builtin_fma(c, z, -0.5);
+    c = __builtin_fma(c, z, 1.0);
+    s = __builtin_fma(s, z, 1.0 / 6227020800.0);
+    s = __builtin_fma(s, z, -1.0 / 39916800.0);
+    s = __builtin_fma(s, z, 1.0 / 362880.0);
+    s = __builtin_fma(s, z, -1.0 / 5040.0);
+    s = __builtin_fma(s, z, 1.0 / 120.0);
+    s = __builtin_fma(s, z, -1.0 / 6.0);
+    s = __builtin_fma(s * z, r, r);
+    const int quarter = (int)(k - 4.0 * floor(k * 0.25));
+    const double cc = quarter & 1 ? s : c, ss = quarter & 1 ? c : s;
+    return make_float2((float)(quarter == 1 || quarter == 2 ? -cc : cc), (float)(quarter >= 2 ? -ss : ss));
+}
+
+struct head_args {
+    uint32_t D, n_half;          // values of a row; rotated pairs, 0 = no rotation
+    int32_t nrot;                // Walsh-Hadamard width, 0 = none
+    int32_t norm;                // 0: rows are taken as they are
+    float hscale, eps;
+    float theta[128];
+};
+
+struct head_src {
+    const uint8_t *data;
+    int type;
+    size_t nb0, nb1, nb2;        // bytes from a dim, a head, a token to the next
+    const float *weight;         // [D] or null
+};
+
+// ---- device: rows ---------------------------------------------------------------
+// LPR lanes hold a row, 4 consecutive dims each, a wave 64 / LPR rows at a time and NI
+// times that in all, loaded before the first is used.
+template <typename T>
+__device__ __forceinline__ T ld_any(const void *p) {
+    T x;
+    __builtin_memcpy(&x, p, sizeof(T));
+    return x;
+}
+__device__ __forceinline__ void load4(const head_src &s, const uint8_t *p, float (&x)[4]) {
+    if (s.type == KVM_TYPE_F32) {
+        if (s.nb0 == 4) {
+            const kvm_f32x4 v = ld_any<kvm_f32x4>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = v[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = ld_any<float>(p + i * s.nb0);
+        }
+        return;
+    }
+    uint32_t u[4];
+    if (s.nb0 == 2) {
+        const kvm_u32x2 v = ld_any<kvm_u32x2>(p);
+        u[0] = v[0] & 0xffffu;
+        u[1] = v[0] >> 16;
+        u[2] = v[1] & 0xffffu;
+        u[3] = v[1] >> 16;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = ld_any<uint16_t>(p + i * s.nb0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = s.type == KVM_TYPE_BF16 ? kvm_bf2f((uint16_t)u[i]) : kvm_h2f((uint16_t)u[i]);
+}
+
+template <int LPR, int NI>
+struct head_rows {
+    static constexpr int RPW = 64 / LPR, ROWS = 4 * RPW * NI;    // rows of a wave at a time, of a workgroup
+    float x[NI][4];
+    uint32_t t[NI], h[NI];       // token of the block, head
+    bool live[NI];
+
+    // The rows of tokens [t0, t0 + nt) and heads [h0, h0 + nh), nt nh <= ROWS.
+    __device__ __forceinline__ void load(const head_args &a, const head_src &s, uint32_t t0, uint32_t nt, uint32_t h0, uint32_t nh) {
+        const uint32_t l = threadIdx.x & 63u, w = threadIdx.x >> 6, d0 = 4 * (l % LPR);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const uint32_t r = (i * 4 + w) * RPW + l / LPR;
+            live[i] = r < nt * nh;
+            t[i] = live[i] ? r / nh : 0u;
+            h[i] = h0 + (live[i] ? r - t[i] * nh : 0u);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[i][j] = 0.0f;
+            if (live[i] && d0 < a.D) load4(s, s.data + (size_t)(t0 + t[i]) * s.nb2 + (size_t)h[i] * s.nb1 + d0 * s.nb0, x[i]);
+        }
+    }
+
+    // norm, rotation, transform; cs: (cos, sin) of [token of the block][pair]
+    __device__ __forceinline__ void turn(const head_args &a, const head_src &s, const float2 *cs) {
+        const uint32_t l = threadIdx.x & 63u, d0 = 4 * (l % LPR);
+        if (a.norm) {
+            float w[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+            if (s.weight && d0 < a.D) {
+                const kvm_f32x4 v = ld_any<kvm_f32x4>(s.weight + d0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = v[j];
+            }
+            double sum[NI];
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                sum[i] = 0.0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[i] = __builtin_fma((double)x[i][j], (double)x[i][j], sum[i]);
+            }
+#pragma unroll
+            for (int o = 1; o < LPR; o <<= 1)
+#pragma unroll
+                for (int i = 0; i < NI; ++i) sum[i] += __shfl_xor(sum[i], o, 64);
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const float r = (float)(1.0 / sqrt(sum[i] / (double)a.D + (double)a.eps));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[i][j] = kvm_fmul(kvm_fmul(x[i][j], r), w[j]);
+            }
+        }
+        if (a.n_half) {
+            // the partner's lane: n_half is a multiple of 4
+            const bool lo = d0 < a.n_half, act = d0 < 2 * a.n_half;
+            const uint32_t pl = a.n_half / 4, p = lo ? l + pl : l - pl, ci = lo ? d0 : act ? d0 - a.n_half : 0u;
+            const uint32_t sm = lo ? 0x80000000u : 0u;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                float y[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    y[j] = __int_as_float(__builtin_amdgcn_ds_bpermute((int)((p & 63u) << 2), __float_as_int(x[i][j])));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 c = cs[t[i] * a.n_half + ci + j];
+                    const float v = kvm_fadd(kvm_fmul(x[i][j], c.x), kvm_fmul(y[j], __uint_as_float(__float_as_uint(c.y) ^ sm)));
+                    x[i][j] = act ? v : x[i][j];
+                }
+            }
+        }
+        if (a.nrot) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                float y[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = kvm_fmul(x[i][j], a.hscale);
+                x[i][0] = kvm_fadd(y[0], y[1]);
+                x[i][1] = kvm_fsub(y[0], y[1]);
+                x[i][2] = kvm_fadd(y[2], y[3]);
+                x[i][3] = kvm_fsub(y[2], y[3]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float u = x[i][j], v = x[i][j + 2];
+                    x[i][j] = kvm_fadd(u, v);
+                    x[i][j + 2] = kvm_fsub(u, v);
+                }
+            }
+            for (int o = 1; 4 * o < a.nrot; o <<= 1) {
+                const float sg = l & o ? -1.0f : 1.0f;           // the lane above takes other - own
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[i][j] = __builtin_fmaf(x[i][j], sg, __shfl_xor(x[i][j], o, 64));
+            }
+        }
+    }
+
+    // rows out [token][n_head][D] of `type`
+    __device__ __forceinline__ void store(const head_args &a, uint8_t *out, int type, uint32_t t0, uint32_t n_head) const {
+        const uint32_t d0 = 4 * ((threadIdx.x & 63u) % LPR);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            if (!live[i] || d0 >= a.D) continue;
+            const size_t at = ((size_t)(t0 + t[i]) * n_head + h[i]) * a.D + d0;
+            if (type == KVM_TYPE_F32) {
+                const kvm_f32x4 v = {x[i][0], x[i][1], x[i][2], x[i][3]};
+                __builtin_memcpy(out + 4 * at, &v, 16);
+                continue;
+            }
+            uint32_t u[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (type == KVM_TYPE_F16) {
+                    u[j] = kvm_f2h(x[i][j]);
+                } else {
+                    __bf16 b = (__bf16)x[i][j];
+                    uint16_t v;
+                    __builtin_memcpy(&v, &b, 2);
+                    u[j] = v;
+                }
+            }
+            const kvm_u32x2 v = {u[0] | u[1] << 16, u[2] | u[3] << 16};
+            __builtin_memcpy(out + 2 * at, &v, 8);
+        }
+    }
+};
+
+// (cos, sin) of the positions of tokens [t0, t0 + nt)
+__device__ __forceinline__ void fill_cs(const head_args &a, const int32_t *pos, uint32_t t0, uint32_t nt, float2 *cs) {
+    if (!a.n_half) return;
+    for (uint32_t i = threadIdx.x; i < nt * a.n_half; i += 256) {
+        const uint32_t t = i / a.n_half, j = i - t * a.n_half;
+        cs[i] = cos_sin(kvm_fmul((float)pos[t0 + t], a.theta[j]));
+    }
+    __syncthreads();
+}
+
+// The rows of a tensor, in units of tt tokens x hb heads.
+struct row_units {
+    uint32_t n_tokens, n_head, tt, hb, units;
+};
+
+template <int LPR, int NI>
+__device__ __forceinline__ void norm_rope_unit(const head_args &a, const head_src &s, const row_units &u, const int32_t *pos,
+                                               uint32_t unit, uint8_t *out, int type, float2 *cs) {
+    const uint32_t nhb = (u.n_head + u.hb - 1) / u.hb, t0 = unit / nhb * u.tt, h0 = unit % nhb * u.hb;
+    const uint32_t nt = min(u.tt, u.n_tokens - t0), nh = min(u.hb, u.n_head - h0);
+    head_rows<LPR, NI> r;
+    r.load(a, s, t0, nt, h0, nh);
+    fill_cs(a, pos, t0, nt, cs);
+    r.turn(a, s, cs);
+    r.store(a, out, type, t0, u.n_head);
+}
+
+struct norm_rope_args {
+    head_args a;
+    head_src q, k;
+    row_units uq, uk;
+    const int32_t *pos;
+    uint8_t *q_out, *k_out;
+    int type;
+};
+
+template <int LPR, int NI>
+__global__ void __launch_bounds__(256) k_norm_rope(norm_rope_args g) {
+    __shared__ float2 s_cs[512 * NI];    // ROWS tokens of 2 LPR pairs at most
+    const uint32_t b = blockIdx.x;
+    if (b < g.uq.units) norm_rope_unit<LPR, NI>(g.a, g.q, g.uq, g.pos, b, g.q_out, g.type, s_cs);
+    else norm_rope_unit<LPR, NI>(g.a, g.k, g.uk, g.pos, b - g.uq.units, g.k_out, g.type, s_cs);
+}
+
+// ---- device: keys and values into a window ---------------------------------------
+// A run: tokens tok0 .. tok0 + n - 1 of the call into cells cell0 .. of a window.  No two
+// runs of a launch touch the same 8-cell group or slot of a window: what is read and
+// written back (the words of 8 cells' nibbles, the slots' counts) has one owner.
+struct run_args {
+    uint8_t *k, *v;
+    int32_t *cell_pos;
+    uint32_t *shadow_rows, *pending;     // null, or the slots' counts
+    uint32_t n_tiles, bt;
+    uint32_t cell0, n, tok0;
+    uint32_t u0;                 // first unit
+};
+
+struct append_args {
+    head_args a;
+    head_src q, k, v;
+    row_units uq;
+    const int32_t *pos;
+    uint8_t *q_out;
+    int q_type;
+    uint32_t H, n_runs;
+    uint32_t tk, hk, ghb;        // tokens and heads of a key unit, (8-cell group, head) pairs of a value unit
+    run_args run[KVM_APPEND_RUNS];
+};
+static_assert(sizeof(append_args) <= 4096, "kernel arguments");
+
+// One (8-cell group, head) of the values: lane d of the D that share it has dim d of the
+// group's tokens, so a word (8 nibbles) or 16 bytes (8 halves) of the tile is a lane's own.
+template <int D, bool QUANT>
+__device__ __forceinline__ void append_v(const append_args &g, const run_args &r, uint32_t h, uint32_t grp, uint32_t d) {
+    const uint32_t c0 = 8 * grp;         // the group's first cell
+    const uint8_t *base = g.v.data + (size_t)h * g.v.nb1 + (size_t)d * g.v.nb0;
+    float x[8];
+    uint32_t valid = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+        const uint32_t i = c0 + j - r.cell0;                     // token of the run (wraps below cell0)
+        const bool in = c0 + j >= r.cell0 && i < r.n;
+        valid |= (uint32_t)in << j;
+        const uint8_t *p = base + (size_t)(r.tok0 + (in ? i : c0 + j < r.cell0 ? 0u : r.n - 1)) * g.v.nb2;
+        x[j] = g.v.type == KVM_TYPE_F32    ? ld_any<float>(p)
+               : g.v.type == KVM_TYPE_BF16 ? kvm_bf2f(ld_any<uint16_t>(p))
+                                           : kvm_h2f(ld_any<uint16_t>(p));
+    }
+    uint8_t *vt = r.v + ((size_t)h * r.n_tiles + c0 / 64) * kvm_vtile_bytes(QUANT ? KVM_TYPE_Q4_0 : KVM_TYPE_F16, D);
+    const uint32_t c = c0 % 64;
+    if constexpr (!QUANT) {
+        uint16_t *dst = (uint16_t *)vt + kvm_vh_idx(c, d);
+        uint32_t y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = kvm_f2h(x[j]);
+        if (valid == 0xffu) {
+            *(kvm_u32x4 *)dst = kvm_u32x4{y[0] | y[1] << 16, y[2] | y[3] << 16, y[4] | y[5] << 16, y[6] | y[7] << 16};
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (valid >> j & 1u) dst[j] = (uint16_t)y[j];
+        }
+    } else {
+        const uint32_t l = threadIdx.x & 31u;
+        uint32_t word = 0, mask = 0;
+        uint16_t *sc = (uint16_t *)(vt + kvm_vd_off(D, c, d / 32));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            // the block's largest magnitude, the first in dim order, with its sign
+            uint32_t top = __float_as_uint(fabsf(x[j]));
+            const float ax = __uint_as_float(top);
+            float m = ax;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+            const uint64_t eq = __builtin_amdgcn_ballot_w64(ax == m);
+            const uint32_t half = (uint32_t)(threadIdx.x & 32u ? eq >> 32 : eq);
+            const int first = half ? __builtin_ctz(half) : 0;
+            const float vmax = __shfl(x[j], (int)(threadIdx.x & 32u) + first, 64);
+            const float dsc = m > 0.0f ? kvm_fmul(vmax, -0.125f) : -0.0f;
+            int n = (int)kvm_fadd(kvm_fmul(x[j], kvm_recip_or0(dsc)), 8.5f);
+            n = n > 15 ? 15 : n;
+            if (valid >> j & 1u) {
+                mask |= 15u << kvm_vq_nib_shift(j);
+                word |= (uint32_t)(n & 15) << kvm_vq_nib_shift(j);
+                if (l == 0) sc[j] = kvm_f2h(dsc);
+            }
+        }
+        uint32_t *dst = (uint32_t *)(vt + kvm_vq_word(d, (c & 31u) >> 3, c >> 5));
+        if (mask != 0xffffffffu) word |= *dst & ~mask;
+        *dst = word;
+    }
+}
+
+// Key rows, 4 dims a lane: into the tile at cell c.
+template <int D, int KT, int NI>
+__device__ __forceinline__ void append_k(const head_rows<D / 4, NI> &r, const run_args &run, uint32_t cell) {
+    const uint32_t l = threadIdx.x & 63u, d0 = 4 * (l % (D / 4)), b = d0 / 32;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const uint32_t at = cell + r.t[i], c = at % 64;
+        uint8_t *kt = run.k + ((size_t)r.h[i] * run.n_tiles + at / 64) * kvm_ktile_bytes(KT, D);
+        if constexpr (KT == KVM_TYPE_F16) {
+            uint32_t y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = kvm_f2h(r.x[i][j]);
+            if (r.live[i]) *(kvm_u32x2 *)((uint16_t *)kt + kvm_kh_idx(D, c, d0)) = kvm_u32x2{y[0] | y[1] << 16, y[2] | y[3] << 16};
+        } else {
+            // a block's 32 dims are 8 lanes'
+            float m = fmaxf(fmaxf(fabsf(r.x[i][0]), fabsf(r.x[i][1])), fmaxf(fabsf(r.x[i][2]), fabsf(r.x[i][3])));
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+            float d;
+            if constexpr (KT == KVM_TYPE_Q8_0) {
+                d = kvm_div127(m);
+            } else {
+                // the sign of the first value of that magnitude in dim order
+                uint32_t first = 0xffu;
+#pragma unroll
+                for (int j = 3; j >= 0; --j)
+                    if (fabsf(r.x[i][j]) == m) first = 2 * (4 * (l & 7u) + j) + (__float_as_uint(r.x[i][j]) >> 31);
+#pragma unroll
+                for (int o = 1; o < 8; o <<= 1) first = min(first, (uint32_t)__shfl_xor((int)first, o, 64));
+                d = m > 0.0f ? kvm_fmul(first & 1u ? -m : m, -0.125f) : -0.0f;
+            }
+            const float id = kvm_recip_or0(d);
+            uint32_t qw = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                int q;
+                if constexpr (KT == KVM_TYPE_Q8_0) {
+                    q = kvm_round_away(kvm_fmul(r.x[i][j], id));
+                } else {
+                    q = (int)kvm_fadd(kvm_fmul(r.x[i][j], id), 8.5f);
+                    q = (q > 15 ? 15 : q) - 8;
+                }
+                qw |= (uint32_t)(uint8_t)(int8_t)q << (8 * j);
+            }
+            if (!r.live[i]) continue;
+            *(uint32_t *)(kt + kvm_kq_off(D, c, d0)) = qw;
+            if ((l & 7u) == 0) *(uint16_t *)(kt + kvm_kd_off(D, c, b)) = kvm_f2h(d);
+        }
+    }
+}
+
+template <int D, int KT, int NI>
+__global__ void __launch_bounds__(256) k_append(append_args g) {
+    __shared__ float2 s_cs[512 * NI];
+    constexpr bool QUANT = KT != KVM_TYPE_F16;
+    uint32_t b = blockIdx.x;
+    if (b < g.uq.units) return norm_rope_unit<D / 4, NI>(g.a, g.q, g.uq, g.pos, b, g.q_out, g.q_type, s_cs);
+    b -= g.uq.units;
+    // the unit's run (their first units ascend)
+    uint32_t ri = 0;
+    while (ri + 1 < g.n_runs && b >= g.run[ri + 1].u0) ++ri;
+    const run_args &r = g.run[ri];
+    b -= r.u0;
+    // the run's units: keys, values, then the positions and the slots' counts
+    const uint32_t nhb = (g.H + g.hk - 1) / g.hk, nk = (r.n + g.tk - 1) / g.tk * nhb;
+    if (b < nk) {
+        const uint32_t i0 = b / nhb * g.tk, nt = min(g.tk, r.n - i0), h0 = b % nhb * g.hk;
+        head_rows<D / 4, NI> rows;
+        rows.load(g.a, g.k, r.tok0 + i0, nt, h0, min(g.hk, g.H - h0));
+        fill_cs(g.a, g.pos, r.tok0 + i0, nt, s_cs);
+        rows.turn(g.a, g.k, s_cs);
+        append_k<D, KT, NI>(rows, r, r.cell0 + i0);
+        return;
+    }
+    b -= nk;
+    const uint32_t g0 = r.cell0 / 8, pairs = ((r.cell0 + r.n - 1) / 8 - g0 + 1) * g.H, nv = (pairs + g.ghb - 1) / g.ghb;
+    if (b < nv) {
+        for (uint32_t i = threadIdx.x / D; i < g.ghb; i += 256 / D) {
+            const uint32_t p = b * g.ghb + i;
+            if (p < pairs) append_v<D, QUANT>(g, r, p % g.H, g0 + p / g.H, threadIdx.x % D);
+        }
+        return;
+    }
+    for (uint32_t i = threadIdx.x; i < r.n; i += 256) r.cell_pos[r.cell0 + i] = g.pos[r.tok0 + i];
+    const uint32_t end = r.cell0 + r.n;
+    for (uint32_t slot = r.cell0 / r.bt + threadIdx.x; slot * r.bt < end; slot += 256) {
+        if (r.shadow_rows) r.shadow_rows[slot] = 0u;
+        if (r.pending) {
+            const uint32_t rows = min((slot + 1) * r.bt, end) - slot * r.bt;
+            r.pending[slot] = max(r.pending[slot], rows);
+        }
+    }
+}
+
+// ---- host -----------------------------------------------------------------------
+static int head_args_of(kvm_state *st, const char *what, uint32_t D, float eps, const kvm_rope_params *rope, int nrot, head_args *a) {
+    if (std::isnan(eps)) return kvm_fail(st, KVM_EINVAL, "%s: eps is not a number", what);
+    a->D = D;
+    a->norm = eps >= 0.0f;
+    a->eps = eps;
+    if (!rope) return KVM_OK;
+    if (rope->n_rot % 8 || rope->n_rot > D)
+        return kvm_fail(st, KVM_EUNSUPPORTED, "%s: n_rot %u (needs a multiple of 8 <= head_dim)", what, rope->n_rot);
+    if (rope->n_rot && !(rope->freq_base > 0.0f))
+        return kvm_fail(st, KVM_EINVAL, "%s: freq_base %g", what, (double)rope->freq_base);
+    if (!kvm_hadamard_ok(nrot, D))
+        return kvm_fail(st, KVM_EUNSUPPORTED, "%s: hadamard width %d", what, nrot);
+    a->n_half = rope->n_rot / 2;
+    a->nrot = nrot;
+    a->hscale = nrot ? 1.0f / sqrtf((float)nrot) : 1.0f;
+    for (uint32_t i = 0; i < a->n_half; ++i)     // kvm_rope_theta's
+        a->theta[i] = powf(rope->freq_base, -2.0f * (float)i / (float)rope->n_rot) * rope->freq_scale;
+    return KVM_OK;
+}
+
+// A view as rows of D dims: [tokens][heads][D], or with the heads of a token packed in
+// one or several longer rows.
+static int head_src_of(kvm_state *st, const char *what, const kvm_view *v, uint32_t D, uint32_t n_head, const float *weight, head_src *s) {
+    kvm_view some = *v;
+    if (v->ne2 == 0 && !v->data) some.data = &some;     // no tokens: no memory either
+    const int rc = view_check(st, &some, n_head * D, what);
+    if (rc) return rc;
+    if (v->ne2 > 0x7fffffff) return kvm_fail(st, KVM_ERANGE, "%s: %lld tokens", what, (long long)v->ne2);
+    *s = head_src{(const uint8_t *)v->data, v->type, v->nb0, v->nb1, v->nb2, weight};
+    if (v->ne0 == (int64_t)D) return KVM_OK;
+    if (v->ne0 % D == 0 && (v->ne1 == 1 || v->nb1 == (size_t)v->ne0 * v->nb0)) {
+        s->nb1 = D * v->nb0;
+        return KVM_OK;
+    }
+    return kvm_fail(st, KVM_EUNSUPPORTED, "%s: view rows of %lld values, heads of %u", what, (long long)v->ne0, D);
+}
+
+// Rows out: the output may be the rows' own memory, packed and of the same type (a row is
+// read before it is written, by the same lanes), but overlap no input otherwise.
+static bool overlaps(const void *out, size_t bytes, const kvm_view *v) {
+    if (!v || v->ne2 == 0) return false;
+    const size_t es = v->type == KVM_TYPE_F32 ? 4 : 2;
+    const uintptr_t a = (uintptr_t)out, b = (uintptr_t)v->data;
+    const uintptr_t e = b + (size_t)(v->ne2 - 1) * v->nb2 + (size_t)(v->ne1 - 1) * v->nb1 + (size_t)(v->ne0 - 1) * v->nb0 + es;
+    return a < e && b < a + bytes;
+}
+static bool in_place(const void *out, int type, const head_src &s, uint32_t D, uint32_t n_head) {
+    const size_t es = type == KVM_TYPE_F32 ? 4 : 2;
+    return out == s.data && type == s.type && s.nb0 == es && s.nb1 == D * es && s.nb2 == (size_t)n_head * D * es;
+}
+
+static bool float_type(int t) { return t == KVM_TYPE_F32 || t == KVM_TYPE_F16 || t == KVM_TYPE_BF16; }
+
+static row_units units_of(uint32_t n_tokens, uint32_t n_head, uint32_t rows) {
+    row_units u{};
+    if (!n_tokens) return u;
+    u.n_tokens = n_tokens;
+    u.n_head = n_head;
+    u.hb = n_head < rows ? n_head : rows;
+    u.tt = rows / u.hb;
+    u.units = kvm_cdiv(n_tokens, u.tt) * kvm_cdiv(n_head, u.hb);
+    return u;
+}
+
+template <typename F>
+static void by_ni(uint64_t n_rows, uint32_t rows1, uint32_t n_cu, F &&f) {
+    if (n_rows <= 8ull * n_cu * rows1) f(std::integral_constant<int, 1>{});
+    else f(std::integral_constant<int, 4>{});
+}
+
+extern "C" int kvm_qk_norm_rope(kvm_state *st, const kvm_view *q, const kvm_view *k, const float *q_weight,
+                                const float *k_weight, float eps, const kvm_rope_params *rope, const int32_t *pos,
+                                int out_type, void *q_out, void *k_out) {
+    const char *what = "qk_norm_rope";
+    if (!q && !k) return kvm_fail(st, KVM_EINVAL, "%s: no queries and no keys", what);
+    if (!float_type(out_type)) return kvm_fail(st, KVM_EUNSUPPORTED, "%s: output type %d", what, out_type);
+    const kvm_view *one = q ? q : k;
+    if (one->ne0 <= 0 || one->ne0 % 8 || one->ne0 > 256) return kvm_fail(st, KVM_EUNSUPPORTED, "%s: head_dim %lld (needs a multiple of 8 <= 256)", what, (long long)one->ne0);
+    if (q && k && (q->ne0 != k->ne0 || q->ne2 != k->ne2)) return kvm_fail(st, KVM_EINVAL, "%s: queries and keys of different head_dim or tokens", what);
+    for (const kvm_view *v : {q, k})
+        if (v && (v->ne1 <= 0 || v->ne1 > (1 << 20))) return kvm_fail(st, KVM_ERANGE, "%s: %lld heads", what, (long long)v->ne1);
+    if (rope && rope->hadamard_nrot < 0) return kvm_fail(st, KVM_EINVAL, "%s: hadamard width %d (there is no window to take it from)", what, rope->hadamard_nrot);
+    norm_rope_args g{};
+    const uint32_t D = (uint32_t)one->ne0;
+    int rc = head_args_of(st, what, D, eps, rope, rope ? rope->hadamard_nrot : 0, &g.a);
+    if (rc) return rc;
+    const size_t es = out_type == KVM_TYPE_F32 ? 4 : 2;
+    uint32_t Hq = 0, Hk = 0;
+    if (q) {
+        Hq = (uint32_t)q->ne1;
+        if ((rc = head_src_of(st, what, q, D, Hq, q_weight, &g.q))) return rc;
+    }
+    if (k) {
+        Hk = (uint32_t)k->ne1;
+        if ((rc = head_src_of(st, what, k, D, Hk, k_weight, &g.k))) return rc;
+    }
+    const uint32_t n = (uint32_t)one->ne2;
+    const uint64_t n_rows = (uint64_t)n * (Hq + Hk);
+    if (n == 0) return KVM_OK;
+    if (n_rows > (1u << 30)) return kvm_fail(st, KVM_ERANGE, "%s: %u tokens", what, n);
+    if ((q && !q_out) || (k && !k_out) || (g.a.n_half && !pos)) return kvm_fail(st, KVM_EINVAL, "%s: null argument", what);
+    const size_t bq = (size_t)n * Hq * D * es, bk = (size_t)n * Hk * D * es;
+    if ((q && ((overlaps(q_out, bq, q) && !in_place(q_out, out_type, g.q, D, Hq)) || overlaps(q_out, bq, k))) ||
+        (k && ((overlaps(k_out, bk, k) && !in_place(k_out, out_type, g.k, D, Hk)) || overlaps(k_out, bk, q))) ||
+        (q && k && (uint8_t *)q_out < (uint8_t *)k_out + bk && (uint8_t *)k_out < (uint8_t *)q_out + bq && bq))
+        return kvm_fail(st, KVM_EINVAL, "%s: an output overlaps an input or the other output", what);
+    if (!st) return KVM_EINVAL;
+    g.pos = pos;
+    g.q_out = (uint8_t *)q_out;
+    g.k_out = (uint8_t *)k_out;
+    g.type = out_type;
+    KVM_HIP(st, hipSetDevice(st->device));
+    auto go = [&](auto lpr) {
+        constexpr int LPR = decltype(lpr)::value;
+        by_ni(n_rows, 4 * (64 / LPR), st->n_cu, [&](auto ni) {
+            constexpr int NI = decltype(ni)::value;
+            constexpr uint32_t ROWS = head_rows<LPR, NI>::ROWS;
+            g.uq = units_of(q ? n : 0, Hq, ROWS);
+            g.uk = units_of(k ? n : 0, Hk, ROWS);
+            hipLaunchKernelGGL((k_norm_rope<LPR, NI>), dim3(g.uq.units + g.uk.units), dim3(256), 0, st->stream, g);
+        });
+    };
+    if (D > 128) go(std::integral_constant<int, 64>{});
+    else if (D > 64) go(std::integral_constant<int, 32>{});
+    else go(std::integral_constant<int, 16>{});
+    KVM_LAUNCH_CHECK(st, what);
+    return KVM_OK;
+}
+
+extern "C" int kvm_window_append(kvm_state *st, const kvm_window *const *windows, const uint32_t *cell0,
+                                 const uint32_t *n_tokens, uint32_t n_runs, const kvm_view *k, const kvm_view *v,
+                                 const float *k_weight, float eps, const kvm_rope_params *rope, const int32_t *pos,
+                                 const kvm_view *q, const float *q_weight, int q_out_type, void *q_out) {
+    const char *what = "window_append";
+    if (n_runs == 0) return KVM_OK;
+    if (!windows || !cell0 || !n_tokens || !k || !v) return kvm_fail(st, KVM_EINVAL, "%s: null argument", what);
+    if (q && !float_type(q_out_type)) return kvm_fail(st, KVM_EUNSUPPORTED, "%s: output type %d", what, q_out_type);
+    uint64_t total = 0;
+    for (uint32_t i = 0; i < n_runs; ++i) {
+        const kvm_window *w = windows[i], *w0 = windows[0];
+        const int rc = kvm_window_check(w);
+        if (rc) return kvm_fail(st, rc, "%s: run %u: bad window", what, i);
+        if (w->n_head_kv != w0->n_head_kv || w->head_dim != w0->head_dim || w->k_type != w0->k_type || w->v_type != w0->v_type)
+            return kvm_fail(st, KVM_EUNSUPPORTED, "%s: run %u: windows of different heads or types", what, i);
+        if ((uint64_t)cell0[i] + n_tokens[i] > w->n_cells) return kvm_fail(st, KVM_ERANGE, "%s: run %u: cells past the window", what, i);
+        total += n_tokens[i];
+    }
+    const kvm_window *w0 = windows[0];
+    const uint32_t D = w0->head_dim, H = w0->n_head_kv;
+    append_args g{};
+    int rc = head_args_of(st, what, D, eps, rope, rope ? kvm_hadamard_width(w0, rope->hadamard_nrot) : 0, &g.a);
+    if (rc) return rc;
+    if ((rc = head_src_of(st, what, k, D, H, k_weight, &g.k)) || (rc = head_src_of(st, what, v, D, H, nullptr, &g.v))) return rc;
+    uint32_t Hq = 0;
+    if (q) {
+        if (q->ne0 <= 0 || q->ne1 <= 0 || (uint64_t)q->ne0 * (uint64_t)q->ne1 % D || (uint64_t)q->ne0 * (uint64_t)q->ne1 > (1u << 28))
+            return kvm_fail(st, KVM_EINVAL, "%s: queries of %lld x %lld values, heads of %u", what, (long long)q->ne0, (long long)q->ne1, D);
+        Hq = (uint32_t)((uint64_t)q->ne0 * (uint64_t)q->ne1 / D);
+        if ((rc = head_src_of(st, what, q, D, Hq, q_weight, &g.q))) return rc;
+    }
+    if ((uint64_t)k->ne2 != total || (uint64_t)v->ne2 != total || (q && (uint64_t)q->ne2 != total))
+        return kvm_fail(st, KVM_EINVAL, "%s: runs of %llu tokens, keys of %lld, values of %lld", what, (unsigned long long)total, (long long)k->ne2, (long long)v->ne2);
+    if (total * (H + Hq) > (1u << 30)) return kvm_fail(st, KVM_ERANGE, "%s: %llu tokens", what, (unsigned long long)total);
+    if (total == 0) return KVM_OK;
+    if (!pos || (q && !q_out)) return kvm_fail(st, KVM_EINVAL, "%s: null argument", what);
+    if (q) {
+        const size_t bytes = total * Hq * D * (q_out_type == KVM_TYPE_F32 ? 4 : 2);
+        if ((overlaps(q_out, bytes, q) && !in_place(q_out, q_out_type, g.q, D, Hq)) || overlaps(q_out, bytes, k) || overlaps(q_out, bytes, v))
+            return kvm_fail(st, KVM_EINVAL, "%s: the query output overlaps an input", what);
+    }
+    if (!st) return KVM_EINVAL;
+    g.pos = pos;
+    g.q_out = (uint8_t *)q_out;
+    g.q_type = q_out_type;
+    g.H = H;
+    KVM_HIP(st, hipSetDevice(st->device));
+
+    // Launches of runs that share no 8-cell group and no slot; the first takes the queries.
+    uint32_t tok = 0;
+    auto shares = [&](uint32_t i, uint32_t j) {
+        const kvm_window *a = windows[i], *b = windows[j];
+        if (a->k != b->k && a->v != b->v && a->cell_pos != b->cell_pos) return false;
+        const uint32_t s = a->block_tokens % 8 ? 1u : a->block_tokens, m = s > 8 && (a->pending_rows || a->shadow_rows) ? s : 8u;
+        if (s == 1u) return true;        // (slots that cut the groups)
+        return cell0[i] / m <= (cell0[j] + n_tokens[j] - 1) / m && cell0[j] / m <= (cell0[i] + n_tokens[i] - 1) / m;
+    };
+    by_ni(total * (H + Hq), 4 * (64 / (D / 4)), st->n_cu, [&](auto ni) {
+        constexpr int NI = decltype(ni)::value;
+        const uint32_t rows = 4 * (256 / D) * NI;
+        g.ghb = NI * (256 / D);
+        g.uq = units_of(q ? (uint32_t)total : 0u, Hq, rows);
+        g.hk = H < rows ? H : rows;
+        g.tk = rows / g.hk;
+        for (uint32_t i = 0; i < n_runs;) {
+            uint32_t first = i, units = 0;
+            g.n_runs = 0;
+            for (; i < n_runs && g.n_runs < KVM_APPEND_RUNS; ++i) {
+                if (!n_tokens[i]) continue;
+                bool clash = false;
+                for (uint32_t j = first; j < i && !clash; ++j) clash = n_tokens[j] && shares(i, j);
+                if (clash) break;
+                const kvm_window *w = windows[i];
+                run_args &r = g.run[g.n_runs++];
+                r = run_args{(uint8_t *)w->k, (uint8_t *)w->v, w->cell_pos, w->shadow_rows, w->pending_rows,
+                             w->n_cells / KVM_TILE_CELLS, w->block_tokens, cell0[i], n_tokens[i], tok, units};
+                const uint32_t pairs = ((cell0[i] + n_tokens[i] - 1) / 8 - cell0[i] / 8 + 1) * H;
+                units += kvm_cdiv(n_tokens[i], g.tk) * kvm_cdiv(H, g.hk) + kvm_cdiv(pairs, g.ghb) + 1;
+                tok += n_tokens[i];
+            }
+            if (!g.n_runs) break;
+            auto go = [&](auto d, auto kt) {
+                hipLaunchKernelGGL((k_append<decltype(d)::value, decltype(kt)::value, NI>), dim3(g.uq.units + units), dim3(256), 0, st->stream, g);
+            };
+            auto go_d = [&](auto d) {
+                if (w0->k_type == KVM_TYPE_Q8_0) go(d, std::integral_constant<int, KVM_TYPE_Q8_0>{});
+                else if (w0->k_type == KVM_TYPE_Q4_0) go(d, std::integral_constant<int, KVM_TYPE_Q4_0>{});
+                else go(d, std::integral_constant<int, KVM_TYPE_F16>{});
+            };
+            if (D == 256) go_d(std::integral_constant<int, 256>{});
+            else go_d(std::integral_constant<int, 128>{});
+            g.uq.units = 0;
+        }
+    });
+    KVM_LAUNCH_CHECK(st, what);
+    return KVM_OK;
+}

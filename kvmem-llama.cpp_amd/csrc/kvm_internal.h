@@ -203,6 +203,19 @@ __host__ __device__ inline uint32_t kvm_vh_idx(uint32_t c, uint32_t d) {
     return ((((d >> 4) * 64u + 16u * g + (d & 15u)) * 2u + ks) << 3) + j;
 }
 
+// Walsh-Hadamard width of a window's keys: as asked for, or (req < 0) the default of the
+// K type (attn_rot_on and kvmem_hadamard_nrot_k, llama-kvmem-quant.h:22-36).
+inline int kvm_hadamard_width(const kvm_window *w, int32_t req) {
+    if (req >= 0) return req;
+    if (!kvm_k_quant(w->k_type) || w->head_dim < 64 || w->head_dim % 64) return 0;
+    int nrot = 64;
+    do { nrot *= 2; } while (w->head_dim % nrot == 0);
+    return nrot / 2;
+}
+inline bool kvm_hadamard_ok(int nrot, uint32_t D) {
+    return nrot == 0 || (nrot >= 64 && nrot <= (int)D && !(nrot & (nrot - 1)) && D % nrot == 0);
+}
+
 // ---------------------------------------------------------------------------
 // Device helpers
 // ---------------------------------------------------------------------------

@@ -41,18 +41,6 @@ static int rope_ctx_for(kvm_state *st, const float *theta, uint32_t n_half, int3
     return KVM_OK;
 }
 
-static int hadamard_width(const kvm_window *w, int32_t req) {
-    if (req >= 0) return req;
-    if (!kvm_k_quant(w->k_type) || w->head_dim < 64 || w->head_dim % 64) return 0;   // attn_rot_on
-    int nrot = 64;                               // kvmem_hadamard_nrot_k, llama-kvmem-quant.h:30-36
-    do { nrot *= 2; } while (w->head_dim % nrot == 0);
-    return nrot / 2;
-}
-
-static bool hadamard_ok(int nrot, uint32_t D) {
-    return nrot == 0 || (nrot >= 64 && nrot <= (int)D && !(nrot & (nrot - 1)) && D % nrot == 0);
-}
-
 // Checks one lane and fills its kernel arguments (all but the RoPE context).
 static int stage_lane_args(kvm_state *st, const kvm_history *h, const kvm_window *w,
                            const kvm_selection *sel, stage_args *a, uint32_t *max_items) {
@@ -128,8 +116,8 @@ int kvm_stage_prepare(kvm_state *st, const kvm_stagein_lane *lanes, uint32_t n_l
     const kvm_window *w0 = lanes[0].w;
     if (rope->n_rot < 8 || rope->n_rot > w0->head_dim || rope->n_rot % 8)
         return kvm_fail(st, KVM_EUNSUPPORTED, "stagein: n_rot %u (needs a multiple of 8 <= head_dim)", rope->n_rot);
-    const int nrot = hadamard_width(w0, rope->hadamard_nrot);
-    if (!hadamard_ok(nrot, w0->head_dim)) return kvm_fail(st, KVM_EUNSUPPORTED, "stagein: hadamard width %d", nrot);
+    const int nrot = kvm_hadamard_width(w0, rope->hadamard_nrot);
+    if (!kvm_hadamard_ok(nrot, w0->head_dim)) return kvm_fail(st, KVM_EUNSUPPORTED, "stagein: hadamard width %d", nrot);
     KVM_HIP(st, hipSetDevice(st->device));
     const std::vector<float> theta = kvm_rope_theta(rope->freq_base, rope->freq_scale, rope->n_rot);
     rope_ctx rc0;
@@ -279,7 +267,7 @@ extern "C" int kvm_stagein_enqueue_k(kvm_state *st, int type, const void *packed
     if ((size_t)nt * (size_t)(n_embd / 32 * kb) != nbytes) return kvm_fail(st, KVM_EINVAL, "enqueue_k: nbytes %zu mismatch", nbytes);
     if (n_rot_rope < 8 || n_rot_rope % 8 || n_rot_rope > n_embd_head || n_theta != n_rot_rope / 2 || !theta)
         return kvm_fail(st, KVM_EUNSUPPORTED, "enqueue_k: n_rot %d / n_theta %d", n_rot_rope, n_theta);
-    if (!hadamard_ok(nrot, w->head_dim)) return kvm_fail(st, KVM_EUNSUPPORTED, "enqueue_k: hadamard width %d", nrot);
+    if (!kvm_hadamard_ok(nrot, w->head_dim)) return kvm_fail(st, KVM_EUNSUPPORTED, "enqueue_k: hadamard width %d", nrot);
     // one theta per flush: a different theta flushes what is queued first
     if (!st->items.empty() && !st->theta.empty() &&
         (st->theta.size() != (size_t)n_theta || std::memcmp(st->theta.data(), theta, n_theta * 4))) {

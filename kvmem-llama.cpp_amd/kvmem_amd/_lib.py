@@ -137,6 +137,11 @@ SIGNATURES = {
     "kvm_slot_free": (C.c_int, [C.POINTER(SlotPool), _i32]),
     "kvm_slot_copy_to_host": (C.c_int, [_P, C.POINTER(_PW), _u32, _i32, _P, C.c_uint64]),
     "kvm_slot_copy_from_host": (C.c_int, [_P, C.POINTER(_PW), _u32, _i32, _P, C.c_uint64]),
+    "kvm_qk_norm_rope": (C.c_int, [_P, C.POINTER(View), C.POINTER(View), _P, _P, _f, C.POINTER(RopeParams), _P, C.c_int,
+                                   _P, _P]),
+    "kvm_window_append": (C.c_int, [_P, C.POINTER(_PW), C.POINTER(_u32), C.POINTER(_u32), _u32, C.POINTER(View),
+                                    C.POINTER(View), _P, _f, C.POINTER(RopeParams), _P, C.POINTER(View), _P, C.c_int,
+                                    _P]),
     "kvm_harvest_block": (C.c_int, [_P, _PW, _u32, _u32, C.POINTER(View), _u32, _P, _P, C.POINTER(MeanKIndex),
                                     _u32, _u32]),
     "kvm_quantize_rows": (C.c_int, [_P, C.c_int, _P, _P, _i64, _i64]),

@@ -693,6 +693,128 @@ def prepare_decode_step_lanes(st, lanes, n_head, scale, n_rot, freq_base, freq_s
                     (st.h, arr, hists, fl, n, C.byref(r), qt, n_head, float(scale)), (keep, arr, hists, fl, r))
 
 
+def _on_device(st, dtype, shape, **tensors):
+    """Refuses what the kernels would read wrongly: a tensor on another device, of
+    another type or shape, or not packed (None passes)."""
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if t.device != torch.device("cuda", st.device) or t.dtype != dtype or tuple(t.shape) != tuple(shape) or \
+                not t.is_contiguous():
+            raise L.KvmError(L.KVM_EINVAL, f"{name}: needs a packed {dtype} tensor {list(shape)} on cuda:{st.device}, got "
+                                           f"{t.dtype} {list(t.shape)} on {t.device}")
+
+
+def _head_views(st, **tensors):
+    """kvm_views of [tokens][heads][dims] tensors on the state's device (None passes)."""
+    for name, t in tensors.items():
+        if t is not None and (t.dim() != 3 or t.dtype not in _VIEW_TYPES or t.device != torch.device("cuda", st.device)):
+            raise L.KvmError(L.KVM_EINVAL, f"{name}: needs [tokens][heads][dims] of fp32, fp16 or bf16 on cuda:{st.device}, "
+                                           f"got {t.dtype} {list(t.shape)} on {t.device}")
+    return [None if t is None else view(t) for t in tensors.values()]
+
+
+def _rope_of(n_rot, freq_base, freq_scale, hadamard_nrot):
+    return L.RopeParams(n_rot or 0, freq_base, freq_scale, hadamard_nrot)
+
+
+def _out_of(st, x, out, dtype, name):
+    """The output rows of x: given, or a new tensor of dtype (x's if None)."""
+    if out is None:
+        return torch.empty(x.shape, dtype=dtype or x.dtype, device=x.device)
+    if dtype is not None and dtype != out.dtype:
+        raise L.KvmError(L.KVM_EINVAL, f"{name}: {out.dtype}, asked for {dtype}")
+    if out.dtype not in _VIEW_TYPES:
+        raise L.KvmError(L.KVM_EINVAL, f"{name}: {out.dtype}")
+    _on_device(st, out.dtype, x.shape, **{name: out})
+    return out
+
+
+def prepare_qk_norm_rope(st, q, k, pos, n_rot, freq_base, freq_scale=1.0, hadamard_nrot=0, q_weight=None, k_weight=None,
+                         eps=None, q_out=None, k_out=None, out_dtype=None):
+    """kvm_qk_norm_rope: head norms (eps = None: none), rotation of the first n_rot dims
+    (0: none) and Walsh-Hadamard transform (0: none) of the queries and keys
+    [tokens][heads][dims], any strides; q or k may be None.  The call's results are its
+    q_out and k_out: given, or new tensors of out_dtype (the input's type if None)."""
+    qv, kv = _head_views(st, q=q, k=k)
+    one = q if q is not None else k
+    if one is None:
+        raise L.KvmError(L.KVM_EINVAL, "qk_norm_rope: no queries and no keys")
+    _on_device(st, torch.int32, (one.shape[0],), pos=pos)
+    _on_device(st, torch.float32, (one.shape[2],), q_weight=q_weight, k_weight=k_weight)
+    q_out = None if q is None else _out_of(st, q, q_out, out_dtype, "q_out")
+    k_out = None if k is None else _out_of(st, k, k_out, out_dtype, "k_out")
+    types = {t.dtype for t in (q_out, k_out) if t is not None}
+    if len(types) > 1:
+        raise L.KvmError(L.KVM_EINVAL, f"qk_norm_rope: outputs of {types}")
+    r = _rope_of(n_rot, freq_base, freq_scale, hadamard_nrot)
+    p = Prepared(st, st.lib.kvm_qk_norm_rope,
+                 (st.h, None if q is None else C.byref(qv), None if k is None else C.byref(kv), _ptr(q_weight),
+                  _ptr(k_weight), -1.0 if eps is None else float(eps), C.byref(r), _ptr(pos), _VIEW_TYPES[types.pop()],
+                  _ptr(q_out), _ptr(k_out)),
+                 (q, k, qv, kv, q_weight, k_weight, r, pos))
+    p.q_out, p.k_out = q_out, k_out
+    return p
+
+
+def qk_norm_rope(st, q, k, pos, n_rot, freq_base, freq_scale=1.0, hadamard_nrot=0, q_weight=None, k_weight=None, eps=None,
+                 q_out=None, k_out=None, out_dtype=None):
+    """Returns (q_out, k_out) of prepare_qk_norm_rope's call."""
+    p = prepare_qk_norm_rope(st, q, k, pos, n_rot, freq_base, freq_scale, hadamard_nrot, q_weight, k_weight, eps, q_out,
+                             k_out, out_dtype)
+    p()
+    return p.q_out, p.k_out
+
+
+def _window_ptrs(st, windows):
+    """Windows (None allowed) as an array of kvm_window pointers."""
+    arr = (C.POINTER(L.Window) * max(len(windows), 1))()
+    for i, w in enumerate(windows):
+        if w is not None:
+            if w.st.device != st.device:
+                raise L.KvmError(L.KVM_EINVAL, f"window {i}: on cuda:{w.st.device}, the state on cuda:{st.device}")
+            arr[i] = C.pointer(w.c)
+    return arr
+
+
+def prepare_window_append(st, windows, cell0, n_tokens, k, v, pos, n_rot, freq_base, freq_scale=1.0, hadamard_nrot=-1,
+                          k_weight=None, eps=None, q=None, q_weight=None, q_out=None, q_out_dtype=None):
+    """kvm_window_append: run i takes the next n_tokens[i] tokens of k and v
+    ([tokens][kv heads][dims], any strides) into cells cell0[i] .. of windows[i]; keys
+    normed (eps = None: not), rotated and transformed on the way (hadamard_nrot = -1: the
+    window type's width).  With q, the call's q_out holds the tokens' queries treated
+    the same."""
+    if not (len(windows) == len(cell0) == len(n_tokens)):
+        raise L.KvmError(L.KVM_EINVAL, f"window_append: {len(windows)} windows, {len(cell0)} cells, {len(n_tokens)} counts")
+    if any(w is None for w in windows) or any(int(x) < 0 for x in (*cell0, *n_tokens)):
+        raise L.KvmError(L.KVM_EINVAL, "window_append: a run without a window, or a negative cell or count")
+    qv, kv, vv = _head_views(st, q=q, k=k, v=v)
+    if k is None or v is None:
+        raise L.KvmError(L.KVM_EINVAL, "window_append: no keys or no values")
+    _on_device(st, torch.int32, (k.shape[0],), pos=pos)
+    _on_device(st, torch.float32, (k.shape[2],), k_weight=k_weight, q_weight=q_weight)
+    q_out = None if q is None else _out_of(st, q, q_out, q_out_dtype, "q_out")
+    n = len(windows)
+    arr, c0, nt = _window_ptrs(st, windows), (L._u32 * max(n, 1))(*map(int, cell0)), (L._u32 * max(n, 1))(*map(int, n_tokens))
+    r = _rope_of(n_rot, freq_base, freq_scale, hadamard_nrot)
+    p = Prepared(st, st.lib.kvm_window_append,
+                 (st.h, arr, c0, nt, n, C.byref(kv), C.byref(vv), _ptr(k_weight), -1.0 if eps is None else float(eps),
+                  C.byref(r), _ptr(pos), None if q is None else C.byref(qv), _ptr(q_weight),
+                  L.T_F32 if q is None else _VIEW_TYPES[q_out.dtype], _ptr(q_out)),
+                 (windows, arr, c0, nt, k, v, kv, vv, k_weight, r, pos, q, qv, q_weight))
+    p.q_out = q_out
+    return p
+
+
+def window_append(st, windows, cell0, n_tokens, k, v, pos, n_rot, freq_base, freq_scale=1.0, hadamard_nrot=-1, k_weight=None,
+                  eps=None, q=None, q_weight=None, q_out=None, q_out_dtype=None):
+    """prepare_window_append's call; returns q_out (None without q)."""
+    p = prepare_window_append(st, windows, cell0, n_tokens, k, v, pos, n_rot, freq_base, freq_scale, hadamard_nrot, k_weight,
+                              eps, q, q_weight, q_out, q_out_dtype)
+    p()
+    return p.q_out
+
+
 def quantize_rows(st, ty, x):
     """x: device fp32 [n_rows][n_per_row] -> uint8 ggml rows."""
     x = x.contiguous()
