@@ -253,6 +253,8 @@ def _handles(case, s):
         for i, w in enumerate(s["windows"]):
             w.import_rows(0, s["lk"][i], s["lv"][i], s["lpos"][i])
         del s["lk"], s["lv"]
+    if case["kind"] in ("append", "step") and case["cache"] == "f16":
+        s["views"] = [_cells(case, w) for w in s["windows"]]
     s["calls"] = _calls(case, s)
     return s
 
@@ -307,7 +309,7 @@ def _run_own(s):
     if append is not None:
         append()
         if case["cache"] == "f16":
-            res["cells"] = [_cells(case, w) for w in s["windows"]]
+            res["cells"] = s["views"]
         else:                             # the values that the cells now hold
             w, n, e = s["windows"][0], s["counts"][0], case["kv_heads"] * case["head_dim"]
             kr, vr = w.export_rows(case["cell0"], n)
