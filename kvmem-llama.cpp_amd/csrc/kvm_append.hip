@@ -21,6 +21,8 @@
 
 #define KVM_APPEND_RUNS 40u      // runs of one launch: their descriptors are kernel arguments
 
+typedef __bf16 kvm_bf16x4 __attribute__((ext_vector_type(4)));
+
 // ---- device: angles -----------------------------------------------------------
 // cos and sin of an fp32 angle to within an ulp of 64 bits: a - k pi/2 with pi/2 in two
 // doubles (one rounding each, by fma), then the Taylor series, whose first terms left
@@ -56,6 +58,7 @@ struct head_args {
     int32_t nrot;                // Walsh-Hadamard width, 0 = none
     int32_t norm;                // 0: rows are taken as they are
     float hscale, eps;
+    double inv_D;
     float theta[128];
 };
 
@@ -75,31 +78,42 @@ __device__ __forceinline__ T ld_any(const void *p) {
     __builtin_memcpy(&x, p, sizeof(T));
     return x;
 }
+__device__ __forceinline__ uint32_t elem_size(int type) { return type == KVM_TYPE_F32 ? 4u : 2u; }
+__device__ __forceinline__ float from16(int type, uint32_t u) { return type == KVM_TYPE_BF16 ? kvm_bf2f((uint16_t)u) : kvm_h2f((uint16_t)u); }
+// 4 dims of a row at p, any strides and type
 __device__ __forceinline__ void load4(const head_src &s, const uint8_t *p, float (&x)[4]) {
-    if (s.type == KVM_TYPE_F32) {
-        if (s.nb0 == 4) {
-            const kvm_f32x4 v = ld_any<kvm_f32x4>(p);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = v[i];
-        } else {
+    for (int i = 0; i < 4; ++i) x[i] = s.type == KVM_TYPE_F32 ? ld_any<float>(p + i * s.nb0) : from16(s.type, ld_any<uint16_t>(p + i * s.nb0));
+}
+
+// A 64-bit value of another lane, as a DPP move of its halves.
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0u, (uint32_t)u, CTRL, 0xf, 0xf, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+#define DPP_QUAD(a, b, c, d) ((a) | (b) << 2 | (c) << 4 | (d) << 6)
+// x of the even and of the odd row of 16 lanes (or half of 32) of a pair, added: the same in both.
+template <int N>
+__device__ __forceinline__ double add_rows_f64(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t l = (uint32_t)u, h = (uint32_t)(u >> 32);
+    const auto a = N == 16 ? __builtin_amdgcn_permlane16_swap(l, l, false, false) : __builtin_amdgcn_permlane32_swap(l, l, false, false);
+    const auto b = N == 16 ? __builtin_amdgcn_permlane16_swap(h, h, false, false) : __builtin_amdgcn_permlane32_swap(h, h, false, false);
+    return __builtin_bit_cast(double, (uint64_t)b[0] << 32 | a[0]) + __builtin_bit_cast(double, (uint64_t)b[1] << 32 | a[1]);
+}
+// 1 / sqrt(m) to within some ulps of 64 bits: two Newton steps from the hardware's
+// estimate (m is at least the square of the smallest fp32, or 0, infinite or no number).
+__device__ __forceinline__ double recip_sqrt(double m) {
+    double y = __builtin_amdgcn_rsq(m);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = ld_any<float>(p + i * s.nb0);
-        }
-        return;
+    for (int i = 0; i < 2; ++i) {
+        const double e = __builtin_fma(-m * y, y, 1.0);
+        y = __builtin_fma(0.5 * y, e, y);
     }
-    uint32_t u[4];
-    if (s.nb0 == 2) {
-        const kvm_u32x2 v = ld_any<kvm_u32x2>(p);
-        u[0] = v[0] & 0xffffu;
-        u[1] = v[0] >> 16;
-        u[2] = v[1] & 0xffffu;
-        u[3] = v[1] >> 16;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = ld_any<uint16_t>(p + i * s.nb0);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = s.type == KVM_TYPE_BF16 ? kvm_bf2f((uint16_t)u[i]) : kvm_h2f((uint16_t)u[i]);
+    return m > 0.0 && m < (double)INFINITY ? y : 1.0 / sqrt(m);
 }
 
 template <int LPR, int NI>
@@ -109,31 +123,72 @@ struct head_rows {
     uint32_t t[NI], h[NI];       // token of the block, head
     bool live[NI];
 
-    // The rows of tokens [t0, t0 + nt) and heads [h0, h0 + nh), nt nh <= ROWS.
-    __device__ __forceinline__ void load(const head_args &a, const head_src &s, uint32_t t0, uint32_t nt, uint32_t h0, uint32_t nh) {
-        const uint32_t l = threadIdx.x & 63u, w = threadIdx.x >> 6, d0 = 4 * (l % LPR);
+    // The rows of tokens [t0, t0 + nt) and heads [h0, h0 + nh), nt nh <= ROWS; heads from
+    // `split` on are the second tensor's.
+    __device__ __forceinline__ void load(const head_args &a, const head_src &s, const head_src &s2, uint32_t split, uint32_t t0,
+                                         uint32_t nt, uint32_t h0, uint32_t nh) {
+        const uint32_t l = threadIdx.x & 63u, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d0 = 4 * (l % LPR);
+        const uint8_t *p[NI];            // the rows (one a wave: in scalar registers)
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const uint32_t r = (i * 4 + w) * RPW + l / LPR;
+            // (a row past the last is the unit's first, its dims past D are dim 0: loaded, not used)
+            const uint32_t r = (i * 4 + w) * RPW + (RPW > 1 ? l / LPR : 0u);
             live[i] = r < nt * nh;
             t[i] = live[i] ? r / nh : 0u;
             h[i] = h0 + (live[i] ? r - t[i] * nh : 0u);
+            const size_t tok = t0 + t[i];
+            p[i] = h[i] < split ? s.data + tok * s.nb2 + (size_t)h[i] * s.nb1 : s2.data + tok * s2.nb2 + (size_t)(h[i] - split) * s2.nb1;
+        }
+        // Rows of packed dims are loaded first and converted after: a conversion waits for
+        // its load, one row's after the other.
+        const uint32_t es = elem_size(s.type), d = d0 < a.D ? d0 : 0u;
+        const bool packed = s.nb0 == es && s2.nb0 == es && elem_size(s2.type) == es;
+        if (packed && es == 4) {
+            kvm_f32x4 v[NI];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[i][j] = 0.0f;
-            if (live[i] && d0 < a.D) load4(s, s.data + (size_t)(t0 + t[i]) * s.nb2 + (size_t)h[i] * s.nb1 + d0 * s.nb0, x[i]);
+            for (int i = 0; i < NI; ++i) v[i] = ld_any<kvm_f32x4>(p[i] + 4 * d);
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[i][j] = v[i][j];
+        } else if (packed) {
+            kvm_u32x2 v[NI];
+#pragma unroll
+            for (int i = 0; i < NI; ++i) v[i] = ld_any<kvm_u32x2>(p[i] + 2 * d);
+            if (s.type == KVM_TYPE_BF16 && s2.type == KVM_TYPE_BF16) {
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[i][j] = __uint_as_float(j & 1 ? v[i][j >> 1] & 0xffff0000u : v[i][j >> 1] << 16);
+            } else {
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[i][j] = from16(h[i] < split ? s.type : s2.type, j & 1 ? v[i][j >> 1] >> 16 : v[i][j >> 1] & 0xffffu);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const head_src &q = h[i] < split ? s : s2;
+                load4(q, p[i] + d * q.nb0, x[i]);
+            }
+        }
+        if (d0 >= a.D) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[i][j] = 0.0f;
         }
     }
 
-    // norm, rotation, transform; cs: (cos, sin) of [token of the block][pair]
-    __device__ __forceinline__ void turn(const head_args &a, const head_src &s, const float2 *cs) {
+    // norm, rotation, transform; cs: (cos, sin) of [token of the block][pair], nt tokens
+    __device__ __forceinline__ void turn(const head_args &a, const float *weight, const float *weight2, uint32_t split,
+                                         const float2 *cs, uint32_t nt) {
         const uint32_t l = threadIdx.x & 63u, d0 = 4 * (l % LPR);
         if (a.norm) {
-            float w[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-            if (s.weight && d0 < a.D) {
-                const kvm_f32x4 v = ld_any<kvm_f32x4>(s.weight + d0);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = v[j];
-            }
+            const kvm_f32x4 ones = {1.0f, 1.0f, 1.0f, 1.0f};
+            const kvm_f32x4 w = weight && d0 < a.D ? ld_any<kvm_f32x4>(weight + d0) : ones;
+            const kvm_f32x4 w2 = weight2 && d0 < a.D ? ld_any<kvm_f32x4>(weight2 + d0) : ones;
             double sum[NI];
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
@@ -141,33 +196,69 @@ struct head_rows {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) sum[i] = __builtin_fma((double)x[i][j], (double)x[i][j], sum[i]);
             }
+            // Over the lanes of a row.  With four rows, lane l keeps row l % 4 after two
+            // exchanges, so that one root serves all four.
+            static_assert(NI == 1 || NI == 4, "rows of a wave");
+            double v;
+            if constexpr (NI == 4) {
+                const bool o1 = l & 1u, o2 = l & 2u;
+                const double a0 = (o1 ? sum[1] : sum[0]) + dpp_f64<DPP_QUAD(1, 0, 3, 2)>(o1 ? sum[0] : sum[1]);
+                const double a1 = (o1 ? sum[3] : sum[2]) + dpp_f64<DPP_QUAD(1, 0, 3, 2)>(o1 ? sum[2] : sum[3]);
+                v = (o2 ? a1 : a0) + dpp_f64<DPP_QUAD(2, 3, 0, 1)>(o2 ? a0 : a1);
+            } else {
+                v = sum[0] + dpp_f64<DPP_QUAD(1, 0, 3, 2)>(sum[0]);
+                v += dpp_f64<DPP_QUAD(2, 3, 0, 1)>(v);
+            }
+            v += dpp_f64<0x124>(v);                      // row_ror:4
+            v += dpp_f64<0x128>(v);                      // row_ror:8
+            if constexpr (LPR >= 32) v = add_rows_f64<16>(v);
+            if constexpr (LPR >= 64) v = add_rows_f64<32>(v);
+            const float root = (float)recip_sqrt(__builtin_fma(v, a.inv_D, (double)a.eps));
+            auto scale = [&](auto row) {
+                constexpr int i = decltype(row)::value;
+                const float r = NI == 1 ? root : __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(root), DPP_QUAD(i, i, i, i), 0xf, 0xf, true));
 #pragma unroll
-            for (int o = 1; o < LPR; o <<= 1)
-#pragma unroll
-                for (int i = 0; i < NI; ++i) sum[i] += __shfl_xor(sum[i], o, 64);
-#pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                const float r = (float)(1.0 / sqrt(sum[i] / (double)a.D + (double)a.eps));
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[i][j] = kvm_fmul(kvm_fmul(x[i][j], r), w[j]);
+                for (int j = 0; j < 4; ++j) x[i][j] = kvm_fmul(kvm_fmul(x[i][j], r), h[i] < split ? w[j] : w2[j]);
+            };
+            scale(std::integral_constant<int, 0>{});
+            if constexpr (NI == 4) {
+                scale(std::integral_constant<int, 1>{});
+                scale(std::integral_constant<int, 2>{});
+                scale(std::integral_constant<int, 3>{});
             }
         }
-        if (a.n_half) {
-            // the partner's lane: n_half is a multiple of 4
-            const bool lo = d0 < a.n_half, act = d0 < 2 * a.n_half;
-            const uint32_t pl = a.n_half / 4, p = lo ? l + pl : l - pl, ci = lo ? d0 : act ? d0 - a.n_half : 0u;
+        if (d0 < 2 * a.n_half) {
+            // the partner's lane, one that turns too: n_half is a multiple of 4
+            const bool lo = d0 < a.n_half;
+            const uint32_t pl = a.n_half / 4, p = (lo ? l + pl : l - pl) << 2, ci = lo ? d0 : d0 - a.n_half;
             const uint32_t sm = lo ? 0x80000000u : 0u;
+            float y[NI][4];
 #pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                float y[4];
+            for (int i = 0; i < NI; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    y[j] = __int_as_float(__builtin_amdgcn_ds_bpermute((int)((p & 63u) << 2), __float_as_int(x[i][j])));
+                for (int j = 0; j < 4; ++j) y[i][j] = __int_as_float(__builtin_amdgcn_ds_bpermute((int)p, __float_as_int(x[i][j])));
+            float c[4], sn[4];
+            auto angles = [&](uint32_t token) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float2 c = cs[t[i] * a.n_half + ci + j];
-                    const float v = kvm_fadd(kvm_fmul(x[i][j], c.x), kvm_fmul(y[j], __uint_as_float(__float_as_uint(c.y) ^ sm)));
-                    x[i][j] = act ? v : x[i][j];
+                    const float2 v = cs[token * a.n_half + ci + j];
+                    c[j] = v.x;
+                    sn[j] = __uint_as_float(__float_as_uint(v.y) ^ sm);
+                }
+            };
+            auto rotate = [&](int i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[i][j] = kvm_fadd(kvm_fmul(x[i][j], c[j]), kvm_fmul(y[i][j], sn[j]));
+            };
+            if (nt == 1) {                       // one token's rows turn alike
+                angles(0);
+#pragma unroll
+                for (int i = 0; i < NI; ++i) rotate(i);
+            } else {
+#pragma unroll
+                for (int i = 0; i < NI; ++i) {
+                    angles(t[i]);
+                    rotate(i);
                 }
             }
         }
@@ -198,32 +289,30 @@ struct head_rows {
         }
     }
 
-    // rows out [token][n_head][D] of `type`
-    __device__ __forceinline__ void store(const head_args &a, uint8_t *out, int type, uint32_t t0, uint32_t n_head) const {
+    // rows out [token][head][D] of `type`, the two tensors' heads (split and the rest of n_head) apart
+    __device__ __forceinline__ void store(const head_args &a, uint8_t *out, uint8_t *out2, uint32_t split, uint32_t n_head, int type,
+                                          uint32_t t0) const {
         const uint32_t d0 = 4 * ((threadIdx.x & 63u) % LPR);
+        if (d0 >= a.D) return;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            if (!live[i] || d0 >= a.D) continue;
-            const size_t at = ((size_t)(t0 + t[i]) * n_head + h[i]) * a.D + d0;
+            if (!live[i]) continue;
+            const bool first = h[i] < split;
+            const size_t row = (size_t)(t0 + t[i]) * (first ? split : n_head - split) + (first ? h[i] : h[i] - split);
+            uint8_t *o = (first ? out : out2) + row * a.D * elem_size(type);
+            const kvm_f32x4 v = {x[i][0], x[i][1], x[i][2], x[i][3]};
             if (type == KVM_TYPE_F32) {
-                const kvm_f32x4 v = {x[i][0], x[i][1], x[i][2], x[i][3]};
-                __builtin_memcpy(out + 4 * at, &v, 16);
-                continue;
-            }
-            uint32_t u[4];
+                __builtin_memcpy(o + 4 * d0, &v, 16);
+            } else if (type == KVM_TYPE_BF16) {
+                const kvm_bf16x4 u = __builtin_convertvector(v, kvm_bf16x4);
+                __builtin_memcpy(o + 2 * d0, &u, 8);
+            } else {
+                uint32_t u[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (type == KVM_TYPE_F16) {
-                    u[j] = kvm_f2h(x[i][j]);
-                } else {
-                    __bf16 b = (__bf16)x[i][j];
-                    uint16_t v;
-                    __builtin_memcpy(&v, &b, 2);
-                    u[j] = v;
-                }
+                for (int j = 0; j < 4; ++j) u[j] = kvm_f2h(v[j]);
+                const kvm_u32x2 y = {u[0] | u[1] << 16, u[2] | u[3] << 16};
+                __builtin_memcpy(o + 2 * d0, &y, 8);
             }
-            const kvm_u32x2 v = {u[0] | u[1] << 16, u[2] | u[3] << 16};
-            __builtin_memcpy(out + 2 * at, &v, 8);
         }
     }
 };
@@ -238,38 +327,36 @@ __device__ __forceinline__ void fill_cs(const head_args &a, const int32_t *pos, 
     __syncthreads();
 }
 
-// The rows of a tensor, in units of tt tokens x hb heads.
-struct row_units {
-    uint32_t n_tokens, n_head, tt, hb, units;
+// The rows of a launch's queries (and keys), in units of tt tokens x hb heads.
+struct rope_args {
+    head_src q, k;
+    const int32_t *pos;
+    uint8_t *q_out, *k_out;
+    int type;
+    uint32_t n_tokens, n_head, split;    // heads of both, of the queries
+    uint32_t tt, hb, units;
 };
 
 template <int LPR, int NI>
-__device__ __forceinline__ void norm_rope_unit(const head_args &a, const head_src &s, const row_units &u, const int32_t *pos,
-                                               uint32_t unit, uint8_t *out, int type, float2 *cs) {
+__device__ __forceinline__ void norm_rope_unit(const head_args &a, const rope_args &u, uint32_t unit, float2 *cs) {
     const uint32_t nhb = (u.n_head + u.hb - 1) / u.hb, t0 = unit / nhb * u.tt, h0 = unit % nhb * u.hb;
     const uint32_t nt = min(u.tt, u.n_tokens - t0), nh = min(u.hb, u.n_head - h0);
     head_rows<LPR, NI> r;
-    r.load(a, s, t0, nt, h0, nh);
-    fill_cs(a, pos, t0, nt, cs);
-    r.turn(a, s, cs);
-    r.store(a, out, type, t0, u.n_head);
+    r.load(a, u.q, u.k, u.split, t0, nt, h0, nh);
+    fill_cs(a, u.pos, t0, nt, cs);
+    r.turn(a, u.q.weight, u.k.weight, u.split, cs, nt);
+    r.store(a, u.q_out, u.k_out, u.split, u.n_head, u.type, t0);
 }
 
 struct norm_rope_args {
     head_args a;
-    head_src q, k;
-    row_units uq, uk;
-    const int32_t *pos;
-    uint8_t *q_out, *k_out;
-    int type;
+    rope_args u;
 };
 
 template <int LPR, int NI>
 __global__ void __launch_bounds__(256) k_norm_rope(norm_rope_args g) {
     __shared__ float2 s_cs[512 * NI];    // ROWS tokens of 2 LPR pairs at most
-    const uint32_t b = blockIdx.x;
-    if (b < g.uq.units) norm_rope_unit<LPR, NI>(g.a, g.q, g.uq, g.pos, b, g.q_out, g.type, s_cs);
-    else norm_rope_unit<LPR, NI>(g.a, g.k, g.uk, g.pos, b - g.uq.units, g.k_out, g.type, s_cs);
+    norm_rope_unit<LPR, NI>(g.a, g.u, blockIdx.x, s_cs);
 }
 
 // ---- device: keys and values into a window ---------------------------------------
@@ -282,18 +369,16 @@ struct run_args {
     uint32_t *shadow_rows, *pending;     // null, or the slots' counts
     uint32_t n_tiles, bt;
     uint32_t cell0, n, tok0;
-    uint32_t u0;                 // first unit
 };
 
 struct append_args {
     head_args a;
-    head_src q, k, v;
-    row_units uq;
+    rope_args u;                 // the queries
+    head_src k, v;
     const int32_t *pos;
-    uint8_t *q_out;
-    int q_type;
     uint32_t H, n_runs;
     uint32_t tk, hk, ghb;        // tokens and heads of a key unit, (8-cell group, head) pairs of a value unit
+    uint32_t u0[KVM_APPEND_RUNS];        // first units, ascending
     run_args run[KVM_APPEND_RUNS];
 };
 static_assert(sizeof(append_args) <= 4096, "kernel arguments");
@@ -304,6 +389,7 @@ template <int D, bool QUANT>
 __device__ __forceinline__ void append_v(const append_args &g, const run_args &r, uint32_t h, uint32_t grp, uint32_t d) {
     const uint32_t c0 = 8 * grp;         // the group's first cell
     const uint8_t *base = g.v.data + (size_t)h * g.v.nb1 + (size_t)d * g.v.nb0;
+    const uint8_t *p[8];
     float x[8];
     uint32_t valid = 0;
 #pragma unroll
@@ -311,10 +397,17 @@ __device__ __forceinline__ void append_v(const append_args &g, const run_args &r
         const uint32_t i = c0 + j - r.cell0;                     // token of the run (wraps below cell0)
         const bool in = c0 + j >= r.cell0 && i < r.n;
         valid |= (uint32_t)in << j;
-        const uint8_t *p = base + (size_t)(r.tok0 + (in ? i : c0 + j < r.cell0 ? 0u : r.n - 1)) * g.v.nb2;
-        x[j] = g.v.type == KVM_TYPE_F32    ? ld_any<float>(p)
-               : g.v.type == KVM_TYPE_BF16 ? kvm_bf2f(ld_any<uint16_t>(p))
-                                           : kvm_h2f(ld_any<uint16_t>(p));
+        p[j] = base + (size_t)(r.tok0 + (in ? i : c0 + j < r.cell0 ? 0u : r.n - 1)) * g.v.nb2;
+    }
+    if (g.v.type == KVM_TYPE_F32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = ld_any<float>(p[j]);
+    } else {
+        uint16_t u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = ld_any<uint16_t>(p[j]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = from16(g.v.type, u[j]);
     }
     uint8_t *vt = r.v + ((size_t)h * r.n_tiles + c0 / 64) * kvm_vtile_bytes(QUANT ? KVM_TYPE_Q4_0 : KVM_TYPE_F16, D);
     const uint32_t c = c0 % 64;
@@ -417,21 +510,23 @@ __global__ void __launch_bounds__(256) k_append(append_args g) {
     __shared__ float2 s_cs[512 * NI];
     constexpr bool QUANT = KT != KVM_TYPE_F16;
     uint32_t b = blockIdx.x;
-    if (b < g.uq.units) return norm_rope_unit<D / 4, NI>(g.a, g.q, g.uq, g.pos, b, g.q_out, g.q_type, s_cs);
-    b -= g.uq.units;
-    // the unit's run (their first units ascend)
-    uint32_t ri = 0;
-    while (ri + 1 < g.n_runs && b >= g.run[ri + 1].u0) ++ri;
+    if (b < g.u.units) return norm_rope_unit<D / 4, NI>(g.a, g.u, b, s_cs);
+    b -= g.u.units;
+    // The unit's run: the last of those that begin at or before it.  (Every wave looks at
+    // all of them at once; one after the other they are a chain of loads.)
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint64_t begun = __builtin_amdgcn_ballot_w64(lane < g.n_runs && g.u0[lane < g.n_runs ? lane : 0u] <= b);
+    const uint32_t ri = __builtin_amdgcn_readfirstlane(__popcll(begun) - 1);
     const run_args &r = g.run[ri];
-    b -= r.u0;
+    b -= g.u0[ri];
     // the run's units: keys, values, then the positions and the slots' counts
     const uint32_t nhb = (g.H + g.hk - 1) / g.hk, nk = (r.n + g.tk - 1) / g.tk * nhb;
     if (b < nk) {
         const uint32_t i0 = b / nhb * g.tk, nt = min(g.tk, r.n - i0), h0 = b % nhb * g.hk;
         head_rows<D / 4, NI> rows;
-        rows.load(g.a, g.k, r.tok0 + i0, nt, h0, min(g.hk, g.H - h0));
+        rows.load(g.a, g.k, g.k, g.H, r.tok0 + i0, nt, h0, min(g.hk, g.H - h0));
         fill_cs(g.a, g.pos, r.tok0 + i0, nt, s_cs);
-        rows.turn(g.a, g.k, s_cs);
+        rows.turn(g.a, g.k.weight, nullptr, g.H, s_cs, nt);
         append_k<D, KT, NI>(rows, r, r.cell0 + i0);
         return;
     }
@@ -459,6 +554,7 @@ __global__ void __launch_bounds__(256) k_append(append_args g) {
 static int head_args_of(kvm_state *st, const char *what, uint32_t D, float eps, const kvm_rope_params *rope, int nrot, head_args *a) {
     if (std::isnan(eps)) return kvm_fail(st, KVM_EINVAL, "%s: eps is not a number", what);
     a->D = D;
+    a->inv_D = 1.0 / (double)D;
     a->norm = eps >= 0.0f;
     a->eps = eps;
     if (!rope) return KVM_OK;
@@ -509,15 +605,11 @@ static bool in_place(const void *out, int type, const head_src &s, uint32_t D, u
 
 static bool float_type(int t) { return t == KVM_TYPE_F32 || t == KVM_TYPE_F16 || t == KVM_TYPE_BF16; }
 
-static row_units units_of(uint32_t n_tokens, uint32_t n_head, uint32_t rows) {
-    row_units u{};
-    if (!n_tokens) return u;
-    u.n_tokens = n_tokens;
-    u.n_head = n_head;
-    u.hb = n_head < rows ? n_head : rows;
-    u.tt = rows / u.hb;
-    u.units = kvm_cdiv(n_tokens, u.tt) * kvm_cdiv(n_head, u.hb);
-    return u;
+// Units of at most `rows` rows: the heads in equal parts, and as many tokens as fit.
+static void units_of(uint32_t n_tokens, uint32_t n_head, uint32_t rows, uint32_t *tt, uint32_t *hb, uint32_t *units) {
+    *hb = kvm_cdiv(n_head, kvm_cdiv(n_head, rows));
+    *tt = rows / *hb;
+    *units = kvm_cdiv(n_tokens, *tt) * kvm_cdiv(n_head, *hb);
 }
 
 template <typename F>
@@ -546,11 +638,11 @@ extern "C" int kvm_qk_norm_rope(kvm_state *st, const kvm_view *q, const kvm_view
     uint32_t Hq = 0, Hk = 0;
     if (q) {
         Hq = (uint32_t)q->ne1;
-        if ((rc = head_src_of(st, what, q, D, Hq, q_weight, &g.q))) return rc;
+        if ((rc = head_src_of(st, what, q, D, Hq, q_weight, &g.u.q))) return rc;
     }
     if (k) {
         Hk = (uint32_t)k->ne1;
-        if ((rc = head_src_of(st, what, k, D, Hk, k_weight, &g.k))) return rc;
+        if ((rc = head_src_of(st, what, k, D, Hk, k_weight, &g.u.k))) return rc;
     }
     const uint32_t n = (uint32_t)one->ne2;
     const uint64_t n_rows = (uint64_t)n * (Hq + Hk);
@@ -558,24 +650,27 @@ extern "C" int kvm_qk_norm_rope(kvm_state *st, const kvm_view *q, const kvm_view
     if (n_rows > (1u << 30)) return kvm_fail(st, KVM_ERANGE, "%s: %u tokens", what, n);
     if ((q && !q_out) || (k && !k_out) || (g.a.n_half && !pos)) return kvm_fail(st, KVM_EINVAL, "%s: null argument", what);
     const size_t bq = (size_t)n * Hq * D * es, bk = (size_t)n * Hk * D * es;
-    if ((q && ((overlaps(q_out, bq, q) && !in_place(q_out, out_type, g.q, D, Hq)) || overlaps(q_out, bq, k))) ||
-        (k && ((overlaps(k_out, bk, k) && !in_place(k_out, out_type, g.k, D, Hk)) || overlaps(k_out, bk, q))) ||
+    if ((q && ((overlaps(q_out, bq, q) && !in_place(q_out, out_type, g.u.q, D, Hq)) || overlaps(q_out, bq, k))) ||
+        (k && ((overlaps(k_out, bk, k) && !in_place(k_out, out_type, g.u.k, D, Hk)) || overlaps(k_out, bk, q))) ||
         (q && k && (uint8_t *)q_out < (uint8_t *)k_out + bk && (uint8_t *)k_out < (uint8_t *)q_out + bq && bq))
         return kvm_fail(st, KVM_EINVAL, "%s: an output overlaps an input or the other output", what);
     if (!st) return KVM_EINVAL;
-    g.pos = pos;
-    g.q_out = (uint8_t *)q_out;
-    g.k_out = (uint8_t *)k_out;
-    g.type = out_type;
+    if (!q) g.u.q = g.u.k;       // (no head is read from it)
+    if (!k) g.u.k = g.u.q;
+    g.u.pos = pos;
+    g.u.q_out = (uint8_t *)q_out;
+    g.u.k_out = (uint8_t *)k_out;
+    g.u.type = out_type;
+    g.u.n_tokens = n;
+    g.u.n_head = Hq + Hk;
+    g.u.split = Hq;
     KVM_HIP(st, hipSetDevice(st->device));
     auto go = [&](auto lpr) {
         constexpr int LPR = decltype(lpr)::value;
         by_ni(n_rows, 4 * (64 / LPR), st->n_cu, [&](auto ni) {
             constexpr int NI = decltype(ni)::value;
-            constexpr uint32_t ROWS = head_rows<LPR, NI>::ROWS;
-            g.uq = units_of(q ? n : 0, Hq, ROWS);
-            g.uk = units_of(k ? n : 0, Hk, ROWS);
-            hipLaunchKernelGGL((k_norm_rope<LPR, NI>), dim3(g.uq.units + g.uk.units), dim3(256), 0, st->stream, g);
+            units_of(n, Hq + Hk, head_rows<LPR, NI>::ROWS, &g.u.tt, &g.u.hb, &g.u.units);
+            hipLaunchKernelGGL((k_norm_rope<LPR, NI>), dim3(g.u.units), dim3(256), 0, st->stream, g);
         });
     };
     if (D > 128) go(std::integral_constant<int, 64>{});
@@ -614,7 +709,7 @@ extern "C" int kvm_window_append(kvm_state *st, const kvm_window *const *windows
         if (q->ne0 <= 0 || q->ne1 <= 0 || (uint64_t)q->ne0 * (uint64_t)q->ne1 % D || (uint64_t)q->ne0 * (uint64_t)q->ne1 > (1u << 28))
             return kvm_fail(st, KVM_EINVAL, "%s: queries of %lld x %lld values, heads of %u", what, (long long)q->ne0, (long long)q->ne1, D);
         Hq = (uint32_t)((uint64_t)q->ne0 * (uint64_t)q->ne1 / D);
-        if ((rc = head_src_of(st, what, q, D, Hq, q_weight, &g.q))) return rc;
+        if ((rc = head_src_of(st, what, q, D, Hq, q_weight, &g.u.q))) return rc;
     }
     if ((uint64_t)k->ne2 != total || (uint64_t)v->ne2 != total || (q && (uint64_t)q->ne2 != total))
         return kvm_fail(st, KVM_EINVAL, "%s: runs of %llu tokens, keys of %lld, values of %lld", what, (unsigned long long)total, (long long)k->ne2, (long long)v->ne2);
@@ -623,13 +718,16 @@ extern "C" int kvm_window_append(kvm_state *st, const kvm_window *const *windows
     if (!pos || (q && !q_out)) return kvm_fail(st, KVM_EINVAL, "%s: null argument", what);
     if (q) {
         const size_t bytes = total * Hq * D * (q_out_type == KVM_TYPE_F32 ? 4 : 2);
-        if ((overlaps(q_out, bytes, q) && !in_place(q_out, q_out_type, g.q, D, Hq)) || overlaps(q_out, bytes, k) || overlaps(q_out, bytes, v))
+        if ((overlaps(q_out, bytes, q) && !in_place(q_out, q_out_type, g.u.q, D, Hq)) || overlaps(q_out, bytes, k) || overlaps(q_out, bytes, v))
             return kvm_fail(st, KVM_EINVAL, "%s: the query output overlaps an input", what);
     }
     if (!st) return KVM_EINVAL;
-    g.pos = pos;
-    g.q_out = (uint8_t *)q_out;
-    g.q_type = q_out_type;
+    g.pos = g.u.pos = pos;
+    g.u.q_out = (uint8_t *)q_out;
+    g.u.type = q_out_type;
+    g.u.n_tokens = (uint32_t)total;
+    g.u.n_head = g.u.split = Hq;
+    g.u.k = g.u.q;
     g.H = H;
     KVM_HIP(st, hipSetDevice(st->device));
 
@@ -646,9 +744,9 @@ extern "C" int kvm_window_append(kvm_state *st, const kvm_window *const *windows
         constexpr int NI = decltype(ni)::value;
         const uint32_t rows = 4 * (256 / D) * NI;
         g.ghb = NI * (256 / D);
-        g.uq = units_of(q ? (uint32_t)total : 0u, Hq, rows);
-        g.hk = H < rows ? H : rows;
-        g.tk = rows / g.hk;
+        if (q) units_of((uint32_t)total, Hq, rows, &g.u.tt, &g.u.hb, &g.u.units);
+        uint32_t unused;
+        units_of((uint32_t)total, H, rows, &g.tk, &g.hk, &unused);
         for (uint32_t i = 0; i < n_runs;) {
             uint32_t first = i, units = 0;
             g.n_runs = 0;
@@ -658,16 +756,16 @@ extern "C" int kvm_window_append(kvm_state *st, const kvm_window *const *windows
                 for (uint32_t j = first; j < i && !clash; ++j) clash = n_tokens[j] && shares(i, j);
                 if (clash) break;
                 const kvm_window *w = windows[i];
-                run_args &r = g.run[g.n_runs++];
-                r = run_args{(uint8_t *)w->k, (uint8_t *)w->v, w->cell_pos, w->shadow_rows, w->pending_rows,
-                             w->n_cells / KVM_TILE_CELLS, w->block_tokens, cell0[i], n_tokens[i], tok, units};
+                g.u0[g.n_runs] = units;
+                g.run[g.n_runs++] = run_args{(uint8_t *)w->k, (uint8_t *)w->v, w->cell_pos, w->shadow_rows, w->pending_rows,
+                             w->n_cells / KVM_TILE_CELLS, w->block_tokens, cell0[i], n_tokens[i], tok};
                 const uint32_t pairs = ((cell0[i] + n_tokens[i] - 1) / 8 - cell0[i] / 8 + 1) * H;
                 units += kvm_cdiv(n_tokens[i], g.tk) * kvm_cdiv(H, g.hk) + kvm_cdiv(pairs, g.ghb) + 1;
                 tok += n_tokens[i];
             }
             if (!g.n_runs) break;
             auto go = [&](auto d, auto kt) {
-                hipLaunchKernelGGL((k_append<decltype(d)::value, decltype(kt)::value, NI>), dim3(g.uq.units + units), dim3(256), 0, st->stream, g);
+                hipLaunchKernelGGL((k_append<decltype(d)::value, decltype(kt)::value, NI>), dim3(g.u.units + units), dim3(256), 0, st->stream, g);
             };
             auto go_d = [&](auto d) {
                 if (w0->k_type == KVM_TYPE_Q8_0) go(d, std::integral_constant<int, KVM_TYPE_Q8_0>{});
@@ -676,7 +774,7 @@ extern "C" int kvm_window_append(kvm_state *st, const kvm_window *const *windows
             };
             if (D == 256) go_d(std::integral_constant<int, 256>{});
             else go_d(std::integral_constant<int, 128>{});
-            g.uq.units = 0;
+            g.u.units = 0;
         }
     });
     KVM_LAUNCH_CHECK(st, what);
