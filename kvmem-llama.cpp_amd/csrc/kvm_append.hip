@@ -86,6 +86,7 @@ __device__ __forceinline__ void load4(const head_src &s, const uint8_t *p, float
     for (int i = 0; i < 4; ++i) x[i] = s.type == KVM_TYPE_F32 ? ld_any<float>(p + i * s.nb0) : from16(s.type, ld_any<uint16_t>(p + i * s.nb0));
 }
 
+#define DPP_QUAD(a, b, c, d) ((a) | (b) << 2 | (c) << 4 | (d) << 6)
 // A 64-bit value of another lane, as a DPP move of its halves.
 template <int CTRL>
 __device__ __forceinline__ double dpp_f64(double x) {
@@ -94,7 +95,24 @@ __device__ __forceinline__ double dpp_f64(double x) {
     const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-#define DPP_QUAD(a, b, c, d) ((a) | (b) << 2 | (c) << 4 | (d) << 6)
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+// x of lane l ^ O (O = 16 and 32: the swap leaves the lower rows' own value and the upper
+// rows' partner in one result, the others in the other)
+template <int O>
+__device__ __forceinline__ float xor_f32(float x) {
+    if constexpr (O == 1) return dpp_f32<DPP_QUAD(1, 0, 3, 2)>(x);
+    else if constexpr (O == 2) return dpp_f32<DPP_QUAD(2, 3, 0, 1)>(x);
+    else if constexpr (O == 4) return dpp_f32<DPP_QUAD(3, 2, 1, 0)>(dpp_f32<0x141>(x));      // row_half_mirror: l ^ 7
+    else if constexpr (O == 8) return dpp_f32<0x128>(x);                                       // row_ror:8
+    else {
+        const uint32_t u = __float_as_uint(x);
+        const auto r = O == 16 ? __builtin_amdgcn_permlane16_swap(u, u, false, false) : __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        return __uint_as_float(threadIdx.x & O ? r[0] : r[1]);
+    }
+}
 // x of the even and of the odd row of 16 lanes (or half of 32) of a pair, added: the same in both.
 template <int N>
 __device__ __forceinline__ double add_rows_f64(double x) {
@@ -279,13 +297,22 @@ struct head_rows {
                     x[i][j + 2] = kvm_fsub(u, v);
                 }
             }
-            for (int o = 1; 4 * o < a.nrot; o <<= 1) {
-                const float sg = l & o ? -1.0f : 1.0f;           // the lane above takes other - own
+            auto stage = [&](auto lanes) {
+                constexpr int O = decltype(lanes)::value;
+                const float sg = l & O ? -1.0f : 1.0f;           // the lane above takes other - own
 #pragma unroll
                 for (int i = 0; i < NI; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x[i][j] = __builtin_fmaf(x[i][j], sg, __shfl_xor(x[i][j], o, 64));
-            }
+                    for (int j = 0; j < 4; ++j) x[i][j] = __builtin_fmaf(x[i][j], sg, xor_f32<O>(x[i][j]));
+            };
+            stage(std::integral_constant<int, 1>{});             // (chunks of 64 dims at least)
+            stage(std::integral_constant<int, 2>{});
+            stage(std::integral_constant<int, 4>{});
+            stage(std::integral_constant<int, 8>{});
+            if constexpr (LPR >= 32)
+                if (a.nrot > 64) stage(std::integral_constant<int, 16>{});
+            if constexpr (LPR >= 64)
+                if (a.nrot > 128) stage(std::integral_constant<int, 32>{});
         }
     }
 
@@ -377,7 +404,7 @@ struct append_args {
     head_src k, v;
     const int32_t *pos;
     uint32_t H, n_runs;
-    uint32_t tk, hk, ghb;        // tokens and heads of a key unit, (8-cell group, head) pairs of a value unit
+    uint32_t tk, hk;             // tokens and heads of a key unit
     uint32_t u0[KVM_APPEND_RUNS];        // first units, ascending
     run_args run[KVM_APPEND_RUNS];
 };
@@ -399,6 +426,11 @@ __device__ __forceinline__ void append_v(const append_args &g, const run_args &r
         valid |= (uint32_t)in << j;
         p[j] = base + (size_t)(r.tok0 + (in ? i : c0 + j < r.cell0 ? 0u : r.n - 1)) * g.v.nb2;
     }
+    uint8_t *vt = r.v + ((size_t)h * r.n_tiles + c0 / 64) * kvm_vtile_bytes(QUANT ? KVM_TYPE_Q4_0 : KVM_TYPE_F16, D);
+    const uint32_t c = c0 % 64;
+    uint32_t *const word_at = (uint32_t *)(vt + kvm_vq_word(d, (c & 31u) >> 3, c >> 5));
+    uint32_t old = 0;
+    if (QUANT && valid != 0xffu) old = *word_at;                 // the other cells' nibbles stay
     if (g.v.type == KVM_TYPE_F32) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = ld_any<float>(p[j]);
@@ -409,8 +441,6 @@ __device__ __forceinline__ void append_v(const append_args &g, const run_args &r
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = from16(g.v.type, u[j]);
     }
-    uint8_t *vt = r.v + ((size_t)h * r.n_tiles + c0 / 64) * kvm_vtile_bytes(QUANT ? KVM_TYPE_Q4_0 : KVM_TYPE_F16, D);
-    const uint32_t c = c0 % 64;
     if constexpr (!QUANT) {
         uint16_t *dst = (uint16_t *)vt + kvm_vh_idx(c, d);
         uint32_t y[8];
@@ -429,17 +459,17 @@ __device__ __forceinline__ void append_v(const append_args &g, const run_args &r
         uint16_t *sc = (uint16_t *)(vt + kvm_vd_off(D, c, d / 32));
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            // the block's largest magnitude, the first in dim order, with its sign
-            uint32_t top = __float_as_uint(fabsf(x[j]));
-            const float ax = __uint_as_float(top);
-            float m = ax;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-            const uint64_t eq = __builtin_amdgcn_ballot_w64(ax == m);
-            const uint32_t half = (uint32_t)(threadIdx.x & 32u ? eq >> 32 : eq);
-            const int first = half ? __builtin_ctz(half) : 0;
-            const float vmax = __shfl(x[j], (int)(threadIdx.x & 32u) + first, 64);
-            const float dsc = m > 0.0f ? kvm_fmul(vmax, -0.125f) : -0.0f;
+            // the block's largest magnitude, with the sign of the first in dim order
+            const float ax = fabsf(x[j]);
+            float m = fmaxf(ax, xor_f32<1>(ax));
+            m = fmaxf(m, xor_f32<2>(m));
+            m = fmaxf(m, dpp_f32<0x124>(m));                     // row_ror:4, :8: the row's four quads
+            m = fmaxf(m, xor_f32<8>(m));
+            m = kvm_max_xor16(m);
+            const uint64_t eq = __builtin_amdgcn_ballot_w64(ax == m), neg = __builtin_amdgcn_ballot_w64(x[j] < 0.0f);
+            const uint32_t eq32 = (uint32_t)(threadIdx.x & 32u ? eq >> 32 : eq), neg32 = (uint32_t)(threadIdx.x & 32u ? neg >> 32 : neg);
+            const bool minus = neg32 & eq32 & (0u - eq32);       // (the lowest set bit)
+            const float dsc = m > 0.0f ? kvm_fmul(minus ? -m : m, -0.125f) : -0.0f;
             int n = (int)kvm_fadd(kvm_fmul(x[j], kvm_recip_or0(dsc)), 8.5f);
             n = n > 15 ? 15 : n;
             if (valid >> j & 1u) {
@@ -448,9 +478,7 @@ __device__ __forceinline__ void append_v(const append_args &g, const run_args &r
                 if (l == 0) sc[j] = kvm_f2h(dsc);
             }
         }
-        uint32_t *dst = (uint32_t *)(vt + kvm_vq_word(d, (c & 31u) >> 3, c >> 5));
-        if (mask != 0xffffffffu) word |= *dst & ~mask;
-        *dst = word;
+        *word_at = word | (old & ~mask);
     }
 }
 
@@ -470,8 +498,9 @@ __device__ __forceinline__ void append_k(const head_rows<D / 4, NI> &r, const ru
         } else {
             // a block's 32 dims are 8 lanes'
             float m = fmaxf(fmaxf(fabsf(r.x[i][0]), fabsf(r.x[i][1])), fmaxf(fabsf(r.x[i][2]), fabsf(r.x[i][3])));
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+            m = fmaxf(m, xor_f32<1>(m));
+            m = fmaxf(m, xor_f32<2>(m));
+            m = fmaxf(m, dpp_f32<0x141>(m));                     // row_half_mirror: the other quad
             float d;
             if constexpr (KT == KVM_TYPE_Q8_0) {
                 d = kvm_div127(m);
@@ -514,9 +543,11 @@ __global__ void __launch_bounds__(256) k_append(append_args g) {
     b -= g.u.units;
     // The unit's run: the last of those that begin at or before it.  (Every wave looks at
     // all of them at once; one after the other they are a chain of loads.)
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint64_t begun = __builtin_amdgcn_ballot_w64(lane < g.n_runs && g.u0[lane < g.n_runs ? lane : 0u] <= b);
-    const uint32_t ri = __builtin_amdgcn_readfirstlane(__popcll(begun) - 1);
+    uint32_t ri = 0;
+    if (g.n_runs > 1) {
+        const uint32_t lane = threadIdx.x & 63u;
+        ri = __builtin_amdgcn_readfirstlane(__popcll(__builtin_amdgcn_ballot_w64(lane < g.n_runs && g.u0[lane < g.n_runs ? lane : 0u] <= b)) - 1);
+    }
     const run_args &r = g.run[ri];
     b -= g.u0[ri];
     // the run's units: keys, values, then the positions and the slots' counts
@@ -531,12 +562,11 @@ __global__ void __launch_bounds__(256) k_append(append_args g) {
         return;
     }
     b -= nk;
-    const uint32_t g0 = r.cell0 / 8, pairs = ((r.cell0 + r.n - 1) / 8 - g0 + 1) * g.H, nv = (pairs + g.ghb - 1) / g.ghb;
+    // (8-cell group, head) pairs, 256 / D of them a unit
+    const uint32_t g0 = r.cell0 / 8, pairs = ((r.cell0 + r.n - 1) / 8 - g0 + 1) * g.H, nv = (pairs + 256 / D - 1) / (256 / D);
     if (b < nv) {
-        for (uint32_t i = threadIdx.x / D; i < g.ghb; i += 256 / D) {
-            const uint32_t p = b * g.ghb + i;
-            if (p < pairs) append_v<D, QUANT>(g, r, p % g.H, g0 + p / g.H, threadIdx.x % D);
-        }
+        const uint32_t p = b * (256 / D) + __builtin_amdgcn_readfirstlane(threadIdx.x / D);
+        if (p < pairs) append_v<D, QUANT>(g, r, p % g.H, g0 + p / g.H, threadIdx.x % D);
         return;
     }
     for (uint32_t i = threadIdx.x; i < r.n; i += 256) r.cell_pos[r.cell0 + i] = g.pos[r.tok0 + i];
@@ -612,9 +642,14 @@ static void units_of(uint32_t n_tokens, uint32_t n_head, uint32_t rows, uint32_t
     *units = kvm_cdiv(n_tokens, *tt) * kvm_cdiv(n_head, *hb);
 }
 
+// Rows of a wave: one, or four with one root for all.  One hides more latency while the
+// chip is not full: us with one and four, keys and values of n tokens of 4 x 256 into a
+// quantised window, 512: 6.6 and 7.2, 1,024: 8.8 and 7.7, 2,048: 12.3 and 11.2; norms and
+// rotation of 28 x 256, 128: 3.8 and 4.8, 256: 6.2 and 5.7, 2,048: 24.6 and 16.9; of 10 x
+// 128, 1,024: 5.9 and 6.1, 2,048: 8.4 and 7.4.
 template <typename F>
 static void by_ni(uint64_t n_rows, uint32_t rows1, uint32_t n_cu, F &&f) {
-    if (n_rows <= 8ull * n_cu * rows1) f(std::integral_constant<int, 1>{});
+    if (n_rows < 4ull * n_cu * rows1) f(std::integral_constant<int, 1>{});
     else f(std::integral_constant<int, 4>{});
 }
 
@@ -743,7 +778,6 @@ extern "C" int kvm_window_append(kvm_state *st, const kvm_window *const *windows
     by_ni(total * (H + Hq), 4 * (64 / (D / 4)), st->n_cu, [&](auto ni) {
         constexpr int NI = decltype(ni)::value;
         const uint32_t rows = 4 * (256 / D) * NI;
-        g.ghb = NI * (256 / D);
         if (q) units_of((uint32_t)total, Hq, rows, &g.u.tt, &g.u.hb, &g.u.units);
         uint32_t unused;
         units_of((uint32_t)total, H, rows, &g.tk, &g.hk, &unused);
@@ -760,7 +794,7 @@ extern "C" int kvm_window_append(kvm_state *st, const kvm_window *const *windows
                 g.run[g.n_runs++] = run_args{(uint8_t *)w->k, (uint8_t *)w->v, w->cell_pos, w->shadow_rows, w->pending_rows,
                              w->n_cells / KVM_TILE_CELLS, w->block_tokens, cell0[i], n_tokens[i], tok};
                 const uint32_t pairs = ((cell0[i] + n_tokens[i] - 1) / 8 - cell0[i] / 8 + 1) * H;
-                units += kvm_cdiv(n_tokens[i], g.tk) * kvm_cdiv(H, g.hk) + kvm_cdiv(pairs, g.ghb) + 1;
+                units += kvm_cdiv(n_tokens[i], g.tk) * kvm_cdiv(H, g.hk) + kvm_cdiv(pairs, 256 / D) + 1;
                 tok += n_tokens[i];
             }
             if (!g.n_runs) break;

@@ -221,6 +221,9 @@ APPEND_CASES = [
     (256, 2, "f16", 64, 63, 1, 0, 0, None, torch.float16, "packed"),
     (128, 1, "q8_0", 8192, 7, 8101, 128, -1, 1e-6, torch.bfloat16, "joint"),
     (256, 4, "q8_0", 4096, 1003, 2047, 64, -1, 1e-6, torch.bfloat16, "joint"),
+    (128, 8, "f16", 4096, 5, 1025, 128, -1, 1e-6, torch.bfloat16, "joint"),
+    (256, 2, "f16", 4096, 1023, 2500, 64, -1, 1e-6, torch.float32, "packed"),
+    (256, 4, "q4_0", 2048, 62, 1300, 64, -1, 1e-6, torch.float16, "joint"),
     (128, 70, "q8_0", 64, 30, 3, 64, -1, 1e-6, torch.bfloat16, "packed"),
     (256, 5, "q4_0", 64, 0, 9, 256, 64, None, torch.float32, "packed"),
 ]
