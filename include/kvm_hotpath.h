@@ -598,6 +598,28 @@ typedef struct kvm_lane {
 int kvm_fa_decode_lanes(kvm_state *st, const kvm_lane *lanes, uint32_t n_lanes, int q_type,
                         uint32_t n_head, float scale);
 
+/* Decode / verify attention of several conversations that share a long prefix
+ * (a system prompt, a document): every token attends over the prefix window's
+ * cells and its own conversation's, one softmax over both, with kvm_fa_decode's
+ * visibility rule in each (positions in a lane's own window go on after the
+ * prefix).  The prefix's keys and values are read once for 32 query rows (a
+ * row is a token and a query head of a kv head's group), of whichever lanes,
+ * not once per lane.  The reference keeps every conversation's cells in that
+ * conversation's window (docs/multi-lane-conversations.md:1-20).
+ * n_tokens: host [n_lanes], tokens of each lane (0 allowed); q, q_pos and out
+ * hold the lanes' tokens after each other: q [tokens][n_head][head_dim] (F32 or
+ * BF16), out the same shape of out_type (F32, BF16 or F16).  windows: host
+ * [n_lanes], NULL entries = a lane without cells of its own (windows NULL: all);
+ * prefix NULL: none.  At most 64 lanes; any number of tokens a lane; all
+ * windows have the same kv heads and head_dim and are all quantised or all f16.
+ * Arithmetic as kvm_fa_prefill's: f16 operands (q, the cells' values, the
+ * probabilities), fp32 sums, one rounding to out_type.  A token that sees no
+ * cell outputs zeros; what cells hold that a token does not see does not reach
+ * its output, be it infinite or no number. */
+int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, const kvm_window *const *windows,
+                         const uint32_t *n_tokens, uint32_t n_lanes, const void *q, int q_type,
+                         const int32_t *q_pos, uint32_t n_head, float scale, int out_type, void *out);
+
 /* A decode step's stage-in and attention in one launch: kvm_stagein_selection
  * of (h, sel) into w, then kvm_fa_decode over w, with the results of those two
  * calls.  The attention's workgroups stage the plan themselves and meet at an

@@ -78,6 +78,12 @@ struct kvm_state {
     // outputs a decode step's attention must not overwrite
     void *fa_ws = nullptr;
     size_t fa_ws_bytes = 0;
+    // pieces of the shared-prefix attention; the buffers that it outgrew stay until the
+    // state is freed, since captured graphs may use them (each at least twice the last)
+    void *fs_ws = nullptr;
+    size_t fs_ws_bytes = 0;
+    void *fs_old[48] = {};
+    uint32_t n_fs_old = 0;
     // staging of the blocks a stage-in plan moves within the window (their
     // shadow K rows and V rows, gathered before any slot is written)
     void *mv_ws = nullptr;
@@ -121,6 +127,9 @@ size_t kvm_fa_sync_bytes();
 void *kvm_workspace(kvm_state *st, size_t bytes);
 // The same for the attention workspace (kvm_state::fa_ws).
 void *kvm_fa_workspace(kvm_state *st, size_t bytes);
+// The pieces of the shared-prefix attention (kvm_state::fs_ws): never freed before the
+// state, and not grown while the stream is captured (*buf; KVM_ENOMEM).
+int kvm_shared_workspace(kvm_state *st, const char *what, size_t bytes, void **buf);
 // The same for the stage-in move staging (kvm_state::mv_ws).
 void *kvm_move_workspace(kvm_state *st, size_t bytes);
 // Workgroups of `threads` threads and `lds` bytes of dynamic LDS of kernel fn

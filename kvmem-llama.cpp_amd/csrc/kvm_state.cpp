@@ -62,6 +62,8 @@ extern "C" void kvm_state_free(kvm_state *st) {
     if (st->fa_sync) (void)hipFree(st->fa_sync);
     if (st->fa_ws) (void)hipFree(st->fa_ws);
     if (st->mv_ws) (void)hipFree(st->mv_ws);
+    if (st->fs_ws) (void)hipFree(st->fs_ws);
+    for (uint32_t i = 0; i < st->n_fs_old; ++i) (void)hipFree(st->fs_old[i]);
     if (st->stage_sync) (void)hipFree(st->stage_sync);
     if (st->slab) (void)hipHostFree(st->slab);
     if (st->ev) (void)hipEventDestroy(st->ev);
@@ -154,6 +156,25 @@ void *kvm_workspace(kvm_state *st, size_t bytes) { return grow(st, &st->ws, &st-
 void *kvm_fa_workspace(kvm_state *st, size_t bytes) { return grow(st, &st->fa_ws, &st->fa_ws_bytes, bytes); }
 
 void *kvm_move_workspace(kvm_state *st, size_t bytes) { return grow(st, &st->mv_ws, &st->mv_ws_bytes, bytes); }
+
+int kvm_shared_workspace(kvm_state *st, const char *what, size_t bytes, void **buf) {
+    *buf = st->fs_ws;
+    if (bytes <= st->fs_ws_bytes) return KVM_OK;
+    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+    KVM_HIP(st, hipStreamIsCapturing(st->stream, &capturing));
+    if (capturing != hipStreamCaptureStatusNone)
+        return kvm_fail(st, KVM_ENOMEM, "%s: the workspace has to grow to %zu bytes: call it once before the capture", what, bytes);
+    const size_t twice = 2 * st->fs_ws_bytes, least = bytes < (4u << 20) ? (4u << 20) : bytes, want = twice > least ? twice : least;
+    void *p = nullptr;
+    if (st->n_fs_old == sizeof(st->fs_old) / sizeof(st->fs_old[0]) || hipMalloc(&p, want) != hipSuccess) {
+        (void)hipGetLastError();
+        return kvm_fail(st, KVM_ENOMEM, "%s: workspace of %zu bytes", what, want);
+    }
+    if (st->fs_ws) st->fs_old[st->n_fs_old++] = st->fs_ws;
+    st->fs_ws = *buf = p;
+    st->fs_ws_bytes = want;
+    return KVM_OK;
+}
 
 int kvm_resident_blocks(kvm_state *st, const void *fn, int threads, size_t lds, int *blocks) {
     struct entry {

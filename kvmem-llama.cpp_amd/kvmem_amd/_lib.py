@@ -177,6 +177,8 @@ SIGNATURES = {
     "kvm_fa_decode": (C.c_int, [_P, _PW, _P, C.c_int, _P, _u32, _u32, _f, _P]),
     "kvm_fa_decode_lanes": (C.c_int, [_P, C.POINTER(Lane), _u32, C.c_int, _u32, _f]),
     "kvm_fa_decode_noalloc": (C.c_int, [_P, _PW, _P, C.c_int, _P, _u32, _u32, _f, _P]),
+    "kvm_fa_decode_shared": (C.c_int, [_P, _PW, C.POINTER(_PW), C.POINTER(_u32), _u32, _P, C.c_int, _P, _u32, _f, C.c_int,
+                                       _P]),
     "kvm_stagein_fa_decode": (C.c_int, [_P, C.POINTER(History), C.POINTER(Selection), C.POINTER(RopeParams), _PW, _P,
                                         C.c_int, _P, _u32, _u32, _f, _P]),
     "kvm_stagein_fa_decode_lanes": (C.c_int, [_P, C.POINTER(StageinLane), C.POINTER(Lane), _u32,

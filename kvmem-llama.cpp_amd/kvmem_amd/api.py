@@ -815,6 +815,40 @@ def window_append(st, windows, cell0, n_tokens, k, v, pos, n_rot, freq_base, fre
     return p.q_out
 
 
+def prepare_fa_decode_shared(st, prefix, windows, n_tokens, q, q_pos, n_head, scale, out=None, out_dtype=None):
+    """kvm_fa_decode_shared: the lanes' tokens (n_tokens[i] of lane i, after each other in
+    q [tokens][n_head][dims] of fp32 or bf16 and q_pos) over the prefix window (or None)
+    and each lane's own (None: none).  The call's result is its out: given, or a new
+    tensor of out_dtype (fp32 if None)."""
+    if len(windows) != len(n_tokens) or any(int(n) < 0 for n in n_tokens):
+        raise L.KvmError(L.KVM_EINVAL, f"fa_decode_shared: {len(windows)} windows, counts {list(n_tokens)}")
+    total = sum(int(n) for n in n_tokens)
+    some = prefix or next((w for w in windows if w is not None), None)
+    if some is None:
+        raise L.KvmError(L.KVM_EINVAL, "fa_decode_shared: no window")
+    if q.dtype not in (torch.float32, torch.bfloat16):
+        raise L.KvmError(L.KVM_EINVAL, f"q: {q.dtype}")
+    _on_device(st, q.dtype, (total, n_head, some.head_dim), q=q)
+    _on_device(st, torch.int32, (total,), q_pos=q_pos)
+    out = _out_of(st, q, out, out_dtype if out is not None or out_dtype is not None else torch.float32, "out")
+    n = len(windows)
+    arr, nt = _window_ptrs(st, windows), (L._u32 * max(n, 1))(*map(int, n_tokens))
+    pre = _window_ptrs(st, [prefix])
+    p = Prepared(st, st.lib.kvm_fa_decode_shared,
+                 (st.h, pre[0] if prefix is not None else None, arr, nt, n, _ptr(q), _VIEW_TYPES[q.dtype], _ptr(q_pos), n_head,
+                  float(scale), _VIEW_TYPES[out.dtype], _ptr(out)),
+                 (prefix, windows, arr, nt, pre, q, q_pos))
+    p.out = out
+    return p
+
+
+def fa_decode_shared(st, prefix, windows, n_tokens, q, q_pos, n_head, scale, out=None, out_dtype=None):
+    """prepare_fa_decode_shared's call; returns its out."""
+    p = prepare_fa_decode_shared(st, prefix, windows, n_tokens, q, q_pos, n_head, scale, out, out_dtype)
+    p()
+    return p.out
+
+
 def quantize_rows(st, ty, x):
     """x: device fp32 [n_rows][n_per_row] -> uint8 ggml rows."""
     x = x.contiguous()

@@ -1,0 +1,407 @@
+"""kvm_fa_decode_shared against softmax attention in 64 bits over the cells' values:
+prefixes and conversations of many sizes, ragged token counts, every type, masks that
+leave a row or a tile empty, what is not finite at cells that are not seen, streams,
+graphs and refusals; and a layer's step: append, then attend."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import oracle as O
+from kvmem_amd import api, _lib as L
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"q8_0": (L.T_Q8_0, L.T_Q4_0), "q4_0": (L.T_Q4_0, L.T_Q4_0), "f16": (L.T_F16, L.T_F16)}
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def window(st, rng, cells, H, D, cache, pos, bt=64):
+    """A window of random rows at the given positions, and the cells' values in 64 bits."""
+    w = api.KVWindow(st, cells, H, D, bt, *TYPES[cache])
+    rows, vals = [], []
+    for t in TYPES[cache]:
+        r = api.quantize_rows(st, t, torch.from_numpy(rng.standard_normal((cells, H * D)).astype(np.float32)).cuda())
+        rows.append(r)
+        vals.append(api.dequantize_rows(st, t, r, H * D).double().view(cells, H, D))
+    p = torch.from_numpy(np.asarray(pos, np.int32)).cuda()
+    w.import_rows(0, rows[0], rows[1], p)
+    return w, vals[0], vals[1], p
+
+
+def expected(q, q_pos, counts, prefix, owns, H, scale):
+    """(softmax attention, bound of the f16 operands' error) in 64 bits.  prefix and owns:
+    (window, K, V, positions) or None.
+
+    Half steps of f16 are u = 2^-11.  A score's terms carry u for q and u for k (a bf16 q
+    and an f16 cell none, not used): |ds| <= 2u scale sum |q k|; p changes by a factor
+    exp(+-2 ds) at most against the others; p and v are rounded: u each.  So an output,
+    a weighted mean, is off by (exp(2 ds) (1 + u)^3 - 1) sum p |v| / sum p at most; fp32
+    sums of n terms add n 2^-24 of it.  Probabilities below f16's range lose up to 2^-25
+    of the row's reference, which is within 2^8 of its maximum: 2^-17 of the largest p
+    each, n of them."""
+    n, Hq, D = q.shape
+    G, u = Hq // H, 2.0 ** -11
+    q = q.double()
+    out, lim = torch.zeros((n, Hq, D), dtype=torch.float64, device="cuda"), torch.zeros((n, Hq, D), dtype=torch.float64, device="cuda")
+    at = 0
+    for m, own in zip(counts, owns):
+        parts = [x for x in (prefix, own) if x is not None]
+        for t in range(at, at + m):
+            seen = [(x[3] >= 0) & (x[3] <= q_pos[t]) for x in parts]
+            if not any(bool(s.any()) for s in seen):
+                continue
+            for h in range(H):
+                k = torch.cat([x[1][s, h] for x, s in zip(parts, seen)])
+                v = torch.cat([x[2][s, h] for x, s in zip(parts, seen)])
+                qq = q[t, h * G:(h + 1) * G]
+                s = (k @ qq.t().contiguous()).t() * scale
+                e = (k.abs() @ qq.abs().t().contiguous()).t().amax(1) * abs(scale) * 2 * u
+                p = torch.softmax(s, 1)
+                mean = p @ v.abs()
+                cells = k.shape[0]
+                out[t, h * G:(h + 1) * G] = p @ v
+                lim[t, h * G:(h + 1) * G] = mean * (torch.exp(2 * e)[:, None] * (1 + u) ** 3 - 1 + cells * 2.0 ** -24) \
+                    + p.amax(1, keepdim=True) * v.abs().sum(0) * 2.0 ** -17
+        at += m
+    return out, lim
+
+
+def check(got, want, lim):
+    err = (got.double() - want).abs()
+    bound = lim + (want.abs() + lim) * HALF_STEP[got.dtype]
+    assert not bool((~(err <= bound)).any()), float((err - bound).max())
+    ref = want.norm()
+    if float(ref):
+        # and far closer on the whole: roundings do not all point one way
+        rel = float((got.double() - want).norm() / ref)
+        assert rel <= 2e-3 + HALF_STEP[got.dtype], rel
+
+
+def run(st, rng, H, G, D, cache, prefix_cells, prefix_pos, lanes, counts, q_dtype, out_dtype, scale=None, q_pos=None):
+    """lanes: (cells, positions) or None for each."""
+    scale = D ** -0.5 if scale is None else scale
+    prefix = None if not prefix_cells else window(st, rng, prefix_cells, H, D, cache, prefix_pos)
+    owns = [None if x is None else window(st, rng, x[0], H, D, cache, x[1]) for x in lanes]
+    n = sum(counts)
+    q = torch.from_numpy(rng.standard_normal((n, H * G, D)).astype(np.float32)).to(q_dtype).cuda()
+    qp = torch.from_numpy(np.asarray(q_pos, np.int32)).cuda()
+    got = api.fa_decode_shared(st, prefix and prefix[0], [x and x[0] for x in owns], counts, q, qp, H * G, scale, out_dtype=out_dtype)
+    check(got, *expected(q, qp, counts, prefix, owns, H, scale))
+    return got, prefix, owns, q, qp
+
+
+def cells(n, live, first, hole=0):
+    """Positions of a window's n cells: `live` from `first` on, the rest empty."""
+    p = np.where(np.arange(n) < live, first + np.arange(n), -1)
+    if hole:
+        p[::hole] = -1
+    return p
+
+
+CASES = [
+    # H, G, D, cache, prefix cells, live, [own cells, live], counts, q, out
+    (2, 4, 128, "f16", 1024, 1000, [(256, 130), (256, 3)], [1, 1], torch.bfloat16, torch.bfloat16),
+    (4, 6, 256, "q8_0", 4096, 4096, [(512, 400)] * 8, [1] * 8, torch.bfloat16, torch.bfloat16),
+    (4, 6, 256, "q8_0", 2048, 1999, [(512, 500), (64, 5), (1024, 700)], [4, 1, 5], torch.float32, torch.float32),
+    (1, 8, 256, "q4_0", 1984, 1961, [(192, 190), (128, 1), (64, 64), (64, 9)], [3, 0, 2, 4], torch.bfloat16, torch.float32),
+    (8, 4, 128, "f16", 640, 640, [(128, 100)] * 5, [3] * 5, torch.float32, torch.float16),
+    (2, 1, 256, "f16", 320, 311, [(64, 33), (64, 2)], [1, 2], torch.bfloat16, torch.float32),
+    (3, 5, 128, "q8_0", 128, 65, [(64, 1), None, (64, 64)], [1, 2, 1], torch.float32, torch.bfloat16),
+    (1, 1, 128, "q4_0", 64, 1, [None], [1], torch.float32, torch.float32),
+    (2, 2, 128, "q8_0", 0, 0, [(64, 10), (4096, 4000)], [1, 1], torch.float32, torch.float32),
+    (1, 64, 128, "f16", 256, 200, [(64, 20)] * 3, [1, 2, 1], torch.bfloat16, torch.bfloat16),
+    (1, 2, 128, "q8_0", 512, 512, [(64, 20)] * 64, [1] * 64, torch.bfloat16, torch.bfloat16),
+    (2, 3, 256, "q4_0", 256, 256, [(64, 40)] * 2, [40, 33], torch.bfloat16, torch.bfloat16),     # chunks, not single tokens
+    (4, 6, 256, "f16", 1024, 1024, [(256, 250)] * 4, [4, 3, 2, 1], torch.bfloat16, torch.float32),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(str(x).replace("torch.", "").replace(" ", "") for x in c)[:90])
+def test_equals_softmax_in_64_bits(kvm_state, case):
+    H, G, D, cache, pc, live, lanes, counts, qd, od = case
+    rng = np.random.default_rng(pc + D + G)
+    own = [x and (x[0], cells(x[0], x[1], live)) for x in lanes]
+    ends = [live + (x[1] if x else 0) for x in lanes]
+    qp = np.concatenate([np.arange(e - m, e) for e, m in zip(ends, counts)])
+    run(kvm_state, rng, H, G, D, cache, pc, cells(pc, live, 0) if pc else None, own, counts, qd, od, q_pos=qp)
+
+
+@pytest.mark.parametrize("cache", ["q8_0", "f16"])
+def test_long_prefix(kvm_state, cache):
+    """Many tiles a wave, several looks at a piece's tiles (one kv head, one row group: all
+    tiles of 524,288 cells are a few workgroups' when the chip has few)."""
+    st, rng, H, G, D = kvm_state, np.random.default_rng(2), 1, 2, 128
+    n = 131072
+    p = cells(n, n - 77, 0, hole=1013)
+    run(st, rng, H, G, D, cache, n, p, [(64, cells(64, 3, n))], [1], torch.bfloat16, torch.float32, q_pos=[n + 2])
+
+
+def test_many_tiles_a_workgroup(kvm_state):
+    """More tiles a workgroup than it looks at at a time: 8 kv heads x 5 row groups x 2,048 tiles."""
+    st, rng, n = kvm_state, np.random.default_rng(14), 131072
+    p = rng.permutation(n)
+    p[rng.random(n) < 0.01] = -1
+    run(st, rng, 8, 4, 128, "q8_0", n, p, [None, None], [20, 20], torch.bfloat16, torch.float32,
+        q_pos=rng.integers(n // 2, n, 40))
+
+
+def test_workspace_under_capture(kvm_state):
+    """A capture that needs a larger workspace is refused; one captured before another call
+    grew it replays on the one it had."""
+    st, rng, H, D = api.State(0), np.random.default_rng(15), 1, 128
+    try:
+        w = window(st, rng, 256, H, D, "q8_0", cells(256, 256, 0))[0]
+        big = window(st, rng, 65536, 8, D, "q8_0", cells(65536, 65536, 0))[0]
+        q = torch.from_numpy(rng.standard_normal((1, 4, D)).astype(np.float32)).cuda()
+        pos = torch.tensor([300], dtype=torch.int32, device="cuda")
+        small = api.prepare_fa_decode_shared(st, w, [None], [1], q, pos, 4, 0.1)
+        qb = torch.from_numpy(rng.standard_normal((64, 64, D)).astype(np.float32)).cuda()
+        pb = torch.full((64,), 70000, dtype=torch.int32, device="cuda")
+        large = api.prepare_fa_decode_shared(st, big, [None], [64], qb, pb, 64, 0.1)
+        small()
+        torch.cuda.synchronize()
+        want = small.out.clone()
+        g = st.capture(small)
+        with pytest.raises(L.KvmError) as e:
+            st.capture(large)
+        assert e.value.code == L.KVM_ENOMEM
+        torch.cuda.synchronize()
+        large()
+        torch.cuda.synchronize()
+        for _ in range(3):
+            small.out.zero_()
+            g.replay()
+            large()
+            torch.cuda.synchronize()
+            assert torch.equal(small.out, want)
+    finally:
+        torch.cuda.synchronize()
+        st.close()
+
+
+def test_rows_that_see_little_or_nothing(kvm_state):
+    """Rows whose positions lie before every cell give zeros; others see a single cell, a part
+    of the prefix and none of their own, or cells in no order with holes and whole empty tiles."""
+    st, rng, H, G, D = kvm_state, np.random.default_rng(3), 2, 3, 128
+    pre = rng.permutation(640).astype(np.int64) + 10
+    pre[64:192] = -1
+    pre[200::7] = -1
+    own = [(128, np.where(np.arange(128) % 3 == 0, 700 + np.arange(128), -1)), (64, np.full(64, -1)), None]
+    for cache in ("q8_0", "f16"):
+        got, prefix, *_ = run(st, rng, H, G, D, cache, 640, pre, own, [3, 2, 2], torch.float32, torch.float32,
+                              q_pos=[5, 11, 760, -1, 300, 2 ** 31 - 1, 9])
+        assert not got[0].any() and not got[3].any() and not got[6].any()
+        first = int(np.flatnonzero((pre >= 0) & (pre <= 11))[0]) if ((pre >= 0) & (pre <= 11)).sum() == 1 else None
+        if first is not None:
+            assert torch.equal(got[1].view(H, G, D)[:, 0], prefix[2][first].float())
+
+
+def test_empty_windows(kvm_state):
+    """Nothing anywhere: zeros, whatever was there; no tokens: nothing is written."""
+    st, rng = kvm_state, np.random.default_rng(4)
+    got, *_ = run(st, rng, 1, 4, 128, "q8_0", 128, np.full(128, -1), [(64, np.full(64, -1))] * 2, [1, 2], torch.float32,
+                  torch.float32, q_pos=[5, 6, 7])
+    assert not got.any()
+    w = window(st, rng, 64, 1, 128, "q8_0", cells(64, 64, 0))[0]
+    none = torch.empty((0, 4, 128), device="cuda")
+    pos = torch.empty((0,), dtype=torch.int32, device="cuda")
+    assert api.fa_decode_shared(st, w, [None, w], [0, 0], none, pos, 4, 1.0).shape == none.shape
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.07, 3.0])
+def test_scales(kvm_state, scale):
+    """Equal weights, a negative scale, scores that grow far past the first tile's."""
+    run(kvm_state, np.random.default_rng(5), 2, 4, 128, "f16", 1024, cells(1024, 1024, 0), [(128, cells(128, 100, 1024))] * 3,
+        [2, 1, 1], torch.bfloat16, torch.float32, scale=scale, q_pos=[1100, 1110, 1123, 1060])
+
+
+def test_scores_that_keep_growing(kvm_state):
+    """Keys along the query, longer from tile to tile: every wave moves its maximum often."""
+    st, rng, H, G, D = kvm_state, np.random.default_rng(6), 1, 2, 128
+    n = 2048
+    q = torch.ones((1, G, D), dtype=torch.float32, device="cuda")
+    k = np.ones((n, D), np.float32) * (np.arange(n)[:, None] // 64 * 0.5)
+    v = rng.standard_normal((n, D)).astype(np.float32)
+    w = api.KVWindow(st, n, H, D, 64, *TYPES["f16"])
+    rows = [api.quantize_rows(st, L.T_F16, torch.from_numpy(x).cuda()) for x in (k, v)]
+    pos = torch.from_numpy(rng.permutation(n).astype(np.int32)).cuda()
+    w.import_rows(0, *rows, pos)
+    kd, vd = (api.dequantize_rows(st, L.T_F16, x, D).double().view(n, H, D) for x in rows)
+    qp = torch.tensor([n], dtype=torch.int32, device="cuda")
+    got = api.fa_decode_shared(st, w, [None], [1], q, qp, G, 0.3)
+    check(got, *expected(q, qp, [1], (w, kd, vd, pos), [None], H, 0.3))
+
+
+@pytest.mark.parametrize("cache", ["q8_0", "f16"])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+def test_what_is_not_seen_is_not_used(kvm_state, cache, what):
+    """NaN and infinities in empty cells, and in cells that some tokens of a unit see and others
+    do not: a token's output is as if what it does not see held zeros."""
+    st, H, G, D = kvm_state, 2, 3, 128
+    lanes, counts = [(128, cells(128, 40, 256)), (64, cells(64, 9, 256))], [4, 3]
+    qp = np.concatenate([np.arange(292, 296), np.arange(262, 265)])
+    outs = []
+    for bad in (False, True):
+        rng = np.random.default_rng(7)
+        got, prefix, owns, q, qpos = run(st, rng, H, G, D, cache, 320, cells(320, 256, 0), lanes, counts, torch.float32, torch.float32,
+                                         q_pos=qp)
+        if bad:
+            raw = {"f16": lambda x: x.view(torch.float16), "q8_0": lambda x: x.view(torch.float16)}[cache]
+            for w, empties in ((prefix[0], range(256, 320)), (owns[0][0], range(40, 128)), (owns[1][0], range(9, 64))):
+                for c in empties:
+                    for h in range(H):
+                        _poison(w, cache, c, h, what)
+            # lane 0's last token (cell 39, position 295) and lane 1's last two: later tokens' own cells
+            _poison(owns[0][0], cache, 39, 1, what)
+            _poison(owns[1][0], cache, 7, 0, what)
+            _poison(owns[1][0], cache, 8, 0, what)
+            got = api.fa_decode_shared(st, prefix[0], [x[0] for x in owns], counts, q, qpos, H * G, D ** -0.5)
+        outs.append(got)
+    clean, dirty = (x.view(7, H, G, D) for x in outs)
+    same = torch.ones((7, H), dtype=torch.bool)
+    same[3, 1] = same[5, 0] = same[6, 0] = False       # these see one
+    assert torch.equal(dirty[same], clean[same])
+    assert not bool(dirty[~same].isfinite().all())
+
+
+def _poison(w, cache, c, h, what):
+    """What is not finite into the values (and keys) of cell c, kv head h."""
+    D, t, i = w.head_dim, c // 64, c % 64
+    if cache == "f16":
+        v = w.v.view(torch.float16).view(w.n_head_kv, -1, 64 * D)[h, t].view(D // 16, 4, 16, 2, 8)
+        k = w.k.view(torch.float16).view(w.n_head_kv, -1, 64 * D)[h, t].view(4, D // 32, 4, 16, 8)
+        v[:, (i & 31) >> 3, :, i >> 5, i & 7] = what
+        if int(w.cell_pos[c]) < 0:
+            k[i >> 4, :, :, i & 15] = what
+    else:
+        NB = D // 32
+        vb = w.v.view(w.n_head_kv, -1, 32 * D + 128 * NB)[h, t][32 * D:].view(torch.float16).view(NB, 2, 4, 8)
+        kb = w.k.view(w.n_head_kv, -1, 64 * D + 128 * NB)[h, t][64 * D:].view(torch.float16).view(4, NB, 16)
+        vb[:, i >> 5, (i & 31) >> 3, i & 7] = what
+        if int(w.cell_pos[c]) < 0:
+            kb[i >> 4, :, i & 15] = what
+
+
+def test_infinite_values_that_are_seen(kvm_state):
+    """An infinite value at a cell that every row sees reaches every row, and only its dims."""
+    st, rng, H, G, D = kvm_state, np.random.default_rng(8), 1, 2, 128
+    w, k, v, pos = window(st, rng, 128, H, D, "f16", cells(128, 128, 0))
+    w.v.view(torch.float16).view(-1, 64 * D)[0].view(D // 16, 4, 16, 2, 8)[3, 0, 5, 0, 2] = float("inf")     # cell 2, dim 53
+    q = torch.from_numpy(rng.standard_normal((2, G, D)).astype(np.float32)).cuda() * 0.1
+    got = api.fa_decode_shared(st, w, [None], [2], q, torch.tensor([200, 200], dtype=torch.int32, device="cuda"), G, D ** -0.5)
+    assert bool((got[..., 53] == float("inf")).all())
+    got[..., 53] = 0
+    assert bool(got.isfinite().all())
+
+
+def test_same_as_one_window(kvm_state):
+    """A prefix and an own window give what one window with all the cells gives (kvm_fa_prefill),
+    to the roundings of both."""
+    st, rng, H, G, D = kvm_state, np.random.default_rng(9), 4, 6, 256
+    P, n, T = 1024, 512, 6
+    kv = [api.quantize_rows(st, t, torch.from_numpy(rng.standard_normal((P + n, H * D)).astype(np.float32)).cuda()) for t in TYPES["q8_0"]]
+    pos = torch.arange(P + n, dtype=torch.int32).cuda()
+    one, pre, own = api.KVWindow(st, P + n, H, D, 64), api.KVWindow(st, P, H, D, 64), api.KVWindow(st, n, H, D, 64)
+    one.import_rows(0, *kv, pos)
+    pre.import_rows(0, kv[0][:P], kv[1][:P], pos[:P])
+    own.import_rows(0, kv[0][P:], kv[1][P:], pos[P:])
+    q = torch.from_numpy(rng.standard_normal((T, H * G, D)).astype(np.float32)).cuda()
+    qp = pos[-T:].contiguous()
+    a = api.fa_prefill(st, one, q, qp, H * G, D ** -0.5)
+    b = api.fa_decode_shared(st, pre, [own], [T], q, qp, H * G, D ** -0.5)
+    rel = float((a - b).norm() / a.norm())
+    assert rel <= 1e-3, rel                             # (two forms of 3e-4 each)
+
+
+def test_order_of_lanes_and_repeats(kvm_state):
+    """The same call twice gives the same bits; a lane's output does not depend on what the
+    other lanes' windows hold."""
+    st, H, G, D = kvm_state, 2, 4, 128
+    args = dict(H=H, G=G, D=D, cache="q8_0", prefix_cells=512, prefix_pos=cells(512, 512, 0),
+                lanes=[(64, cells(64, 20, 512)), (128, cells(128, 99, 512))], counts=[2, 1], q_dtype=torch.bfloat16,
+                out_dtype=torch.float32, q_pos=[530, 531, 610])
+    got, prefix, owns, q, qp = run(st, np.random.default_rng(10), **args)
+    again = api.fa_decode_shared(st, prefix[0], [x[0] for x in owns], [2, 1], q, qp, H * G, D ** -0.5)
+    assert torch.equal(got, again)
+    other = window(st, np.random.default_rng(11), 64, H, D, "q8_0", cells(64, 64, 512))
+    mixed = api.fa_decode_shared(st, prefix[0], [other[0], owns[1][0]], [2, 1], q, qp, H * G, D ** -0.5)
+    assert torch.equal(mixed[2], got[2]) and not torch.equal(mixed[:2], got[:2])
+
+
+def test_step_append_then_attend(kvm_state):
+    """A layer's step of a batch: new keys, values and queries of each conversation into its window
+    (norms and rotation on the way), then the shared attention, against the same from the
+    cells' values; on a stream of its own, and captured and replayed with other inputs."""
+    rng, H, G, D, P = np.random.default_rng(12), 2, 4, 128, 512
+    s = torch.cuda.Stream()
+    st = api.State(0, stream=s.cuda_stream)
+    try:
+        with torch.cuda.stream(s):
+            prefix = window(st, rng, P, H, D, "q8_0", cells(P, P, 0))
+            counts, fill = [3, 1, 2], [10, 63, 100]
+            owns = [window(st, rng, 128, H, D, "q8_0", cells(128, f, P)) for f in fill]
+            n = sum(counts)
+            q, k, v = (torch.from_numpy(rng.standard_normal((n, h, D)).astype(np.float32)).bfloat16().cuda() for h in (H * G, H, H))
+            qw, kw = torch.ones(D, device="cuda"), torch.ones(D, device="cuda") * 0.9
+            pos = torch.from_numpy(np.concatenate([P + f + np.arange(m) for f, m in zip(fill, counts)]).astype(np.int32)).cuda()
+            app = api.prepare_window_append(st, [x[0] for x in owns], fill, counts, k, v, pos, 64, 1e6, k_weight=kw, eps=1e-6, q=q,
+                                            q_weight=qw, q_out_dtype=torch.float32)
+            att = api.prepare_fa_decode_shared(st, prefix[0], [x[0] for x in owns], counts, app.q_out, pos, H * G, D ** -0.5)
+
+            def want():
+                held = []
+                for w, *_ in owns:
+                    kr, vr = w.export_rows(0, 128)
+                    held.append((w, *(api.dequantize_rows(st, t, r, H * D).double().view(128, H, D) for t, r in
+                                      ((w.k_type, kr), (w.v_type, vr))), w.cell_pos))
+                return expected(app.q_out, pos, counts, prefix, held, H, D ** -0.5)
+
+            app()
+            att()
+            torch.cuda.synchronize()
+            check(att.out, *want())
+        g = st.capture(lambda: (app(), att()))
+        for i in range(3):
+            with torch.cuda.stream(s):
+                for x in (q, k, v):
+                    x.copy_(torch.from_numpy(rng.standard_normal(x.shape).astype(np.float32)))
+                torch.cuda.synchronize()
+                att.out.fill_(-7.0)
+                torch.cuda.synchronize()
+                g.replay()
+                torch.cuda.synchronize()
+                got = att.out.clone()
+                check(got, *want())
+                app()
+                att()
+                torch.cuda.synchronize()
+                assert torch.equal(att.out, got)
+    finally:
+        torch.cuda.synchronize()
+        st.close()
+
+
+def test_refusals(kvm_state):
+    st, rng, H, D = kvm_state, np.random.default_rng(13), 2, 128
+    w = window(st, rng, 64, H, D, "q8_0", cells(64, 64, 0))[0]
+    q, pos = torch.zeros((2, 8, D), device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+
+    def refused(code, *a, **kw):
+        with pytest.raises(L.KvmError) as e:
+            api.fa_decode_shared(st, *a, **kw)
+        assert e.value.code == code, e.value
+
+    refused(L.KVM_EUNSUPPORTED, w, [api.KVWindow(st, 64, H, D, 64, *TYPES["f16"])], [2], q, pos, 8, 1.0)
+    refused(L.KVM_EUNSUPPORTED, w, [api.KVWindow(st, 64, 4, D, 64)], [2], q, pos, 8, 1.0)
+    refused(L.KVM_ERANGE, w, [None] * 65, [1, 1] + [0] * 63, q, pos, 8, 1.0)
+    refused(L.KVM_EINVAL, None, [None], [2], q, pos, 8, 1.0)
+    refused(L.KVM_EINVAL, w, [None], [3], q, pos, 8, 1.0)
+    refused(L.KVM_EINVAL, w, [None, None], [2], q, pos, 8, 1.0)
+    refused(L.KVM_EINVAL, w, [None], [2], q[:, :7].contiguous(), pos, 7, 1.0)
+    refused(L.KVM_EINVAL, w, [None], [2], q.half(), pos, 8, 1.0)
+    refused(L.KVM_EINVAL, w, [None], [2], q.cpu(), pos, 8, 1.0)
+    refused(L.KVM_EINVAL, w, [None], [2], q, pos.long(), 8, 1.0)
+    refused(L.KVM_EINVAL, w, [None], [2], q, pos, 8, float("nan"))
+    refused(L.KVM_EINVAL, w, [None], [2], q, pos, 8, 1.0, out=torch.empty((2, 8, D), dtype=torch.float64, device="cuda"))
