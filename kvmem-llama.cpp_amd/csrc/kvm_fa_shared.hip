@@ -35,6 +35,7 @@
 #define FS_LAZY 8.0f             // log2 growth of a row's maximum tolerated before a rescale
 
 typedef float kvm_f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void *fs_lds_ptr;
 typedef float kvm_f32x2 __attribute__((ext_vector_type(2)));
 
 // A window with the rows that attend over it.
@@ -76,13 +77,16 @@ __host__ __device__ inline uint32_t fs_owner(uint32_t tiles, uint32_t log_p, uin
     return p;
 }
 
+// Workgroups of a CU: the f16 tiles of 256 dims take the registers of two waves.
+__host__ __device__ constexpr uint32_t fs_resident(uint32_t D, bool quant) { return D == 256 && !quant ? 1 : 2; }
+
 template <int D, bool QUANT>
 struct fs_geo {
     static constexpr int KS = D / 16, NB = D / 32, DT = D / 32;              // k-steps, 32-dim blocks, dim tiles
     static constexpr int DW = DT / 4;                     // dim tiles that a wave adds up at the end
     static constexpr uint32_t KB = QUANT ? 64u * D + 128u * NB : 128u * D, VB = QUANT ? 32u * D + 128u * NB : 128u * D;
     static constexpr int KH = QUANT ? NB : 2 * NB;        // 16-byte loads of a half tile's K
-    static constexpr int SETS = D == 256 && !QUANT ? 1 : 2;                  // half tiles of K (and f16 V) in registers
+    static constexpr int SETS = D == 256 ? 1 : 2;                  // half tiles of K (and f16 V) in registers
     static constexpr uint32_t QU = 528;                   // LDS bytes of a unit of Q: 8 dims of 32 rows, 16 bytes apart in the banks
 };
 
@@ -90,14 +94,23 @@ template <int D, bool QUANT>
 struct fs_lds {
     using G = fs_geo<D, QUANT>;
     alignas(16) uint8_t q[2 * G::KS * G::QU];
-    alignas(16) uint8_t sc[4][2][128 * G::NB];            // a wave's tile: K scales, V scales
-    alignas(16) int32_t cp[4][64];
+    alignas(16) uint8_t sc[4][2][QUANT ? 2 : 1][QUANT ? 1024 : 16];           // a wave's tile and its next: K scales, V scales
+    alignas(16) int32_t cp[4][2][64];                     // and their cells' positions
     alignas(16) float x[4][G::DW * 4 * 256];              // chunks of O on their way
     float ml[4][2][32];
     uint32_t odd[4][2];
     uint32_t list[FS_BATCH];
     uint8_t flag[FS_BATCH];
 };
+
+// x, from which the compiler cannot tell that a value formed of it does not change in a
+// loop: hoisted, lane addresses take the registers that the accumulators need.
+__device__ __forceinline__ uint32_t fs_opaque(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+// K row i of a half tile is this key: bits 2 and 3 swapped.
+__device__ __forceinline__ uint32_t fs_key(uint32_t i) { return (i & 0x13) | (i & 4) << 1 | (i & 8) >> 1; }
 
 // Nothing moves over it.
 #define FS_FENCE() __builtin_amdgcn_sched_barrier(0)
@@ -149,8 +162,8 @@ __device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_
 #pragma unroll
         for (int r = 0; r < 16; ++r) O[dt][r] = 0.0f;
 
-    // operand addresses of a lane: K row m2 is key m2 with bits 2 and 3 swapped
-    const uint32_t key = (m2 & 0x13) | (m2 & 4) << 1 | (m2 & 8) >> 1;
+    // operand addresses of a lane
+    const uint32_t key = fs_key(m2);
     const uint32_t k_lane = ((key >> 4) * (QUANT ? NB / 2 : NB) * 64 + 16 * g2 + (key & 15)) * 16;
     const uint32_t v_lane = ((m2 >> 4) * 64 + 16 * g2 + (m2 & 15)) * (QUANT ? 8 : 32);
     const uint8_t *const k_head = sg.k + (uint64_t)h * sg.n_tiles * KB, *const v_head = sg.v + (uint64_t)h * sg.n_tiles * VB;
@@ -190,9 +203,8 @@ __device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_
 
         // ---- the wave's tiles: list entries w, w + 4, ..  Registers of a half tile are
         // loaded for the next tile where this one's are used up.
-        kvm_u32x4 kr[SETS][KH], vh[QUANT ? 1 : SETS][QUANT ? 1 : 2 * DT], sck, scv;
-        kvm_u32x2 vq[QUANT ? 2 * DT : 1];                 // quantised V: both halves
-        uint32_t cp;
+        kvm_u32x4 kr[SETS][KH], vh[QUANT ? 1 : SETS][QUANT ? 1 : 2 * DT];
+        uint32_t vq[QUANT ? 2 * DT : 1];                  // quantised V of a half tile
         // (past the wave's last tile the bounds let nothing through)
         auto rsrc = [&](const void *head, uint32_t e, uint32_t bytes, bool more) {
             return __builtin_amdgcn_make_buffer_rsrc((void *)((const uint8_t *)head + (uint64_t)(e & 0x7fffffffu) * bytes), (short)0, more ? bytes : 0u, 0x00020000);
@@ -205,18 +217,28 @@ __device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_
         auto load_v = [&](__amdgpu_buffer_rsrc_t r, int half) {
 #pragma unroll
             for (int i = 0; i < 2 * DT; ++i) {
-                if constexpr (QUANT) vq[i] = __builtin_amdgcn_raw_buffer_load_b64(r, v_lane + (i & 1) * 256, (i >> 1) * 1024, 0);
+                if constexpr (QUANT) vq[i] = __builtin_amdgcn_raw_buffer_load_b32(r, v_lane + (i & 1) * 256 + half * 4, (i >> 1) * 1024, 0);
                 else vh[half % SETS][i] = __builtin_amdgcn_raw_buffer_load_b128(r, v_lane + (i & 1) * 1024 + half * 16, (i >> 1) * 4096, 0);
             }
         };
-        auto load_sc = [&](__amdgpu_buffer_rsrc_t rk, __amdgpu_buffer_rsrc_t rv) {
-            if constexpr (QUANT) {
-                sck = __builtin_amdgcn_raw_buffer_load_b128(rk, 16 * l, 64 * D, 0);
-                scv = __builtin_amdgcn_raw_buffer_load_b128(rv, 16 * l, 32 * D, 0);
-            }
+        // Scales and positions go to LDS by direct copies (lane l writes 16 or 4 bytes at M0 +
+        // 16 l or 4 l), issued from asm, so that the compiler adds no wait for them; the asm
+        // restores M0, which the compiler reserves.
+        auto copy16 = [&](const uint8_t *src, void *dst) {
+            const uint32_t off = 16u * (fs_opaque(l) & (D == 256 ? 63u : 31u));   // (128 dims: 512 bytes of scales)
+            uint32_t m0_saved;
+            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
+                         : "=&s"(m0_saved) : "v"(off), "s"((uint32_t)(uintptr_t)(fs_lds_ptr)dst), "s"(src) : "memory");
         };
-        auto load_cp = [&](uint32_t e, bool more) {
-            cp = __builtin_amdgcn_raw_buffer_load_b32(rsrc(sg.cell_pos, e, 256u, more), 4 * l, 0, 0);
+        auto copies = [&](uint32_t e, uint32_t buf) {
+            const uint32_t t = e & 0x7fffffffu;
+            if constexpr (QUANT) {
+                copy16(k_head + (uint64_t)t * KB + 64 * D, sm.sc[w][buf][0]);
+                copy16(v_head + (uint64_t)t * VB + 32 * D, sm.sc[w][buf][1]);
+            }
+            uint32_t m0_saved;
+            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, %3\n\ts_mov_b32 m0, %0"
+                         : "=&s"(m0_saved) : "v"(4u * fs_opaque(l)), "s"((uint32_t)(uintptr_t)(fs_lds_ptr)&sm.cp[w][buf][0]), "s"(sg.cell_pos + (uint64_t)t * 64) : "memory");
         };
         // keys base .. base + 7 of the lanes' bits, together
         auto gather = [&](uint32_t base, uint32_t bits) {
@@ -230,14 +252,16 @@ __device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_
         if ((uint32_t)w < n_t) {
             e = __builtin_amdgcn_readfirstlane(sm.list[w]);
             const auto rk = rsrc(k_head, e, KB, true), rv = rsrc(v_head, e, VB, true);
-            load_sc(rk, rv);
-            load_cp(e, true);
+            copies(e, 0);
             load_k(rk, 0);
             if (SETS == 2) load_k(rk, 1);
             load_v(rv, 0);
             if (!QUANT && SETS == 2) load_v(rv, 1);
         }
-        for (uint32_t j = w; j < n_t; j += 4) {
+        uint32_t buf = 0;
+        for (uint32_t j = w; j < n_t; j += 4, buf ^= 1) {
+            // the tile's copies: the first tile's half tiles, or more, were loaded after them
+            asm volatile("s_waitcnt vmcnt(%0)" : : "n"(SETS * KH + (QUANT ? 1 : SETS) * 2 * DT) : "memory");
             const bool more = j + 4 < n_t;
             const uint32_t en = __builtin_amdgcn_readfirstlane(sm.list[more ? j + 4 : j]);
             const auto rk = rsrc(k_head, en, KB, more), rv = rsrc(v_head, en, VB, more);
@@ -247,59 +271,59 @@ __device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_
             uint64_t seen = ~0ull, part = 0, odd = 0;
             if (!full) {
                 asm volatile("" ::: "memory");            // keep it on this (rare) path
+                const uint32_t cp = (uint32_t)sm.cp[w][buf][fs_opaque(l)];
                 seen = __builtin_amdgcn_ballot_w64(cp < some_lim);
                 part = seen & ~__builtin_amdgcn_ballot_w64(cp < all_lim);
-                sm.cp[w][l] = (int32_t)cp;
                 if constexpr (QUANT) {
                     // What no row sees counts nothing, whatever it holds: a scale of 0.  (Lane
                     // l has the scales of 8 keys of a block.)
-                    const uint32_t base = 32 * (l >> 2 & 1u) + 8 * (l & 3u), on = (uint32_t)(seen >> base) & 0xffu, pt = (uint32_t)(part >> base) & 0xffu;
+                    const uint32_t lo = fs_opaque(l), base = 32 * (lo >> 2 & 1u) + 8 * (lo & 3u), on = (uint32_t)(seen >> base) & 0xffu, pt = (uint32_t)(part >> base) & 0xffu;
+                    kvm_u32x4 scv = *(const kvm_u32x4 *)(sm.sc[w][buf][1] + 16 * lo);
                     uint32_t bad = 0;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const uint32_t sh = 16 * (i & 1), v = scv[i >> 1] >> sh & 0xffffu;
-                        if (l < 8u * NB && (pt >> i & 1u) && (v & 0x7c00u) == 0x7c00u) bad |= 1u << i;
+                        if (lo < 8u * NB && (pt >> i & 1u) && (v & 0x7c00u) == 0x7c00u) bad |= 1u << i;
                         if (!(on >> i & 1u) || (bad >> i & 1u)) scv[i >> 1] &= ~(0xffffu << sh);
                     }
+                    *(kvm_u32x4 *)(sm.sc[w][buf][1] + 16 * lo) = scv;
                     if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) odd = gather(base, bad);
                 }
             }
-            if constexpr (QUANT) {
-                if (l < 8u * NB) {
-                    *(kvm_u32x4 *)(sm.sc[w][0] + 16 * l) = sck;
-                    *(kvm_u32x4 *)(sm.sc[w][1] + 16 * l) = scv;
-                }
-            }
-            load_sc(rk, rv);
-            load_cp(en, more);
+            if (more) copies(en, buf ^ 1);
 
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                // ---- S^T of 32 keys: operand ks + 1 is made while the MFMAs of ks run
+                // ---- S^T of 32 keys: K operand i + 1 is made while the MFMA of i runs; what
+                // comes from LDS is read two steps ahead
                 kvm_f32x16 S;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) S[r] = 0.0f;
-                const uint8_t *const sk = sm.sc[w][0] + (2 * half + (key >> 4)) * NB * 32 + 2 * (key & 15);
+                uint32_t ksc[NB];                         // the scales of the lane's key
+                if constexpr (QUANT) {
+                    const uint32_t k = fs_key(fs_opaque(l) & 31u);
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) ksc[b] = *(const uint16_t *)(sm.sc[w][buf][0] + ((2 * half + (k >> 4)) * NB + b) * 32 + 2 * (k & 15));
+                }
                 const uint8_t *const sq = sm.q + g2 * QU + m2 * 16;
                 // operands in the order of the K loads: (block pair, 16-dim half | block of the pair)
                 auto ks_of = [](int i) { return QUANT ? 4 * (i >> 2) + 2 * (i & 1) + (i >> 1 & 1) : i; };
                 auto k_op = [&](int i) {
                     if constexpr (QUANT) {
                         const kvm_u32x4 x = kr[half % SETS][i >> 1];
-                        return pf_q8(x[2 * (i & 1)], x[2 * (i & 1) + 1], *(const uint16_t *)(sk + 32 * (2 * (i >> 2) + (i & 1))));
+                        return pf_q8(x[2 * (i & 1)], x[2 * (i & 1) + 1], ksc[2 * (i >> 2) + (i & 1)]);
                     } else {
                         return __builtin_bit_cast(kvm_f16x8, kr[half % SETS][i]);
                     }
                 };
                 auto q_op = [&](int i) { return *(const kvm_f16x8 *)(sq + 2 * ks_of(i) * QU); };
-                kvm_f16x8 kop = k_op(0), qop = q_op(0);
+                kvm_f16x8 kop = k_op(0), qr[3] = {q_op(0), q_op(1)};
 #pragma unroll
                 for (int i = 0; i < KS; ++i) {
-                    kvm_f16x8 qn = qop;
-                    if (i + 1 < KS) qn = q_op(i + 1);
-                    S = __builtin_amdgcn_mfma_f32_32x32x16_f16(kop, qop, S, 0, 0, 0);
+                    if (i + 2 < KS) qr[(i + 2) % 3] = q_op(i + 2);
+                    FS_FENCE();
+                    S = __builtin_amdgcn_mfma_f32_32x32x16_f16(kop, qr[i % 3], S, 0, 0, 0);
                     if (i + 1 < KS) kop = k_op(i + 1);
-                    qop = qn;
                     FS_FENCE();
                 }
                 if (SETS == 2) load_k(rk, half);
@@ -311,7 +335,7 @@ __device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_
                     asm volatile("" ::: "memory");
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const kvm_u32x4 x = *(const kvm_u32x4 *)(&sm.cp[w][32 * half + 16 * (i >> 1) + 8 * g2 + 4 * (i & 1)]);
+                        const kvm_u32x4 x = *(const kvm_u32x4 *)(&sm.cp[w][buf][32 * half + 16 * (i >> 1) + 8 * (fs_opaque(l) >> 5) + 4 * (i & 1)]);
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
                             if (!(x[r] < qlim)) S[4 * i + r] = -INFINITY;
@@ -366,14 +390,21 @@ __device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_
                             odd |= gather(32 * half + 8 * g2, bad[0] | bad[1] << 16);
                     }
                 }
+                kvm_u32x4 vs[3];
+                auto v_scale = [&](int i) {
+                    if constexpr (QUANT) vs[i % 3] = *(const kvm_u32x4 *)(sm.sc[w][buf][1] + (((i >> 1) * 2 + half) * 4 + 2 * (i & 1) + g2) * 16);
+                };
                 auto v_op = [&](int i) {
-                    if constexpr (QUANT)
-                        return pf_q4(vq[i][half], *(const kvm_u32x4 *)(sm.sc[w][1] + (((i >> 1) * 2 + half) * 4 + 2 * (i & 1) + g2) * 16));
+                    if constexpr (QUANT) return pf_q4(vq[i], vs[i % 3]);
                     else return __builtin_bit_cast(kvm_f16x8, vh[half % SETS][i]);
                 };
+                v_scale(0);
+                v_scale(1);
                 kvm_f16x8 vop = v_op(0);
 #pragma unroll
                 for (int i = 0; i < 2 * DT; ++i) {
+                    if (i + 2 < 2 * DT) v_scale(i + 2);
+                    FS_FENCE();
                     O[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vop, pb[i & 1], O[i >> 1], 0, 0, 0);
                     if (i + 1 < 2 * DT) vop = v_op(i + 1);
                     FS_FENCE();
@@ -382,15 +413,15 @@ __device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_
                     // A value that is no finite number, at a key that some rows see and others
                     // do not: 0 times it is not 0.  The product took 0 for it; here it is added
                     // where p is not 0 (p times it is itself).
-                    asm volatile("" ::: "memory");
+                    asm volatile("" : "+v"(pb[0]), "+v"(pb[1]) : : "memory");     // keep it on this (rare) path
                     const uint8_t *const v_tile = v_head + (uint64_t)(e & 0x7fffffffu) * VB;
                     float *const sx = sm.x[w];
                     for (uint32_t k = 0; k < 32; ++k) {
-                        const uint32_t c = 32 * half + k;
+                        const uint32_t c = 32 * half + k, lo = fs_opaque(l);
                         if (!(odd >> c & 1u)) continue;
                         // the key's values that are not finite, and where its p are not 0
 #pragma unroll
-                        for (uint32_t d = l; d < D; d += 64) {
+                        for (uint32_t d = lo; d < D; d += 64) {
                             float v;
                             if constexpr (QUANT)
                                 v = (float)((int)(v_tile[kvm_vq_byte(c, d)] >> kvm_vq_shift(c) & 15u) - 8) * kvm_h2f(*(const uint16_t *)(v_tile + kvm_vd_off(D, c, d / 32)));
@@ -399,13 +430,13 @@ __device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_
                         }
                         bool has = false;
 #pragma unroll
-                        for (uint32_t r = 0; r < 16; ++r) has |= g2 == (k >> 3 & 1u) && r == (k >> 4) * 8 + (k & 7u) && !((float)pb[r >> 3][r & 7] == 0.0f);
+                        for (uint32_t r = 0; r < 16; ++r) has |= lo >> 5 == (k >> 3 & 1u) && r == (k >> 4) * 8 + (k & 7u) && !((float)pb[r >> 3][r & 7] == 0.0f);
                         const uint64_t b = __builtin_amdgcn_ballot_w64(has);
-                        const bool mine = ((uint32_t)b | (uint32_t)(b >> 32)) >> m2 & 1u;
+                        const bool mine = ((uint32_t)b | (uint32_t)(b >> 32)) >> (lo & 31u) & 1u;
                         __builtin_amdgcn_wave_barrier();
 #pragma unroll
                         for (int x = 0; x < 4 * DT; ++x) {
-                            const kvm_f32x4 v = *(const kvm_f32x4 *)(sx + 8 * x + 4 * g2);
+                            const kvm_f32x4 v = *(const kvm_f32x4 *)(sx + 8 * x + 4 * (lo >> 5));
 #pragma unroll
                             for (int r = 0; r < 4; ++r) O[x >> 2][4 * (x & 3) + r] += mine ? v[r] : 0.0f;
                             FS_FENCE();
@@ -413,14 +444,9 @@ __device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_
                         __builtin_amdgcn_wave_barrier();
                     }
                 }
-                if constexpr (QUANT) {
-                    if (half == 1) load_v(rv, 0);
-                } else if (SETS == 2) {
-                    load_v(rv, half);
-                } else {
-                    if (half == 0) load_v(rsrc(v_head, e, VB, true), 1);
-                    else load_v(rv, 0);
-                }
+                if (!QUANT && SETS == 2) load_v(rv, half);
+                else if (half == 0) load_v(rsrc(v_head, e, VB, true), 1);
+                else load_v(rv, 0);
             }
             e = en;
         }
@@ -477,7 +503,7 @@ __device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_
 }
 
 template <int D, bool QUANT>
-__global__ void __launch_bounds__(256, 1) k_fs_attn(fs_args a) {
+__global__ void __launch_bounds__(256, fs_resident(D, QUANT)) k_fs_attn(fs_args a) {
     __shared__ fs_lds<D, QUANT> sm;
     const uint32_t tid = threadIdx.x, l = tid & 63u;
     // neighbouring shares on one XCD: their units read the same tiles
@@ -613,7 +639,7 @@ static uint32_t fs_stride(uint32_t n) {
 
 // Fills the segments, their tiles and the number of workgroups.
 static int fs_shape(kvm_state *st, const char *what, const kvm_window *prefix, const kvm_window *const *windows,
-                    const uint32_t *n_tokens, uint32_t n_lanes, uint32_t n_cu, fs_args *a, uint32_t *units) {
+                    const uint32_t *n_tokens, uint32_t n_lanes, uint32_t n_wg, fs_args *a, uint32_t *units) {
     uint64_t unit = 0, tiles = 0;
     uint32_t n = 0;
     auto add = [&](const kvm_window *w, uint32_t row0, uint32_t n_rows) {
@@ -643,7 +669,7 @@ static int fs_shape(kvm_state *st, const char *what, const kvm_window *prefix, c
     a->n_seg = n;
     // a share of four tiles at least: one a wave
     a->log_p = 0;
-    while ((2u << a->log_p) <= n_cu && (8ull << a->log_p) <= tiles) ++a->log_p;
+    while ((2u << a->log_p) <= n_wg && (8ull << a->log_p) <= tiles) ++a->log_p;
     *units = (uint32_t)unit;
     return KVM_OK;
 }
@@ -694,7 +720,9 @@ extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, con
     a.q_sign = scale < 0.0f ? -1.0f : scale > 0.0f ? 1.0f : 0.0f;
     a.c = scale != 0.0f ? fabsf(scale) * 1.4426950408889634f : 1.0f;
     uint32_t units = 0;
-    const int rc = fs_shape(st, what, prefix, windows, n_tokens, n_lanes, st ? st->n_cu : 256u, &a, &units);
+    const bool quant = kvm_k_quant(w0->k_type);
+    const uint32_t n_wg = (st ? st->n_cu : 256u) * fs_resident(D, quant);
+    const int rc = fs_shape(st, what, prefix, windows, n_tokens, n_lanes, n_wg, &a, &units);
     if (rc) return rc;
     if (!st) return KVM_EINVAL;
     const uint64_t slots = a.n_seg ? (1ull << a.log_p) + units : 0;
@@ -706,7 +734,6 @@ extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, con
         a.ws_o = (float *)ws;
         a.ws_ml = (float *)((uint8_t *)a.ws_o + bytes_o);
     }
-    const bool quant = kvm_k_quant(w0->k_type);
     auto go = [&](auto d) {
         constexpr int DD = decltype(d)::value;
         if (a.n_seg) {
