@@ -6,26 +6,29 @@
 //   both windows with 0 <= position <= the query's
 //
 // splits over any parts of the cells into (m, l, o) of each part, joined by the parts'
-// maxima.  A part is a piece: some tiles of one window for at most 32 rows of a kv head (a
-// row is a token and a query head of the group).  The prefix's rows are all conversations'
-// tokens side by side, so its keys and values are read, and brought to f16, once for 32
-// rows; a conversation's own window is one for its rows.  k_fs_attn forms the pieces,
-// k_fs_join joins those of each row.
+// maxima.  A part is a piece: some tiles of one window for a unit, 32 or 128 rows of a kv
+// head (a row is a token and a query head of the group).  The prefix's rows are all
+// conversations' tokens side by side, so its keys and values are read, and brought to f16,
+// once for a unit's rows; a conversation's own window has that conversation's rows.
+// k_fs_wide and k_fs_narrow form the pieces, k_fs_join joins those of each row.
 //
-// A workgroup is 4 waves, one a SIMD; each takes every fourth of the piece's tiles, for all
-// its rows, so that nothing is shared in the loop and no barrier is in it: tiles go from
-// memory into registers (the tile layout is the matrix operands'), a half tile's registers
-// are loaded for the next tile as soon as they are used.  S^T = K Q^T and O^T += V^T P^T on
-// 32x32x16 f16 MFMAs; Q is in LDS as operands.  Quantised tiles become f16 on the way: K and
-// V as (f16)(q d), Q and P rounded to f16, everything else fp32.  Key order: score row i of a
-// half tile is key i with bits 2 and 3 swapped, so that a lane's scores are 8 consecutive
-// keys of each 16, what the P V operand wants.  The waves' sums meet in LDS at the end.
-//
-// The tiles of all units (32 rows of a head over one window) are dealt to the workgroups in
-// equal shares, in an order that steps through a window in strides: a
-// part-filled window's live tiles are spread evenly over its pieces.
+// S^T = K Q^T and O^T += V^T P^T on 32x32x16 f16 MFMAs, 32 rows a wave.  Quantised tiles
+// become f16 on the way: K and V as (f16)(q d); Q and P are rounded to f16, everything else
+// is fp32.  Key order: score row i of a half tile is key i with bits 2 and 3 swapped, so that
+// a lane's scores are 8 consecutive keys of each 16, what the P V operand wants.
+//   narrow units (quantised windows of few rows): workgroups of 4 waves, two a CU.
+//     Each wave takes every fourth of the piece's tiles.  Nothing is shared in the loop and no
+//     barrier is in it: tiles go from memory into registers (the tile layout is the matrix
+//     operands') and are converted there; the waves' sums meet in LDS at the end.
+//   wide units: workgroups of 8 waves, one a CU.  Waves 0 - 3 have 32 rows each and take every
+//     key; waves 4 - 7 bring the next tile into one of two LDS buffers, converted, while the
+//     other is worked on.
+// The tiles of all units of a kind are dealt to the workgroups in equal shares, in an order
+// that steps through a window in strides: a part-filled window's live tiles are spread
+// evenly over its pieces.
 #include "kvm_f16_dev.h"
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -46,61 +49,80 @@ struct fs_seg {
     uint32_t row0, n_rows;       // rows [row0, row0 + n_rows) of every kv head
 };
 
+// The tiles [base, base + ..) of a kind's units, dealt to p workgroups: each has q, the first
+// r one more.
+struct fs_deal {
+    uint32_t base, p, q, r;
+    // workgroup i has the tiles from here to the next's
+    __host__ __device__ uint32_t first(uint32_t i) const { return base + i * q + (i < r ? i : r); }
+    // the workgroup that has tile x
+    __host__ __device__ uint32_t owner(uint32_t x) const {
+        x -= base;
+        return x < r * (q + 1) ? x / (q + 1) : r + (x - r * (q + 1)) / q;
+    }
+};
+
 struct fs_args {
     const void *q;
     const int32_t *q_pos;
     void *out;
-    float *ws_o;                 // pieces [slot][dim / 8][lane][4]
+    float *ws_o;                 // pieces of 32 rows: [slot][dim / 8][lane][4]
     float *ws_ml;                // [slot][row][2]: scaled maximum, sum
     uint32_t H, G, n_head, n_rows;
-    uint32_t n_seg, log_p;       // workgroups: 1 << log_p
+    uint32_t n_seg, n_wide;      // segments, the wide ones before the narrow ones
+    fs_deal wide, narrow;
     float c, q_sign;             // |scale| log2(e); q times -1 for a negative scale, and 0 (c = 1) for none
     int q_type, out_type;
     uint32_t has_prefix;         // segment 0 is the prefix
     uint32_t tile0[FS_SEGS + 1]; // tiles of the units of the segments before
-    uint32_t unit0[FS_SEGS];     // units before
+    uint32_t slot0[FS_SEGS];     // unit u's piece of workgroup p: slots slot0 + (p + u) groups .. (mod 2^32)
     uint32_t lane0[FS_LANES];    // first row of the conversations' segments, the rest ~0
+    uint8_t lane_seg[FS_LANES];  // and their segments
     fs_seg seg[FS_SEGS];
 };
 static_assert(sizeof(fs_args) <= 4096, "kernel arguments");
 
-__host__ __device__ inline uint32_t fs_row_tiles(uint32_t n_rows) { return (n_rows + 31) / 32; }
-// Workgroup p has tiles [fs_share(p), fs_share(p + 1)) of the units' after each other.
-__host__ __device__ inline uint32_t fs_share(uint32_t tiles, uint32_t log_p, uint32_t p) { return (uint32_t)((uint64_t)p * tiles >> log_p); }
-// The workgroup whose share holds tile x.
-__host__ __device__ inline uint32_t fs_owner(uint32_t tiles, uint32_t log_p, uint32_t x) {
-    const uint32_t n = 1u << log_p;
-    uint32_t p = (uint32_t)((float)x * ((float)n / (float)tiles));
-    p = p < n ? p : n - 1;
-    while (p > 0 && fs_share(tiles, log_p, p) > x) --p;
-    while (p + 1 < n && fs_share(tiles, log_p, p + 1) <= x) ++p;
-    return p;
-}
-
-// Workgroups of a CU: the f16 tiles of 256 dims take the registers of two waves.
-__host__ __device__ constexpr uint32_t fs_resident(uint32_t D, bool quant) { return D == 256 && !quant ? 1 : 2; }
+__host__ __device__ inline uint32_t fs_unit_rows(bool wide) { return wide ? 128u : 32u; }
+__host__ __device__ inline uint32_t fs_row_tiles(bool wide, uint32_t n_rows) { return (n_rows + fs_unit_rows(wide) - 1) / fs_unit_rows(wide); }
 
 template <int D, bool QUANT>
 struct fs_geo {
     static constexpr int KS = D / 16, NB = D / 32, DT = D / 32;              // k-steps, 32-dim blocks, dim tiles
-    static constexpr int DW = DT / 4;                     // dim tiles that a wave adds up at the end
     static constexpr uint32_t KB = QUANT ? 64u * D + 128u * NB : 128u * D, VB = QUANT ? 32u * D + 128u * NB : 128u * D;
-    static constexpr int KH = QUANT ? NB : 2 * NB;        // 16-byte loads of a half tile's K
-    static constexpr int SETS = D == 256 ? 1 : 2;                  // half tiles of K (and f16 V) in registers
+    static constexpr uint32_t TB = 128u * D;              // bytes of an f16 K (or V) tile
     static constexpr uint32_t QU = 528;                   // LDS bytes of a unit of Q: 8 dims of 32 rows, 16 bytes apart in the banks
+    static constexpr int NQ = D / 32;                     // quads that a wave adds up at the end of a narrow piece
 };
 
-template <int D, bool QUANT>
-struct fs_lds {
-    using G = fs_geo<D, QUANT>;
-    alignas(16) uint8_t q[2 * G::KS * G::QU];
-    alignas(16) uint8_t sc[4][2][QUANT ? 2 : 1][QUANT ? 1024 : 16];           // a wave's tile and its next: K scales, V scales
-    alignas(16) int32_t cp[4][2][64];                     // and their cells' positions
-    alignas(16) float x[4][G::DW * 4 * 256];              // chunks of O on their way
-    float ml[4][2][32];
-    uint32_t odd[4][2];
+// What both kinds have in LDS; NW: waves.
+template <int D, int NW>
+struct fs_list {
+    alignas(16) float odd_v[4][D];
+    uint32_t odd;                // the batch has values that are no finite numbers where not all rows see them
     uint32_t list[FS_BATCH];
     uint8_t flag[FS_BATCH];
+};
+template <int D>
+struct fs_lds_narrow : fs_list<D, 4> {
+    using G = fs_geo<D, true>;
+    union {
+        struct {                                          // a wave's tile and its next
+            alignas(16) uint8_t q[2 * G::KS * G::QU];
+            alignas(16) uint8_t sc[4][2][2][1024];        // K scales, V scales
+            alignas(16) int32_t cp[4][2][64];             // and the cells' positions
+        };
+        alignas(16) float x[4][2][G::NQ * 256];           // at the end: chunks of O on their way
+    };
+    float ml[4][2][32];
+};
+template <int D, bool QUANT>
+struct fs_lds_wide : fs_list<D, 8> {
+    using G = fs_geo<D, QUANT>;
+    union {
+        alignas(16) uint8_t q4[4][2 * G::KS * G::QU];     // at the start: the four waves' rows
+        alignas(16) uint8_t ring[2][2 * G::TB];           // K, V tile; V in units of 8 keys of a dim: [32-key half][16-dim tile][8-key group][dim]
+    };
+    alignas(16) int32_t cp[2][64];
 };
 
 // x, from which the compiler cannot tell that a value formed of it does not change in a
@@ -115,44 +137,206 @@ __device__ __forceinline__ uint32_t fs_key(uint32_t i) { return (i & 0x13) | (i 
 // Nothing moves over it.
 #define FS_FENCE() __builtin_amdgcn_sched_barrier(0)
 
-// A piece: tiles [i_lo, i_hi) in the unit's order.
+// Q rows [row_g, row_g + rows) of head h, RG groups of 32: loaded, then as f16 operands into
+// LDS (rows past the last: zeros).  8 rows x 8 units of 8 dims an instruction.
+template <int D, int RG, int NW>
+struct fs_rows {
+    static constexpr uint32_t KS = D / 16, QU = 528;
+    static constexpr int N = 32 * RG * 2 * KS / (64 * NW);
+    kvm_u32x4 y[N][2];
+    __device__ __forceinline__ void load(const fs_args &a, uint32_t h, uint32_t row_g, uint32_t rows) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t x = threadIdx.x + 64 * NW * i, b = x >> 6, r = b % (4 * RG) * 8 + (x & 63u) / 8, u = b / (4 * RG) * 8 + (x & 7u);
+            const uint32_t row = row_g + (r < rows ? r : 0u), t = row / a.G;
+            const uint64_t e = ((uint64_t)t * a.n_head + h * a.G + (row - t * a.G)) * D + 8 * u;
+            if (a.q_type == KVM_TYPE_F32) __builtin_memcpy(y[i], (const float *)a.q + e, 32);
+            else __builtin_memcpy(y[i], (const uint16_t *)a.q + e, 16);
+        }
+    }
+    __device__ __forceinline__ void store(const fs_args &a, uint32_t rows, uint8_t *dst) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t x = threadIdx.x + 64 * NW * i, b = x >> 6, r = b % (4 * RG) * 8 + (x & 63u) / 8, u = b / (4 * RG) * 8 + (x & 7u);
+            kvm_f16x8 o;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t v = a.q_type == KVM_TYPE_F32 ? y[i][j >> 2][j & 3] : j & 1 ? y[i][0][j >> 1] & 0xffff0000u : y[i][0][j >> 1] << 16;
+                o[j] = r < rows ? (_Float16)(__uint_as_float(v) * a.q_sign) : (_Float16)0.0f;
+            }
+            *(kvm_f16x8 *)(dst + (r >> 5) * (2 * KS * QU) + u * QU + (r & 31u) * 16) = o;
+        }
+    }
+};
+
+// A row's limit: it sees the cells with (unsigned)position below it.
+__device__ __forceinline__ uint32_t fs_limit(const fs_args &a, uint32_t row_g, uint32_t rows, uint32_t r) {
+    const int32_t qp = r < rows ? a.q_pos[(row_g + r) / a.G] : -1;
+    return qp >= 0 ? (uint32_t)qp + 1u : 0u;
+}
+
+// Tile i of a unit's order.
+__device__ __forceinline__ uint32_t fs_tile(const fs_seg &sg, uint32_t i) { return i * sg.mult % sg.n_tiles; }      // (n_tiles < 2^16)
+
+// Positions of the cells of tiles b0 + r0 .. of nb in the unit's order: 4 tiles a wave and load.
+template <int NW>
+struct fs_cells {
+    kvm_u32x4 c[4];
+    __device__ __forceinline__ static uint32_t at(uint32_t r0, int r) { return r0 + 4 * NW * r + 4 * (threadIdx.x >> 6) + ((threadIdx.x & 63u) >> 4); }
+    __device__ __forceinline__ void load(const fs_seg &sg, uint32_t b0, uint32_t nb, uint32_t r0) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t i = at(r0, r);
+            c[r] = *(const kvm_u32x4 *)(sg.cell_pos + (uint64_t)fs_tile(sg, b0 + (i < nb ? i : 0u)) * 64 + 4 * (threadIdx.x & 15u));
+        }
+    }
+};
+
+// The tiles b0 .. b0 + nb - 1 in the unit's order that some row sees, in sm.list (bit 31: every
+// cell is visible to every row); returns how many.  Every wave takes part; two barriers.
+// cells: loaded for r0 = 0.
+template <int D, int NW>
+__device__ __forceinline__ uint32_t fs_tiles(const fs_seg &sg, fs_list<D, NW> &sm, uint32_t b0, uint32_t nb, uint32_t some_lim,
+                                             uint32_t all_lim, fs_cells<NW> &cells) {
+    const uint32_t l = fs_opaque(threadIdx.x & 63u), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (uint32_t r0 = 0;;) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t i = cells.at(r0, r);
+            const kvm_u32x4 c = cells.c[r];
+            const uint32_t least = min(min(c[0], c[1]), min(c[2], c[3])), most = max(max(c[0], c[1]), max(c[2], c[3]));
+            const uint32_t some = (uint32_t)(__builtin_amdgcn_ballot_w64(least < some_lim) >> (l & 48)) & 0xffffu;
+            const uint32_t all = (uint32_t)(__builtin_amdgcn_ballot_w64(most < all_lim) >> (l & 48)) & 0xffffu;
+            if (i < nb && (l & 15) == 0) sm.flag[i] = (uint8_t)((some != 0) | (all == 0xffffu) << 1);
+        }
+        r0 += 16 * NW;
+        if (r0 >= nb) break;
+        cells.load(sg, b0, nb, r0);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) sm.odd = 0;
+    uint32_t n_t = 0;
+#pragma unroll
+    for (uint32_t x = 0; x < FS_BATCH / 64; ++x) {
+        const uint32_t f = 64 * x + l < nb ? sm.flag[64 * x + l] : 0u;
+        const uint64_t bal = __builtin_amdgcn_ballot_w64(f & 1u);
+        const uint32_t rank = n_t + __builtin_amdgcn_mbcnt_hi((uint32_t)(bal >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bal, 0u));
+        if ((f & 1u) && x == w) sm.list[rank] = fs_tile(sg, b0 + 64 * x + l) | (f >> 1) << 31;
+        n_t += __popcll(bal);
+    }
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(n_t);
+}
+
+// The scores of a half tile that its cells' positions mask.
+__device__ __forceinline__ void fs_mask(kvm_f32x16 &S, const int32_t *cp, uint32_t qlim) {
+    asm volatile("" ::: "memory");                        // keep it on the (rare) masked path
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const kvm_u32x4 x = *(const kvm_u32x4 *)(cp + 16 * (i >> 1) + 8 * (fs_opaque(threadIdx.x & 63u) >> 5) + 4 * (i & 1));
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (!(x[r] < qlim)) S[4 * i + r] = -INFINITY;
+    }
+}
+
+// Halves of v (values, or scales of values) whose keys, base .. base + 7, no row sees become
+// 0, and so do those that are no finite numbers where not all rows see the key (0 times them
+// would not be 0): whether there are such.
+__device__ __forceinline__ bool fs_clear(kvm_u32x4 &v, uint32_t base, uint64_t seen, uint64_t part) {
+    const uint32_t on = (uint32_t)(seen >> base) & 0xffu, pt = (uint32_t)(part >> base) & 0xffu;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t sh = 16 * (i & 1), x = v[i >> 1] >> sh & 0xffffu;
+        const bool no = (pt >> i & 1u) && (x & 0x7c00u) == 0x7c00u;
+        odd |= no;
+        if (!(on >> i & 1u) || no) v[i >> 1] &= ~(0xffffu << sh);
+    }
+    return odd;
+}
+
+// What fs_clear took out of the list's tiles j0, j0 + step, ..: values that are no finite
+// numbers are added to the rows that see them (a positive p times one is itself).  sx: the
+// wave's own.
 template <int D, bool QUANT>
-__device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_lds<D, QUANT> &sm, uint32_t rt, uint32_t h, uint32_t slot,
-                                         uint32_t i_lo, uint32_t i_hi) {
-    using G = fs_geo<D, QUANT>;
-    constexpr int KS = G::KS, NB = G::NB, DT = G::DT, DW = G::DW, KH = G::KH, SETS = G::SETS;
+__device__ __forceinline__ void fs_add_odd(kvm_f32x16 (&O)[D / 32], const fs_seg &sg, const uint8_t *v_head, const uint32_t *list, uint32_t j0,
+                                           uint32_t step, uint32_t n_t, uint32_t some_lim, uint32_t all_lim, uint32_t qlim, float *sx) {
+    const uint32_t l = threadIdx.x & 63u;
+    for (uint32_t j = j0; j < n_t; j += step) {
+        const uint32_t e = list[j], t = e & 0x7fffffffu;
+        if (e >> 31) continue;
+        const uint8_t *v_tile = v_head + (uint64_t)t * fs_geo<D, QUANT>::VB;
+        for (uint32_t k = 0; k < 64; ++k) {
+            const uint32_t cp = (uint32_t)sg.cell_pos[(uint64_t)t * 64 + k];
+            if (!(cp < some_lim) || cp < all_lim) continue;
+            bool any = false;
+            for (uint32_t d = l; d < D; d += 64) {
+                bool bad;
+                float v;
+                if constexpr (QUANT) {
+                    const float sc = kvm_h2f(*(const uint16_t *)(v_tile + kvm_vd_off(D, k, d / 32)));
+                    bad = !(sc - sc == 0.0f);
+                    v = (float)((int)(v_tile[kvm_vq_byte(k, d)] >> kvm_vq_shift(k) & 15u) - 8) * sc;
+                } else {
+                    v = kvm_h2f(((const uint16_t *)v_tile)[kvm_vh_idx(k, d)]);
+                    bad = !(v - v == 0.0f);
+                }
+                sx[d] = bad ? v : 0.0f;
+                any |= bad;
+            }
+            if (__builtin_amdgcn_ballot_w64(any) == 0) continue;
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const kvm_f32x4 v = *(const kvm_f32x4 *)(sx + 32 * dt + 8 * x + 4 * (l >> 5));
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) O[dt][4 * x + r] += cp < qlim ? v[r] : 0.0f;
+                }
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+}
+
+// Direct copies to LDS (lane l writes 16 or 4 bytes at M0 + 16 l or 4 l), issued from asm, so
+// that the compiler adds no wait for them; the asm restores M0, which the compiler reserves.
+// Whoever reads waits by vmcnt first.
+__device__ __forceinline__ void fs_copy16(const uint8_t *src, uint32_t off, void *dst) {
+    uint32_t m0_saved;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0_saved) : "v"(off), "s"((uint32_t)(uintptr_t)(fs_lds_ptr)dst), "s"(src) : "memory");
+}
+__device__ __forceinline__ void fs_copy4(const int32_t *src, uint32_t off, void *dst) {
+    uint32_t m0_saved;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0_saved) : "v"(off), "s"((uint32_t)(uintptr_t)(fs_lds_ptr)dst), "s"(src) : "memory");
+}
+
+// A piece of a narrow unit (32 rows over a quantised window): tiles [i_lo, i_hi) in the
+// unit's order.  What bounds it: instruction issue (a tile's conversion is ~900 of a wave's
+// ~1,700 instructions), or the memory where no two units read the same tiles.
+template <int D>
+__device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs_lds_narrow<D> &sm, uint32_t rt, uint32_t h, uint32_t slot,
+                                          uint32_t i_lo, uint32_t i_hi) {
+    using G = fs_geo<D, true>;
+    constexpr int KS = G::KS, NB = G::NB, DT = G::DT, NQ = G::NQ;
+    constexpr int SETS = D == 256 ? 1 : 2;                // half tiles of K in registers
     constexpr uint32_t KB = G::KB, VB = G::VB, QU = G::QU;
-    const uint32_t tid = threadIdx.x, l = tid & 63u, g2 = l >> 5, m2 = l & 31u;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t l = fs_opaque(threadIdx.x & 63u), g2 = l >> 5, m2 = l & 31u;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t rows = min(32u, sg.n_rows - 32 * rt), row_g = sg.row0 + 32 * rt;
 
-    // ---- the rows: Q as f16 operands in LDS, the rows' limits
-    for (uint32_t x = tid; x < 32u * 2 * KS; x += 256) {
-        // 8 rows x 8 units an instruction
-        const uint32_t b = x >> 6, r = b % 4 * 8 + (x & 63u) / 8, u = b / 4 * 8 + (x & 7u);
-        float v[8];
-        if (r < rows) {
-            const uint32_t t = (row_g + r) / a.G;
-            const uint64_t e = ((uint64_t)t * a.n_head + h * a.G + (row_g + r - t * a.G)) * D + 8 * u;
-            if (a.q_type == KVM_TYPE_F32) {
-                __builtin_memcpy(v, (const float *)a.q + e, 32);
-            } else {
-                kvm_u32x4 y;
-                __builtin_memcpy(&y, (const uint16_t *)a.q + e, 16);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(j & 1 ? y[j >> 1] & 0xffff0000u : y[j >> 1] << 16);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-        }
-        kvm_f16x8 o;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = (_Float16)(v[j] * a.q_sign);
-        *(kvm_f16x8 *)(sm.q + u * QU + r * 16) = o;
+    // the loads of the start, all issued before any is used
+    fs_cells<4> cells;
+    cells.load(sg, i_lo, min(FS_BATCH, i_hi - i_lo), 0);
+    const uint32_t qlim = fs_limit(a, row_g, rows, m2);
+    {
+        fs_rows<D, 1, 4> q;
+        q.load(a, h, row_g, rows);
+        q.store(a, rows, sm.q);
     }
-    const int32_t qp = m2 < rows ? a.q_pos[(row_g + m2) / a.G] : -1;
-    const uint32_t qlim = qp >= 0 ? (uint32_t)qp + 1u : 0u;      // a cell is visible iff (unsigned)position < qlim
     const uint32_t all_lim = kvm_wave_min_u32(m2 < rows ? qlim : 0xffffffffu), some_lim = ~kvm_wave_min_u32(~qlim);
 
     kvm_f32x16 O[DT];
@@ -164,89 +348,37 @@ __device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_
 
     // operand addresses of a lane
     const uint32_t key = fs_key(m2);
-    const uint32_t k_lane = ((key >> 4) * (QUANT ? NB / 2 : NB) * 64 + 16 * g2 + (key & 15)) * 16;
-    const uint32_t v_lane = ((m2 >> 4) * 64 + 16 * g2 + (m2 & 15)) * (QUANT ? 8 : 32);
+    const uint32_t k_lane = ((key >> 4) * (NB / 2) * 64 + 16 * g2 + (key & 15)) * 16, v_lane = ((m2 >> 4) * 64 + 16 * g2 + (m2 & 15)) * 8;
     const uint8_t *const k_head = sg.k + (uint64_t)h * sg.n_tiles * KB, *const v_head = sg.v + (uint64_t)h * sg.n_tiles * VB;
 
     for (uint32_t b0 = i_lo; b0 < i_hi; b0 += FS_BATCH) {
-        // ---- the batch's tiles that some row sees; bit 31: every cell visible to every row
-        const uint32_t nb = min(FS_BATCH, i_hi - b0);
-        auto tile_of = [&](uint32_t i) { return (b0 + i) * sg.mult % sg.n_tiles; };     // (n_tiles < 2^16)
-        for (uint32_t r0 = 0; r0 < nb; r0 += 64) {
-            kvm_u32x4 c[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint32_t i = r0 + 16 * r + 4 * w + (l >> 4);
-                c[r] = *(const kvm_u32x4 *)(sg.cell_pos + (uint64_t)tile_of(i < nb ? i : 0u) * 64 + 4 * (l & 15));
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint32_t i = r0 + 16 * r + 4 * w + (l >> 4);
-                const uint32_t least = min(min(c[r][0], c[r][1]), min(c[r][2], c[r][3])), most = max(max(c[r][0], c[r][1]), max(c[r][2], c[r][3]));
-                const uint32_t some = (uint32_t)(__builtin_amdgcn_ballot_w64(least < some_lim) >> (l & 48)) & 0xffffu;
-                const uint32_t all = (uint32_t)(__builtin_amdgcn_ballot_w64(most < all_lim) >> (l & 48)) & 0xffffu;
-                if (i < nb && (l & 15) == 0) sm.flag[i] = (uint8_t)((some != 0) | (all == 0xffffu) << 1);
-            }
-        }
-        __syncthreads();                                  // flags, and Q
-        uint32_t n_t = 0;
-#pragma unroll
-        for (uint32_t x = 0; x < FS_BATCH / 64; ++x) {
-            const uint32_t f = 64 * x + l < nb ? sm.flag[64 * x + l] : 0u;
-            const uint64_t bal = __builtin_amdgcn_ballot_w64(f & 1u);
-            const uint32_t rank = n_t + __builtin_amdgcn_mbcnt_hi((uint32_t)(bal >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bal, 0u));
-            if ((f & 1u) && (int)x == w) sm.list[rank] = tile_of(64 * x + l) | (f >> 1) << 31;
-            n_t += __popcll(bal);
-        }
-        n_t = __builtin_amdgcn_readfirstlane(n_t);
-        __syncthreads();
+        if (b0 != i_lo) cells.load(sg, b0, min(FS_BATCH, i_hi - b0), 0);
+        const uint32_t n_t = fs_tiles<D, 4>(sg, sm, b0, min(FS_BATCH, i_hi - b0), some_lim, all_lim, cells);      // (its barriers: Q, too)
 
-        // ---- the wave's tiles: list entries w, w + 4, ..  Registers of a half tile are
-        // loaded for the next tile where this one's are used up.
-        kvm_u32x4 kr[SETS][KH], vh[QUANT ? 1 : SETS][QUANT ? 1 : 2 * DT];
-        uint32_t vq[QUANT ? 2 * DT : 1];                  // quantised V of a half tile
-        // (past the wave's last tile the bounds let nothing through)
-        auto rsrc = [&](const void *head, uint32_t e, uint32_t bytes, bool more) {
-            return __builtin_amdgcn_make_buffer_rsrc((void *)((const uint8_t *)head + (uint64_t)(e & 0x7fffffffu) * bytes), (short)0, more ? bytes : 0u, 0x00020000);
+        // The wave's tiles: list entries w, w + 4, ..  Registers of a half tile are loaded for
+        // the next where this one's are used up; past the wave's last tile the bounds let
+        // nothing through.
+        kvm_u32x4 kr[SETS][NB];
+        uint32_t vq[2 * DT];
+        auto rsrc = [&](const uint8_t *head, uint32_t e, uint32_t bytes, bool more) {
+            return __builtin_amdgcn_make_buffer_rsrc((void *)(head + (uint64_t)(e & 0x7fffffffu) * bytes), (short)0, more ? bytes : 0u, 0x00020000);
         };
         auto load_k = [&](__amdgpu_buffer_rsrc_t r, int half) {
+            const uint32_t at = fs_opaque(k_lane);
 #pragma unroll
-            for (int i = 0; i < KH; ++i)
-                kr[half % SETS][i] = __builtin_amdgcn_raw_buffer_load_b128(r, k_lane + (i & 1) * 512, half * (QUANT ? NB : 2 * NB) * 1024 + (i >> 1) * 1024, 0);
+            for (int i = 0; i < NB; ++i)
+                kr[half % SETS][i] = __builtin_amdgcn_raw_buffer_load_b128(r, at + (i & 1) * 512, half * NB * 1024 + (i >> 1) * 1024, 0);
         };
         auto load_v = [&](__amdgpu_buffer_rsrc_t r, int half) {
+            const uint32_t at = fs_opaque(v_lane);
 #pragma unroll
-            for (int i = 0; i < 2 * DT; ++i) {
-                if constexpr (QUANT) vq[i] = __builtin_amdgcn_raw_buffer_load_b32(r, v_lane + (i & 1) * 256 + half * 4, (i >> 1) * 1024, 0);
-                else vh[half % SETS][i] = __builtin_amdgcn_raw_buffer_load_b128(r, v_lane + (i & 1) * 1024 + half * 16, (i >> 1) * 4096, 0);
-            }
-        };
-        // Scales and positions go to LDS by direct copies (lane l writes 16 or 4 bytes at M0 +
-        // 16 l or 4 l), issued from asm, so that the compiler adds no wait for them; the asm
-        // restores M0, which the compiler reserves.
-        auto copy16 = [&](const uint8_t *src, void *dst) {
-            const uint32_t off = 16u * (fs_opaque(l) & (D == 256 ? 63u : 31u));   // (128 dims: 512 bytes of scales)
-            uint32_t m0_saved;
-            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
-                         : "=&s"(m0_saved) : "v"(off), "s"((uint32_t)(uintptr_t)(fs_lds_ptr)dst), "s"(src) : "memory");
+            for (int i = 0; i < 2 * DT; ++i) vq[i] = __builtin_amdgcn_raw_buffer_load_b32(r, at + (i & 1) * 256 + half * 4, (i >> 1) * 1024, 0);
         };
         auto copies = [&](uint32_t e, uint32_t buf) {
-            const uint32_t t = e & 0x7fffffffu;
-            if constexpr (QUANT) {
-                copy16(k_head + (uint64_t)t * KB + 64 * D, sm.sc[w][buf][0]);
-                copy16(v_head + (uint64_t)t * VB + 32 * D, sm.sc[w][buf][1]);
-            }
-            uint32_t m0_saved;
-            asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, %3\n\ts_mov_b32 m0, %0"
-                         : "=&s"(m0_saved) : "v"(4u * fs_opaque(l)), "s"((uint32_t)(uintptr_t)(fs_lds_ptr)&sm.cp[w][buf][0]), "s"(sg.cell_pos + (uint64_t)t * 64) : "memory");
-        };
-        // keys base .. base + 7 of the lanes' bits, together
-        auto gather = [&](uint32_t base, uint32_t bits) {
-            if (l < 2) sm.odd[w][l] = 0;
-            __builtin_amdgcn_wave_barrier();
-            if (bits) atomicOr(&sm.odd[w][base >> 5], bits << (base & 31u));
-            __builtin_amdgcn_wave_barrier();
-            return (uint64_t)__builtin_amdgcn_readfirstlane(sm.odd[w][1]) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane(sm.odd[w][0]);
+            const uint32_t t = e & 0x7fffffffu, off = 16u * (fs_opaque(l) & (D == 256 ? 63u : 31u));     // (128 dims: 512 bytes of scales)
+            fs_copy16(k_head + (uint64_t)t * KB + 64 * D, off, sm.sc[w][buf][0]);
+            fs_copy16(v_head + (uint64_t)t * VB + 32 * D, off, sm.sc[w][buf][1]);
+            fs_copy4(sg.cell_pos + (uint64_t)t * 64, 4u * fs_opaque(l), &sm.cp[w][buf][0]);
         };
         uint32_t e = 0;
         if ((uint32_t)w < n_t) {
@@ -256,39 +388,25 @@ __device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_
             load_k(rk, 0);
             if (SETS == 2) load_k(rk, 1);
             load_v(rv, 0);
-            if (!QUANT && SETS == 2) load_v(rv, 1);
         }
         uint32_t buf = 0;
         for (uint32_t j = w; j < n_t; j += 4, buf ^= 1) {
             // the tile's copies: the first tile's half tiles, or more, were loaded after them
-            asm volatile("s_waitcnt vmcnt(%0)" : : "n"(SETS * KH + (QUANT ? 1 : SETS) * 2 * DT) : "memory");
+            asm volatile("s_waitcnt vmcnt(%0)" : : "n"(SETS * NB + 2 * DT) : "memory");
             const bool more = j + 4 < n_t;
             const uint32_t en = __builtin_amdgcn_readfirstlane(sm.list[more ? j + 4 : j]);
             const auto rk = rsrc(k_head, en, KB, more), rv = rsrc(v_head, en, VB, more);
             const bool full = e >> 31;
-            // keys that some row sees; those of them that not all do and whose value is no
-            // finite number
-            uint64_t seen = ~0ull, part = 0, odd = 0;
             if (!full) {
                 asm volatile("" ::: "memory");            // keep it on this (rare) path
-                const uint32_t cp = (uint32_t)sm.cp[w][buf][fs_opaque(l)];
-                seen = __builtin_amdgcn_ballot_w64(cp < some_lim);
-                part = seen & ~__builtin_amdgcn_ballot_w64(cp < all_lim);
-                if constexpr (QUANT) {
-                    // What no row sees counts nothing, whatever it holds: a scale of 0.  (Lane
-                    // l has the scales of 8 keys of a block.)
-                    const uint32_t lo = fs_opaque(l), base = 32 * (lo >> 2 & 1u) + 8 * (lo & 3u), on = (uint32_t)(seen >> base) & 0xffu, pt = (uint32_t)(part >> base) & 0xffu;
-                    kvm_u32x4 scv = *(const kvm_u32x4 *)(sm.sc[w][buf][1] + 16 * lo);
-                    uint32_t bad = 0;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint32_t sh = 16 * (i & 1), v = scv[i >> 1] >> sh & 0xffffu;
-                        if (lo < 8u * NB && (pt >> i & 1u) && (v & 0x7c00u) == 0x7c00u) bad |= 1u << i;
-                        if (!(on >> i & 1u) || (bad >> i & 1u)) scv[i >> 1] &= ~(0xffffu << sh);
-                    }
-                    *(kvm_u32x4 *)(sm.sc[w][buf][1] + 16 * lo) = scv;
-                    if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) odd = gather(base, bad);
-                }
+                const uint32_t lo = fs_opaque(l), cp = (uint32_t)sm.cp[w][buf][lo];
+                const uint64_t seen = __builtin_amdgcn_ballot_w64(cp < some_lim), part = seen & ~__builtin_amdgcn_ballot_w64(cp < all_lim);
+                // lane l has the scales of 8 keys of a block
+                const uint32_t base = 32 * (lo >> 2 & 1u) + 8 * (lo & 3u);
+                kvm_u32x4 scv = *(const kvm_u32x4 *)(sm.sc[w][buf][1] + 16 * lo);
+                const bool odd = fs_clear(scv, base, seen, part);
+                *(kvm_u32x4 *)(sm.sc[w][buf][1] + 16 * lo) = scv;
+                if (odd && lo < 8u * NB) sm.odd = 1;
             }
             if (more) copies(en, buf ^ 1);
 
@@ -300,23 +418,19 @@ __device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_
 #pragma unroll
                 for (int r = 0; r < 16; ++r) S[r] = 0.0f;
                 uint32_t ksc[NB];                         // the scales of the lane's key
-                if constexpr (QUANT) {
+                {
                     const uint32_t k = fs_key(fs_opaque(l) & 31u);
 #pragma unroll
                     for (int b = 0; b < NB; ++b) ksc[b] = *(const uint16_t *)(sm.sc[w][buf][0] + ((2 * half + (k >> 4)) * NB + b) * 32 + 2 * (k & 15));
                 }
-                const uint8_t *const sq = sm.q + g2 * QU + m2 * 16;
+                const uint32_t lq = fs_opaque(l);
+                const uint8_t *const sq = sm.q + (lq >> 5) * QU + (lq & 31u) * 16;
                 // operands in the order of the K loads: (block pair, 16-dim half | block of the pair)
-                auto ks_of = [](int i) { return QUANT ? 4 * (i >> 2) + 2 * (i & 1) + (i >> 1 & 1) : i; };
                 auto k_op = [&](int i) {
-                    if constexpr (QUANT) {
-                        const kvm_u32x4 x = kr[half % SETS][i >> 1];
-                        return pf_q8(x[2 * (i & 1)], x[2 * (i & 1) + 1], ksc[2 * (i >> 2) + (i & 1)]);
-                    } else {
-                        return __builtin_bit_cast(kvm_f16x8, kr[half % SETS][i]);
-                    }
+                    const kvm_u32x4 x = kr[half % SETS][i >> 1];
+                    return pf_q8(x[2 * (i & 1)], x[2 * (i & 1) + 1], ksc[2 * (i >> 2) + (i & 1)]);
                 };
-                auto q_op = [&](int i) { return *(const kvm_f16x8 *)(sq + 2 * ks_of(i) * QU); };
+                auto q_op = [&](int i) { return *(const kvm_f16x8 *)(sq + 2 * (4 * (i >> 2) + 2 * (i & 1) + (i >> 1 & 1)) * QU); };
                 kvm_f16x8 kop = k_op(0), qr[3] = {q_op(0), q_op(1)};
 #pragma unroll
                 for (int i = 0; i < KS; ++i) {
@@ -331,16 +445,7 @@ __device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_
                 else load_k(rk, 0);
 
                 // ---- softmax: P as f16 operands
-                if (!full) {
-                    asm volatile("" ::: "memory");
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const kvm_u32x4 x = *(const kvm_u32x4 *)(&sm.cp[w][buf][32 * half + 16 * (i >> 1) + 8 * (fs_opaque(l) >> 5) + 4 * (i & 1)]);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (!(x[r] < qlim)) S[4 * i + r] = -INFINITY;
-                    }
-                }
+                if (!full) fs_mask(S, &sm.cp[w][buf][32 * half], qlim);
                 float x = S[0];
 #pragma unroll
                 for (int r = 1; r < 16; ++r) x = fmaxf(x, S[r]);
@@ -368,129 +473,72 @@ __device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_
                 lp += sum;
 
                 // ---- O^T += V^T P^T
-                if constexpr (!QUANT) {
-                    if (!full) {
-                        // values of keys that no row sees become 0
-                        asm volatile("" ::: "memory");
-                        uint32_t bad[2] = {0, 0};
-#pragma unroll
-                        for (int i = 0; i < 2 * DT; ++i) {
-                            const uint32_t base = 32 * half + 16 * (i & 1) + 8 * g2;
-                            const uint32_t on = (uint32_t)(seen >> base) & 0xffu, pt = (uint32_t)(part >> base) & 0xffu;
-                            kvm_u32x4 &v = vh[half % SETS][i];
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) {
-                                const uint32_t sh = 16 * (k & 1);
-                                const bool no = (pt >> k & 1u) && (v[k >> 1] >> sh & 0x7c00u) == 0x7c00u;
-                                if (no) bad[i & 1] |= 1u << k;
-                                if (!(on >> k & 1u) || no) v[k >> 1] &= ~(0xffffu << sh);
-                            }
-                        }
-                        if (__builtin_amdgcn_ballot_w64((bad[0] | bad[1]) != 0) != 0)
-                            odd |= gather(32 * half + 8 * g2, bad[0] | bad[1] << 16);
-                    }
-                }
                 kvm_u32x4 vs[3];
-                auto v_scale = [&](int i) {
-                    if constexpr (QUANT) vs[i % 3] = *(const kvm_u32x4 *)(sm.sc[w][buf][1] + (((i >> 1) * 2 + half) * 4 + 2 * (i & 1) + g2) * 16);
-                };
-                auto v_op = [&](int i) {
-                    if constexpr (QUANT) return pf_q4(vq[i], vs[i % 3]);
-                    else return __builtin_bit_cast(kvm_f16x8, vh[half % SETS][i]);
-                };
+                const uint8_t *const sv = sm.sc[w][buf][1] + (fs_opaque(l) >> 5) * 16;
+                auto v_scale = [&](int i) { vs[i % 3] = *(const kvm_u32x4 *)(sv + (((i >> 1) * 2 + half) * 4 + 2 * (i & 1)) * 16); };
                 v_scale(0);
                 v_scale(1);
-                kvm_f16x8 vop = v_op(0);
+                kvm_f16x8 vop = pf_q4(vq[0], vs[0]);
 #pragma unroll
                 for (int i = 0; i < 2 * DT; ++i) {
                     if (i + 2 < 2 * DT) v_scale(i + 2);
                     FS_FENCE();
                     O[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vop, pb[i & 1], O[i >> 1], 0, 0, 0);
-                    if (i + 1 < 2 * DT) vop = v_op(i + 1);
+                    if (i + 1 < 2 * DT) vop = pf_q4(vq[i + 1], vs[(i + 1) % 3]);
                     FS_FENCE();
                 }
-                if ((uint32_t)(odd >> (32 * half)) != 0) {
-                    // A value that is no finite number, at a key that some rows see and others
-                    // do not: 0 times it is not 0.  The product took 0 for it; here it is added
-                    // where p is not 0 (p times it is itself).
-                    asm volatile("" : "+v"(pb[0]), "+v"(pb[1]) : : "memory");     // keep it on this (rare) path
-                    const uint8_t *const v_tile = v_head + (uint64_t)(e & 0x7fffffffu) * VB;
-                    float *const sx = sm.x[w];
-                    for (uint32_t k = 0; k < 32; ++k) {
-                        const uint32_t c = 32 * half + k, lo = fs_opaque(l);
-                        if (!(odd >> c & 1u)) continue;
-                        // the key's values that are not finite, and where its p are not 0
-#pragma unroll
-                        for (uint32_t d = lo; d < D; d += 64) {
-                            float v;
-                            if constexpr (QUANT)
-                                v = (float)((int)(v_tile[kvm_vq_byte(c, d)] >> kvm_vq_shift(c) & 15u) - 8) * kvm_h2f(*(const uint16_t *)(v_tile + kvm_vd_off(D, c, d / 32)));
-                            else v = kvm_h2f(((const uint16_t *)v_tile)[kvm_vh_idx(c, d)]);
-                            sx[d] = v - v == 0.0f ? 0.0f : v;
-                        }
-                        bool has = false;
-#pragma unroll
-                        for (uint32_t r = 0; r < 16; ++r) has |= lo >> 5 == (k >> 3 & 1u) && r == (k >> 4) * 8 + (k & 7u) && !((float)pb[r >> 3][r & 7] == 0.0f);
-                        const uint64_t b = __builtin_amdgcn_ballot_w64(has);
-                        const bool mine = ((uint32_t)b | (uint32_t)(b >> 32)) >> (lo & 31u) & 1u;
-                        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                        for (int x = 0; x < 4 * DT; ++x) {
-                            const kvm_f32x4 v = *(const kvm_f32x4 *)(sx + 8 * x + 4 * (lo >> 5));
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) O[x >> 2][4 * (x & 3) + r] += mine ? v[r] : 0.0f;
-                            FS_FENCE();
-                        }
-                        __builtin_amdgcn_wave_barrier();
-                    }
-                }
-                if (!QUANT && SETS == 2) load_v(rv, half);
-                else if (half == 0) load_v(rsrc(v_head, e, VB, true), 1);
+                if (half == 0) load_v(rsrc(v_head, e, VB, true), 1);
                 else load_v(rv, 0);
             }
             e = en;
         }
-        __syncthreads();                                  // the next batch's flags and list
+        if (__builtin_amdgcn_readfirstlane(sm.odd)) fs_add_odd<D, true>(O, sg, v_head, sm.list, w, 4, n_t, some_lim, all_lim, qlim, sm.odd_v[w]);
     }
 
-    // ---- the waves' sums: one maximum, then chunk by chunk to the wave that adds it up
+    // ---- the waves' sums: one maximum, then each wave's quarter of the dims from the others,
+    // two waves' and the third's
     const float lr = kvm_add_xor32(lp);
     if (g2 == 0) {
         sm.ml[w][0][m2] = ms;
         sm.ml[w][1][m2] = lr;
     }
     __syncthreads();
-    const float M = fmaxf(fmaxf(sm.ml[0][0][m2], sm.ml[1][0][m2]), fmaxf(sm.ml[2][0][m2], sm.ml[3][0][m2]));
-    float L = 0.0f;
+    float M = sm.ml[0][0][m2], L = 0.0f;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) L += sm.ml[x][0][m2] == -INFINITY ? 0.0f : sm.ml[x][1][m2] * __builtin_amdgcn_exp2f(sm.ml[x][0][m2] - M);
-    const float wgt = __builtin_amdgcn_exp2f(ms - M);
+    for (int x = 1; x < 4; ++x) M = fmaxf(M, sm.ml[x][0][m2]);
+    const float top = M == -INFINITY ? 0.0f : M;          // (a wave that saw nothing of the row: weight, sum and O are 0)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) L += sm.ml[x][1][m2] * __builtin_amdgcn_exp2f(sm.ml[x][0][m2] - top);
+    const float wgt = __builtin_amdgcn_exp2f(ms - top);
     // quad i of O: dims 8 i + 4 g2 .. + 3 of the lane's row, weighted
     auto quad = [&](int i) {
         kvm_f32x4 v;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = ms == -INFINITY ? 0.0f : O[i >> 2][4 * (i & 3) + k] * wgt;
+        for (int k = 0; k < 4; ++k) v[k] = O[i >> 2][4 * (i & 3) + k] * wgt;
         return v;
     };
-    constexpr int NQ = DW * 4;                            // quads of a chunk
     kvm_f32x4 acc[NQ];
+    for (int round = 0; round < 2; ++round) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-        if (q == w) {
+        for (int q = 0; q < 4; ++q) {
+            const int k = (q - w) & 3;                    // the (k - 1)-th of the waves that give to q
+            if (k == 0) {
+                if (round == 0) {
 #pragma unroll
-            for (int x = 0; x < NQ; ++x) acc[x] = quad(q * NQ + x);
-        }
-    for (int round = 1; round < 4; ++round) {
-        const int to = (w + round) & 3;
+                    for (int x = 0; x < NQ; ++x) acc[x] = quad(q * NQ + x);
+                }
+            } else if ((k - 1) >> 1 == round) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (q == to) {
-#pragma unroll
-                for (int x = 0; x < NQ; ++x) *(kvm_f32x4 *)(sm.x[q] + 256 * x + 4 * l) = quad(q * NQ + x);
+                for (int x = 0; x < NQ; ++x) *(kvm_f32x4 *)(sm.x[q][(k - 1) & 1] + 256 * x + 4 * l) = quad(q * NQ + x);
             }
+        }
         __syncthreads();
 #pragma unroll
-        for (int x = 0; x < NQ; ++x) acc[x] += *(const kvm_f32x4 *)(sm.x[w] + 256 * x + 4 * l);
+        for (int k = 0; k < 2; ++k) {
+            if (round == 1 && k == 1) break;
+#pragma unroll
+            for (int x = 0; x < NQ; ++x) acc[x] += *(const kvm_f32x4 *)(sm.x[w][k] + 256 * x + 4 * l);
+        }
         __syncthreads();
     }
 #pragma unroll
@@ -502,85 +550,418 @@ __device__ __forceinline__ void fs_piece(const fs_args &a, const fs_seg &sg, fs_
     }
 }
 
+// x stays where it is: nothing moves over it, the MFMA that wrote it included.
+#define FS_PIN(x)                                    \
+    do {                                             \
+        asm volatile("" : "+v"(x) : : "memory");     \
+        FS_FENCE();                                  \
+    } while (0)
+
+// A piece of a wide unit.  What bounds it: the attention waves' chain, one a SIMD (of a tile
+// of 256 dims, 2,048 cycles on the matrix cores); over an f16 window the memory where no two
+// units read the same tiles.
 template <int D, bool QUANT>
-__global__ void __launch_bounds__(256, fs_resident(D, QUANT)) k_fs_attn(fs_args a) {
-    __shared__ fs_lds<D, QUANT> sm;
-    const uint32_t tid = threadIdx.x, l = tid & 63u;
+__device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg, fs_lds_wide<D, QUANT> &sm, uint32_t rt, uint32_t h,
+                                              uint32_t slot, uint32_t i_lo, uint32_t i_hi) {
+    using G = fs_geo<D, QUANT>;
+    constexpr int KS = G::KS, NB = G::NB, DT = G::DT;     // (2 DT = KS)
+    constexpr uint32_t KB = G::KB, VB = G::VB, TB = G::TB, QU = G::QU;
+    const uint32_t l = fs_opaque(threadIdx.x & 63u);
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = w & 3;
+    const uint32_t rows = min(128u, sg.n_rows - 128 * rt), row_g = sg.row0 + 128 * rt;
+
+    // the loads of the start, all issued before any is used
+    fs_cells<8> cells;
+    cells.load(sg, i_lo, min(FS_BATCH, i_hi - i_lo), 0);
+    const uint32_t lim0 = fs_limit(a, row_g, rows, l), lim1 = fs_limit(a, row_g, rows, l + 64);
+    {
+        fs_rows<D, 4, 8> q;
+        q.load(a, h, row_g, rows);
+        q.store(a, rows, sm.q4[0]);
+    }
+    const uint32_t all_lim = kvm_wave_min_u32(min(l < rows ? lim0 : 0xffffffffu, l + 64 < rows ? lim1 : 0xffffffffu));
+    const uint32_t some_lim = ~kvm_wave_min_u32(~max(lim0, lim1));
+    const uint8_t *const k_head = sg.k + (uint64_t)h * sg.n_tiles * KB, *const v_head = sg.v + (uint64_t)h * sg.n_tiles * VB;
+    uint32_t n_t = fs_tiles<D, 8>(sg, sm, i_lo, min(FS_BATCH, i_hi - i_lo), some_lim, all_lim, cells);   // (its barriers: Q, too)
+
+    // Both roles take the same barriers: one when Q is in registers, and for a batch of tiles
+    // one when the first is in LDS, one a tile, and those of the next batch's list.
+    if (w < 4) {
+        // ======== 32 rows: S^T = K Q^T, softmax, O^T += V^T P^T
+        const float c = a.c;
+        const uint32_t lc = fs_opaque(l), m2 = lc & 31u, g2 = lc >> 5;
+        // operand rings: R1 where a softmax is under way (registers), R0 elsewhere
+        constexpr std::integral_constant<int, D == 256 ? 4 : 6> R0;
+        constexpr std::integral_constant<int, D == 256 ? 2 : 4> R1;
+        kvm_f32x16 O[DT];
+        float ms = -INFINITY, lp = 0.0f;
+        kvm_f16x8 qop[KS];       // lane (g2, m2): Q[row m2][16 ks + 8 g2 .. + 7]
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qop[ks] = *(const kvm_f16x8 *)(sm.q4[rg] + (2 * ks + g2) * QU + m2 * 16);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) O[dt][r] = 0.0f;
+        const uint32_t qlim = fs_limit(a, row_g, rows, 32 * rg + m2);
+        const uint32_t key = fs_key(m2);
+        const uint32_t k_ofs = ((key >> 4) * NB * 64 + 16 * g2 + (key & 15)) * 16, v_ofs = ((m2 >> 4) * 64 + 16 * g2 + (m2 & 15)) * 16;
+        const bool active = 32u * rg < rows;              // not a wave of padding rows
+        KVM_LDS_BARRIER();                                // Q is in registers
+
+        // S^T of a half tile: K operand ks at sk + .., KR - 1 ahead; between(ks) follows MFMA ks
+        auto scores = [&](auto ring, const uint8_t *sk, auto &&between) {
+            constexpr int KR = decltype(ring)::value;
+            kvm_f32x16 S;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[r] = 0.0f;
+            kvm_f16x8 kr[KR];
+            auto ld = [&](int ks) { return *(const kvm_f16x8 *)(sk + ks * 512); };
+#pragma unroll
+            for (int i = 0; i < KR - 1; ++i) kr[i] = ld(i);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (ks + KR - 1 < KS) kr[(ks + KR - 1) % KR] = ld(ks + KR - 1);
+                FS_FENCE();
+                S = __builtin_amdgcn_mfma_f32_32x32x16_f16(kr[ks % KR], qop[ks], S, 0, 0, 0);
+                between(ks);
+                FS_PIN(S);
+            }
+            return S;
+        };
+        // O^T += V^T P^T: operand i = (16 keys i / DT, dim tile i % DT)
+        auto accumulate = [&](auto ring, const uint8_t *sv, const kvm_f16x8 (&pb)[2], auto &&between) {
+            constexpr int VR = decltype(ring)::value;
+            kvm_f16x8 vr[VR];
+            auto ld = [&](int i) { return *(const kvm_f16x8 *)(sv + (i % DT) * 2048 + (i / DT) * 512); };
+#pragma unroll
+            for (int i = 0; i < VR - 1; ++i) vr[i] = ld(i);
+#pragma unroll
+            for (int i = 0; i < 2 * DT; ++i) {
+                if (i + VR - 1 < 2 * DT) vr[(i + VR - 1) % VR] = ld(i + VR - 1);
+                FS_FENCE();
+                O[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vr[i % VR], pb[i / DT], O[i % DT], 0, 0, 0);
+                between(i);
+                FS_PIN(O[i % DT]);
+            }
+        };
+        // The softmax of a half tile in KS steps, taken between another's MFMAs: the maximum
+        // (KS / 4 steps), the running maximum's move (one), the probabilities (KS / 2).
+        float x = 0.0f, ref = 0.0f, alpha = 1.0f, sum = 0.0f;
+        bool moved = false;
+        auto soft = [&](const kvm_f32x16 &S, kvm_f16x8 (&pb)[2], int i) {
+            constexpr int NM = KS / 4, EM = 16 / NM, EP = 16 / (KS / 2);
+            if (i < NM) {
+#pragma unroll
+                for (int r = 0; r < EM; ++r) x = i == 0 && r == 0 ? S[0] : fmaxf(x, S[EM * i + r]);
+            } else if (i == NM) {
+                x = kvm_max_xor32(x);
+                const bool up = fmaf(x, c, -ms) > FS_LAZY;        // false for a row with nothing visible yet
+                moved = __builtin_amdgcn_ballot_w64(up) != 0;
+                const float mnew = up ? x * c : ms;
+                alpha = up ? __builtin_amdgcn_exp2f(ms - mnew) : 1.0f;
+                ms = mnew;
+                ref = ms == -INFINITY ? 0.0f : ms;
+                sum = 0.0f;
+            } else if (i >= KS / 2) {
+#pragma unroll
+                for (int j = 0; j < EP; ++j) {
+                    // (the row sum takes p before its rounding)
+                    const int r = EP * (i - KS / 2) + j;
+                    const float y = __builtin_amdgcn_exp2f(fmaf(S[r], c, -ref));
+                    pb[r >> 3][r & 7] = (_Float16)y;
+                    sum += y;
+                }
+            }
+        };
+        // what the moved maximum asks of the sums so far
+        auto settle = [&]() {
+            if (moved) {
+                asm volatile("" ::: "memory");            // keep it on this (rare) path
+                lp *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) O[dt] *= alpha;
+            }
+            lp += sum;
+        };
+        auto nothing = [](int) {};
+
+        for (uint32_t b0 = i_lo;;) {
+            KVM_LDS_BARRIER();                            // the first tile is in LDS
+            for (uint32_t k = 0; k < n_t; ++k) {
+                if (!active) {
+                    KVM_LDS_BARRIER();
+                    continue;
+                }
+                const bool masked = (__builtin_amdgcn_readfirstlane(sm.list[k]) >> 31) == 0;
+                const uint8_t *sk = sm.ring[k & 1u] + k_ofs, *sv = sm.ring[k & 1u] + TB + v_ofs;
+                kvm_f16x8 pb[2], pb1[2];
+                kvm_f32x16 S0 = scores(R0, sk, nothing);
+                if (masked) fs_mask(S0, &sm.cp[k & 1u][0], qlim);
+                kvm_f32x16 S1 = scores(R1, sk + 2 * NB * 1024, [&](int i) { soft(S0, pb, i); });
+                settle();
+                if (masked) fs_mask(S1, &sm.cp[k & 1u][32], qlim);
+                accumulate(R1, sv, pb, [&](int i) { soft(S1, pb1, i); });
+                settle();
+                accumulate(R0, sv + TB / 2, pb1, nothing);
+                KVM_LDS_BARRIER();
+            }
+            if (__builtin_amdgcn_readfirstlane(sm.odd)) fs_add_odd<D, QUANT>(O, sg, v_head, sm.list, 0, 1, n_t, some_lim, all_lim, qlim, sm.odd_v[w]);
+            b0 += FS_BATCH;
+            if (b0 >= i_hi) break;
+            fs_cells<8> next;
+            next.load(sg, b0, min(FS_BATCH, i_hi - b0), 0);
+            n_t = fs_tiles<D, 8>(sg, sm, b0, min(FS_BATCH, i_hi - b0), some_lim, all_lim, next);
+        }
+        if (active) {
+            // quad i of O: dims 8 i + 4 g2 .. + 3 of the lane's row
+            const float lr = kvm_add_xor32(lp);
+            const uint32_t le = fs_opaque(l);
+            float *o = a.ws_o + (uint64_t)(slot + rg) * 32 * D + 4 * le;
+            if (__builtin_amdgcn_ballot_w64(ms != -INFINITY) != 0) {
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i)
+                    *(kvm_f32x4 *)(o + 256 * i) = kvm_f32x4{O[i >> 2][4 * (i & 3)], O[i >> 2][4 * (i & 3) + 1], O[i >> 2][4 * (i & 3) + 2], O[i >> 2][4 * (i & 3) + 3]};
+            }
+            if (le < 32) {
+                float *ml = a.ws_ml + ((uint64_t)(slot + rg) * 32 + le) * 2;
+                ml[0] = ms;
+                ml[1] = lr;
+            }
+        }
+    } else {
+        // ======== tile k + 1 into one buffer while the others work on tile k
+        const int pw = w - 4;
+        KVM_LDS_BARRIER();                                // Q is in registers
+        auto tile = [&](uint32_t k) { return __builtin_amdgcn_readfirstlane(sm.list[k < n_t ? k : n_t - 1]); };
+        auto cells_of = [&](uint32_t e) { return sg.cell_pos[(uint64_t)(e & 0x7fffffffu) * 64 + l]; };
+        // what the tile's masks say: the keys that some row sees, and those that not all do
+        auto masks = [&](int32_t cp, uint64_t &seen, uint64_t &part) {
+            seen = __builtin_amdgcn_ballot_w64((uint32_t)cp < some_lim);
+            part = seen & ~__builtin_amdgcn_ballot_w64((uint32_t)cp < all_lim);
+        };
+        for (uint32_t b0 = i_lo;;) {
+            if constexpr (QUANT) {
+                // The quantised tile goes through registers (two sets: tiles k + 2 and k + 3 are
+                // in flight while tile k + 1 is converted).  Thread (pw, l): K units 4 j + pw
+                // (lane l of (sub, block pair)), V dim tiles VJ pw + j.
+                constexpr int KJ = D / 64, VJ = D / 64, VB2 = VJ / 2;
+                struct raw_tile {
+                    kvm_u32x4 k[KJ];
+                    uint32_t kd[KJ][2];
+                    kvm_u32x2 v[VJ];
+                    kvm_u32x4 vs[VB2][2];
+                    int32_t cp;
+                    uint32_t e;
+                };
+                raw_tile rt2[2] = {};
+                auto load = [&](raw_tile &r, uint32_t e) {
+                    const uint32_t ln = fs_opaque(l), t = e & 0x7fffffffu;
+                    const uint8_t *kt = k_head + (uint64_t)t * KB, *vt = v_head + (uint64_t)t * VB;
+#pragma unroll
+                    for (int j = 0; j < KJ; ++j) {
+                        const uint32_t sp = 4 * j + pw, s = sp / (NB / 2), pr = sp % (NB / 2);
+                        r.k[j] = *(const kvm_u32x4 *)(kt + (sp * 64 + ln) * 16);
+                        r.kd[j][0] = *(const uint16_t *)(kt + kvm_kd_off(D, 16 * s + (ln & 15), 2 * pr));
+                        r.kd[j][1] = *(const uint16_t *)(kt + kvm_kd_off(D, 16 * s + (ln & 15), 2 * pr + 1));
+                    }
+#pragma unroll
+                    for (int j = 0; j < VJ; ++j) r.v[j] = *(const kvm_u32x2 *)(vt + ((VJ * pw + j) * 64 + ln) * 8);
+#pragma unroll
+                    for (int b = 0; b < VB2; ++b)
+#pragma unroll
+                        for (int ks = 0; ks < 2; ++ks) r.vs[b][ks] = *(const kvm_u32x4 *)(vt + 32 * D + (((VB2 * pw + b) * 2 + ks) * 4 + (ln >> 4)) * 16);
+                    r.cp = cells_of(e);
+                    r.e = e;
+                };
+                auto convert = [&](raw_tile &r, uint32_t buf) {
+                    if (!(r.e >> 31)) {
+                        asm volatile("" ::: "memory");    // keep it on this (rare) path
+                        uint64_t seen, part;
+                        masks(r.cp, seen, part);
+                        bool odd = false;
+#pragma unroll
+                        for (int b = 0; b < VB2; ++b)
+#pragma unroll
+                            for (int ks = 0; ks < 2; ++ks) odd |= fs_clear(r.vs[b][ks], 32 * ks + 8 * (fs_opaque(l) >> 4), seen, part);
+                        if (odd) sm.odd = 1;
+                    }
+                    uint8_t *dk = sm.ring[buf] + 16 * fs_opaque(l), *dv = dk + TB;
+#pragma unroll
+                    for (int j = 0; j < KJ; ++j) {
+                        const uint32_t sp = 4 * j + pw, s = sp / (NB / 2), pr = sp % (NB / 2);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) *(kvm_f16x8 *)(dk + (s * NB + 2 * pr + i) * 1024) = pf_q8(r.k[j][2 * i], r.k[j][2 * i + 1], r.kd[j][i]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < VJ; ++j)
+#pragma unroll
+                        for (int ks = 0; ks < 2; ++ks) *(kvm_f16x8 *)(dv + ks * (TB / 2) + (VJ * pw + j) * 1024) = pf_q4(r.v[j][ks], r.vs[j / 2][ks]);
+                    if (pw == 0) sm.cp[buf][l] = r.cp;
+                };
+                if (n_t != 0) {
+                    load(rt2[0], tile(0));
+                    load(rt2[1], tile(1));
+                    convert(rt2[0], 0);
+                }
+                KVM_LDS_BARRIER();                        // the first tile is in LDS
+                if (2 < n_t) load(rt2[0], tile(2));
+                auto step = [&](raw_tile &r, uint32_t k) {
+                    if (k + 1 < n_t) convert(r, (k + 1) & 1u);
+                    if (k + 3 < n_t) load(r, tile(k + 3));
+                    KVM_LDS_BARRIER();
+                };
+                uint32_t k = 0;
+                for (; k + 2 <= n_t; k += 2) {
+                    step(rt2[1], k);
+                    step(rt2[0], k + 1);
+                }
+                if (k < n_t) step(rt2[1], k);
+            } else {
+                // An f16 window's tiles are copied.  Its V tile holds the two key halves of a
+                // dim side by side, so the copies read every second unit of a dim tile.
+                constexpr int NC = (int)TB / 4096;        // 1 KB copies of a wave, of K and of V
+                auto bring = [&](uint32_t e, uint32_t buf) {
+                    const uint32_t t = e & 0x7fffffffu;
+                    uint8_t *const dst = sm.ring[buf];
+                    const uint8_t *kt = k_head + (uint64_t)t * TB, *vt = v_head + (uint64_t)t * TB;
+                    const int32_t cp = cells_of(e);
+#pragma unroll
+                    for (int i = 0; i < NC; ++i) fs_copy16(kt + (pw * NC + i) * 1024u, 16u * fs_opaque(l), dst + (pw * NC + i) * 1024u);
+#pragma unroll
+                    for (int i = 0; i < NC; ++i) {
+                        const uint32_t x = pw * NC + i;   // key half, dim tile
+                        fs_copy16(vt + (x % (D / 16)) * 2048u + (x / (D / 16)) * 16u, 32u * fs_opaque(l), dst + TB + x * 1024u);
+                    }
+                    if (pw == 0) sm.cp[buf][l] = cp;
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    if (!(e >> 31)) {
+                        asm volatile("" ::: "memory");
+                        uint64_t seen, part;
+                        masks(cp, seen, part);
+                        const uint32_t ln = fs_opaque(l);
+                        bool odd = false;
+                        for (int i = 0; i < NC; ++i) {
+                            const uint32_t x = pw * NC + i;
+                            kvm_u32x4 *const u = (kvm_u32x4 *)(dst + TB + x * 1024u + 16 * ln);
+                            kvm_u32x4 v = *u;
+                            odd |= fs_clear(v, 32 * (x / (D / 16)) + 8 * (ln >> 4), seen, part);
+                            *u = v;
+                        }
+                        if (odd) sm.odd = 1;
+                    }
+                };
+                if (n_t != 0) bring(tile(0), 0);
+                KVM_LDS_BARRIER();                        // the first tile is in LDS
+                for (uint32_t k = 0; k < n_t; ++k) {
+                    if (k + 1 < n_t) bring(tile(k + 1), (k + 1) & 1u);
+                    KVM_LDS_BARRIER();
+                }
+            }
+            b0 += FS_BATCH;
+            if (b0 >= i_hi) break;
+            fs_cells<8> next;
+            next.load(sg, b0, min(FS_BATCH, i_hi - b0), 0);
+            n_t = fs_tiles<D, 8>(sg, sm, b0, min(FS_BATCH, i_hi - b0), some_lim, all_lim, next);
+        }
+    }
+    __syncthreads();                                      // the LDS is the next piece's
+}
+
+// The pieces of a workgroup: tiles [lo, hi) of the kind's, the segments s .. one after another.
+template <bool WIDE, class F>
+__device__ __forceinline__ void fs_pieces(const fs_args &a, F &&piece) {
+    const uint32_t l = threadIdx.x & 63u;
+    const fs_deal &dl = WIDE ? a.wide : a.narrow;
     // neighbouring shares on one XCD: their units read the same tiles
     uint32_t p = blockIdx.x;
-    if (a.log_p >= 3) p = (p & 7u) << (a.log_p - 3) | p >> 3;
-    const uint32_t tiles = a.tile0[a.n_seg], lo = fs_share(tiles, a.log_p, p), hi = fs_share(tiles, a.log_p, p + 1);
+    if (dl.p % 8 == 0) p = (p & 7u) * (dl.p / 8) + (p >> 3);
+    const uint32_t lo = dl.first(p), hi = dl.first(p + 1);
     uint32_t s = __popcll(__builtin_amdgcn_ballot_w64(l < a.n_seg && a.tile0[l < a.n_seg ? l : 0u] <= lo)) - 1;
     if (a.n_seg > 64 && a.tile0[64] <= lo) s = 64;
     s = __builtin_amdgcn_readfirstlane(s);
     for (uint32_t at = lo; at < hi;) {
         const fs_seg &sg = a.seg[s];
-        const uint32_t n_rt = fs_row_tiles(sg.n_rows), ul = (at - a.tile0[s]) / sg.n_tiles, t0 = a.tile0[s] + ul * sg.n_tiles;
-        fs_piece<D, QUANT>(a, sg, sm, ul % n_rt, ul / n_rt, p + a.unit0[s] + ul, at - t0, min(hi - t0, sg.n_tiles));
-        at = t0 + sg.n_tiles;
+        const uint32_t n_rt = fs_row_tiles(WIDE, sg.n_rows);
+        const uint32_t u = (at - a.tile0[s]) / sg.n_tiles, c0 = a.tile0[s] + u * sg.n_tiles, h = u / n_rt;
+        piece(sg, u - h * n_rt, h, a.slot0[s] + (p + u) * (WIDE ? 4u : 1u), at - c0, min(hi - c0, sg.n_tiles));
+        at = c0 + sg.n_tiles;
         if (at >= a.tile0[s + 1]) ++s;
     }
 }
 
+template <int D, bool QUANT>
+__global__ void __launch_bounds__(512) k_fs_wide(fs_args a) {
+    __shared__ fs_lds_wide<D, QUANT> sm;
+    fs_pieces<true>(a, [&](const fs_seg &sg, uint32_t rt, uint32_t h, uint32_t slot, uint32_t i_lo, uint32_t i_hi) {
+        fs_wide_piece<D, QUANT>(a, sg, sm, rt, h, slot, i_lo, i_hi);
+    });
+}
+
+template <int D>
+__global__ void __launch_bounds__(256, 2) k_fs_narrow(fs_args a) {
+    __shared__ fs_lds_narrow<D> sm;
+    fs_pieces<false>(a, [&](const fs_seg &sg, uint32_t rt, uint32_t h, uint32_t slot, uint32_t i_lo, uint32_t i_hi) {
+        fs_narrow<D>(a, sg, sm, rt, h, slot, i_lo, i_hi);
+    });
+}
+
 // The pieces of 32 rows' 8 dims: a lane has 4 dims of a row; the workgroup's four waves share
-// the prefix's pieces, wave 0 also takes the conversation's.
-template <int D, int NP>
+// the row's pieces, the prefix's and the conversation's.
+template <int D, bool QUANT, int NP>
 __global__ void __launch_bounds__(256) k_fs_join(fs_args a) {
     const uint32_t l = threadIdx.x & 63u, w = threadIdx.x >> 6, m2 = l & 31u, i = blockIdx.y, h = blockIdx.z, row = 32 * blockIdx.x + m2;
-    const uint32_t tiles = a.tile0[a.n_seg];
+    const bool live = row < a.n_rows;
+    // the pieces of the unit of segment s that has the segment's row r: n slots, step apart
+    auto pieces = [&](uint32_t s, uint32_t r, uint32_t &n, uint32_t &step) {
+        const fs_seg &sg = a.seg[s];
+        const bool wide = !QUANT || s < a.n_wide;
+        const uint32_t ur = fs_unit_rows(wide), u = h * fs_row_tiles(wide, sg.n_rows) + r / ur;
+        const fs_deal &dl = wide ? a.wide : a.narrow;
+        const uint32_t c0 = a.tile0[s] + u * sg.n_tiles, q0 = dl.owner(c0), q1 = dl.owner(c0 + sg.n_tiles - 1);
+        step = ur / 32;
+        n = q1 - q0 + 1;
+        return a.slot0[s] + (q0 + u) * step + r % ur / 32;
+    };
+    // the conversation that the row is in
+    uint32_t s = 0;
+#pragma unroll
+    for (uint32_t x = 0; x < FS_LANES; ++x) s += row >= a.lane0[x];
+    s = a.lane_seg[s > 0 ? s - 1 : 0u];
+    const uint32_t row0 = a.lane0[0] == 0xffffffffu ? 0xffffffffu : a.seg[s].row0, r_own = row - row0;
+    const bool own = live && row >= a.lane0[0] && r_own < a.seg[s].n_rows;
+    uint32_t n_pre = 0, step_pre = 1, slot_pre = 0, n_own = 0, step_own = 1, slot_own = 0;
+    if (a.has_prefix) slot_pre = pieces(0, live ? row : 0u, n_pre, step_pre);     // (the prefix's rows are all rows)
+    if (own) slot_own = pieces(s, r_own, n_own, step_own);
     float M = -INFINITY, L = 0.0f;
     kvm_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    // pieces first, first + step, .. of unit ul of segment s; r: the row in the unit
-    auto take = [&](uint32_t s, uint32_t ul, uint32_t r, uint32_t first, uint32_t step, bool live) {
-        const fs_seg &sg = a.seg[s];
-        const uint32_t t0 = a.tile0[s] + ul * sg.n_tiles;
-        const uint32_t q0 = fs_owner(tiles, a.log_p, t0), q1 = fs_owner(tiles, a.log_p, t0 + sg.n_tiles - 1);
-        const uint64_t u = a.unit0[s] + ul;
-        for (uint32_t q = q0 + first; q <= q1; q += step * NP) {
-            kvm_f32x4 x[NP];
-            float m[NP], sum[NP];
+    for (uint32_t q = w; q < n_pre + n_own; q += 4 * NP) {
+        kvm_f32x4 x[NP];
+        float m[NP], sum[NP];
 #pragma unroll
-            for (uint32_t j = 0; j < NP; ++j) {
-                const uint64_t slot = min(q + step * j, q1) + u;
-                x[j] = *(const kvm_f32x4 *)(a.ws_o + (slot * (D / 8) + i) * 256 + 128 * (l >> 5) + 4 * r);
-                const kvm_f32x2 ml = *(const kvm_f32x2 *)(a.ws_ml + (slot * 32 + r) * 2);
-                m[j] = live && q + step * j <= q1 ? ml[0] : -INFINITY;
-                sum[j] = ml[1];
-            }
-            float mb = M;
-#pragma unroll
-            for (uint32_t j = 0; j < NP; ++j) mb = fmaxf(mb, m[j]);
-            const float keep = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mb);
-            L *= keep;
-            acc *= keep;
-#pragma unroll
-            for (uint32_t j = 0; j < NP; ++j) {
-                // (a piece that saw nothing, or is not the lane's, holds anything)
-                const float wgt = __builtin_amdgcn_exp2f(m[j] - mb);
-                const bool no = m[j] == -INFINITY;
-                L += no ? 0.0f : sum[j] * wgt;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) acc[k] += no ? 0.0f : x[j][k] * wgt;
-            }
-            M = mb;
+        for (uint32_t j = 0; j < NP; ++j) {
+            const uint32_t k = min(q + 4 * j, n_pre + n_own - 1), r = k < n_pre ? m2 : r_own & 31u;
+            const uint64_t slot = k < n_pre ? slot_pre + k * step_pre : slot_own + (k - n_pre) * step_own;
+            x[j] = *(const kvm_f32x4 *)(a.ws_o + (slot * (D / 8) + i) * 256 + 128 * (l >> 5) + 4 * r);
+            const kvm_f32x2 ml = *(const kvm_f32x2 *)(a.ws_ml + (slot * 32 + r) * 2);
+            m[j] = live && q + 4 * j < n_pre + n_own ? ml[0] : -INFINITY;
+            sum[j] = ml[1];
         }
-    };
-    const bool live = row < a.n_rows;
-    if (a.has_prefix) {
-        // the prefix's rows are all rows
-        const uint32_t n_rt = fs_row_tiles(a.n_rows);
-        take(0, h * n_rt + blockIdx.x, m2, w, 4, live);
-    }
-    if (w == 0) {
-        // the conversation that the row is in
-        uint32_t s = 0;
+        float mb = M;
 #pragma unroll
-        for (uint32_t x = 0; x < FS_LANES; ++x) s += row >= a.lane0[x];
-        const bool own = live && s > 0 && row < a.seg[a.has_prefix + s - 1].row0 + a.seg[a.has_prefix + s - 1].n_rows;
-        if (own) {
-            const uint32_t x = a.has_prefix + s - 1, r = row - a.seg[x].row0;
-            take(x, h * fs_row_tiles(a.seg[x].n_rows) + r / 32, r % 32, 0, 1, true);
+        for (uint32_t j = 0; j < NP; ++j) mb = fmaxf(mb, m[j]);
+        const float keep = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mb);
+        L *= keep;
+        acc *= keep;
+#pragma unroll
+        for (uint32_t j = 0; j < NP; ++j) {
+            // (a piece that saw nothing, or is not the lane's, holds anything)
+            const float wgt = __builtin_amdgcn_exp2f(m[j] - mb);
+            const bool no = m[j] == -INFINITY;
+            L += no ? 0.0f : sum[j] * wgt;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[k] += no ? 0.0f : x[j][k] * wgt;
         }
+        M = mb;
     }
     __shared__ __align__(16) float s_x[4][64][4];
     __shared__ float s_m[4][64], s_l[4][64];
@@ -637,40 +1018,85 @@ static uint32_t fs_stride(uint32_t n) {
     return m;
 }
 
-// Fills the segments, their tiles and the number of workgroups.
+// The rows from which on a window's units are wide.  An f16 window has nothing to convert: all.
+// A CU's workgroup takes a tile of a wide unit of 256 dims in 2.6 - 3.1 us, its two narrow ones
+// a tile of theirs in 1.5: a wide unit pays from three narrow ones' rows on.  Where some windows
+// stay narrow all the same, the wide ones are a launch more (10 us for its start and end) and
+// have to save that: 288 rows over 5,003 cells with 16 x 18 over 8,192, all narrow 79 us, else
+// 28 + 61; 768 rows over 32,768 with 32 x 24 over 2,048, 277 us and 175 + 41.
+static uint32_t fs_wide_rows(const kvm_window *prefix, const kvm_window *const *windows, const uint32_t *n_tokens, uint32_t n_lanes, bool quant,
+                             uint32_t n_cu, uint32_t H, uint32_t G, uint32_t n_rows) {
+    if (!quant) return 1;
+    double saved = 0.0;              // us
+    bool narrow = false;
+    auto add = [&](const kvm_window *w, uint32_t r) {
+        if (!w || !r) return;
+        if (r <= 64) narrow = true;
+        else saved += (double)(w->n_cells / KVM_TILE_CELLS) * H / n_cu * (1.5 * fs_row_tiles(false, r) - 2.8 * fs_row_tiles(true, r));
+    };
+    add(prefix, n_rows);
+    for (uint32_t i = 0; i < n_lanes; ++i) add(windows ? windows[i] : nullptr, n_tokens[i] * G);
+    return narrow && saved < 10.0 ? 0xffffffffu : 65;
+}
+
+// Fills the segments, their tiles and slots, and the numbers of workgroups.
 static int fs_shape(kvm_state *st, const char *what, const kvm_window *prefix, const kvm_window *const *windows,
-                    const uint32_t *n_tokens, uint32_t n_lanes, uint32_t n_wg, fs_args *a, uint32_t *units) {
-    uint64_t unit = 0, tiles = 0;
+                    const uint32_t *n_tokens, uint32_t n_lanes, bool quant, uint32_t n_cu, fs_args *a, uint64_t *slots) {
+    const uint32_t wide_rows = fs_wide_rows(prefix, windows, n_tokens, n_lanes, quant, n_cu, a->H, a->G, a->n_rows);
+    uint64_t tiles = 0, units = 0, wide = 0;
     uint32_t n = 0;
     auto add = [&](const kvm_window *w, uint32_t row0, uint32_t n_rows) {
         const uint32_t t = w->n_cells / KVM_TILE_CELLS;
+        const bool iw = n_rows >= wide_rows;
         a->tile0[n] = (uint32_t)tiles;
-        a->unit0[n] = (uint32_t)unit;
         a->seg[n++] = fs_seg{(const uint8_t *)w->k, (const uint8_t *)w->v, w->cell_pos, t, fs_stride(t), row0, n_rows};
-        const uint64_t u = (uint64_t)fs_row_tiles(n_rows) * a->H;
-        unit += u;
+        const uint64_t u = (uint64_t)fs_row_tiles(iw, n_rows) * a->H;
+        units += u;
         tiles += u * t;
+        if (iw) wide = tiles, a->n_wide = n;
     };
     a->has_prefix = prefix && a->n_rows;
-    if (a->has_prefix) add(prefix, 0, a->n_rows);
-    uint32_t row = 0, own = 0;
+    if (a->has_prefix) add(prefix, 0, a->n_rows);          // (wide where a conversation is)
     for (uint32_t i = 0; i < FS_LANES; ++i) a->lane0[i] = 0xffffffffu;
-    for (uint32_t i = 0; i < n_lanes; ++i) {
-        const uint32_t r = n_tokens[i] * a->G;
-        if (windows && windows[i] && r) {
-            a->lane0[own++] = row;
-            add(windows[i], row, r);
+    for (int narrow = 0; narrow < 2; ++narrow) {
+        uint32_t row = 0, own = 0;
+        for (uint32_t i = 0; i < n_lanes; ++i) {
+            const uint32_t r = n_tokens[i] * a->G;
+            if (windows && windows[i] && r) {
+                if ((r >= wide_rows) == !narrow) {
+                    a->lane0[own] = row;
+                    a->lane_seg[own] = (uint8_t)n;
+                    add(windows[i], row, r);
+                }
+                ++own;
+            }
+            row += r;
         }
-        row += r;
     }
-    if (tiles > 0x7fffffffu || unit > (1u << 24))
+    if (tiles > 0x7fffffffu || units > (1u << 22))
         return kvm_fail(st, KVM_ERANGE, "%s: %u rows over these windows are too many for one call", what, a->n_rows);
     a->tile0[n] = (uint32_t)tiles;
     a->n_seg = n;
-    // a share of four tiles at least: one a wave
-    a->log_p = 0;
-    while ((2u << a->log_p) <= n_wg && (8ull << a->log_p) <= tiles) ++a->log_p;
-    *units = (uint32_t)unit;
+    // Workgroups: what the CUs hold at once, and a tile or more for each of the attention's
+    // waves; eighths, one for each XCD
+    auto deal = [](uint32_t base, uint32_t of, uint32_t most) {
+        uint32_t p = std::min(most, std::max(of / 4, 1u));
+        if (p > 8) p &= ~7u;
+        return fs_deal{base, p, of / p, of % p};
+    };
+    a->wide = deal(0, (uint32_t)wide, n_cu);
+    a->narrow = deal((uint32_t)wide, (uint32_t)(tiles - wide), 2 * n_cu);
+    // A unit's pieces are those of the workgroups that its tiles reach over; from one piece
+    // of a segment to the next the workgroup, the unit or both go on by one.
+    uint64_t slot = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+        const bool iw = i < a->n_wide;
+        const fs_deal &dl = iw ? a->wide : a->narrow;
+        const uint32_t gr = fs_unit_rows(iw) / 32, p0 = dl.owner(a->tile0[i]), p1 = dl.owner(a->tile0[i + 1] - 1);
+        a->slot0[i] = (uint32_t)slot - p0 * gr;
+        slot += (uint64_t)(p1 - p0 + fs_row_tiles(iw, a->seg[i].n_rows) * a->H) * gr;
+    }
+    *slots = slot;
     return KVM_OK;
 }
 
@@ -719,13 +1145,11 @@ extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, con
     a.out_type = out_type;
     a.q_sign = scale < 0.0f ? -1.0f : scale > 0.0f ? 1.0f : 0.0f;
     a.c = scale != 0.0f ? fabsf(scale) * 1.4426950408889634f : 1.0f;
-    uint32_t units = 0;
+    uint64_t slots = 0;
     const bool quant = kvm_k_quant(w0->k_type);
-    const uint32_t n_wg = (st ? st->n_cu : 256u) * fs_resident(D, quant);
-    const int rc = fs_shape(st, what, prefix, windows, n_tokens, n_lanes, n_wg, &a, &units);
+    const int rc = fs_shape(st, what, prefix, windows, n_tokens, n_lanes, quant, st ? st->n_cu : 256u, &a, &slots);
     if (rc) return rc;
     if (!st) return KVM_EINVAL;
-    const uint64_t slots = a.n_seg ? (1ull << a.log_p) + units : 0;
     const size_t bytes_o = (size_t)slots * 32 * D * 4, bytes = bytes_o + (size_t)slots * 32 * 8;
     KVM_HIP(st, hipSetDevice(st->device));
     if (slots) {
@@ -734,16 +1158,19 @@ extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, con
         a.ws_o = (float *)ws;
         a.ws_ml = (float *)((uint8_t *)a.ws_o + bytes_o);
     }
-    auto go = [&](auto d) {
+    auto go = [&](auto d, auto qt) {
         constexpr int DD = decltype(d)::value;
-        if (a.n_seg) {
-            if (quant) hipLaunchKernelGGL((k_fs_attn<DD, true>), dim3(1u << a.log_p), dim3(256), 0, st->stream, a);
-            else hipLaunchKernelGGL((k_fs_attn<DD, false>), dim3(1u << a.log_p), dim3(256), 0, st->stream, a);
-        }
-        hipLaunchKernelGGL((k_fs_join<DD, 4>), dim3(kvm_cdiv(a.n_rows, 32), DD / 8, H), dim3(256), 0, st->stream, a);
+        constexpr bool Q = decltype(qt)::value;
+        if (a.n_wide) hipLaunchKernelGGL((k_fs_wide<DD, Q>), dim3(a.wide.p), dim3(512), 0, st->stream, a);
+        if (Q && a.n_wide < a.n_seg) hipLaunchKernelGGL((k_fs_narrow<DD>), dim3(a.narrow.p), dim3(256), 0, st->stream, a);
+        hipLaunchKernelGGL((k_fs_join<DD, Q, 4>), dim3(kvm_cdiv(a.n_rows, 32), DD / 8, H), dim3(256), 0, st->stream, a);
     };
-    if (D == 256) go(std::integral_constant<int, 256>{});
-    else go(std::integral_constant<int, 128>{});
+    auto go_d = [&](auto d) {
+        if (quant) go(d, std::true_type{});
+        else go(d, std::false_type{});
+    };
+    if (D == 256) go_d(std::integral_constant<int, 256>{});
+    else go_d(std::integral_constant<int, 128>{});
     KVM_LAUNCH_CHECK(st, what);
     return KVM_OK;
 }

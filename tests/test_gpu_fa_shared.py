@@ -128,6 +128,18 @@ def test_equals_softmax_in_64_bits(kvm_state, case):
     run(kvm_state, rng, H, G, D, cache, pc, cells(pc, live, 0) if pc else None, own, counts, qd, od, q_pos=qp)
 
 
+@pytest.mark.parametrize("H,D,cache", [(8, 128, "q8_0"), (4, 256, "q4_0")])
+def test_few_rows_beside_many(kvm_state, H, D, cache):
+    """A prefix of many rows, and conversations of one token and of many, in no order: what
+    quantised windows of few rows and of many take different ways for, in one call."""
+    rng, G, P = np.random.default_rng(16), 8, 2048
+    counts = [1, 9, 8, 0, 20, 8, 17, 3, 16, 16, 8, 8, 8, 8]
+    lanes = [(64 * (1 + i % 5), 40 + 11 * (i % 9)) for i in range(len(counts))]
+    own = [None if i == 5 else (n, cells(n, min(n, m), P)) for i, (n, m) in enumerate(lanes)]
+    qp = np.concatenate([P + min(n, m) - c + np.arange(c) for (n, m), c in zip(lanes, counts)])
+    run(kvm_state, rng, H, G, D, cache, P, cells(P, P, 0), own, counts, torch.bfloat16, torch.float32, q_pos=qp)
+
+
 @pytest.mark.parametrize("cache", ["q8_0", "f16"])
 def test_long_prefix(kvm_state, cache):
     """Many tiles a wave, several looks at a piece's tiles (one kv head, one row group: all
@@ -264,6 +276,30 @@ def test_what_is_not_seen_is_not_used(kvm_state, cache, what):
     same[3, 1] = same[5, 0] = same[6, 0] = False       # these see one
     assert torch.equal(dirty[same], clean[same])
     assert not bool(dirty[~same].isfinite().all())
+
+
+@pytest.mark.parametrize("cache", ["q8_0", "f16"])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+def test_what_is_not_seen_is_not_used_by_many_rows(kvm_state, cache, what):
+    """The same where a window has hundreds of rows, of which some see the cell: theirs hold it,
+    the others' are as if it held zeros."""
+    st, H, G, D = kvm_state, 2, 7, 128
+    counts, fills = [30, 21], [100, 64]
+    qp = np.concatenate([256 + f - c + np.arange(c) for f, c in zip(fills, counts)])
+    rng = np.random.default_rng(17)
+    clean, prefix, owns, q, qpos = run(st, rng, H, G, D, cache, 320, cells(320, 256, 0), [(128, cells(128, f, 256)) for f in fills],
+                                       counts, torch.float32, torch.float32, q_pos=qp)
+    _poison(prefix[0], cache, 300, 0, what)             # empty
+    _poison(owns[0][0], cache, 120, 1, what)
+    for c in (80, 99):
+        _poison(owns[0][0], cache, c, 1, what)          # lane 0's token 10 sees the first, its last token both
+    _poison(owns[1][0], cache, 63, 0, what)             # lane 1's last token
+    got = api.fa_decode_shared(st, prefix[0], [x[0] for x in owns], counts, q, qpos, H * G, D ** -0.5)
+    same = torch.ones((51, H), dtype=torch.bool)
+    same[10:30, 1] = same[50, 0] = False
+    clean, dirty = (x.view(51, H, G, D) for x in (clean, got))
+    assert torch.equal(dirty[same], clean[same])
+    assert not bool(dirty[~same].isfinite().flatten(1).all(1).any())
 
 
 def _poison(w, cache, c, h, what):
