@@ -58,29 +58,39 @@ struct fs_deal {
     // the workgroup that has tile x
     __host__ __device__ uint32_t owner(uint32_t x) const {
         x -= base;
-        return x < r * (q + 1) ? x / (q + 1) : r + (x - r * (q + 1)) / q;
+        const bool more = x < r * (q + 1);
+        return (more ? x : x - r * (q + 1)) / (more ? q + 1 : q) + (more ? 0 : r);
     }
 };
 
 struct fs_args {
     const void *q;
     const int32_t *q_pos;
-    void *out;
     float *ws_o;                 // pieces of 32 rows: [slot][dim / 8][lane][4]
     float *ws_ml;                // [slot][row][2]: scaled maximum, sum
     uint32_t H, G, n_head, n_rows;
     uint32_t n_seg, n_wide;      // segments, the wide ones before the narrow ones
     fs_deal wide, narrow;
     float c, q_sign;             // |scale| log2(e); q times -1 for a negative scale, and 0 (c = 1) for none
-    int q_type, out_type;
-    uint32_t has_prefix;         // segment 0 is the prefix
+    int q_type;
     uint32_t tile0[FS_SEGS + 1]; // tiles of the units of the segments before
     uint32_t slot0[FS_SEGS];     // unit u's piece of workgroup p: slots slot0 + (p + u) groups .. (mod 2^32)
-    uint32_t lane0[FS_LANES];    // first row of the conversations' segments, the rest ~0
-    uint8_t lane_seg[FS_LANES];  // and their segments
     fs_seg seg[FS_SEGS];
 };
 static_assert(sizeof(fs_args) <= 4096, "kernel arguments");
+
+// What the join reads.
+struct fs_join_args {
+    const float *ws_o, *ws_ml;
+    void *out;
+    int out_type;
+    uint32_t G, n_head, n_rows;
+    fs_deal wide, narrow;
+    uint32_t pre_tiles, pre_wide, pre_slot0;              // the prefix's (no tiles: none)
+    // conversations with a window, in order: first row (the rest: ~0), rows, tiles before, tiles
+    // (bit 31: wide), first slot
+    uint32_t row0[FS_LANES], rows[FS_LANES], tile0[FS_LANES], tiles[FS_LANES], slot0[FS_LANES];
+};
 
 __host__ __device__ inline uint32_t fs_unit_rows(bool wide) { return wide ? 128u : 32u; }
 __host__ __device__ inline uint32_t fs_row_tiles(bool wide, uint32_t n_rows) { return (n_rows + fs_unit_rows(wide) - 1) / fs_unit_rows(wide); }
@@ -905,98 +915,125 @@ __global__ void __launch_bounds__(256, 2) k_fs_narrow(fs_args a) {
     });
 }
 
-// The pieces of 32 rows' 8 dims: a lane has 4 dims of a row; the workgroup's four waves share
-// the row's pieces, the prefix's and the conversation's.
-template <int D, bool QUANT, int NP>
-__global__ void __launch_bounds__(256) k_fs_join(fs_args a) {
-    const uint32_t l = threadIdx.x & 63u, w = threadIdx.x >> 6, m2 = l & 31u, i = blockIdx.y, h = blockIdx.z, row = 32 * blockIdx.x + m2;
-    const bool live = row < a.n_rows;
-    // the pieces of the unit of segment s that has the segment's row r: n slots, step apart
-    auto pieces = [&](uint32_t s, uint32_t r, uint32_t &n, uint32_t &step) {
-        const fs_seg &sg = a.seg[s];
-        const bool wide = !QUANT || s < a.n_wide;
-        const uint32_t ur = fs_unit_rows(wide), u = h * fs_row_tiles(wide, sg.n_rows) + r / ur;
-        const fs_deal &dl = wide ? a.wide : a.narrow;
-        const uint32_t c0 = a.tile0[s] + u * sg.n_tiles, q0 = dl.owner(c0), q1 = dl.owner(c0 + sg.n_tiles - 1);
-        step = ur / 32;
-        n = q1 - q0 + 1;
-        return a.slot0[s] + (q0 + u) * step + r % ur / 32;
-    };
-    // the conversation that the row is in
-    uint32_t s = 0;
-#pragma unroll
-    for (uint32_t x = 0; x < FS_LANES; ++x) s += row >= a.lane0[x];
-    s = a.lane_seg[s > 0 ? s - 1 : 0u];
-    const uint32_t row0 = a.lane0[0] == 0xffffffffu ? 0xffffffffu : a.seg[s].row0, r_own = row - row0;
-    const bool own = live && row >= a.lane0[0] && r_own < a.seg[s].n_rows;
-    uint32_t n_pre = 0, step_pre = 1, slot_pre = 0, n_own = 0, step_own = 1, slot_own = 0;
-    if (a.has_prefix) slot_pre = pieces(0, live ? row : 0u, n_pre, step_pre);     // (the prefix's rows are all rows)
-    if (own) slot_own = pieces(s, r_own, n_own, step_own);
-    float M = -INFINITY, L = 0.0f;
-    kvm_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t q = w; q < n_pre + n_own; q += 4 * NP) {
-        kvm_f32x4 x[NP];
-        float m[NP], sum[NP];
-#pragma unroll
-        for (uint32_t j = 0; j < NP; ++j) {
-            const uint32_t k = min(q + 4 * j, n_pre + n_own - 1), r = k < n_pre ? m2 : r_own & 31u;
-            const uint64_t slot = k < n_pre ? slot_pre + k * step_pre : slot_own + (k - n_pre) * step_own;
-            x[j] = *(const kvm_f32x4 *)(a.ws_o + (slot * (D / 8) + i) * 256 + 128 * (l >> 5) + 4 * r);
-            const kvm_f32x2 ml = *(const kvm_f32x2 *)(a.ws_ml + (slot * 32 + r) * 2);
-            m[j] = live && q + 4 * j < n_pre + n_own ? ml[0] : -INFINITY;
-            sum[j] = ml[1];
-        }
-        float mb = M;
-#pragma unroll
-        for (uint32_t j = 0; j < NP; ++j) mb = fmaxf(mb, m[j]);
-        const float keep = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - mb);
-        L *= keep;
-        acc *= keep;
-#pragma unroll
-        for (uint32_t j = 0; j < NP; ++j) {
-            // (a piece that saw nothing, or is not the lane's, holds anything)
-            const float wgt = __builtin_amdgcn_exp2f(m[j] - mb);
-            const bool no = m[j] == -INFINITY;
-            L += no ? 0.0f : sum[j] * wgt;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) acc[k] += no ? 0.0f : x[j][k] * wgt;
-        }
-        M = mb;
-    }
+// The pieces of 32 rows: a lane has 4 dims of a row; the workgroup's four waves share the row's
+// pieces, the prefix's and the conversation's, 8 of them in flight each.  What bounds it: the way
+// through the launch, the arguments and one load (3.9 us for 8 rows of 128 dims; with a wait for
+// every argument 5.7), past some MB of pieces their reading (768 rows of 256 dims, 52 MB: 13.1).
+template <int D>
+__global__ void __launch_bounds__(256) k_fs_join(fs_join_args a) {
+    constexpr uint32_t NP = 8;
     __shared__ __align__(16) float s_x[4][64][4];
     __shared__ float s_m[4][64], s_l[4][64];
-    *(kvm_f32x4 *)s_x[w][l] = acc;
-    s_m[w][l] = M;
-    s_l[w][l] = L;
-    __syncthreads();
-    if (w != 0 || !live) return;
-    float mb = M;
-#pragma unroll
-    for (int j = 1; j < 4; ++j) mb = fmaxf(mb, s_m[j][l]);
-    L = 0.0f;
-    acc = kvm_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const bool no = s_m[j][l] == -INFINITY;
-        const float wgt = __builtin_amdgcn_exp2f(s_m[j][l] - mb);
-        L += no ? 0.0f : s_l[j][l] * wgt;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) acc[k] += no ? 0.0f : s_x[j][l][k] * wgt;
+    const uint32_t l = threadIdx.x & 63u, w = threadIdx.x >> 6, m2 = l & 31u, h = blockIdx.z, row_b = 32 * blockIdx.x, row = row_b + m2;
+    // lane x has conversation x's entries
+    const uint32_t t_row0 = a.row0[l], t_rows = a.rows[l], t_tile0 = a.tile0[l], t_tiles = a.tiles[l], t_slot0 = a.slot0[l];
+    // (as values: the compiler would load where each is used, one wait after another)
+    auto pin = [](uint32_t x) {
+        asm volatile("" : "+s"(x));
+        return x;
+    };
+    const uint32_t wb = pin(a.wide.base), wq = pin(a.wide.q), wr = pin(a.wide.r), nb = pin(a.narrow.base), nq = pin(a.narrow.q), nr = pin(a.narrow.r);
+    const uint32_t pre_tiles = pin(a.pre_tiles), pre_wide = pin(a.pre_wide), pre_slot0 = pin(a.pre_slot0), n_rows = pin(a.n_rows);
+    const bool live = row < n_rows;
+    // the pieces of unit u (with `tiles` tiles, tile0 before the segment's) : n of them from p0 on
+    auto pieces = [&](bool wide, uint32_t tile0, uint32_t tiles, uint32_t u, uint32_t &n) {
+        fs_deal dl;
+        dl.base = wide ? wb : nb;
+        dl.q = wide ? wq : nq;
+        dl.r = wide ? wr : nr;
+        const uint32_t c0 = tile0 + u * tiles, p0 = dl.owner(c0);
+        n = dl.owner(c0 + tiles - 1) - p0 + 1;
+        return p0;
+    };
+    uint32_t n_pre = 0, step_pre = 0, slot_pre = 0, n_own = 0, step_own = 0, slot_own = 0, r_own = 0;
+    if (pre_tiles) {                                      // (its rows are all rows)
+        const uint32_t ur = fs_unit_rows(pre_wide), u = h * fs_row_tiles(pre_wide, n_rows) + row_b / ur;
+        const uint32_t p0 = pieces(pre_wide, 0, pre_tiles, u, n_pre);
+        step_pre = ur / 32;
+        slot_pre = pre_slot0 + (p0 + u) * step_pre + row_b % ur / 32;
     }
-    // nothing visible: zeros
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    const uint32_t t = row / a.G;
-    const uint64_t at = ((uint64_t)t * a.n_head + h * a.G + (row - t * a.G)) * D + 8 * i + 4 * (l >> 5);
-    acc *= inv;
-    if (a.out_type == KVM_TYPE_F32) {
-        __builtin_memcpy((float *)a.out + at, &acc, 16);
-    } else if (a.out_type == KVM_TYPE_BF16) {
-        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-        const bf16x4 y = __builtin_convertvector(acc, bf16x4);
-        __builtin_memcpy((uint16_t *)a.out + at, &y, 8);
-    } else {
-        const kvm_f16x4 y = {(_Float16)acc[0], (_Float16)acc[1], (_Float16)acc[2], (_Float16)acc[3]};
-        __builtin_memcpy((uint16_t *)a.out + at, &y, 8);
+    // the conversation that the row is in: the last that begins at or before it
+    const uint32_t c_lo = __popcll(__builtin_amdgcn_ballot_w64(t_row0 <= row_b)), c_hi = __popcll(__builtin_amdgcn_ballot_w64(t_row0 <= row_b + 31));
+    uint32_t cv = c_lo;
+    for (uint32_t x = c_lo; x < c_hi; ++x) cv += row >= (uint32_t)__builtin_amdgcn_readlane((int)t_row0, (int)x);
+    if (c_hi) {
+        auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_ds_bpermute((int)(4 * (cv ? cv - 1 : 0)), (int)v); };
+        const uint32_t row0 = of(t_row0), n = of(t_rows), tile0 = of(t_tile0), tiles = of(t_tiles), slot0 = of(t_slot0);
+        if (live && cv && row - row0 < n) {
+            const bool wide = tiles >> 31;
+            r_own = row - row0;
+            const uint32_t ur = fs_unit_rows(wide), u = h * fs_row_tiles(wide, n) + r_own / ur;
+            const uint32_t p0 = pieces(wide, tile0, tiles & 0x7fffffffu, u, n_own);
+            step_own = ur / 32;
+            slot_own = slot0 + (p0 + u) * step_own + r_own % ur / 32;
+        }
+    }
+    const uint32_t n = live ? n_pre + n_own : 0u, t = row / a.G;
+    for (uint32_t i = blockIdx.y; i < D / 8; i += gridDim.y) {
+        float M = -INFINITY, L = 0.0f;
+        kvm_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (uint32_t q = w; q < n; q += 4 * NP) {
+            kvm_u32x4 x[NP];
+            kvm_f32x2 ml[NP];
+#pragma unroll
+            for (uint32_t j = 0; j < NP; ++j) {
+                const uint32_t k = min(q + 4 * j, n - 1), r = k < n_pre ? m2 : r_own & 31u;
+                const uint64_t slot = k < n_pre ? slot_pre + k * step_pre : slot_own + (k - n_pre) * step_own;
+                x[j] = *(const kvm_u32x4 *)(a.ws_o + (slot * (D / 8) + i) * 256 + 128 * (l >> 5) + 4 * r);
+                ml[j] = *(const kvm_f32x2 *)(a.ws_ml + (slot * 32 + r) * 2);
+            }
+            float mb = M;
+#pragma unroll
+            for (uint32_t j = 0; j < NP; ++j) {
+                if (q + 4 * j >= n) ml[j][0] = -INFINITY;
+                mb = fmaxf(mb, ml[j][0]);
+            }
+            const float top = mb == -INFINITY ? 0.0f : mb, keep = __builtin_amdgcn_exp2f(M - top);
+            L *= keep;
+            acc *= keep;
+#pragma unroll
+            for (uint32_t j = 0; j < NP; ++j) {
+                // (a piece that saw nothing of the row holds anything)
+                const float wgt = __builtin_amdgcn_exp2f(ml[j][0] - top);
+                const uint32_t has = ml[j][0] == -INFINITY ? 0u : 0xffffffffu;
+                L = fmaf(__uint_as_float(__float_as_uint(ml[j][1]) & has), wgt, L);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[k] = fmaf(__uint_as_float(x[j][k] & has), wgt, acc[k]);
+            }
+            M = mb;
+        }
+        *(kvm_f32x4 *)s_x[w][l] = acc;
+        s_m[w][l] = M;
+        s_l[w][l] = L;
+        __syncthreads();
+        if (w == 0 && live) {
+            float mb = M;
+#pragma unroll
+            for (int j = 1; j < 4; ++j) mb = fmaxf(mb, s_m[j][l]);
+            const float top = mb == -INFINITY ? 0.0f : mb;
+            L = 0.0f;
+            acc = kvm_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {                 // (a wave without pieces: zeros)
+                const float wgt = __builtin_amdgcn_exp2f(s_m[j][l] - top);
+                L = fmaf(s_l[j][l], wgt, L);
+                acc += *(const kvm_f32x4 *)s_x[j][l] * wgt;
+            }
+            // nothing visible: zeros
+            acc *= L == 0.0f ? 0.0f : 1.0f / L;
+            const uint64_t at = ((uint64_t)t * a.n_head + h * a.G + (row - t * a.G)) * D + 8 * i + 4 * (l >> 5);
+            if (a.out_type == KVM_TYPE_F32) {
+                __builtin_memcpy((float *)a.out + at, &acc, 16);
+            } else if (a.out_type == KVM_TYPE_BF16) {
+                typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+                const bf16x4 y = __builtin_convertvector(acc, bf16x4);
+                __builtin_memcpy((uint16_t *)a.out + at, &y, 8);
+            } else {
+                const kvm_f16x4 y = {(_Float16)acc[0], (_Float16)acc[1], (_Float16)acc[2], (_Float16)acc[3]};
+                __builtin_memcpy((uint16_t *)a.out + at, &y, 8);
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -1041,7 +1078,7 @@ static uint32_t fs_wide_rows(const kvm_window *prefix, const kvm_window *const *
 
 // Fills the segments, their tiles and slots, and the numbers of workgroups.
 static int fs_shape(kvm_state *st, const char *what, const kvm_window *prefix, const kvm_window *const *windows,
-                    const uint32_t *n_tokens, uint32_t n_lanes, bool quant, uint32_t n_cu, fs_args *a, uint64_t *slots) {
+                    const uint32_t *n_tokens, uint32_t n_lanes, bool quant, uint32_t n_cu, fs_args *a, fs_join_args *j, uint64_t *slots) {
     const uint32_t wide_rows = fs_wide_rows(prefix, windows, n_tokens, n_lanes, quant, n_cu, a->H, a->G, a->n_rows);
     uint64_t tiles = 0, units = 0, wide = 0;
     uint32_t n = 0;
@@ -1055,17 +1092,20 @@ static int fs_shape(kvm_state *st, const char *what, const kvm_window *prefix, c
         tiles += u * t;
         if (iw) wide = tiles, a->n_wide = n;
     };
-    a->has_prefix = prefix && a->n_rows;
-    if (a->has_prefix) add(prefix, 0, a->n_rows);          // (wide where a conversation is)
-    for (uint32_t i = 0; i < FS_LANES; ++i) a->lane0[i] = 0xffffffffu;
+    uint32_t lane_seg[FS_LANES], own = 0;
+    if (prefix) {                                          // (wide where a conversation is)
+        add(prefix, 0, a->n_rows);
+        j->pre_tiles = a->seg[0].n_tiles;
+        j->pre_wide = a->n_wide;
+    }
     for (int narrow = 0; narrow < 2; ++narrow) {
-        uint32_t row = 0, own = 0;
+        uint32_t row = 0;
+        own = 0;
         for (uint32_t i = 0; i < n_lanes; ++i) {
             const uint32_t r = n_tokens[i] * a->G;
             if (windows && windows[i] && r) {
                 if ((r >= wide_rows) == !narrow) {
-                    a->lane0[own] = row;
-                    a->lane_seg[own] = (uint8_t)n;
+                    lane_seg[own] = n;
                     add(windows[i], row, r);
                 }
                 ++own;
@@ -1077,15 +1117,16 @@ static int fs_shape(kvm_state *st, const char *what, const kvm_window *prefix, c
         return kvm_fail(st, KVM_ERANGE, "%s: %u rows over these windows are too many for one call", what, a->n_rows);
     a->tile0[n] = (uint32_t)tiles;
     a->n_seg = n;
-    // Workgroups: what the CUs hold at once, and a tile or more for each of the attention's
-    // waves; eighths, one for each XCD
-    auto deal = [](uint32_t base, uint32_t of, uint32_t most) {
-        uint32_t p = std::min(most, std::max(of / 4, 1u));
+    // Workgroups: what the CUs hold at once, and a tile or more for each wave that has tiles of
+    // its own (8 rows over 1,024 + 2 x 256 f16 cells of 2 heads: 8.7 us, with 4 tiles a workgroup
+    // 15.6); eighths, one for each XCD
+    auto deal = [](uint32_t base, uint32_t of, uint32_t most, uint32_t least) {
+        uint32_t p = std::min(most, std::max(of / least, 1u));
         if (p > 8) p &= ~7u;
         return fs_deal{base, p, of / p, of % p};
     };
-    a->wide = deal(0, (uint32_t)wide, n_cu);
-    a->narrow = deal((uint32_t)wide, (uint32_t)(tiles - wide), 2 * n_cu);
+    a->wide = deal(0, (uint32_t)wide, n_cu, 1);
+    a->narrow = deal((uint32_t)wide, (uint32_t)(tiles - wide), 2 * n_cu, 4);
     // A unit's pieces are those of the workgroups that its tiles reach over; from one piece
     // of a segment to the next the workgroup, the unit or both go on by one.
     uint64_t slot = 0;
@@ -1097,6 +1138,18 @@ static int fs_shape(kvm_state *st, const char *what, const kvm_window *prefix, c
         slot += (uint64_t)(p1 - p0 + fs_row_tiles(iw, a->seg[i].n_rows) * a->H) * gr;
     }
     *slots = slot;
+    j->wide = a->wide;
+    j->narrow = a->narrow;
+    if (prefix) j->pre_slot0 = a->slot0[0];
+    for (uint32_t i = 0; i < FS_LANES; ++i) j->row0[i] = 0xffffffffu;
+    for (uint32_t i = 0; i < own; ++i) {
+        const uint32_t s = lane_seg[i];
+        j->row0[i] = a->seg[s].row0;
+        j->rows[i] = a->seg[s].n_rows;
+        j->tile0[i] = a->tile0[s];
+        j->tiles[i] = a->seg[s].n_tiles | (s < a->n_wide ? 0x80000000u : 0u);
+        j->slot0[i] = a->slot0[s];
+    }
     return KVM_OK;
 }
 
@@ -1134,6 +1187,7 @@ extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, con
     if (total == 0) return KVM_OK;
     if (!q || !q_pos || !out) return kvm_fail(st, KVM_EINVAL, "%s: null argument", what);
     fs_args a{};
+    fs_join_args j{};
     a.H = H;
     a.G = n_head / H;
     a.n_head = n_head;
@@ -1141,13 +1195,16 @@ extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, con
     a.q = q;
     a.q_type = q_type;
     a.q_pos = q_pos;
-    a.out = out;
-    a.out_type = out_type;
+    j.out = out;
+    j.out_type = out_type;
+    j.G = a.G;
+    j.n_head = n_head;
+    j.n_rows = a.n_rows;
     a.q_sign = scale < 0.0f ? -1.0f : scale > 0.0f ? 1.0f : 0.0f;
     a.c = scale != 0.0f ? fabsf(scale) * 1.4426950408889634f : 1.0f;
     uint64_t slots = 0;
     const bool quant = kvm_k_quant(w0->k_type);
-    const int rc = fs_shape(st, what, prefix, windows, n_tokens, n_lanes, quant, st ? st->n_cu : 256u, &a, &slots);
+    const int rc = fs_shape(st, what, prefix, windows, n_tokens, n_lanes, quant, st ? st->n_cu : 256u, &a, &j, &slots);
     if (rc) return rc;
     if (!st) return KVM_EINVAL;
     const size_t bytes_o = (size_t)slots * 32 * D * 4, bytes = bytes_o + (size_t)slots * 32 * 8;
@@ -1157,13 +1214,20 @@ extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, con
         if (const int bad = kvm_shared_workspace(st, what, bytes, &ws)) return bad;
         a.ws_o = (float *)ws;
         a.ws_ml = (float *)((uint8_t *)a.ws_o + bytes_o);
+        j.ws_o = a.ws_o;
+        j.ws_ml = a.ws_ml;
     }
+    // a workgroup of the join has 8 dims, or more of them where all CUs have two all the same
+    // (its start is most of its work: 768 rows of 256 dims, 15.6 us by 8 dims)
+    const uint32_t blocks = kvm_cdiv(a.n_rows, 32) * H;
+    uint32_t by = D / 8;
+    while (by > 1 && (uint64_t)blocks * by >= 4ull * st->n_cu) by /= 2;
     auto go = [&](auto d, auto qt) {
         constexpr int DD = decltype(d)::value;
         constexpr bool Q = decltype(qt)::value;
         if (a.n_wide) hipLaunchKernelGGL((k_fs_wide<DD, Q>), dim3(a.wide.p), dim3(512), 0, st->stream, a);
         if (Q && a.n_wide < a.n_seg) hipLaunchKernelGGL((k_fs_narrow<DD>), dim3(a.narrow.p), dim3(256), 0, st->stream, a);
-        hipLaunchKernelGGL((k_fs_join<DD, Q, 4>), dim3(kvm_cdiv(a.n_rows, 32), DD / 8, H), dim3(256), 0, st->stream, a);
+        hipLaunchKernelGGL((k_fs_join<DD>), dim3(kvm_cdiv(a.n_rows, 32), by, H), dim3(256), 0, st->stream, j);
     };
     auto go_d = [&](auto d) {
         if (quant) go(d, std::true_type{});
