@@ -17,7 +17,7 @@
 // is fp32.  Key order: score row i of a half tile is key i with bits 2 and 3 swapped, so that
 // a lane's scores are 8 consecutive keys of each 16, what the P V operand wants.
 //   narrow units (quantised windows of few rows): workgroups of 4 waves, two a CU.
-//     Each wave takes every fourth of the piece's tiles.  Nothing is shared in the loop and no
+//     Each wave takes every fourth half of the piece's tiles.  Nothing is shared in the loop and no
 //     barrier is in it: tiles go from memory into registers (the tile layout is the matrix
 //     operands') and are converted there; the waves' sums meet in LDS at the end.
 //   wide units: workgroups of 8 waves, one a CU.  Waves 0 - 3 have 32 rows each and take every
@@ -101,6 +101,7 @@ struct fs_geo {
     static constexpr uint32_t KB = QUANT ? 64u * D + 128u * NB : 128u * D, VB = QUANT ? 32u * D + 128u * NB : 128u * D;
     static constexpr uint32_t TB = 128u * D;              // bytes of an f16 K (or V) tile
     static constexpr uint32_t QU = 528;                   // LDS bytes of a unit of Q: 8 dims of 32 rows, 16 bytes apart in the banks
+    static constexpr int SETS = D == 256 ? 1 : 2;         // half tiles that a wave has in registers
     static constexpr int NQ = D / 32;                     // quads that a wave adds up at the end of a narrow piece
 };
 
@@ -116,10 +117,10 @@ template <int D>
 struct fs_lds_narrow : fs_list<D, 4> {
     using G = fs_geo<D, true>;
     union {
-        struct {                                          // a wave's tile and its next
+        struct {                                          // a wave's half tile and its next
             alignas(16) uint8_t q[2 * G::KS * G::QU];
-            alignas(16) uint8_t sc[4][2][2][1024];        // K scales, V scales
-            alignas(16) int32_t cp[4][2][64];             // and the cells' positions
+            alignas(16) uint8_t sc[4][G::SETS + 1][1024]; // K scales, V scales
+            alignas(16) int32_t cp[4][G::SETS + 1][64];   // and the tile's cells' positions
         };
         alignas(16) float x[4][2][G::NQ * 256];           // at the end: chunks of O on their way
     };
@@ -266,18 +267,18 @@ __device__ __forceinline__ bool fs_clear(kvm_u32x4 &v, uint32_t base, uint64_t s
     return odd;
 }
 
-// What fs_clear took out of the list's tiles j0, j0 + step, ..: values that are no finite
+// What fs_clear took out of keys k0 .. k0 + n_k - 1 of the list's tiles j0, j0 + step, ..: values that are no finite
 // numbers are added to the rows that see them (a positive p times one is itself).  sx: the
 // wave's own.
 template <int D, bool QUANT>
 __device__ __forceinline__ void fs_add_odd(kvm_f32x16 (&O)[D / 32], const fs_seg &sg, const uint8_t *v_head, const uint32_t *list, uint32_t j0,
-                                           uint32_t step, uint32_t n_t, uint32_t some_lim, uint32_t all_lim, uint32_t qlim, float *sx) {
+                                           uint32_t step, uint32_t n_t, uint32_t k0, uint32_t n_k, uint32_t some_lim, uint32_t all_lim, uint32_t qlim, float *sx) {
     const uint32_t l = threadIdx.x & 63u;
     for (uint32_t j = j0; j < n_t; j += step) {
         const uint32_t e = list[j], t = e & 0x7fffffffu;
         if (e >> 31) continue;
         const uint8_t *v_tile = v_head + (uint64_t)t * fs_geo<D, QUANT>::VB;
-        for (uint32_t k = 0; k < 64; ++k) {
+        for (uint32_t k = k0; k < k0 + n_k; ++k) {
             const uint32_t cp = (uint32_t)sg.cell_pos[(uint64_t)t * 64 + k];
             if (!(cp < some_lim) || cp < all_lim) continue;
             bool any = false;
@@ -318,6 +319,11 @@ __device__ __forceinline__ void fs_copy16(const uint8_t *src, uint32_t off, void
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
                  : "=&s"(m0_saved) : "v"(off), "s"((uint32_t)(uintptr_t)(fs_lds_ptr)dst), "s"(src) : "memory");
 }
+__device__ __forceinline__ void fs_copy16(const uint8_t *lane_src, void *dst) {
+    uint32_t m0_saved;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0_saved) : "v"(lane_src), "s"((uint32_t)(uintptr_t)(fs_lds_ptr)dst) : "memory");
+}
 __device__ __forceinline__ void fs_copy4(const int32_t *src, uint32_t off, void *dst) {
     uint32_t m0_saved;
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, %3\n\ts_mov_b32 m0, %0"
@@ -331,8 +337,7 @@ template <int D>
 __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs_lds_narrow<D> &sm, uint32_t rt, uint32_t h, uint32_t slot,
                                           uint32_t i_lo, uint32_t i_hi) {
     using G = fs_geo<D, true>;
-    constexpr int KS = G::KS, NB = G::NB, DT = G::DT, NQ = G::NQ;
-    constexpr int SETS = D == 256 ? 1 : 2;                // half tiles of K in registers
+    constexpr int KS = G::KS, NB = G::NB, DT = G::DT, NQ = G::NQ, SETS = G::SETS;
     constexpr uint32_t KB = G::KB, VB = G::VB, QU = G::QU;
     const uint32_t l = fs_opaque(threadIdx.x & 63u), g2 = l >> 5, m2 = l & 31u;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -365,144 +370,153 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
         if (b0 != i_lo) cells.load(sg, b0, min(FS_BATCH, i_hi - b0), 0);
         const uint32_t n_t = fs_tiles<D, 4>(sg, sm, b0, min(FS_BATCH, i_hi - b0), some_lim, all_lim, cells);      // (its barriers: Q, too)
 
-        // The wave's tiles: list entries w, w + 4, ..  Registers of a half tile are loaded for
-        // the next where this one's are used up; past the wave's last tile the bounds let
-        // nothing through.
+        // The wave's half tiles: half w & 1 of list entries w / 2, w / 2 + 2, ..  Their
+        // registers are loaded for the next one where this one's are used up; past the wave's
+        // last the bounds let nothing through.
+        const uint32_t half = w & 1;
         kvm_u32x4 kr[SETS][NB];
-        uint32_t vq[2 * DT];
+        uint32_t vq[SETS][2 * DT];
         auto rsrc = [&](const uint8_t *head, uint32_t e, uint32_t bytes, bool more) {
             return __builtin_amdgcn_make_buffer_rsrc((void *)(head + (uint64_t)(e & 0x7fffffffu) * bytes), (short)0, more ? bytes : 0u, 0x00020000);
         };
-        auto load_k = [&](__amdgpu_buffer_rsrc_t r, int half) {
+        auto load_k = [&](__amdgpu_buffer_rsrc_t r, int set) {
             const uint32_t at = fs_opaque(k_lane);
 #pragma unroll
             for (int i = 0; i < NB; ++i)
-                kr[half % SETS][i] = __builtin_amdgcn_raw_buffer_load_b128(r, at + (i & 1) * 512, half * NB * 1024 + (i >> 1) * 1024, 0);
+                kr[set][i] = __builtin_amdgcn_raw_buffer_load_b128(r, at + (i & 1) * 512, half * NB * 1024 + (i >> 1) * 1024, 0);
         };
-        auto load_v = [&](__amdgpu_buffer_rsrc_t r, int half) {
+        auto load_v = [&](__amdgpu_buffer_rsrc_t r, int set) {
             const uint32_t at = fs_opaque(v_lane);
 #pragma unroll
-            for (int i = 0; i < 2 * DT; ++i) vq[i] = __builtin_amdgcn_raw_buffer_load_b32(r, at + (i & 1) * 256 + half * 4, (i >> 1) * 1024, 0);
+            for (int i = 0; i < 2 * DT; ++i) vq[set][i] = __builtin_amdgcn_raw_buffer_load_b32(r, at + (i & 1) * 256, half * 4 + (i >> 1) * 1024, 0);
         };
+        // lanes below 2 NB: the half's K scales, from 32 on its V scales (units of 8 keys of a block)
         auto copies = [&](uint32_t e, uint32_t buf) {
-            const uint32_t t = e & 0x7fffffffu, off = 16u * (fs_opaque(l) & (D == 256 ? 63u : 31u));     // (128 dims: 512 bytes of scales)
-            fs_copy16(k_head + (uint64_t)t * KB + 64 * D, off, sm.sc[w][buf][0]);
-            fs_copy16(v_head + (uint64_t)t * VB + 32 * D, off, sm.sc[w][buf][1]);
-            fs_copy4(sg.cell_pos + (uint64_t)t * 64, 4u * fs_opaque(l), &sm.cp[w][buf][0]);
+            const uint32_t t = e & 0x7fffffffu, ln = fs_opaque(l), x = ln & (4u * NB - 1);
+            const uint8_t *const src = ln < 32 ? k_head + (uint64_t)t * KB + 64 * D + half * (64u * NB) + 16 * x
+                                               : v_head + (uint64_t)t * VB + 32 * D + (x >> 2) * 128 + half * 64 + (x & 3u) * 16;
+            fs_copy16(src, sm.sc[w][buf]);
+            fs_copy4(sg.cell_pos + (uint64_t)t * 64, 4u * ln, &sm.cp[w][buf][0]);
         };
-        uint32_t e = 0;
-        if ((uint32_t)w < n_t) {
-            e = __builtin_amdgcn_readfirstlane(sm.list[w]);
-            const auto rk = rsrc(k_head, e, KB, true), rv = rsrc(v_head, e, VB, true);
-            copies(e, 0);
-            load_k(rk, 0);
-            if (SETS == 2) load_k(rk, 1);
-            load_v(rv, 0);
+        auto entry = [&](uint32_t j) { return __builtin_amdgcn_readfirstlane(sm.list[min(j, n_t - 1)]); };
+        const uint32_t j0 = w >> 1;
+        if (j0 < n_t) {
+#pragma unroll
+            for (int x = 0; x < SETS; ++x) {
+                const uint32_t e = entry(j0 + 2 * x);
+                const bool more = j0 + 2 * x < n_t;
+                copies(e, x);
+                load_k(rsrc(k_head, e, KB, more), x);
+                load_v(rsrc(v_head, e, VB, more), x);
+            }
         }
         uint32_t buf = 0;
-        for (uint32_t j = w; j < n_t; j += 4, buf ^= 1) {
-            // the tile's copies: the first tile's half tiles, or more, were loaded after them
-            asm volatile("s_waitcnt vmcnt(%0)" : : "n"(SETS * NB + 2 * DT) : "memory");
-            const bool more = j + 4 < n_t;
-            const uint32_t en = __builtin_amdgcn_readfirstlane(sm.list[more ? j + 4 : j]);
+        auto item = [&](uint32_t j, auto which) {
+            constexpr int set = decltype(which)::value;
+            // the half tile's copies: its registers' loads, and the next ones', are younger
+            asm volatile("s_waitcnt vmcnt(%0)" : : "n"(SETS * (NB + 2 * DT) + 2 * (SETS - 1)) : "memory");
+            const uint32_t e = entry(j), en = entry(j + 2 * SETS);
+            const bool more = j + 2 * SETS < n_t, full = e >> 31;
             const auto rk = rsrc(k_head, en, KB, more), rv = rsrc(v_head, en, VB, more);
-            const bool full = e >> 31;
             if (!full) {
                 asm volatile("" ::: "memory");            // keep it on this (rare) path
                 const uint32_t lo = fs_opaque(l), cp = (uint32_t)sm.cp[w][buf][lo];
                 const uint64_t seen = __builtin_amdgcn_ballot_w64(cp < some_lim), part = seen & ~__builtin_amdgcn_ballot_w64(cp < all_lim);
                 // lane l has the scales of 8 keys of a block
-                const uint32_t base = 32 * (lo >> 2 & 1u) + 8 * (lo & 3u);
-                kvm_u32x4 scv = *(const kvm_u32x4 *)(sm.sc[w][buf][1] + 16 * lo);
-                const bool odd = fs_clear(scv, base, seen, part);
-                *(kvm_u32x4 *)(sm.sc[w][buf][1] + 16 * lo) = scv;
-                if (odd && lo < 8u * NB) sm.odd = 1;
+                if (lo < 4u * NB) {
+                    kvm_u32x4 *const at = (kvm_u32x4 *)(sm.sc[w][buf] + 512 + 16 * lo);
+                    kvm_u32x4 scv = *at;
+                    if (fs_clear(scv, 32 * half + 8 * (lo & 3u), seen, part)) sm.odd = 1;
+                    *at = scv;
+                }
             }
-            if (more) copies(en, buf ^ 1);
+            copies(en, buf ? buf - 1 : SETS);
 
+            // ---- S^T of 32 keys: K operand i + 1 is made while the MFMA of i runs; what
+            // comes from LDS is read two steps ahead
+            kvm_f32x16 S;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                // ---- S^T of 32 keys: K operand i + 1 is made while the MFMA of i runs; what
-                // comes from LDS is read two steps ahead
-                kvm_f32x16 S;
+            for (int r = 0; r < 16; ++r) S[r] = 0.0f;
+            uint32_t ksc[NB];                         // the scales of the lane's key
+            {
+                const uint32_t k = fs_key(fs_opaque(l) & 31u);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) S[r] = 0.0f;
-                uint32_t ksc[NB];                         // the scales of the lane's key
-                {
-                    const uint32_t k = fs_key(fs_opaque(l) & 31u);
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) ksc[b] = *(const uint16_t *)(sm.sc[w][buf][0] + ((2 * half + (k >> 4)) * NB + b) * 32 + 2 * (k & 15));
-                }
-                const uint32_t lq = fs_opaque(l);
-                const uint8_t *const sq = sm.q + (lq >> 5) * QU + (lq & 31u) * 16;
-                // operands in the order of the K loads: (block pair, 16-dim half | block of the pair)
-                auto k_op = [&](int i) {
-                    const kvm_u32x4 x = kr[half % SETS][i >> 1];
-                    return pf_q8(x[2 * (i & 1)], x[2 * (i & 1) + 1], ksc[2 * (i >> 2) + (i & 1)]);
-                };
-                auto q_op = [&](int i) { return *(const kvm_f16x8 *)(sq + 2 * (4 * (i >> 2) + 2 * (i & 1) + (i >> 1 & 1)) * QU); };
-                kvm_f16x8 kop = k_op(0), qr[3] = {q_op(0), q_op(1)};
-#pragma unroll
-                for (int i = 0; i < KS; ++i) {
-                    if (i + 2 < KS) qr[(i + 2) % 3] = q_op(i + 2);
-                    FS_FENCE();
-                    S = __builtin_amdgcn_mfma_f32_32x32x16_f16(kop, qr[i % 3], S, 0, 0, 0);
-                    if (i + 1 < KS) kop = k_op(i + 1);
-                    FS_FENCE();
-                }
-                if (SETS == 2) load_k(rk, half);
-                else if (half == 0) load_k(rsrc(k_head, e, KB, true), 1);
-                else load_k(rk, 0);
-
-                // ---- softmax: P as f16 operands
-                if (!full) fs_mask(S, &sm.cp[w][buf][32 * half], qlim);
-                float x = S[0];
-#pragma unroll
-                for (int r = 1; r < 16; ++r) x = fmaxf(x, S[r]);
-                x = kvm_max_xor32(x);
-                const bool up = fmaf(x, a.c, -ms) > FS_LAZY;      // false for a row with nothing visible yet
-                if (__builtin_amdgcn_ballot_w64(up) != 0) {
-                    const float mnew = up ? x * a.c : ms;
-                    const float alpha = up ? __builtin_amdgcn_exp2f(ms - mnew) : 1.0f;
-                    ms = mnew;
-                    lp *= alpha;
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) O[dt] *= alpha;
-                }
-                const float ref = ms == -INFINITY ? 0.0f : ms;
-                kvm_f16x8 pb[2];
-                float sum = 0.0f;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    // the row sum takes p before its rounding to the f16 operand: within
-                    // 2^-11 of it per element
-                    const float y = __builtin_amdgcn_exp2f(fmaf(S[r], a.c, -ref));
-                    pb[r >> 3][r & 7] = (_Float16)y;
-                    sum += y;
-                }
-                lp += sum;
-
-                // ---- O^T += V^T P^T
-                kvm_u32x4 vs[3];
-                const uint8_t *const sv = sm.sc[w][buf][1] + (fs_opaque(l) >> 5) * 16;
-                auto v_scale = [&](int i) { vs[i % 3] = *(const kvm_u32x4 *)(sv + (((i >> 1) * 2 + half) * 4 + 2 * (i & 1)) * 16); };
-                v_scale(0);
-                v_scale(1);
-                kvm_f16x8 vop = pf_q4(vq[0], vs[0]);
-#pragma unroll
-                for (int i = 0; i < 2 * DT; ++i) {
-                    if (i + 2 < 2 * DT) v_scale(i + 2);
-                    FS_FENCE();
-                    O[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vop, pb[i & 1], O[i >> 1], 0, 0, 0);
-                    if (i + 1 < 2 * DT) vop = pf_q4(vq[i + 1], vs[(i + 1) % 3]);
-                    FS_FENCE();
-                }
-                if (half == 0) load_v(rsrc(v_head, e, VB, true), 1);
-                else load_v(rv, 0);
+                for (int b = 0; b < NB; ++b) ksc[b] = *(const uint16_t *)(sm.sc[w][buf] + ((k >> 4) * NB + b) * 32 + 2 * (k & 15));
             }
-            e = en;
+            const uint32_t lq = fs_opaque(l);
+            const uint8_t *const sq = sm.q + (lq >> 5) * QU + (lq & 31u) * 16;
+            // operands in the order of the K loads: (block pair, 16-dim half | block of the pair)
+            auto k_op = [&](int i) {
+                const kvm_u32x4 x = kr[set][i >> 1];
+                return pf_q8(x[2 * (i & 1)], x[2 * (i & 1) + 1], ksc[2 * (i >> 2) + (i & 1)]);
+            };
+            auto q_op = [&](int i) { return *(const kvm_f16x8 *)(sq + 2 * (4 * (i >> 2) + 2 * (i & 1) + (i >> 1 & 1)) * QU); };
+            kvm_f16x8 kop = k_op(0), qr[3] = {q_op(0), q_op(1)};
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                if (i + 2 < KS) qr[(i + 2) % 3] = q_op(i + 2);
+                FS_FENCE();
+                S = __builtin_amdgcn_mfma_f32_32x32x16_f16(kop, qr[i % 3], S, 0, 0, 0);
+                if (i + 1 < KS) kop = k_op(i + 1);
+                FS_FENCE();
+            }
+            load_k(rk, set);
+
+            // ---- softmax: P as f16 operands
+            if (!full) fs_mask(S, &sm.cp[w][buf][32 * half], qlim);
+            float x = S[0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) x = fmaxf(x, S[r]);
+            x = kvm_max_xor32(x);
+            const bool up = fmaf(x, a.c, -ms) > FS_LAZY;      // false for a row with nothing visible yet
+            if (__builtin_amdgcn_ballot_w64(up) != 0) {
+                const float mnew = up ? x * a.c : ms;
+                const float alpha = up ? __builtin_amdgcn_exp2f(ms - mnew) : 1.0f;
+                ms = mnew;
+                lp *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) O[dt] *= alpha;
+            }
+            const float ref = ms == -INFINITY ? 0.0f : ms;
+            kvm_f16x8 pb[2];
+            float sum = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                // the row sum takes p before its rounding to the f16 operand: within
+                // 2^-11 of it per element
+                const float y = __builtin_amdgcn_exp2f(fmaf(S[r], a.c, -ref));
+                pb[r >> 3][r & 7] = (_Float16)y;
+                sum += y;
+            }
+            lp += sum;
+
+            // ---- O^T += V^T P^T
+            kvm_u32x4 vs[3];
+            const uint8_t *const sv = sm.sc[w][buf] + 512 + (fs_opaque(l) >> 5) * 16;
+            auto v_scale = [&](int i) { vs[i % 3] = *(const kvm_u32x4 *)(sv + ((i >> 1) * 4 + 2 * (i & 1)) * 16); };
+            v_scale(0);
+            v_scale(1);
+            kvm_f16x8 vop = pf_q4(vq[set][0], vs[0]);
+#pragma unroll
+            for (int i = 0; i < 2 * DT; ++i) {
+                if (i + 2 < 2 * DT) v_scale(i + 2);
+                FS_FENCE();
+                O[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vop, pb[i & 1], O[i >> 1], 0, 0, 0);
+                if (i + 1 < 2 * DT) vop = pf_q4(vq[set][i + 1], vs[(i + 1) % 3]);
+                FS_FENCE();
+            }
+            load_v(rv, set);
+            buf = buf == SETS ? 0 : buf + 1;
+        };
+        for (uint32_t j = j0; j < n_t; j += 2) {
+            item(j, std::integral_constant<int, 0>{});
+            if constexpr (SETS == 2) {
+                if ((j += 2) >= n_t) break;
+                item(j, std::integral_constant<int, 1>{});
+            }
         }
-        if (__builtin_amdgcn_readfirstlane(sm.odd)) fs_add_odd<D, true>(O, sg, v_head, sm.list, w, 4, n_t, some_lim, all_lim, qlim, sm.odd_v[w]);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the last items' copies, which nobody reads)
+        if (__builtin_amdgcn_readfirstlane(sm.odd)) fs_add_odd<D, true>(O, sg, v_head, sm.list, j0, 2, n_t, 32 * half, 32, some_lim, all_lim, qlim, sm.odd_v[w]);
     }
 
     // ---- the waves' sums: one maximum, then each wave's quarter of the dims from the others,
@@ -715,7 +729,7 @@ __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg
                 accumulate(R0, sv + TB / 2, pb1, nothing);
                 KVM_LDS_BARRIER();
             }
-            if (__builtin_amdgcn_readfirstlane(sm.odd)) fs_add_odd<D, QUANT>(O, sg, v_head, sm.list, 0, 1, n_t, some_lim, all_lim, qlim, sm.odd_v[w]);
+            if (__builtin_amdgcn_readfirstlane(sm.odd)) fs_add_odd<D, QUANT>(O, sg, v_head, sm.list, 0, 1, n_t, 0, 64, some_lim, all_lim, qlim, sm.odd_v[w]);
             b0 += FS_BATCH;
             if (b0 >= i_hi) break;
             fs_cells<8> next;
