@@ -379,16 +379,11 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
         auto rsrc = [&](const uint8_t *head, uint32_t e, uint32_t bytes, bool more) {
             return __builtin_amdgcn_make_buffer_rsrc((void *)(head + (uint64_t)(e & 0x7fffffffu) * bytes), (short)0, more ? bytes : 0u, 0x00020000);
         };
-        auto load_k = [&](__amdgpu_buffer_rsrc_t r, int set) {
-            const uint32_t at = fs_opaque(k_lane);
-#pragma unroll
-            for (int i = 0; i < NB; ++i)
-                kr[set][i] = __builtin_amdgcn_raw_buffer_load_b128(r, at + (i & 1) * 512, half * NB * 1024 + (i >> 1) * 1024, 0);
+        auto load_k = [&](__amdgpu_buffer_rsrc_t r, int set, int i) {
+            kr[set][i] = __builtin_amdgcn_raw_buffer_load_b128(r, fs_opaque(k_lane) + (i & 1) * 512, half * NB * 1024 + (i >> 1) * 1024, 0);
         };
-        auto load_v = [&](__amdgpu_buffer_rsrc_t r, int set) {
-            const uint32_t at = fs_opaque(v_lane);
-#pragma unroll
-            for (int i = 0; i < 2 * DT; ++i) vq[set][i] = __builtin_amdgcn_raw_buffer_load_b32(r, at + (i & 1) * 256, half * 4 + (i >> 1) * 1024, 0);
+        auto load_v = [&](__amdgpu_buffer_rsrc_t r, int set, int i) {
+            vq[set][i] = __builtin_amdgcn_raw_buffer_load_b32(r, fs_opaque(v_lane) + (i & 1) * 256, half * 4 + (i >> 1) * 1024, 0);
         };
         // lanes below 2 NB: the half's K scales, from 32 on its V scales (units of 8 keys of a block)
         auto copies = [&](uint32_t e, uint32_t buf) {
@@ -406,8 +401,10 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
                 const uint32_t e = entry(j0 + 2 * x);
                 const bool more = j0 + 2 * x < n_t;
                 copies(e, x);
-                load_k(rsrc(k_head, e, KB, more), x);
-                load_v(rsrc(v_head, e, VB, more), x);
+#pragma unroll
+                for (int i = 0; i < NB; ++i) load_k(rsrc(k_head, e, KB, more), x, i);
+#pragma unroll
+                for (int i = 0; i < 2 * DT; ++i) load_v(rsrc(v_head, e, VB, more), x, i);
             }
         }
         uint32_t buf = 0;
@@ -458,9 +455,9 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
                 FS_FENCE();
                 S = __builtin_amdgcn_mfma_f32_32x32x16_f16(kop, qr[i % 3], S, 0, 0, 0);
                 if (i + 1 < KS) kop = k_op(i + 1);
+                if (i & 1) load_k(rk, set, i >> 1);
                 FS_FENCE();
             }
-            load_k(rk, set);
 
             // ---- softmax: P as f16 operands
             if (!full) fs_mask(S, &sm.cp[w][buf][32 * half], qlim);
@@ -503,9 +500,9 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
                 FS_FENCE();
                 O[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vop, pb[i & 1], O[i >> 1], 0, 0, 0);
                 if (i + 1 < 2 * DT) vop = pf_q4(vq[set][i + 1], vs[(i + 1) % 3]);
+                load_v(rv, set, i);
                 FS_FENCE();
             }
-            load_v(rv, set);
             buf = buf == SETS ? 0 : buf + 1;
         };
         for (uint32_t j = j0; j < n_t; j += 2) {
