@@ -101,6 +101,9 @@ struct fs_geo {
     static constexpr uint32_t KB = QUANT ? 64u * D + 128u * NB : 128u * D, VB = QUANT ? 32u * D + 128u * NB : 128u * D;
     static constexpr uint32_t TB = 128u * D;              // bytes of an f16 K (or V) tile
     static constexpr uint32_t QU = 528;                   // LDS bytes of a unit of Q: 8 dims of 32 rows, 16 bytes apart in the banks
+    // Of 256 dims every third Q operand of a wide unit is read from LDS: all 16 in registers
+    // are 24 too many (spilled, their reloads were half of a tile's time)
+    static constexpr int QL = D == 256 ? 5 : 0;
     static constexpr int SETS = D == 256 ? 1 : 2;         // half tiles that a wave has in registers
     static constexpr int NQ = D / 32;                     // quads that a wave adds up at the end of a narrow piece
 };
@@ -134,6 +137,7 @@ struct fs_lds_wide : fs_list<D, 8> {
         alignas(16) uint8_t ring[2][2 * G::TB];           // K, V tile; V in units of 8 keys of a dim: [32-key half][16-dim tile][8-key group][dim]
     };
     alignas(16) int32_t cp[2][64];
+    alignas(16) uint8_t ql[4][G::QL ? G::QL : 1][1024];   // the Q operands that stay here
 };
 
 // x, from which the compiler cannot tell that a value formed of it does not change in a
@@ -617,8 +621,14 @@ __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg
         kvm_f32x16 O[DT];
         float ms = -INFINITY, lp = 0.0f;
         kvm_f16x8 qop[KS];       // lane (g2, m2): Q[row m2][16 ks + 8 g2 .. + 7]
+        auto in_lds = [](int ks) { return G::QL && ks % 3 == 1; };
+        uint8_t *const ql = sm.ql[rg][0] + 16 * lc;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) qop[ks] = *(const kvm_f16x8 *)(sm.q4[rg] + (2 * ks + g2) * QU + m2 * 16);
+        for (int ks = 0; ks < KS; ++ks) {
+            const kvm_f16x8 v = *(const kvm_f16x8 *)(sm.q4[rg] + (2 * ks + g2) * QU + m2 * 16);
+            if (in_lds(ks)) *(kvm_f16x8 *)(ql + ks / 3 * 1024) = v;
+            else qop[ks] = v;
+        }
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -637,13 +647,19 @@ __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg
             for (int r = 0; r < 16; ++r) S[r] = 0.0f;
             kvm_f16x8 kr[KR];
             auto ld = [&](int ks) { return *(const kvm_f16x8 *)(sk + ks * 512); };
+            kvm_f16x8 qn;
+            auto ldq = [&](int ks) {
+                if (in_lds(ks)) qn = *(const kvm_f16x8 *)(sm.ql[rg][0] + 16 * fs_opaque(l) + ks / 3 * 1024);
+            };
+            ldq(1);
 #pragma unroll
             for (int i = 0; i < KR - 1; ++i) kr[i] = ld(i);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 if (ks + KR - 1 < KS) kr[(ks + KR - 1) % KR] = ld(ks + KR - 1);
                 FS_FENCE();
-                S = __builtin_amdgcn_mfma_f32_32x32x16_f16(kr[ks % KR], qop[ks], S, 0, 0, 0);
+                S = __builtin_amdgcn_mfma_f32_32x32x16_f16(kr[ks % KR], in_lds(ks) ? qn : qop[ks], S, 0, 0, 0);
+                if (in_lds(ks) && ks + 3 < KS) ldq(ks + 3);
                 between(ks);
                 FS_PIN(S);
             }
@@ -685,12 +701,16 @@ __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg
                 sum = 0.0f;
             } else if (i >= KS / 2) {
 #pragma unroll
-                for (int j = 0; j < EP; ++j) {
+                for (int j = 0; j < EP; j += 2) {
                     // (the row sum takes p before its rounding)
                     const int r = EP * (i - KS / 2) + j;
-                    const float y = __builtin_amdgcn_exp2f(fmaf(S[r], c, -ref));
-                    pb[r >> 3][r & 7] = (_Float16)y;
-                    sum += y;
+                    const float y0 = __builtin_amdgcn_exp2f(fmaf(S[r], c, -ref)), y1 = __builtin_amdgcn_exp2f(fmaf(S[r + 1], c, -ref));
+                    kvm_f16x2 h = {(_Float16)y0, (_Float16)y1};
+                    sum += y0;
+                    sum += y1;
+                    asm volatile("" : "+v"(h), "+v"(sum)); // here, not where they are used
+                    pb[r >> 3][r & 7] = h[0];
+                    pb[r >> 3][(r & 7) + 1] = h[1];
                 }
             }
         };
