@@ -1087,11 +1087,12 @@ static uint32_t fs_stride(uint32_t n) {
 }
 
 // The rows from which on a window's units are wide.  An f16 window has nothing to convert: all.
-// A CU's workgroup takes a tile of a wide unit of 256 dims in 2.6 - 3.1 us, its two narrow ones
-// a tile of theirs in 1.5: a wide unit pays from three narrow ones' rows on.  Where some windows
+// A CU's workgroup takes a tile of a wide unit of 256 dims in 2.0 us, its two narrow ones a tile
+// of theirs in 1.4: a wide unit pays from three narrow ones' rows on (two's: 48 rows over 32,768
+// cells with 8 x 6 over 2,048, all narrow 43 us, else 34 + 16).  Where some windows
 // stay narrow all the same, the wide ones are a launch more (10 us for its start and end) and
-// have to save that: 288 rows over 5,003 cells with 16 x 18 over 8,192, all narrow 79 us, else
-// 28 + 61; 768 rows over 32,768 with 32 x 24 over 2,048, 277 us and 175 + 41.
+// have to save that: 288 rows over 5,003 cells with 16 x 18 over 8,192, all narrow 73 us, else
+// 37 + 52; 768 rows over 32,768 with 32 x 24 over 2,048, 246 us and 136 + 37.
 static uint32_t fs_wide_rows(const kvm_window *prefix, const kvm_window *const *windows, const uint32_t *n_tokens, uint32_t n_lanes, bool quant,
                              uint32_t n_cu, uint32_t H, uint32_t G, uint32_t n_rows) {
     if (!quant) return 1;
@@ -1100,7 +1101,7 @@ static uint32_t fs_wide_rows(const kvm_window *prefix, const kvm_window *const *
     auto add = [&](const kvm_window *w, uint32_t r) {
         if (!w || !r) return;
         if (r <= 64) narrow = true;
-        else saved += (double)(w->n_cells / KVM_TILE_CELLS) * H / n_cu * (1.5 * fs_row_tiles(false, r) - 2.8 * fs_row_tiles(true, r));
+        else saved += (double)(w->n_cells / KVM_TILE_CELLS) * H / n_cu * (1.4 * fs_row_tiles(false, r) - 2.0 * fs_row_tiles(true, r));
     };
     add(prefix, n_rows);
     for (uint32_t i = 0; i < n_lanes; ++i) add(windows ? windows[i] : nullptr, n_tokens[i] * G);
