@@ -602,8 +602,8 @@ int kvm_fa_decode_lanes(kvm_state *st, const kvm_lane *lanes, uint32_t n_lanes, 
  * (a system prompt, a document): every token attends over the prefix window's
  * cells and its own conversation's, one softmax over both, with kvm_fa_decode's
  * visibility rule in each (positions in a lane's own window go on after the
- * prefix).  The prefix's keys and values are read once for 32 query rows (a
- * row is a token and a query head of a kv head's group), of whichever lanes,
+ * prefix).  The prefix's keys and values are read once for 32 or 128 query rows
+ * (a row is a token and a query head of a kv head's group), of whichever lanes,
  * not once per lane.  The reference keeps every conversation's cells in that
  * conversation's window (docs/multi-lane-conversations.md:1-20).
  * n_tokens: host [n_lanes], tokens of each lane (0 allowed); q, q_pos and out
@@ -615,7 +615,10 @@ int kvm_fa_decode_lanes(kvm_state *st, const kvm_lane *lanes, uint32_t n_lanes, 
  * Arithmetic as kvm_fa_prefill's: f16 operands (q, the cells' values, the
  * probabilities), fp32 sums, one rounding to out_type.  A token that sees no
  * cell outputs zeros; what cells hold that a token does not see does not reach
- * its output, be it infinite or no number. */
+ * its output, be it infinite or no number.  Windows' k, v and cell_pos: 16-byte
+ * aligned.  Partial sums go through the state's workspace: calls of one state, and
+ * replays of graphs captured from it, follow one another.  A capture cannot grow
+ * it (KVM_ENOMEM): call once before with as many tokens and cells. */
 int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, const kvm_window *const *windows,
                          const uint32_t *n_tokens, uint32_t n_lanes, const void *q, int q_type,
                          const int32_t *q_pos, uint32_t n_head, float scale, int out_type, void *out);

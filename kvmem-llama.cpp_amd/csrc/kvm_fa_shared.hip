@@ -1209,11 +1209,13 @@ extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, con
         if (rc) return kvm_fail(st, rc, "%s: %s %u: bad window", what, i == n_lanes ? "prefix," : "lane", i);
         if (w->n_head_kv != w0->n_head_kv || w->head_dim != w0->head_dim || kvm_k_quant(w->k_type) != kvm_k_quant(w0->k_type))
             return kvm_fail(st, KVM_EUNSUPPORTED, "%s: lane %u: windows of different heads or types", what, i);
+        if (((uintptr_t)w->k | (uintptr_t)w->v | (uintptr_t)w->cell_pos) & 15)
+            return kvm_fail(st, KVM_EINVAL, "%s: lane %u: a window that is not aligned to 16 bytes", what, i);
         if (w->n_cells / KVM_TILE_CELLS > 65535) return kvm_fail(st, KVM_ERANGE, "%s: lane %u: %u cells", what, i, w->n_cells);
     }
     const uint32_t H = w0->n_head_kv, D = w0->head_dim;
     if (n_head == 0 || n_head % H) return kvm_fail(st, KVM_EINVAL, "%s: %u heads on %u", what, n_head, H);
-    if (!std::isfinite(scale)) return kvm_fail(st, KVM_EINVAL, "%s: scale %g", what, (double)scale);
+    if (!std::isfinite(scale * 1.4426950408889634f)) return kvm_fail(st, KVM_EINVAL, "%s: scale %g", what, (double)scale);
     if (total * (n_head / H) > (1u << 24)) return kvm_fail(st, KVM_ERANGE, "%s: %llu tokens", what, (unsigned long long)total);
     if (H > 65535) return kvm_fail(st, KVM_ERANGE, "%s: %u kv heads", what, H);
     if (total == 0) return KVM_OK;
@@ -1251,9 +1253,9 @@ extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, con
     }
     // a workgroup of the join has 8 dims, or more of them where all CUs have two all the same
     // (its start is most of its work: 768 rows of 256 dims, 15.6 us by 8 dims)
-    const uint32_t blocks = kvm_cdiv(a.n_rows, 32) * H;
+    const uint64_t blocks = (uint64_t)kvm_cdiv(a.n_rows, 32) * H;
     uint32_t by = D / 8;
-    while (by > 1 && (uint64_t)blocks * by >= 4ull * st->n_cu) by /= 2;
+    while (by > 1 && blocks * by >= 4ull * st->n_cu) by /= 2;
     auto go = [&](auto d, auto qt) {
         constexpr int DD = decltype(d)::value;
         constexpr bool Q = decltype(qt)::value;

@@ -12,6 +12,11 @@ def _window(cells=128, H=2, D=128, kt=L.T_Q8_0, vt=L.T_Q4_0):
     return w
 
 
+def _at(w, off):
+    w.v += off
+    return w
+
+
 def _call(prefix, windows, counts, heads=8, q_type=L.T_F32, out_type=L.T_F32, scale=1.0, lanes=None):
     n = len(counts)
     arr = (C.POINTER(L.Window) * max(n, 1))(*[C.pointer(w) if w else None for w in windows])
@@ -36,7 +41,10 @@ def _call(prefix, windows, counts, heads=8, q_type=L.T_F32, out_type=L.T_F32, sc
     (L.KVM_EINVAL, lambda: _call(_window(), [None], [1], heads=7)),
     (L.KVM_EINVAL, lambda: _call(_window(), [None], [1], heads=0)),
     (L.KVM_EINVAL, lambda: _call(_window(), [None], [1], scale=float("nan"))),
+    (L.KVM_EINVAL, lambda: _call(_window(), [None], [1], scale=3e38)),
     (L.KVM_EINVAL, lambda: _call(_window(cells=100), [None], [1])),
+    (L.KVM_EINVAL, lambda: _call(_at(_window(), 8), [None], [1])),
+    (L.KVM_EINVAL, lambda: _call(_window(), [_at(_window(), 4)], [1])),
 ])
 def test_refusals(code, call):
     assert call() == code

@@ -141,6 +141,39 @@ def test_few_rows_beside_many(kvm_state, H, D, cache):
 
 
 @pytest.mark.parametrize("cache", ["q8_0", "f16"])
+def test_no_prefix(kvm_state, cache):
+    """Conversations alone, of hundreds of rows and of few, one without cells: its tokens give
+    zeros, whatever was there."""
+    rng, H, G, D = np.random.default_rng(18), 4, 8, 128
+    lanes, counts = [(192, 150), (4096, 4000), None, (64, 1), (640, 600)], [1, 80, 3, 1, 6]
+    qp = np.concatenate([(x[1] if x else 5) - c + np.arange(c) for x, c in zip(lanes, counts)])
+    got, *_ = run(kvm_state, rng, H, G, D, cache, 0, None, [x and (x[0], cells(x[0], x[1], 0)) for x in lanes], counts,
+                  torch.float32, torch.bfloat16, q_pos=qp)
+    assert not got[81:84].any() and bool(got[:81].any(2).all()) and bool(got[84:].any(2).all())
+
+
+def test_a_window_twice(kvm_state):
+    """The prefix's window as a lane's own too, and one window for two lanes: its cells count twice."""
+    st, rng, H, G, D = kvm_state, np.random.default_rng(19), 2, 4, 128
+    pre, own = (window(st, rng, n, H, D, "q8_0", cells(n, n, 0)) for n in (256, 64))
+    q = torch.from_numpy(rng.standard_normal((3, H * G, D)).astype(np.float32)).cuda()
+    qp = torch.tensor([200, 40, 63], dtype=torch.int32, device="cuda")
+    owns = [pre, own, own]
+    got = api.fa_decode_shared(st, pre[0], [x[0] for x in owns], [1, 1, 1], q, qp, H * G, D ** -0.5)
+    check(got, *expected(q, qp, [1, 1, 1], pre, owns, H, D ** -0.5))
+
+
+def test_output_over_the_queries(kvm_state):
+    """The output may be the queries' memory: they are read before it is written."""
+    st, rng, H, G, D = kvm_state, np.random.default_rng(20), 2, 4, 128
+    w = window(st, rng, 512, H, D, "q8_0", cells(512, 512, 0))
+    q = torch.from_numpy(rng.standard_normal((2, H * G, D)).astype(np.float32)).cuda()
+    qp = torch.tensor([511, 300], dtype=torch.int32, device="cuda")
+    want = api.fa_decode_shared(st, w[0], [None, None], [1, 1], q, qp, H * G, D ** -0.5)
+    assert torch.equal(api.fa_decode_shared(st, w[0], [None, None], [1, 1], q, qp, H * G, D ** -0.5, out=q), want)
+
+
+@pytest.mark.parametrize("cache", ["q8_0", "f16"])
 def test_long_prefix(kvm_state, cache):
     """Many tiles a wave, several looks at a piece's tiles (one kv head, one row group: all
     tiles of 524,288 cells are a few workgroups' when the chip has few)."""
