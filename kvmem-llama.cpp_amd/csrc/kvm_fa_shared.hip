@@ -56,12 +56,12 @@ struct fs_args {
     float *ws_o;                 // pieces of 32 rows: [slot][dim / 8][lane][4]
     float *ws_ml;                // [slot][row][2]: scaled maximum, sum
     uint32_t H, G, n_head, n_rows;
-    uint32_t n_seg, n_wide;      // segments, the wide ones before the narrow ones
+    uint32_t wide, narrow;       // pieces; the wide ones' segments come first
     float c, q_sign;             // |scale| log2(e); q times -1 for a negative scale, and 0 (c = 1) for none
     int q_type;
     // Pieces of the segments before; a segment's: [head][piece of the unit][unit of the head],
     // so that neighbours read the same tiles.  A wide piece has 4 slots, a narrow one 1.
-    uint32_t piece0[FS_SEGS + 1];
+    uint32_t piece0[FS_SEGS];    // (past the last segment: ~0)
     fs_seg seg[FS_SEGS];
 };
 static_assert(sizeof(fs_args) <= 4096, "kernel arguments");
@@ -896,15 +896,14 @@ __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg
 // The workgroup's piece.
 template <bool WIDE, class F>
 __device__ __forceinline__ void fs_piece(const fs_args &a, F &&piece) {
-    const uint32_t l = threadIdx.x & 63u, n_before = a.piece0[a.n_wide], n = WIDE ? n_before : a.piece0[a.n_seg] - n_before;
+    // (loads that wait for no other)
+    const uint32_t piece0 = a.piece0[threadIdx.x & 63u], last0 = a.piece0[64], n_before = a.wide, n = WIDE ? n_before : a.narrow;
     // neighbours on one XCD
-    uint32_t p = blockIdx.x;
-    if (gridDim.x >= 8) p = (p & 7u) * (gridDim.x / 8) + (p >> 3);
+    const uint32_t each = (n + 7) / 8;
+    uint32_t p = n < 8 ? blockIdx.x : (blockIdx.x & 7u) * each + (blockIdx.x >> 3);
     if (p >= n) return;
     if (!WIDE) p += n_before;
-    uint32_t s = __popcll(__builtin_amdgcn_ballot_w64(l < a.n_seg && a.piece0[l < a.n_seg ? l : 0u] <= p)) - 1;
-    if (a.n_seg > 64 && a.piece0[64] <= p) s = 64;
-    s = __builtin_amdgcn_readfirstlane(s);
+    const uint32_t s = __builtin_amdgcn_readfirstlane(last0 <= p ? 64u : (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(piece0 <= p)) - 1);
     const fs_seg &sg = a.seg[s];
     const uint32_t n_rt = fs_row_tiles(WIDE, sg.n_rows), x = p - a.piece0[s], y = x / n_rt, h = y / sg.pieces, j = y - h * sg.pieces;
     const uint32_t i_lo = j * sg.per + min(j, sg.more);
@@ -1115,11 +1114,11 @@ static uint32_t fs_piece_tiles(const fs_seg *seg, uint32_t n, bool wide, uint32_
 static int fs_shape(kvm_state *st, const char *what, const kvm_window *prefix, const kvm_window *const *windows,
                     const uint32_t *n_tokens, uint32_t n_lanes, bool quant, uint32_t n_cu, fs_args *a, fs_join_args *j, uint64_t *slots) {
     const uint32_t wide_rows = fs_wide_rows(prefix, windows, n_tokens, n_lanes, quant, n_cu, a->H, a->G, a->n_rows);
-    uint32_t n = 0, lane_seg[FS_LANES], own = 0;
+    uint32_t n = 0, nw = 0, lane_seg[FS_LANES], own = 0;
     auto add = [&](const kvm_window *w, uint32_t row0, uint32_t n_rows) {
         const uint32_t t = w->n_cells / KVM_TILE_CELLS;
         a->seg[n++] = fs_seg{(const uint8_t *)w->k, (const uint8_t *)w->v, w->cell_pos, t, fs_stride(t), row0, n_rows, 1, t, 0};
-        if (n_rows >= wide_rows) a->n_wide = n;
+        if (n_rows >= wide_rows) nw = n;
     };
     if (prefix) add(prefix, 0, a->n_rows);                 // (wide where a conversation is)
     for (int narrow = 0; narrow < 2; ++narrow) {
@@ -1137,13 +1136,11 @@ static int fs_shape(kvm_state *st, const char *what, const kvm_window *prefix, c
             row += r;
         }
     }
-    a->n_seg = n;
     // Workgroups: what the CUs hold at once.  A tile or more for each wave that has tiles of its
     // own, or half a one where that leaves CUs idle (8 rows over 1,024 + 2 x 256 f16 cells of 2
     // heads: 8.7 us, with 4 tiles a workgroup 15.6; 12 over 1,024 + 2 x 256 q8_0 cells of 4: 2
     // tiles 12.1 us, 4 13.8); a second narrow workgroup a CU for pieces of 4 tiles or more (48 over
     // 4,032 + 4 x 512: 320 workgroups of 2 tiles 19.0, 160 of 4 16.5).
-    const uint32_t nw = a->n_wide;
     const uint32_t tw = fs_piece_tiles(a->seg, nw, true, a->H, n_cu, 1);
     uint32_t tn = fs_piece_tiles(a->seg + nw, n - nw, false, a->H, n_cu, 2);
     if (tn > 4) tn = fs_piece_tiles(a->seg + nw, n - nw, false, a->H, 2 * n_cu, 4);
@@ -1160,7 +1157,9 @@ static int fs_shape(kvm_state *st, const char *what, const kvm_window *prefix, c
         if (piece > (1u << 24))
             return kvm_fail(st, KVM_ERANGE, "%s: %u rows over these windows are too many for one call", what, a->n_rows);
     }
-    a->piece0[n] = (uint32_t)piece;
+    for (uint32_t i = n; i < FS_SEGS; ++i) a->piece0[i] = 0xffffffffu;
+    a->wide = (uint32_t)wide;
+    a->narrow = (uint32_t)(piece - wide);
     *slots = 4 * wide + (piece - wide);
     if (prefix) {
         j->pre_pieces = a->seg[0].pieces;
@@ -1252,9 +1251,8 @@ extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, con
         constexpr int DD = decltype(d)::value;
         constexpr bool Q = decltype(qt)::value;
         auto grid = [](uint32_t n) { return dim3(n < 8 ? n : (n + 7) / 8 * 8); };       // (a grid of 8 for each XCD's)
-        const uint32_t wide = a.piece0[a.n_wide], narrow = a.piece0[a.n_seg] - wide;
-        if (wide) hipLaunchKernelGGL((k_fs_wide<DD, Q>), grid(wide), dim3(512), 0, st->stream, a);
-        if (Q && narrow) hipLaunchKernelGGL((k_fs_narrow<DD>), grid(narrow), dim3(256), 0, st->stream, a);
+        if (a.wide) hipLaunchKernelGGL((k_fs_wide<DD, Q>), grid(a.wide), dim3(512), 0, st->stream, a);
+        if (Q && a.narrow) hipLaunchKernelGGL((k_fs_narrow<DD>), grid(a.narrow), dim3(256), 0, st->stream, a);
         hipLaunchKernelGGL((k_fs_join<DD>), dim3(kvm_cdiv(a.n_rows, 32), by, H), dim3(256), 0, st->stream, j);
     };
     auto go_d = [&](auto d) {
