@@ -1,0 +1,1274 @@
+// kvm_fa_shared.hip -- decode / verify attention of several conversations that share a
+// long prefix (kvm_fa_decode_shared): every query attends over the prefix window's cells
+// and its own conversation's, one softmax over both.
+//
+//   o_t = sum_c p_tc v_c / sum_c p_tc, p_tc = exp(scale q_t . k_c - m_t) over the cells c of
+//   both windows with 0 <= position <= the query's
+//
+// splits over any parts of the cells into (m, l, o) of each part, joined by the parts'
+// maxima.  A part is a piece: some tiles of one window for a unit, 32 or 128 rows of a kv
+// head (a row is a token and a query head of the group).  The prefix's rows are all
+// conversations' tokens side by side, so its keys and values are read, and brought to f16,
+// once for a unit's rows; a conversation's own window has that conversation's rows.
+// k_fs_wide and k_fs_narrow form the pieces, k_fs_join joins those of each row.
+//
+// S^T = K Q^T and O^T += V^T P^T on 32x32x16 f16 MFMAs, 32 rows a wave.  Quantised tiles
+// become f16 on the way: K and V as (f16)(q d); Q and P are rounded to f16, everything else
+// is fp32.  Key order: score row i of a half tile is key i with bits 2 and 3 swapped, so that
+// a lane's scores are 8 consecutive keys of each 16, what the P V operand wants.
+//   narrow units (quantised windows of few rows): workgroups of 4 waves, two a CU.
+//     Each wave takes every fourth half of the piece's tiles.  Nothing is shared in the loop and no
+//     barrier is in it: tiles go from memory into registers (the tile layout is the matrix
+//     operands') and are converted there; the waves' sums meet in LDS at the end.
+//   wide units: workgroups of 8 waves, one a CU.  Waves 0 - 3 have 32 rows each and take every
+//     key; waves 4 - 7 bring the next tile into one of two LDS buffers, converted, while the
+//     other is worked on.
+// The tiles of all units of a kind are dealt to the workgroups in equal shares, in an order
+// that steps through a window in strides: a part-filled window's live tiles are spread
+// evenly over its pieces.
+#include "kvm_f16_dev.h"
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#define FS_LANES 64u             // conversations of a call
+#define FS_SEGS (FS_LANES + 1)   // windows: theirs and the prefix
+#define FS_BATCH 256u            // tiles of a piece that are looked at at a time
+#define FS_LAZY 8.0f             // log2 growth of a row's maximum tolerated before a rescale
+
+typedef float kvm_f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void *fs_lds_ptr;
+typedef float kvm_f32x2 __attribute__((ext_vector_type(2)));
+
+// A window with the rows that attend over it.
+struct fs_seg {
+    const uint8_t *k, *v;
+    const int32_t *cell_pos;
+    uint32_t n_tiles, mult;      // tile i of a unit's order is (i mult) mod n_tiles
+    uint32_t row0, n_rows;       // rows [row0, row0 + n_rows) of every kv head
+};
+
+// The tiles [base, base + ..) of a kind's units, dealt to p workgroups: each has q, the first
+// r one more.
+struct fs_deal {
+    uint32_t base, p, q, r;
+    // workgroup i has the tiles from here to the next's
+    __host__ __device__ uint32_t first(uint32_t i) const { return base + i * q + (i < r ? i : r); }
+    // the workgroup that has tile x
+    __host__ __device__ uint32_t owner(uint32_t x) const {
+        x -= base;
+        const bool more = x < r * (q + 1);
+        return (more ? x : x - r * (q + 1)) / (more ? q + 1 : q) + (more ? 0 : r);
+    }
+};
+
+struct fs_args {
+    const void *q;
+    const int32_t *q_pos;
+    float *ws_o;                 // pieces of 32 rows: [slot][dim / 8][lane][4]
+    float *ws_ml;                // [slot][row][2]: scaled maximum, sum
+    uint32_t H, G, n_head, n_rows;
+    uint32_t n_seg, n_wide;      // segments, the wide ones before the narrow ones
+    fs_deal wide, narrow;
+    float c, q_sign;             // |scale| log2(e); q times -1 for a negative scale, and 0 (c = 1) for none
+    int q_type;
+    uint32_t tile0[FS_SEGS + 1]; // tiles of the units of the segments before
+    uint32_t slot0[FS_SEGS];     // unit u's piece of workgroup p: slots slot0 + (p + u) groups .. (mod 2^32)
+    fs_seg seg[FS_SEGS];
+};
+static_assert(sizeof(fs_args) <= 4096, "kernel arguments");
+
+// What the join reads.
+struct fs_join_args {
+    const float *ws_o, *ws_ml;
+    void *out;
+    int out_type;
+    uint32_t G, n_head, n_rows;
+    fs_deal wide, narrow;
+    uint32_t pre_tiles, pre_wide, pre_slot0;              // the prefix's (no tiles: none)
+    // conversations with a window, in order: first row (the rest: ~0), rows, tiles before, tiles
+    // (bit 31: wide), first slot
+    uint32_t row0[FS_LANES], rows[FS_LANES], tile0[FS_LANES], tiles[FS_LANES], slot0[FS_LANES];
+};
+
+__host__ __device__ inline uint32_t fs_unit_rows(bool wide) { return wide ? 128u : 32u; }
+__host__ __device__ inline uint32_t fs_row_tiles(bool wide, uint32_t n_rows) { return (n_rows + fs_unit_rows(wide) - 1) / fs_unit_rows(wide); }
+
+template <int D, bool QUANT>
+struct fs_geo {
+    static constexpr int KS = D / 16, NB = D / 32, DT = D / 32;              // k-steps, 32-dim blocks, dim tiles
+    static constexpr uint32_t KB = QUANT ? 64u * D + 128u * NB : 128u * D, VB = QUANT ? 32u * D + 128u * NB : 128u * D;
+    static constexpr uint32_t TB = 128u * D;              // bytes of an f16 K (or V) tile
+    static constexpr uint32_t QU = 528;                   // LDS bytes of a unit of Q: 8 dims of 32 rows, 16 bytes apart in the banks
+    // Of 256 dims every third Q operand of a wide unit is read from LDS: all 16 in registers
+    // are 24 too many (spilled, their reloads were half of a tile's time)
+    static constexpr int QL = D == 256 ? 5 : 0;
+    static constexpr int SETS = D == 256 ? 1 : 2;         // half tiles that a wave has in registers
+    static constexpr int NQ = D / 32;                     // quads that a wave adds up at the end of a narrow piece
+};
+
+// What both kinds have in LDS; NW: waves.
+template <int D, int NW>
+struct fs_list {
+    alignas(16) float odd_v[4][D];
+    uint32_t odd;                // the batch has values that are no finite numbers where not all rows see them
+    uint32_t list[FS_BATCH];
+    uint8_t flag[FS_BATCH];
+};
+template <int D>
+struct fs_lds_narrow : fs_list<D, 4> {
+    using G = fs_geo<D, true>;
+    union {
+        struct {                                          // a wave's half tile and its next
+            alignas(16) uint8_t q[2 * G::KS * G::QU];
+            alignas(16) uint8_t sc[4][G::SETS + 1][1024]; // K scales, V scales
+            alignas(16) int32_t cp[4][G::SETS + 1][64];   // and the tile's cells' positions
+        };
+        alignas(16) float x[4][2][G::NQ * 256];           // at the end: chunks of O on their way
+    };
+    float ml[4][2][32];
+};
+template <int D, bool QUANT>
+struct fs_lds_wide : fs_list<D, 8> {
+    using G = fs_geo<D, QUANT>;
+    union {
+        alignas(16) uint8_t q4[4][2 * G::KS * G::QU];     // at the start: the four waves' rows
+        alignas(16) uint8_t ring[2][2 * G::TB];           // K, V tile; V in units of 8 keys of a dim: [32-key half][16-dim tile][8-key group][dim]
+    };
+    alignas(16) int32_t cp[2][64];
+    alignas(16) uint8_t ql[4][G::QL ? G::QL : 1][1024];   // the Q operands that stay here
+};
+
+// x, from which the compiler cannot tell that a value formed of it does not change in a
+// loop: hoisted, lane addresses take the registers that the accumulators need.
+__device__ __forceinline__ uint32_t fs_opaque(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+// K row i of a half tile is this key: bits 2 and 3 swapped.
+__device__ __forceinline__ uint32_t fs_key(uint32_t i) { return (i & 0x13) | (i & 4) << 1 | (i & 8) >> 1; }
+
+// Nothing moves over it.
+#define FS_FENCE() __builtin_amdgcn_sched_barrier(0)
+
+// Q rows [row_g, row_g + rows) of head h, RG groups of 32: loaded, then as f16 operands into
+// LDS (rows past the last: zeros).  8 rows x 8 units of 8 dims an instruction.
+template <int D, int RG, int NW>
+struct fs_rows {
+    static constexpr uint32_t KS = D / 16, QU = 528;
+    static constexpr int N = 32 * RG * 2 * KS / (64 * NW);
+    kvm_u32x4 y[N][2];
+    __device__ __forceinline__ void load(const fs_args &a, uint32_t h, uint32_t row_g, uint32_t rows) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t x = threadIdx.x + 64 * NW * i, b = x >> 6, r = b % (4 * RG) * 8 + (x & 63u) / 8, u = b / (4 * RG) * 8 + (x & 7u);
+            const uint32_t row = row_g + (r < rows ? r : 0u), t = row / a.G;
+            const uint64_t e = ((uint64_t)t * a.n_head + h * a.G + (row - t * a.G)) * D + 8 * u;
+            if (a.q_type == KVM_TYPE_F32) __builtin_memcpy(y[i], (const float *)a.q + e, 32);
+            else __builtin_memcpy(y[i], (const uint16_t *)a.q + e, 16);
+        }
+    }
+    __device__ __forceinline__ void store(const fs_args &a, uint32_t rows, uint8_t *dst) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t x = threadIdx.x + 64 * NW * i, b = x >> 6, r = b % (4 * RG) * 8 + (x & 63u) / 8, u = b / (4 * RG) * 8 + (x & 7u);
+            kvm_f16x8 o;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t v = a.q_type == KVM_TYPE_F32 ? y[i][j >> 2][j & 3] : j & 1 ? y[i][0][j >> 1] & 0xffff0000u : y[i][0][j >> 1] << 16;
+                o[j] = r < rows ? (_Float16)(__uint_as_float(v) * a.q_sign) : (_Float16)0.0f;
+            }
+            *(kvm_f16x8 *)(dst + (r >> 5) * (2 * KS * QU) + u * QU + (r & 31u) * 16) = o;
+        }
+    }
+};
+
+// A row's limit: it sees the cells with (unsigned)position below it.
+__device__ __forceinline__ uint32_t fs_limit(const fs_args &a, uint32_t row_g, uint32_t rows, uint32_t r) {
+    const int32_t qp = r < rows ? a.q_pos[(row_g + r) / a.G] : -1;
+    return qp >= 0 ? (uint32_t)qp + 1u : 0u;
+}
+
+// Tile i of a unit's order.
+__device__ __forceinline__ uint32_t fs_tile(const fs_seg &sg, uint32_t i) { return i * sg.mult % sg.n_tiles; }      // (n_tiles < 2^16)
+
+// Positions of the cells of tiles b0 + r0 .. of nb in the unit's order: 4 tiles a wave and load.
+template <int NW>
+struct fs_cells {
+    kvm_u32x4 c[4];
+    __device__ __forceinline__ static uint32_t at(uint32_t r0, int r) { return r0 + 4 * NW * r + 4 * (threadIdx.x >> 6) + ((threadIdx.x & 63u) >> 4); }
+    __device__ __forceinline__ void load(const fs_seg &sg, uint32_t b0, uint32_t nb, uint32_t r0) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t i = at(r0, r);
+            c[r] = *(const kvm_u32x4 *)(sg.cell_pos + (uint64_t)fs_tile(sg, b0 + (i < nb ? i : 0u)) * 64 + 4 * (threadIdx.x & 15u));
+        }
+    }
+};
+
+// The tiles b0 .. b0 + nb - 1 in the unit's order that some row sees, in sm.list (bit 31: every
+// cell is visible to every row); returns how many.  Every wave takes part; two barriers.
+// cells: loaded for r0 = 0.
+template <int D, int NW>
+__device__ __forceinline__ uint32_t fs_tiles(const fs_seg &sg, fs_list<D, NW> &sm, uint32_t b0, uint32_t nb, uint32_t some_lim,
+                                             uint32_t all_lim, fs_cells<NW> &cells) {
+    const uint32_t l = fs_opaque(threadIdx.x & 63u), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (uint32_t r0 = 0;;) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t i = cells.at(r0, r);
+            const kvm_u32x4 c = cells.c[r];
+            const uint32_t least = min(min(c[0], c[1]), min(c[2], c[3])), most = max(max(c[0], c[1]), max(c[2], c[3]));
+            const uint32_t some = (uint32_t)(__builtin_amdgcn_ballot_w64(least < some_lim) >> (l & 48)) & 0xffffu;
+            const uint32_t all = (uint32_t)(__builtin_amdgcn_ballot_w64(most < all_lim) >> (l & 48)) & 0xffffu;
+            if (i < nb && (l & 15) == 0) sm.flag[i] = (uint8_t)((some != 0) | (all == 0xffffu) << 1);
+        }
+        r0 += 16 * NW;
+        if (r0 >= nb) break;
+        cells.load(sg, b0, nb, r0);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) sm.odd = 0;
+    uint32_t n_t = 0;
+#pragma unroll
+    for (uint32_t x = 0; x < FS_BATCH / 64; ++x) {
+        const uint32_t f = 64 * x + l < nb ? sm.flag[64 * x + l] : 0u;
+        const uint64_t bal = __builtin_amdgcn_ballot_w64(f & 1u);
+        const uint32_t rank = n_t + __builtin_amdgcn_mbcnt_hi((uint32_t)(bal >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bal, 0u));
+        if ((f & 1u) && x == w) sm.list[rank] = fs_tile(sg, b0 + 64 * x + l) | (f >> 1) << 31;
+        n_t += __popcll(bal);
+    }
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(n_t);
+}
+
+// The scores of a half tile that its cells' positions mask.
+__device__ __forceinline__ void fs_mask(kvm_f32x16 &S, const int32_t *cp, uint32_t qlim) {
+    asm volatile("" ::: "memory");                        // keep it on the (rare) masked path
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const kvm_u32x4 x = *(const kvm_u32x4 *)(cp + 16 * (i >> 1) + 8 * (fs_opaque(threadIdx.x & 63u) >> 5) + 4 * (i & 1));
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (!(x[r] < qlim)) S[4 * i + r] = -INFINITY;
+    }
+}
+
+// Halves of v (values, or scales of values) whose keys, base .. base + 7, no row sees become
+// 0, and so do those that are no finite numbers where not all rows see the key (0 times them
+// would not be 0): whether there are such.
+__device__ __forceinline__ bool fs_clear(kvm_u32x4 &v, uint32_t base, uint64_t seen, uint64_t part) {
+    const uint32_t on = (uint32_t)(seen >> base) & 0xffu, pt = (uint32_t)(part >> base) & 0xffu;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t sh = 16 * (i & 1), x = v[i >> 1] >> sh & 0xffffu;
+        const bool no = (pt >> i & 1u) && (x & 0x7c00u) == 0x7c00u;
+        odd |= no;
+        if (!(on >> i & 1u) || no) v[i >> 1] &= ~(0xffffu << sh);
+    }
+    return odd;
+}
+
+// What fs_clear took out of keys k0 .. k0 + n_k - 1 of the list's tiles j0, j0 + step, ..: values that are no finite
+// numbers are added to the rows that see them (a positive p times one is itself).  sx: the
+// wave's own.
+template <int D, bool QUANT>
+__device__ __forceinline__ void fs_add_odd(kvm_f32x16 (&O)[D / 32], const fs_seg &sg, const uint8_t *v_head, const uint32_t *list, uint32_t j0,
+                                           uint32_t step, uint32_t n_t, uint32_t k0, uint32_t n_k, uint32_t some_lim, uint32_t all_lim, uint32_t qlim, float *sx) {
+    const uint32_t l = threadIdx.x & 63u;
+    for (uint32_t j = j0; j < n_t; j += step) {
+        const uint32_t e = list[j], t = e & 0x7fffffffu;
+        if (e >> 31) continue;
+        const uint8_t *v_tile = v_head + (uint64_t)t * fs_geo<D, QUANT>::VB;
+        for (uint32_t k = k0; k < k0 + n_k; ++k) {
+            const uint32_t cp = (uint32_t)sg.cell_pos[(uint64_t)t * 64 + k];
+            if (!(cp < some_lim) || cp < all_lim) continue;
+            bool any = false;
+            for (uint32_t d = l; d < D; d += 64) {
+                bool bad;
+                float v;
+                if constexpr (QUANT) {
+                    const float sc = kvm_h2f(*(const uint16_t *)(v_tile + kvm_vd_off(D, k, d / 32)));
+                    bad = !(sc - sc == 0.0f);
+                    v = (float)((int)(v_tile[kvm_vq_byte(k, d)] >> kvm_vq_shift(k) & 15u) - 8) * sc;
+                } else {
+                    v = kvm_h2f(((const uint16_t *)v_tile)[kvm_vh_idx(k, d)]);
+                    bad = !(v - v == 0.0f);
+                }
+                sx[d] = bad ? v : 0.0f;
+                any |= bad;
+            }
+            if (__builtin_amdgcn_ballot_w64(any) == 0) continue;
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const kvm_f32x4 v = *(const kvm_f32x4 *)(sx + 32 * dt + 8 * x + 4 * (l >> 5));
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) O[dt][4 * x + r] += cp < qlim ? v[r] : 0.0f;
+                }
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+}
+
+// Direct copies to LDS (lane l writes 16 or 4 bytes at M0 + 16 l or 4 l), issued from asm, so
+// that the compiler adds no wait for them; the asm restores M0, which the compiler reserves.
+// Whoever reads waits by vmcnt first.
+__device__ __forceinline__ void fs_copy16(const uint8_t *src, uint32_t off, void *dst) {
+    uint32_t m0_saved;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0_saved) : "v"(off), "s"((uint32_t)(uintptr_t)(fs_lds_ptr)dst), "s"(src) : "memory");
+}
+__device__ __forceinline__ void fs_copy16(const uint8_t *lane_src, void *dst) {
+    uint32_t m0_saved;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0_saved) : "v"(lane_src), "s"((uint32_t)(uintptr_t)(fs_lds_ptr)dst) : "memory");
+}
+__device__ __forceinline__ void fs_copy4(const int32_t *src, uint32_t off, void *dst) {
+    uint32_t m0_saved;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0_saved) : "v"(off), "s"((uint32_t)(uintptr_t)(fs_lds_ptr)dst), "s"(src) : "memory");
+}
+
+// A piece of a narrow unit (32 rows over a quantised window): tiles [i_lo, i_hi) in the
+// unit's order.  What bounds it: instruction issue (a tile's conversion is ~900 of a wave's
+// ~1,700 instructions), or the memory where no two units read the same tiles.
+template <int D>
+__device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs_lds_narrow<D> &sm, uint32_t rt, uint32_t h, uint32_t slot,
+                                          uint32_t i_lo, uint32_t i_hi) {
+    using G = fs_geo<D, true>;
+    constexpr int KS = G::KS, NB = G::NB, DT = G::DT, NQ = G::NQ, SETS = G::SETS;
+    constexpr uint32_t KB = G::KB, VB = G::VB, QU = G::QU;
+    const uint32_t l = fs_opaque(threadIdx.x & 63u), g2 = l >> 5, m2 = l & 31u;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t rows = min(32u, sg.n_rows - 32 * rt), row_g = sg.row0 + 32 * rt;
+
+    // the loads of the start, all issued before any is used
+    fs_cells<4> cells;
+    cells.load(sg, i_lo, min(FS_BATCH, i_hi - i_lo), 0);
+    const uint32_t qlim = fs_limit(a, row_g, rows, m2);
+    {
+        fs_rows<D, 1, 4> q;
+        q.load(a, h, row_g, rows);
+        q.store(a, rows, sm.q);
+    }
+    const uint32_t all_lim = kvm_wave_min_u32(m2 < rows ? qlim : 0xffffffffu), some_lim = ~kvm_wave_min_u32(~qlim);
+
+    kvm_f32x16 O[DT];
+    float ms = -INFINITY, lp = 0.0f;     // the row's reference maximum (times c), the lane's share of its sum
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) O[dt][r] = 0.0f;
+
+    // operand addresses of a lane
+    const uint32_t key = fs_key(m2);
+    const uint32_t k_lane = ((key >> 4) * (NB / 2) * 64 + 16 * g2 + (key & 15)) * 16, v_lane = ((m2 >> 4) * 64 + 16 * g2 + (m2 & 15)) * 8;
+    const uint8_t *const k_head = sg.k + (uint64_t)h * sg.n_tiles * KB, *const v_head = sg.v + (uint64_t)h * sg.n_tiles * VB;
+
+    for (uint32_t b0 = i_lo; b0 < i_hi; b0 += FS_BATCH) {
+        if (b0 != i_lo) cells.load(sg, b0, min(FS_BATCH, i_hi - b0), 0);
+        const uint32_t n_t = fs_tiles<D, 4>(sg, sm, b0, min(FS_BATCH, i_hi - b0), some_lim, all_lim, cells);      // (its barriers: Q, too)
+
+        // The wave's half tiles: half w & 1 of list entries w / 2, w / 2 + 2, ..  Their
+        // registers are loaded for the next one where this one's are used up; past the wave's
+        // last the bounds let nothing through.
+        const uint32_t half = w & 1;
+        kvm_u32x4 kr[SETS][NB];
+        uint32_t vq[SETS][2 * DT];
+        auto rsrc = [&](const uint8_t *head, uint32_t e, uint32_t bytes, bool more) {
+            return __builtin_amdgcn_make_buffer_rsrc((void *)(head + (uint64_t)(e & 0x7fffffffu) * bytes), (short)0, more ? bytes : 0u, 0x00020000);
+        };
+        auto load_k = [&](__amdgpu_buffer_rsrc_t r, int set, int i) {
+            kr[set][i] = __builtin_amdgcn_raw_buffer_load_b128(r, fs_opaque(k_lane) + (i & 1) * 512, half * NB * 1024 + (i >> 1) * 1024, 0);
+        };
+        auto load_v = [&](__amdgpu_buffer_rsrc_t r, int set, int i) {
+            vq[set][i] = __builtin_amdgcn_raw_buffer_load_b32(r, fs_opaque(v_lane) + (i & 1) * 256, half * 4 + (i >> 1) * 1024, 0);
+        };
+        // lanes below 2 NB: the half's K scales, from 32 on its V scales (units of 8 keys of a block)
+        auto copies = [&](uint32_t e, uint32_t buf) {
+            const uint32_t t = e & 0x7fffffffu, ln = fs_opaque(l), x = ln & (4u * NB - 1);
+            const uint8_t *const src = ln < 32 ? k_head + (uint64_t)t * KB + 64 * D + half * (64u * NB) + 16 * x
+                                               : v_head + (uint64_t)t * VB + 32 * D + (x >> 2) * 128 + half * 64 + (x & 3u) * 16;
+            fs_copy16(src, sm.sc[w][buf]);
+            fs_copy4(sg.cell_pos + (uint64_t)t * 64, 4u * ln, &sm.cp[w][buf][0]);
+        };
+        auto entry = [&](uint32_t j) { return __builtin_amdgcn_readfirstlane(sm.list[min(j, n_t - 1)]); };
+        const uint32_t j0 = w >> 1;
+        if (j0 < n_t) {
+#pragma unroll
+            for (int x = 0; x < SETS; ++x) {
+                const uint32_t e = entry(j0 + 2 * x);
+                const bool more = j0 + 2 * x < n_t;
+                copies(e, x);
+#pragma unroll
+                for (int i = 0; i < NB; ++i) load_k(rsrc(k_head, e, KB, more), x, i);
+#pragma unroll
+                for (int i = 0; i < 2 * DT; ++i) load_v(rsrc(v_head, e, VB, more), x, i);
+            }
+        }
+        uint32_t buf = 0;
+        auto item = [&](uint32_t j, auto which) {
+            constexpr int set = decltype(which)::value;
+            // the half tile's copies: its registers' loads, and the next ones', are younger
+            asm volatile("s_waitcnt vmcnt(%0)" : : "n"(SETS * (NB + 2 * DT) + 2 * (SETS - 1)) : "memory");
+            const uint32_t e = entry(j), en = entry(j + 2 * SETS);
+            const bool more = j + 2 * SETS < n_t, full = e >> 31;
+            const auto rk = rsrc(k_head, en, KB, more), rv = rsrc(v_head, en, VB, more);
+            if (!full) {
+                asm volatile("" ::: "memory");            // keep it on this (rare) path
+                const uint32_t lo = fs_opaque(l), cp = (uint32_t)sm.cp[w][buf][lo];
+                const uint64_t seen = __builtin_amdgcn_ballot_w64(cp < some_lim), part = seen & ~__builtin_amdgcn_ballot_w64(cp < all_lim);
+                // lane l has the scales of 8 keys of a block
+                if (lo < 4u * NB) {
+                    kvm_u32x4 *const at = (kvm_u32x4 *)(sm.sc[w][buf] + 512 + 16 * lo);
+                    kvm_u32x4 scv = *at;
+                    if (fs_clear(scv, 32 * half + 8 * (lo & 3u), seen, part)) sm.odd = 1;
+                    *at = scv;
+                }
+            }
+            copies(en, buf ? buf - 1 : SETS);
+
+            // ---- S^T of 32 keys: K operand i + 1 is made while the MFMA of i runs; what
+            // comes from LDS is read two steps ahead
+            kvm_f32x16 S;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[r] = 0.0f;
+            uint32_t ksc[NB];                         // the scales of the lane's key
+            {
+                const uint32_t k = fs_key(fs_opaque(l) & 31u);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) ksc[b] = *(const uint16_t *)(sm.sc[w][buf] + ((k >> 4) * NB + b) * 32 + 2 * (k & 15));
+            }
+            const uint32_t lq = fs_opaque(l);
+            const uint8_t *const sq = sm.q + (lq >> 5) * QU + (lq & 31u) * 16;
+            // operands in the order of the K loads: (block pair, 16-dim half | block of the pair)
+            auto k_op = [&](int i) {
+                const kvm_u32x4 x = kr[set][i >> 1];
+                return pf_q8(x[2 * (i & 1)], x[2 * (i & 1) + 1], ksc[2 * (i >> 2) + (i & 1)]);
+            };
+            auto q_op = [&](int i) { return *(const kvm_f16x8 *)(sq + 2 * (4 * (i >> 2) + 2 * (i & 1) + (i >> 1 & 1)) * QU); };
+            kvm_f16x8 kop = k_op(0), qr[3] = {q_op(0), q_op(1)};
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                if (i + 2 < KS) qr[(i + 2) % 3] = q_op(i + 2);
+                FS_FENCE();
+                S = __builtin_amdgcn_mfma_f32_32x32x16_f16(kop, qr[i % 3], S, 0, 0, 0);
+                if (i + 1 < KS) kop = k_op(i + 1);
+                if (i & 1) load_k(rk, set, i >> 1);
+                FS_FENCE();
+            }
+
+            // ---- softmax: P as f16 operands
+            if (!full) fs_mask(S, &sm.cp[w][buf][32 * half], qlim);
+            float x = S[0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) x = fmaxf(x, S[r]);
+            x = kvm_max_xor32(x);
+            const bool up = fmaf(x, a.c, -ms) > FS_LAZY;      // false for a row with nothing visible yet
+            if (__builtin_amdgcn_ballot_w64(up) != 0) {
+                const float mnew = up ? x * a.c : ms;
+                const float alpha = up ? __builtin_amdgcn_exp2f(ms - mnew) : 1.0f;
+                ms = mnew;
+                lp *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) O[dt] *= alpha;
+            }
+            const float ref = ms == -INFINITY ? 0.0f : ms;
+            kvm_f16x8 pb[2];
+            float sum = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                // the row sum takes p before its rounding to the f16 operand: within
+                // 2^-11 of it per element
+                const float y = __builtin_amdgcn_exp2f(fmaf(S[r], a.c, -ref));
+                pb[r >> 3][r & 7] = (_Float16)y;
+                sum += y;
+            }
+            lp += sum;
+
+            // ---- O^T += V^T P^T
+            kvm_u32x4 vs[3];
+            const uint8_t *const sv = sm.sc[w][buf] + 512 + (fs_opaque(l) >> 5) * 16;
+            auto v_scale = [&](int i) { vs[i % 3] = *(const kvm_u32x4 *)(sv + ((i >> 1) * 4 + 2 * (i & 1)) * 16); };
+            v_scale(0);
+            v_scale(1);
+            kvm_f16x8 vop = pf_q4(vq[set][0], vs[0]);
+#pragma unroll
+            for (int i = 0; i < 2 * DT; ++i) {
+                if (i + 2 < 2 * DT) v_scale(i + 2);
+                FS_FENCE();
+                O[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vop, pb[i & 1], O[i >> 1], 0, 0, 0);
+                if (i + 1 < 2 * DT) vop = pf_q4(vq[set][i + 1], vs[(i + 1) % 3]);
+                load_v(rv, set, i);
+                FS_FENCE();
+            }
+            buf = buf == SETS ? 0 : buf + 1;
+        };
+        for (uint32_t j = j0; j < n_t; j += 2) {
+            item(j, std::integral_constant<int, 0>{});
+            if constexpr (SETS == 2) {
+                if ((j += 2) >= n_t) break;
+                item(j, std::integral_constant<int, 1>{});
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the last items' copies, which nobody reads)
+        if (__builtin_amdgcn_readfirstlane(sm.odd)) fs_add_odd<D, true>(O, sg, v_head, sm.list, j0, 2, n_t, 32 * half, 32, some_lim, all_lim, qlim, sm.odd_v[w]);
+    }
+
+    // ---- the waves' sums: one maximum, then each wave's quarter of the dims from the others,
+    // two waves' and the third's
+    const float lr = kvm_add_xor32(lp);
+    if (g2 == 0) {
+        sm.ml[w][0][m2] = ms;
+        sm.ml[w][1][m2] = lr;
+    }
+    __syncthreads();
+    float M = sm.ml[0][0][m2], L = 0.0f;
+#pragma unroll
+    for (int x = 1; x < 4; ++x) M = fmaxf(M, sm.ml[x][0][m2]);
+    const float top = M == -INFINITY ? 0.0f : M;          // (a wave that saw nothing of the row: weight, sum and O are 0)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) L += sm.ml[x][1][m2] * __builtin_amdgcn_exp2f(sm.ml[x][0][m2] - top);
+    const float wgt = __builtin_amdgcn_exp2f(ms - top);
+    // quad i of O: dims 8 i + 4 g2 .. + 3 of the lane's row, weighted
+    auto quad = [&](int i) {
+        kvm_f32x4 v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = O[i >> 2][4 * (i & 3) + k] * wgt;
+        return v;
+    };
+    kvm_f32x4 acc[NQ];
+    for (int round = 0; round < 2; ++round) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int k = (q - w) & 3;                    // the (k - 1)-th of the waves that give to q
+            if (k == 0) {
+                if (round == 0) {
+#pragma unroll
+                    for (int x = 0; x < NQ; ++x) acc[x] = quad(q * NQ + x);
+                }
+            } else if ((k - 1) >> 1 == round) {
+#pragma unroll
+                for (int x = 0; x < NQ; ++x) *(kvm_f32x4 *)(sm.x[q][(k - 1) & 1] + 256 * x + 4 * l) = quad(q * NQ + x);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (round == 1 && k == 1) break;
+#pragma unroll
+            for (int x = 0; x < NQ; ++x) acc[x] += *(const kvm_f32x4 *)(sm.x[w][k] + 256 * x + 4 * l);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) *(kvm_f32x4 *)(a.ws_o + ((uint64_t)slot * (D / 8) + w * NQ + x) * 256 + 4 * l) = acc[x];
+    if (w == 0 && g2 == 0) {
+        float *ml = a.ws_ml + ((uint64_t)slot * 32 + m2) * 2;
+        ml[0] = M;
+        ml[1] = L;
+    }
+}
+
+// x stays where it is: nothing moves over it, the MFMA that wrote it included.
+#define FS_PIN(x)                                    \
+    do {                                             \
+        asm volatile("" : "+v"(x) : : "memory");     \
+        FS_FENCE();                                  \
+    } while (0)
+
+// A piece of a wide unit.  What bounds it: the attention waves' chain, one a SIMD (of a tile
+// of 256 dims, 2,048 cycles on the matrix cores); over an f16 window the memory where no two
+// units read the same tiles.
+template <int D, bool QUANT>
+__device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg, fs_lds_wide<D, QUANT> &sm, uint32_t rt, uint32_t h,
+                                              uint32_t slot, uint32_t i_lo, uint32_t i_hi) {
+    using G = fs_geo<D, QUANT>;
+    constexpr int KS = G::KS, NB = G::NB, DT = G::DT;     // (2 DT = KS)
+    constexpr uint32_t KB = G::KB, VB = G::VB, TB = G::TB, QU = G::QU;
+    const uint32_t l = fs_opaque(threadIdx.x & 63u);
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = w & 3;
+    const uint32_t rows = min(128u, sg.n_rows - 128 * rt), row_g = sg.row0 + 128 * rt;
+
+    // the loads of the start, all issued before any is used
+    fs_cells<8> cells;
+    cells.load(sg, i_lo, min(FS_BATCH, i_hi - i_lo), 0);
+    const uint32_t lim0 = fs_limit(a, row_g, rows, l), lim1 = fs_limit(a, row_g, rows, l + 64);
+    {
+        fs_rows<D, 4, 8> q;
+        q.load(a, h, row_g, rows);
+        q.store(a, rows, sm.q4[0]);
+    }
+    const uint32_t all_lim = kvm_wave_min_u32(min(l < rows ? lim0 : 0xffffffffu, l + 64 < rows ? lim1 : 0xffffffffu));
+    const uint32_t some_lim = ~kvm_wave_min_u32(~max(lim0, lim1));
+    const uint8_t *const k_head = sg.k + (uint64_t)h * sg.n_tiles * KB, *const v_head = sg.v + (uint64_t)h * sg.n_tiles * VB;
+    uint32_t n_t = fs_tiles<D, 8>(sg, sm, i_lo, min(FS_BATCH, i_hi - i_lo), some_lim, all_lim, cells);   // (its barriers: Q, too)
+
+    // Both roles take the same barriers: one when Q is in registers, and for a batch of tiles
+    // one when the first is in LDS, one a tile, and those of the next batch's list.
+    if (w < 4) {
+        // ======== 32 rows: S^T = K Q^T, softmax, O^T += V^T P^T
+        const float c = a.c;
+        const uint32_t lc = fs_opaque(l), m2 = lc & 31u, g2 = lc >> 5;
+        // operand rings: R1 where a softmax is under way (registers), R0 elsewhere
+        constexpr std::integral_constant<int, D == 256 ? 4 : 6> R0;
+        constexpr std::integral_constant<int, D == 256 ? 2 : 4> R1;
+        kvm_f32x16 O[DT];
+        float ms = -INFINITY, lp = 0.0f;
+        kvm_f16x8 qop[KS];       // lane (g2, m2): Q[row m2][16 ks + 8 g2 .. + 7]
+        auto in_lds = [](int ks) { return G::QL && ks % 3 == 1; };
+        uint8_t *const ql = sm.ql[rg][0] + 16 * lc;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const kvm_f16x8 v = *(const kvm_f16x8 *)(sm.q4[rg] + (2 * ks + g2) * QU + m2 * 16);
+            if (in_lds(ks)) *(kvm_f16x8 *)(ql + ks / 3 * 1024) = v;
+            else qop[ks] = v;
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) O[dt][r] = 0.0f;
+        const uint32_t qlim = fs_limit(a, row_g, rows, 32 * rg + m2);
+        const uint32_t key = fs_key(m2);
+        const uint32_t k_ofs = ((key >> 4) * NB * 64 + 16 * g2 + (key & 15)) * 16, v_ofs = ((m2 >> 4) * 64 + 16 * g2 + (m2 & 15)) * 16;
+        const bool active = 32u * rg < rows;              // not a wave of padding rows
+        KVM_LDS_BARRIER();                                // Q is in registers
+
+        // S^T of a half tile: K operand ks at sk + .., KR - 1 ahead; between(ks) follows MFMA ks
+        auto scores = [&](auto ring, const uint8_t *sk, auto &&between) {
+            constexpr int KR = decltype(ring)::value;
+            kvm_f32x16 S;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[r] = 0.0f;
+            kvm_f16x8 kr[KR];
+            auto ld = [&](int ks) { return *(const kvm_f16x8 *)(sk + ks * 512); };
+            kvm_f16x8 qn;
+            auto ldq = [&](int ks) {
+                if (in_lds(ks)) qn = *(const kvm_f16x8 *)(sm.ql[rg][0] + 16 * fs_opaque(l) + ks / 3 * 1024);
+            };
+            ldq(1);
+#pragma unroll
+            for (int i = 0; i < KR - 1; ++i) kr[i] = ld(i);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (ks + KR - 1 < KS) kr[(ks + KR - 1) % KR] = ld(ks + KR - 1);
+                FS_FENCE();
+                S = __builtin_amdgcn_mfma_f32_32x32x16_f16(kr[ks % KR], in_lds(ks) ? qn : qop[ks], S, 0, 0, 0);
+                if (in_lds(ks) && ks + 3 < KS) ldq(ks + 3);
+                between(ks);
+                FS_PIN(S);
+            }
+            return S;
+        };
+        // O^T += V^T P^T: operand i = (16 keys i / DT, dim tile i % DT)
+        auto accumulate = [&](auto ring, const uint8_t *sv, const kvm_f16x8 (&pb)[2], auto &&between) {
+            constexpr int VR = decltype(ring)::value;
+            kvm_f16x8 vr[VR];
+            auto ld = [&](int i) { return *(const kvm_f16x8 *)(sv + (i % DT) * 2048 + (i / DT) * 512); };
+#pragma unroll
+            for (int i = 0; i < VR - 1; ++i) vr[i] = ld(i);
+#pragma unroll
+            for (int i = 0; i < 2 * DT; ++i) {
+                if (i + VR - 1 < 2 * DT) vr[(i + VR - 1) % VR] = ld(i + VR - 1);
+                FS_FENCE();
+                O[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vr[i % VR], pb[i / DT], O[i % DT], 0, 0, 0);
+                between(i);
+                FS_PIN(O[i % DT]);
+            }
+        };
+        // The softmax of a half tile in KS steps, taken between another's MFMAs: the maximum
+        // (KS / 4 steps), the running maximum's move (one), the probabilities (KS / 2).
+        float x = 0.0f, ref = 0.0f, alpha = 1.0f, sum = 0.0f;
+        bool moved = false;
+        auto soft = [&](const kvm_f32x16 &S, kvm_f16x8 (&pb)[2], int i) {
+            constexpr int NM = KS / 4, EM = 16 / NM, EP = 16 / (KS / 2);
+            if (i < NM) {
+#pragma unroll
+                for (int r = 0; r < EM; ++r) x = i == 0 && r == 0 ? S[0] : fmaxf(x, S[EM * i + r]);
+            } else if (i == NM) {
+                x = kvm_max_xor32(x);
+                const bool up = fmaf(x, c, -ms) > FS_LAZY;        // false for a row with nothing visible yet
+                moved = __builtin_amdgcn_ballot_w64(up) != 0;
+                const float mnew = up ? x * c : ms;
+                alpha = up ? __builtin_amdgcn_exp2f(ms - mnew) : 1.0f;
+                ms = mnew;
+                ref = ms == -INFINITY ? 0.0f : ms;
+                sum = 0.0f;
+            } else if (i >= KS / 2) {
+#pragma unroll
+                for (int j = 0; j < EP; j += 2) {
+                    // (the row sum takes p before its rounding)
+                    const int r = EP * (i - KS / 2) + j;
+                    const float y0 = __builtin_amdgcn_exp2f(fmaf(S[r], c, -ref)), y1 = __builtin_amdgcn_exp2f(fmaf(S[r + 1], c, -ref));
+                    kvm_f16x2 h = {(_Float16)y0, (_Float16)y1};
+                    sum += y0;
+                    sum += y1;
+                    asm volatile("" : "+v"(h), "+v"(sum)); // here, not where they are used
+                    pb[r >> 3][r & 7] = h[0];
+                    pb[r >> 3][(r & 7) + 1] = h[1];
+                }
+            }
+        };
+        // what the moved maximum asks of the sums so far
+        auto settle = [&]() {
+            if (moved) {
+                asm volatile("" ::: "memory");            // keep it on this (rare) path
+                lp *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) O[dt] *= alpha;
+            }
+            lp += sum;
+        };
+        auto nothing = [](int) {};
+
+        for (uint32_t b0 = i_lo;;) {
+            KVM_LDS_BARRIER();                            // the first tile is in LDS
+            for (uint32_t k = 0; k < n_t; ++k) {
+                if (!active) {
+                    KVM_LDS_BARRIER();
+                    continue;
+                }
+                const bool masked = (__builtin_amdgcn_readfirstlane(sm.list[k]) >> 31) == 0;
+                const uint8_t *sk = sm.ring[k & 1u] + k_ofs, *sv = sm.ring[k & 1u] + TB + v_ofs;
+                kvm_f16x8 pb[2], pb1[2];
+                kvm_f32x16 S0 = scores(R0, sk, nothing);
+                if (masked) fs_mask(S0, &sm.cp[k & 1u][0], qlim);
+                kvm_f32x16 S1 = scores(R1, sk + 2 * NB * 1024, [&](int i) { soft(S0, pb, i); });
+                settle();
+                if (masked) fs_mask(S1, &sm.cp[k & 1u][32], qlim);
+                accumulate(R1, sv, pb, [&](int i) { soft(S1, pb1, i); });
+                settle();
+                accumulate(R0, sv + TB / 2, pb1, nothing);
+                KVM_LDS_BARRIER();
+            }
+            if (__builtin_amdgcn_readfirstlane(sm.odd)) fs_add_odd<D, QUANT>(O, sg, v_head, sm.list, 0, 1, n_t, 0, 64, some_lim, all_lim, qlim, sm.odd_v[w]);
+            b0 += FS_BATCH;
+            if (b0 >= i_hi) break;
+            fs_cells<8> next;
+            next.load(sg, b0, min(FS_BATCH, i_hi - b0), 0);
+            n_t = fs_tiles<D, 8>(sg, sm, b0, min(FS_BATCH, i_hi - b0), some_lim, all_lim, next);
+        }
+        if (active) {
+            // quad i of O: dims 8 i + 4 g2 .. + 3 of the lane's row
+            const float lr = kvm_add_xor32(lp);
+            const uint32_t le = fs_opaque(l);
+            float *o = a.ws_o + (uint64_t)(slot + rg) * 32 * D + 4 * le;
+            if (__builtin_amdgcn_ballot_w64(ms != -INFINITY) != 0) {
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i)
+                    *(kvm_f32x4 *)(o + 256 * i) = kvm_f32x4{O[i >> 2][4 * (i & 3)], O[i >> 2][4 * (i & 3) + 1], O[i >> 2][4 * (i & 3) + 2], O[i >> 2][4 * (i & 3) + 3]};
+            }
+            if (le < 32) {
+                float *ml = a.ws_ml + ((uint64_t)(slot + rg) * 32 + le) * 2;
+                ml[0] = ms;
+                ml[1] = lr;
+            }
+        }
+    } else {
+        // ======== tile k + 1 into one buffer while the others work on tile k
+        const int pw = w - 4;
+        KVM_LDS_BARRIER();                                // Q is in registers
+        auto tile = [&](uint32_t k) { return __builtin_amdgcn_readfirstlane(sm.list[k < n_t ? k : n_t - 1]); };
+        auto cells_of = [&](uint32_t e) { return sg.cell_pos[(uint64_t)(e & 0x7fffffffu) * 64 + l]; };
+        // what the tile's masks say: the keys that some row sees, and those that not all do
+        auto masks = [&](int32_t cp, uint64_t &seen, uint64_t &part) {
+            seen = __builtin_amdgcn_ballot_w64((uint32_t)cp < some_lim);
+            part = seen & ~__builtin_amdgcn_ballot_w64((uint32_t)cp < all_lim);
+        };
+        for (uint32_t b0 = i_lo;;) {
+            if constexpr (QUANT) {
+                // The quantised tile goes through registers (two sets: tiles k + 2 and k + 3 are
+                // in flight while tile k + 1 is converted).  Thread (pw, l): K units 4 j + pw
+                // (lane l of (sub, block pair)), V dim tiles VJ pw + j.
+                constexpr int KJ = D / 64, VJ = D / 64, VB2 = VJ / 2;
+                struct raw_tile {
+                    kvm_u32x4 k[KJ];
+                    uint32_t kd[KJ][2];
+                    kvm_u32x2 v[VJ];
+                    kvm_u32x4 vs[VB2][2];
+                    int32_t cp;
+                    uint32_t e;
+                };
+                raw_tile rt2[2] = {};
+                auto load = [&](raw_tile &r, uint32_t e) {
+                    const uint32_t ln = fs_opaque(l), t = e & 0x7fffffffu;
+                    const uint8_t *kt = k_head + (uint64_t)t * KB, *vt = v_head + (uint64_t)t * VB;
+#pragma unroll
+                    for (int j = 0; j < KJ; ++j) {
+                        const uint32_t sp = 4 * j + pw, s = sp / (NB / 2), pr = sp % (NB / 2);
+                        r.k[j] = *(const kvm_u32x4 *)(kt + (sp * 64 + ln) * 16);
+                        r.kd[j][0] = *(const uint16_t *)(kt + kvm_kd_off(D, 16 * s + (ln & 15), 2 * pr));
+                        r.kd[j][1] = *(const uint16_t *)(kt + kvm_kd_off(D, 16 * s + (ln & 15), 2 * pr + 1));
+                    }
+#pragma unroll
+                    for (int j = 0; j < VJ; ++j) r.v[j] = *(const kvm_u32x2 *)(vt + ((VJ * pw + j) * 64 + ln) * 8);
+#pragma unroll
+                    for (int b = 0; b < VB2; ++b)
+#pragma unroll
+                        for (int ks = 0; ks < 2; ++ks) r.vs[b][ks] = *(const kvm_u32x4 *)(vt + 32 * D + (((VB2 * pw + b) * 2 + ks) * 4 + (ln >> 4)) * 16);
+                    r.cp = cells_of(e);
+                    r.e = e;
+                };
+                auto convert = [&](raw_tile &r, uint32_t buf) {
+                    if (!(r.e >> 31)) {
+                        asm volatile("" ::: "memory");    // keep it on this (rare) path
+                        uint64_t seen, part;
+                        masks(r.cp, seen, part);
+                        bool odd = false;
+#pragma unroll
+                        for (int b = 0; b < VB2; ++b)
+#pragma unroll
+                            for (int ks = 0; ks < 2; ++ks) odd |= fs_clear(r.vs[b][ks], 32 * ks + 8 * (fs_opaque(l) >> 4), seen, part);
+                        if (odd) sm.odd = 1;
+                    }
+                    uint8_t *dk = sm.ring[buf] + 16 * fs_opaque(l), *dv = dk + TB;
+#pragma unroll
+                    for (int j = 0; j < KJ; ++j) {
+                        const uint32_t sp = 4 * j + pw, s = sp / (NB / 2), pr = sp % (NB / 2);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) *(kvm_f16x8 *)(dk + (s * NB + 2 * pr + i) * 1024) = pf_q8(r.k[j][2 * i], r.k[j][2 * i + 1], r.kd[j][i]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < VJ; ++j)
+#pragma unroll
+                        for (int ks = 0; ks < 2; ++ks) *(kvm_f16x8 *)(dv + ks * (TB / 2) + (VJ * pw + j) * 1024) = pf_q4(r.v[j][ks], r.vs[j / 2][ks]);
+                    if (pw == 0) sm.cp[buf][l] = r.cp;
+                };
+                if (n_t != 0) {
+                    load(rt2[0], tile(0));
+                    load(rt2[1], tile(1));
+                    convert(rt2[0], 0);
+                }
+                KVM_LDS_BARRIER();                        // the first tile is in LDS
+                if (2 < n_t) load(rt2[0], tile(2));
+                auto step = [&](raw_tile &r, uint32_t k) {
+                    if (k + 1 < n_t) convert(r, (k + 1) & 1u);
+                    if (k + 3 < n_t) load(r, tile(k + 3));
+                    KVM_LDS_BARRIER();
+                };
+                uint32_t k = 0;
+                for (; k + 2 <= n_t; k += 2) {
+                    step(rt2[1], k);
+                    step(rt2[0], k + 1);
+                }
+                if (k < n_t) step(rt2[1], k);
+            } else {
+                // An f16 window's tiles are copied.  Its V tile holds the two key halves of a
+                // dim side by side, so the copies read every second unit of a dim tile.
+                constexpr int NC = (int)TB / 4096;        // 1 KB copies of a wave, of K and of V
+                auto bring = [&](uint32_t e, uint32_t buf) {
+                    const uint32_t t = e & 0x7fffffffu;
+                    uint8_t *const dst = sm.ring[buf];
+                    const uint8_t *kt = k_head + (uint64_t)t * TB, *vt = v_head + (uint64_t)t * TB;
+                    const int32_t cp = cells_of(e);
+#pragma unroll
+                    for (int i = 0; i < NC; ++i) fs_copy16(kt + (pw * NC + i) * 1024u, 16u * fs_opaque(l), dst + (pw * NC + i) * 1024u);
+#pragma unroll
+                    for (int i = 0; i < NC; ++i) {
+                        const uint32_t x = pw * NC + i;   // key half, dim tile
+                        fs_copy16(vt + (x % (D / 16)) * 2048u + (x / (D / 16)) * 16u, 32u * fs_opaque(l), dst + TB + x * 1024u);
+                    }
+                    if (pw == 0) sm.cp[buf][l] = cp;
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    if (!(e >> 31)) {
+                        asm volatile("" ::: "memory");
+                        uint64_t seen, part;
+                        masks(cp, seen, part);
+                        const uint32_t ln = fs_opaque(l);
+                        bool odd = false;
+                        for (int i = 0; i < NC; ++i) {
+                            const uint32_t x = pw * NC + i;
+                            kvm_u32x4 *const u = (kvm_u32x4 *)(dst + TB + x * 1024u + 16 * ln);
+                            kvm_u32x4 v = *u;
+                            odd |= fs_clear(v, 32 * (x / (D / 16)) + 8 * (ln >> 4), seen, part);
+                            *u = v;
+                        }
+                        if (odd) sm.odd = 1;
+                    }
+                };
+                if (n_t != 0) bring(tile(0), 0);
+                KVM_LDS_BARRIER();                        // the first tile is in LDS
+                for (uint32_t k = 0; k < n_t; ++k) {
+                    if (k + 1 < n_t) bring(tile(k + 1), (k + 1) & 1u);
+                    KVM_LDS_BARRIER();
+                }
+            }
+            b0 += FS_BATCH;
+            if (b0 >= i_hi) break;
+            fs_cells<8> next;
+            next.load(sg, b0, min(FS_BATCH, i_hi - b0), 0);
+            n_t = fs_tiles<D, 8>(sg, sm, b0, min(FS_BATCH, i_hi - b0), some_lim, all_lim, next);
+        }
+    }
+    __syncthreads();                                      // the LDS is the next piece's
+}
+
+// The pieces of a workgroup: tiles [lo, hi) of the kind's, the segments s .. one after another.
+template <bool WIDE, class F>
+__device__ __forceinline__ void fs_pieces(const fs_args &a, F &&piece) {
+    const uint32_t l = threadIdx.x & 63u;
+    const fs_deal &dl = WIDE ? a.wide : a.narrow;
+    // neighbouring shares on one XCD: their units read the same tiles
+    uint32_t p = blockIdx.x;
+    if (dl.p % 8 == 0) p = (p & 7u) * (dl.p / 8) + (p >> 3);
+    const uint32_t lo = dl.first(p), hi = dl.first(p + 1);
+    uint32_t s = __popcll(__builtin_amdgcn_ballot_w64(l < a.n_seg && a.tile0[l < a.n_seg ? l : 0u] <= lo)) - 1;
+    if (a.n_seg > 64 && a.tile0[64] <= lo) s = 64;
+    s = __builtin_amdgcn_readfirstlane(s);
+    for (uint32_t at = lo; at < hi;) {
+        const fs_seg &sg = a.seg[s];
+        const uint32_t n_rt = fs_row_tiles(WIDE, sg.n_rows);
+        const uint32_t u = (at - a.tile0[s]) / sg.n_tiles, c0 = a.tile0[s] + u * sg.n_tiles, h = u / n_rt;
+        piece(sg, u - h * n_rt, h, a.slot0[s] + (p + u) * (WIDE ? 4u : 1u), at - c0, min(hi - c0, sg.n_tiles));
+        at = c0 + sg.n_tiles;
+        if (at >= a.tile0[s + 1]) ++s;
+    }
+}
+
+template <int D, bool QUANT>
+__global__ void __launch_bounds__(512) k_fs_wide(fs_args a) {
+    __shared__ fs_lds_wide<D, QUANT> sm;
+    fs_pieces<true>(a, [&](const fs_seg &sg, uint32_t rt, uint32_t h, uint32_t slot, uint32_t i_lo, uint32_t i_hi) {
+        fs_wide_piece<D, QUANT>(a, sg, sm, rt, h, slot, i_lo, i_hi);
+    });
+}
+
+template <int D>
+__global__ void __launch_bounds__(256, 2) k_fs_narrow(fs_args a) {
+    __shared__ fs_lds_narrow<D> sm;
+    fs_pieces<false>(a, [&](const fs_seg &sg, uint32_t rt, uint32_t h, uint32_t slot, uint32_t i_lo, uint32_t i_hi) {
+        fs_narrow<D>(a, sg, sm, rt, h, slot, i_lo, i_hi);
+    });
+}
+
+// The pieces of 32 rows: a lane has 4 dims of a row; the workgroup's four waves share the row's
+// pieces, the prefix's and the conversation's, 8 of them in flight each.  What bounds it: the way
+// through the launch, the arguments and one load (3.9 us for 8 rows of 128 dims; with a wait for
+// every argument 5.7), past some MB of pieces their reading (768 rows of 256 dims, 52 MB: 13.1).
+template <int D>
+__global__ void __launch_bounds__(256) k_fs_join(fs_join_args a) {
+    constexpr uint32_t NP = 8;
+    __shared__ __align__(16) float s_x[4][64][4];
+    __shared__ float s_m[4][64], s_l[4][64];
+    const uint32_t l = threadIdx.x & 63u, w = threadIdx.x >> 6, m2 = l & 31u, h = blockIdx.z, row_b = 32 * blockIdx.x, row = row_b + m2;
+    // lane x has conversation x's entries
+    const uint32_t t_row0 = a.row0[l], t_rows = a.rows[l], t_tile0 = a.tile0[l], t_tiles = a.tiles[l], t_slot0 = a.slot0[l];
+    // (as values: the compiler would load where each is used, one wait after another)
+    auto pin = [](uint32_t x) {
+        asm volatile("" : "+s"(x));
+        return x;
+    };
+    const uint32_t wb = pin(a.wide.base), wq = pin(a.wide.q), wr = pin(a.wide.r), nb = pin(a.narrow.base), nq = pin(a.narrow.q), nr = pin(a.narrow.r);
+    const uint32_t pre_tiles = pin(a.pre_tiles), pre_wide = pin(a.pre_wide), pre_slot0 = pin(a.pre_slot0), n_rows = pin(a.n_rows);
+    const bool live = row < n_rows;
+    // the pieces of unit u (with `tiles` tiles, tile0 before the segment's) : n of them from p0 on
+    auto pieces = [&](bool wide, uint32_t tile0, uint32_t tiles, uint32_t u, uint32_t &n) {
+        fs_deal dl;
+        dl.base = wide ? wb : nb;
+        dl.q = wide ? wq : nq;
+        dl.r = wide ? wr : nr;
+        const uint32_t c0 = tile0 + u * tiles, p0 = dl.owner(c0);
+        n = dl.owner(c0 + tiles - 1) - p0 + 1;
+        return p0;
+    };
+    uint32_t n_pre = 0, step_pre = 0, slot_pre = 0, n_own = 0, step_own = 0, slot_own = 0, r_own = 0;
+    if (pre_tiles) {                                      // (its rows are all rows)
+        const uint32_t ur = fs_unit_rows(pre_wide), u = h * fs_row_tiles(pre_wide, n_rows) + row_b / ur;
+        const uint32_t p0 = pieces(pre_wide, 0, pre_tiles, u, n_pre);
+        step_pre = ur / 32;
+        slot_pre = pre_slot0 + (p0 + u) * step_pre + row_b % ur / 32;
+    }
+    // the conversation that the row is in: the last that begins at or before it
+    const uint32_t c_lo = __popcll(__builtin_amdgcn_ballot_w64(t_row0 <= row_b)), c_hi = __popcll(__builtin_amdgcn_ballot_w64(t_row0 <= row_b + 31));
+    uint32_t cv = c_lo;
+    for (uint32_t x = c_lo; x < c_hi; ++x) cv += row >= (uint32_t)__builtin_amdgcn_readlane((int)t_row0, (int)x);
+    if (c_hi) {
+        auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_ds_bpermute((int)(4 * (cv ? cv - 1 : 0)), (int)v); };
+        const uint32_t row0 = of(t_row0), n = of(t_rows), tile0 = of(t_tile0), tiles = of(t_tiles), slot0 = of(t_slot0);
+        if (live && cv && row - row0 < n) {
+            const bool wide = tiles >> 31;
+            r_own = row - row0;
+            const uint32_t ur = fs_unit_rows(wide), u = h * fs_row_tiles(wide, n) + r_own / ur;
+            const uint32_t p0 = pieces(wide, tile0, tiles & 0x7fffffffu, u, n_own);
+            step_own = ur / 32;
+            slot_own = slot0 + (p0 + u) * step_own + r_own % ur / 32;
+        }
+    }
+    const uint32_t n = live ? n_pre + n_own : 0u, t = row / a.G;
+    for (uint32_t i = blockIdx.y; i < D / 8; i += gridDim.y) {
+        float M = -INFINITY, L = 0.0f;
+        kvm_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (uint32_t q = w; q < n; q += 4 * NP) {
+            kvm_u32x4 x[NP];
+            kvm_f32x2 ml[NP];
+#pragma unroll
+            for (uint32_t j = 0; j < NP; ++j) {
+                const uint32_t k = min(q + 4 * j, n - 1), r = k < n_pre ? m2 : r_own & 31u;
+                const uint64_t slot = k < n_pre ? slot_pre + k * step_pre : slot_own + (k - n_pre) * step_own;
+                x[j] = *(const kvm_u32x4 *)(a.ws_o + (slot * (D / 8) + i) * 256 + 128 * (l >> 5) + 4 * r);
+                ml[j] = *(const kvm_f32x2 *)(a.ws_ml + (slot * 32 + r) * 2);
+            }
+            float mb = M;
+#pragma unroll
+            for (uint32_t j = 0; j < NP; ++j) {
+                if (q + 4 * j >= n) ml[j][0] = -INFINITY;
+                mb = fmaxf(mb, ml[j][0]);
+            }
+            const float top = mb == -INFINITY ? 0.0f : mb, keep = __builtin_amdgcn_exp2f(M - top);
+            L *= keep;
+            acc *= keep;
+#pragma unroll
+            for (uint32_t j = 0; j < NP; ++j) {
+                // (a piece that saw nothing of the row holds anything)
+                const float wgt = __builtin_amdgcn_exp2f(ml[j][0] - top);
+                const uint32_t has = ml[j][0] == -INFINITY ? 0u : 0xffffffffu;
+                L = fmaf(__uint_as_float(__float_as_uint(ml[j][1]) & has), wgt, L);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[k] = fmaf(__uint_as_float(x[j][k] & has), wgt, acc[k]);
+            }
+            M = mb;
+        }
+        *(kvm_f32x4 *)s_x[w][l] = acc;
+        s_m[w][l] = M;
+        s_l[w][l] = L;
+        __syncthreads();
+        if (w == 0 && live) {
+            float mb = M;
+#pragma unroll
+            for (int j = 1; j < 4; ++j) mb = fmaxf(mb, s_m[j][l]);
+            const float top = mb == -INFINITY ? 0.0f : mb;
+            L = 0.0f;
+            acc = kvm_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {                 // (a wave without pieces: zeros)
+                const float wgt = __builtin_amdgcn_exp2f(s_m[j][l] - top);
+                L = fmaf(s_l[j][l], wgt, L);
+                acc += *(const kvm_f32x4 *)s_x[j][l] * wgt;
+            }
+            // nothing visible: zeros
+            acc *= L == 0.0f ? 0.0f : 1.0f / L;
+            const uint64_t at = ((uint64_t)t * a.n_head + h * a.G + (row - t * a.G)) * D + 8 * i + 4 * (l >> 5);
+            if (a.out_type == KVM_TYPE_F32) {
+                __builtin_memcpy((float *)a.out + at, &acc, 16);
+            } else if (a.out_type == KVM_TYPE_BF16) {
+                typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+                const bf16x4 y = __builtin_convertvector(acc, bf16x4);
+                __builtin_memcpy((uint16_t *)a.out + at, &y, 8);
+            } else {
+                const kvm_f16x4 y = {(_Float16)acc[0], (_Float16)acc[1], (_Float16)acc[2], (_Float16)acc[3]};
+                __builtin_memcpy((uint16_t *)a.out + at, &y, 8);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- host -----------------------------------------------------------------------
+// A step through a window of n tiles that no two of its multiples share a tile with: the
+// one from 0.618 n on that has no divisor in common with n.
+static uint32_t fs_stride(uint32_t n) {
+    auto gcd = [](uint32_t a, uint32_t b) {
+        while (b) {
+            const uint32_t r = a % b;
+            a = b;
+            b = r;
+        }
+        return a;
+    };
+    uint32_t m = (uint32_t)(0.6180339887 * n);
+    m = m ? m : 1;
+    while (gcd(m, n) != 1) ++m;
+    return m;
+}
+
+// The rows from which on a window's units are wide.  An f16 window has nothing to convert: all.
+// A CU's workgroup takes a tile of a wide unit of 256 dims in 2.0 us, its two narrow ones a tile
+// of theirs in 1.4: a wide unit pays from three narrow ones' rows on (two's: 48 rows over 32,768
+// cells with 8 x 6 over 2,048, all narrow 43 us, else 34 + 16).  Where some windows
+// stay narrow all the same, the wide ones are a launch more (10 us for its start and end) and
+// have to save that: 288 rows over 5,003 cells with 16 x 18 over 8,192, all narrow 73 us, else
+// 37 + 52; 768 rows over 32,768 with 32 x 24 over 2,048, 246 us and 136 + 37.
+static uint32_t fs_wide_rows(const kvm_window *prefix, const kvm_window *const *windows, const uint32_t *n_tokens, uint32_t n_lanes, bool quant,
+                             uint32_t n_cu, uint32_t H, uint32_t G, uint32_t n_rows) {
+    if (!quant) return 1;
+    double saved = 0.0;              // us
+    bool narrow = false;
+    auto add = [&](const kvm_window *w, uint32_t r) {
+        if (!w || !r) return;
+        if (r <= 64) narrow = true;
+        else saved += (double)(w->n_cells / KVM_TILE_CELLS) * H / n_cu * (1.4 * fs_row_tiles(false, r) - 2.0 * fs_row_tiles(true, r));
+    };
+    add(prefix, n_rows);
+    for (uint32_t i = 0; i < n_lanes; ++i) add(windows ? windows[i] : nullptr, n_tokens[i] * G);
+    return narrow && saved < 10.0 ? 0xffffffffu : 65;
+}
+
+// Fills the segments, their tiles and slots, and the numbers of workgroups.
+static int fs_shape(kvm_state *st, const char *what, const kvm_window *prefix, const kvm_window *const *windows,
+                    const uint32_t *n_tokens, uint32_t n_lanes, bool quant, uint32_t n_cu, fs_args *a, fs_join_args *j, uint64_t *slots) {
+    const uint32_t wide_rows = fs_wide_rows(prefix, windows, n_tokens, n_lanes, quant, n_cu, a->H, a->G, a->n_rows);
+    uint64_t tiles = 0, units = 0, wide = 0;
+    uint32_t n = 0;
+    auto add = [&](const kvm_window *w, uint32_t row0, uint32_t n_rows) {
+        const uint32_t t = w->n_cells / KVM_TILE_CELLS;
+        const bool iw = n_rows >= wide_rows;
+        a->tile0[n] = (uint32_t)tiles;
+        a->seg[n++] = fs_seg{(const uint8_t *)w->k, (const uint8_t *)w->v, w->cell_pos, t, fs_stride(t), row0, n_rows};
+        const uint64_t u = (uint64_t)fs_row_tiles(iw, n_rows) * a->H;
+        units += u;
+        tiles += u * t;
+        if (iw) wide = tiles, a->n_wide = n;
+    };
+    uint32_t lane_seg[FS_LANES], own = 0;
+    if (prefix) {                                          // (wide where a conversation is)
+        add(prefix, 0, a->n_rows);
+        j->pre_tiles = a->seg[0].n_tiles;
+        j->pre_wide = a->n_wide;
+    }
+    for (int narrow = 0; narrow < 2; ++narrow) {
+        uint32_t row = 0;
+        own = 0;
+        for (uint32_t i = 0; i < n_lanes; ++i) {
+            const uint32_t r = n_tokens[i] * a->G;
+            if (windows && windows[i] && r) {
+                if ((r >= wide_rows) == !narrow) {
+                    lane_seg[own] = n;
+                    add(windows[i], row, r);
+                }
+                ++own;
+            }
+            row += r;
+        }
+    }
+    if (tiles > 0x7fffffffu || units > (1u << 22))
+        return kvm_fail(st, KVM_ERANGE, "%s: %u rows over these windows are too many for one call", what, a->n_rows);
+    a->tile0[n] = (uint32_t)tiles;
+    a->n_seg = n;
+    // Workgroups: what the CUs hold at once, and a tile or more for each wave that has tiles of
+    // its own (8 rows over 1,024 + 2 x 256 f16 cells of 2 heads: 8.7 us, with 4 tiles a workgroup
+    // 15.6); eighths, one for each XCD
+    auto deal = [](uint32_t base, uint32_t of, uint32_t most, uint32_t least) {
+        uint32_t p = std::min(most, std::max(of / least, 1u));
+        if (p > 8) p &= ~7u;
+        return fs_deal{base, p, of / p, of % p};
+    };
+    a->wide = deal(0, (uint32_t)wide, n_cu, 1);
+    a->narrow = deal((uint32_t)wide, (uint32_t)(tiles - wide), 2 * n_cu, 1);
+    // A unit's pieces are those of the workgroups that its tiles reach over; from one piece
+    // of a segment to the next the workgroup, the unit or both go on by one.
+    uint64_t slot = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+        const bool iw = i < a->n_wide;
+        const fs_deal &dl = iw ? a->wide : a->narrow;
+        const uint32_t gr = fs_unit_rows(iw) / 32, p0 = dl.owner(a->tile0[i]), p1 = dl.owner(a->tile0[i + 1] - 1);
+        a->slot0[i] = (uint32_t)slot - p0 * gr;
+        slot += (uint64_t)(p1 - p0 + fs_row_tiles(iw, a->seg[i].n_rows) * a->H) * gr;
+    }
+    *slots = slot;
+    j->wide = a->wide;
+    j->narrow = a->narrow;
+    if (prefix) j->pre_slot0 = a->slot0[0];
+    for (uint32_t i = 0; i < FS_LANES; ++i) j->row0[i] = 0xffffffffu;
+    for (uint32_t i = 0; i < own; ++i) {
+        const uint32_t s = lane_seg[i];
+        j->row0[i] = a->seg[s].row0;
+        j->rows[i] = a->seg[s].n_rows;
+        j->tile0[i] = a->tile0[s];
+        j->tiles[i] = a->seg[s].n_tiles | (s < a->n_wide ? 0x80000000u : 0u);
+        j->slot0[i] = a->slot0[s];
+    }
+    return KVM_OK;
+}
+
+extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, const kvm_window *const *windows,
+                                    const uint32_t *n_tokens, uint32_t n_lanes, const void *q, int q_type,
+                                    const int32_t *q_pos, uint32_t n_head, float scale, int out_type, void *out) {
+    const char *what = "fa_decode_shared";
+    if (n_lanes == 0) return KVM_OK;
+    if (!n_tokens) return kvm_fail(st, KVM_EINVAL, "%s: null argument", what);
+    if (n_lanes > FS_LANES) return kvm_fail(st, KVM_ERANGE, "%s: %u lanes > %u", what, n_lanes, FS_LANES);
+    if (q_type != KVM_TYPE_F32 && q_type != KVM_TYPE_BF16) return kvm_fail(st, KVM_EUNSUPPORTED, "%s: q type %d", what, q_type);
+    if (out_type != KVM_TYPE_F32 && out_type != KVM_TYPE_BF16 && out_type != KVM_TYPE_F16)
+        return kvm_fail(st, KVM_EUNSUPPORTED, "%s: output type %d", what, out_type);
+    const kvm_window *w0 = prefix;
+    uint64_t total = 0;
+    for (uint32_t i = 0; i < n_lanes; ++i) {
+        total += n_tokens[i];
+        if (!w0 && windows) w0 = windows[i];
+    }
+    if (!w0) return kvm_fail(st, KVM_EINVAL, "%s: no window", what);
+    for (uint32_t i = 0; i <= n_lanes; ++i) {
+        const kvm_window *w = i == n_lanes ? prefix : windows ? windows[i] : nullptr;
+        if (!w) continue;
+        const int rc = kvm_window_check(w);
+        if (rc) return kvm_fail(st, rc, "%s: %s %u: bad window", what, i == n_lanes ? "prefix," : "lane", i);
+        if (w->n_head_kv != w0->n_head_kv || w->head_dim != w0->head_dim || kvm_k_quant(w->k_type) != kvm_k_quant(w0->k_type))
+            return kvm_fail(st, KVM_EUNSUPPORTED, "%s: lane %u: windows of different heads or types", what, i);
+        if (((uintptr_t)w->k | (uintptr_t)w->v | (uintptr_t)w->cell_pos) & 15)
+            return kvm_fail(st, KVM_EINVAL, "%s: lane %u: a window that is not aligned to 16 bytes", what, i);
+        if (w->n_cells / KVM_TILE_CELLS > 65535) return kvm_fail(st, KVM_ERANGE, "%s: lane %u: %u cells", what, i, w->n_cells);
+    }
+    const uint32_t H = w0->n_head_kv, D = w0->head_dim;
+    if (n_head == 0 || n_head % H) return kvm_fail(st, KVM_EINVAL, "%s: %u heads on %u", what, n_head, H);
+    if (!std::isfinite(scale * 1.4426950408889634f)) return kvm_fail(st, KVM_EINVAL, "%s: scale %g", what, (double)scale);
+    if (total * (n_head / H) > (1u << 24)) return kvm_fail(st, KVM_ERANGE, "%s: %llu tokens", what, (unsigned long long)total);
+    if (H > 65535) return kvm_fail(st, KVM_ERANGE, "%s: %u kv heads", what, H);
+    if (total == 0) return KVM_OK;
+    if (!q || !q_pos || !out) return kvm_fail(st, KVM_EINVAL, "%s: null argument", what);
+    fs_args a{};
+    fs_join_args j{};
+    a.H = H;
+    a.G = n_head / H;
+    a.n_head = n_head;
+    a.n_rows = (uint32_t)total * a.G;
+    a.q = q;
+    a.q_type = q_type;
+    a.q_pos = q_pos;
+    j.out = out;
+    j.out_type = out_type;
+    j.G = a.G;
+    j.n_head = n_head;
+    j.n_rows = a.n_rows;
+    a.q_sign = scale < 0.0f ? -1.0f : scale > 0.0f ? 1.0f : 0.0f;
+    a.c = scale != 0.0f ? fabsf(scale) * 1.4426950408889634f : 1.0f;
+    uint64_t slots = 0;
+    const bool quant = kvm_k_quant(w0->k_type);
+    const int rc = fs_shape(st, what, prefix, windows, n_tokens, n_lanes, quant, st ? st->n_cu : 256u, &a, &j, &slots);
+    if (rc) return rc;
+    if (!st) return KVM_EINVAL;
+    const size_t bytes_o = (size_t)slots * 32 * D * 4, bytes = bytes_o + (size_t)slots * 32 * 8;
+    KVM_HIP(st, hipSetDevice(st->device));
+    if (slots) {
+        void *ws = nullptr;
+        if (const int bad = kvm_shared_workspace(st, what, bytes, &ws)) return bad;
+        a.ws_o = (float *)ws;
+        a.ws_ml = (float *)((uint8_t *)a.ws_o + bytes_o);
+        j.ws_o = a.ws_o;
+        j.ws_ml = a.ws_ml;
+    }
+    // a workgroup of the join has 8 dims, or more of them where all CUs have two all the same
+    // (its start is most of its work: 768 rows of 256 dims, 15.6 us by 8 dims)
+    const uint64_t blocks = (uint64_t)kvm_cdiv(a.n_rows, 32) * H;
+    uint32_t by = D / 8;
+    while (by > 1 && blocks * by >= 4ull * st->n_cu) by /= 2;
+    auto go = [&](auto d, auto qt) {
+        constexpr int DD = decltype(d)::value;
+        constexpr bool Q = decltype(qt)::value;
+        if (a.n_wide) hipLaunchKernelGGL((k_fs_wide<DD, Q>), dim3(a.wide.p), dim3(512), 0, st->stream, a);
+        if (Q && a.n_wide < a.n_seg) hipLaunchKernelGGL((k_fs_narrow<DD>), dim3(a.narrow.p), dim3(256), 0, st->stream, a);
+        hipLaunchKernelGGL((k_fs_join<DD>), dim3(kvm_cdiv(a.n_rows, 32), by, H), dim3(256), 0, st->stream, j);
+    };
+    auto go_d = [&](auto d) {
+        if (quant) go(d, std::true_type{});
+        else go(d, std::false_type{});
+    };
+    if (D == 256) go_d(std::integral_constant<int, 256>{});
+    else go_d(std::integral_constant<int, 128>{});
+    KVM_LAUNCH_CHECK(st, what);
+    return KVM_OK;
+}

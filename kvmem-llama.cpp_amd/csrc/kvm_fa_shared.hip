@@ -321,8 +321,12 @@ __device__ __forceinline__ void fs_copy4(const int32_t *src, uint32_t off, void 
 }
 
 // A piece of a narrow unit (32 rows over a quantised window): tiles [i_lo, i_hi) in the
-// unit's order.  What bounds it: instruction issue (a tile's conversion is ~900 of a wave's
-// ~1,700 instructions), or the memory where no two units read the same tiles.
+// unit's order.  A tile of 256 dims is ~1,650 instructions of a wave, 930 of them its conversion,
+// and 64 MFMAs (2,048 cycles): the issue of two waves a SIMD bounds it (~2.1 us a tile and
+// workgroup; everything in the L2, a third less), next to the memory where no two units read the
+// same tiles, and for short pieces the start (8.6 us to the first half tile) and the sums' meeting
+// (2.2).  8 lanes x 6 rows of 4 heads over 32,768 + 2,048 cells of q8_0: 33 us for 74.5 MB, 2.3
+// TB/s; 16 x 18 over 5,003 + 8,192 of q4_0: 67 us, 154 MB.
 template <int D>
 __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs_lds_narrow<D> &sm, uint32_t rt, uint32_t h, uint32_t slot,
                                           uint32_t i_lo, uint32_t i_hi) {
@@ -568,9 +572,11 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
         FS_FENCE();                                  \
     } while (0)
 
-// A piece of a wide unit.  What bounds it: the attention waves' chain, one a SIMD (of a tile
-// of 256 dims, 2,048 cycles on the matrix cores); over an f16 window the memory where no two
-// units read the same tiles.
+// A piece of a wide unit.  A tile of 256 dims is 64 MFMAs of an attention wave (2,048 cycles) in
+// ~4,600: its softmax and the other wave's conversion share the SIMD's issue, at the clock that
+// the power limit leaves.  768 rows of 4 heads over 32,768 cells of q8_0 (103 GFLOP): 137 us, 750
+// TFLOP/s.  Over an f16 window of few rows the memory: 36 tokens x 4 rows of 8 heads of 128 dims
+// over 8,192 + 12 x 1,024 cells, 24 us for 84 MB, the prefix read twice.
 template <int D, bool QUANT>
 __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg, fs_lds_wide<D, QUANT> &sm, uint32_t rt, uint32_t h,
                                               uint32_t slot, uint32_t i_lo, uint32_t i_hi) {
