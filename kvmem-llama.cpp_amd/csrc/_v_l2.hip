@@ -23,9 +23,9 @@
 //   wide units: workgroups of 8 waves, one a CU.  Waves 0 - 3 have 32 rows each and take every
 //     key; waves 4 - 7 bring the next tile into one of two LDS buffers, converted, while the
 //     other is worked on.
-// The tiles of all units of a kind are dealt to the workgroups in equal shares, in an order
-// that steps through a window in strides: a part-filled window's live tiles are spread
-// evenly over its pieces.
+// A workgroup has one piece: the units of a window are cut into equal numbers of pieces, and
+// longer ones into more.  The tiles are taken in an order that steps through a window in
+// strides: a part-filled window's live tiles are spread evenly over its pieces.
 #include "kvm_f16_dev.h"
 
 #include <algorithm>
@@ -47,20 +47,7 @@ struct fs_seg {
     const int32_t *cell_pos;
     uint32_t n_tiles, mult;      // tile i of a unit's order is (i mult) mod n_tiles
     uint32_t row0, n_rows;       // rows [row0, row0 + n_rows) of every kv head
-};
-
-// The tiles [base, base + ..) of a kind's units, dealt to p workgroups: each has q, the first
-// r one more.
-struct fs_deal {
-    uint32_t base, p, q, r;
-    // workgroup i has the tiles from here to the next's
-    __host__ __device__ uint32_t first(uint32_t i) const { return base + i * q + (i < r ? i : r); }
-    // the workgroup that has tile x
-    __host__ __device__ uint32_t owner(uint32_t x) const {
-        x -= base;
-        const bool more = x < r * (q + 1);
-        return (more ? x : x - r * (q + 1)) / (more ? q + 1 : q) + (more ? 0 : r);
-    }
+    uint32_t pieces, per, more;  // of a unit: pieces of `per` tiles, the first `more` of one more
 };
 
 struct fs_args {
@@ -69,12 +56,12 @@ struct fs_args {
     float *ws_o;                 // pieces of 32 rows: [slot][dim / 8][lane][4]
     float *ws_ml;                // [slot][row][2]: scaled maximum, sum
     uint32_t H, G, n_head, n_rows;
-    uint32_t n_seg, n_wide;      // segments, the wide ones before the narrow ones
-    fs_deal wide, narrow;
+    uint32_t wide, narrow;       // pieces; the wide ones' segments come first
     float c, q_sign;             // |scale| log2(e); q times -1 for a negative scale, and 0 (c = 1) for none
     int q_type;
-    uint32_t tile0[FS_SEGS + 1]; // tiles of the units of the segments before
-    uint32_t slot0[FS_SEGS];     // unit u's piece of workgroup p: slots slot0 + (p + u) groups .. (mod 2^32)
+    // Pieces of the segments before; a segment's: [head][piece of the unit][unit of the head],
+    // so that neighbours read the same tiles.  A wide piece has 4 slots, a narrow one 1.
+    uint32_t piece0[FS_SEGS];    // (past the last segment: ~0)
     fs_seg seg[FS_SEGS];
 };
 static_assert(sizeof(fs_args) <= 4096, "kernel arguments");
@@ -85,11 +72,10 @@ struct fs_join_args {
     void *out;
     int out_type;
     uint32_t G, n_head, n_rows;
-    fs_deal wide, narrow;
-    uint32_t pre_tiles, pre_wide, pre_slot0;              // the prefix's (no tiles: none)
-    // conversations with a window, in order: first row (the rest: ~0), rows, tiles before, tiles
+    uint32_t pre_pieces, pre_wide;                        // a prefix unit's (none: no prefix)
+    // conversations with a window, in order: first row (the rest: ~0), rows, pieces of a unit
     // (bit 31: wide), first slot
-    uint32_t row0[FS_LANES], rows[FS_LANES], tile0[FS_LANES], tiles[FS_LANES], slot0[FS_LANES];
+    uint32_t row0[FS_LANES], rows[FS_LANES], pieces[FS_LANES], slot0[FS_LANES];
 };
 
 __host__ __device__ inline uint32_t fs_unit_rows(bool wide) { return wide ? 128u : 32u; }
@@ -236,7 +222,7 @@ __device__ __forceinline__ uint32_t fs_tiles(const fs_seg &sg, fs_list<D, NW> &s
         const uint32_t f = 64 * x + l < nb ? sm.flag[64 * x + l] : 0u;
         const uint64_t bal = __builtin_amdgcn_ballot_w64(f & 1u);
         const uint32_t rank = n_t + __builtin_amdgcn_mbcnt_hi((uint32_t)(bal >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)bal, 0u));
-        if ((f & 1u) && x == w) sm.list[rank] = fs_tile(sg, b0 + 64 * x + l) | (f >> 1) << 31;
+        if ((f & 1u) && x == w) sm.list[rank] = (fs_tile(sg, b0 + 64 * x + l) & 3u) | (f >> 1) << 31;
         n_t += __popcll(bal);
     }
     __syncthreads();
@@ -335,8 +321,12 @@ __device__ __forceinline__ void fs_copy4(const int32_t *src, uint32_t off, void 
 }
 
 // A piece of a narrow unit (32 rows over a quantised window): tiles [i_lo, i_hi) in the
-// unit's order.  What bounds it: instruction issue (a tile's conversion is ~900 of a wave's
-// ~1,700 instructions), or the memory where no two units read the same tiles.
+// unit's order.  A tile of 256 dims is ~1,650 instructions of a wave, 930 of them its conversion,
+// and 64 MFMAs (2,048 cycles): the issue of two waves a SIMD bounds it (~2.1 us a tile and
+// workgroup; everything in the L2, a third less), next to the memory where no two units read the
+// same tiles, and for short pieces the start (8.6 us to the first half tile) and the sums' meeting
+// (2.2).  8 lanes x 6 rows of 4 heads over 32,768 + 2,048 cells of q8_0: 33 us for 74.5 MB, 2.3
+// TB/s; 16 x 18 over 5,003 + 8,192 of q4_0: 67 us, 154 MB.
 template <int D>
 __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs_lds_narrow<D> &sm, uint32_t rt, uint32_t h, uint32_t slot,
                                           uint32_t i_lo, uint32_t i_hi) {
@@ -582,9 +572,11 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
         FS_FENCE();                                  \
     } while (0)
 
-// A piece of a wide unit.  What bounds it: the attention waves' chain, one a SIMD (of a tile
-// of 256 dims, 2,048 cycles on the matrix cores); over an f16 window the memory where no two
-// units read the same tiles.
+// A piece of a wide unit.  A tile of 256 dims is 64 MFMAs of an attention wave (2,048 cycles) in
+// ~4,600: its softmax and the other wave's conversion share the SIMD's issue, at the clock that
+// the power limit leaves.  768 rows of 4 heads over 32,768 cells of q8_0 (103 GFLOP): 137 us, 750
+// TFLOP/s.  Over an f16 window of few rows the memory: 36 tokens x 4 rows of 8 heads of 128 dims
+// over 8,192 + 12 x 1,024 cells, 24 us for 84 MB, the prefix read twice.
 template <int D, bool QUANT>
 __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg, fs_lds_wide<D, QUANT> &sm, uint32_t rt, uint32_t h,
                                               uint32_t slot, uint32_t i_lo, uint32_t i_hi) {
@@ -905,35 +897,29 @@ __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg
             n_t = fs_tiles<D, 8>(sg, sm, b0, min(FS_BATCH, i_hi - b0), some_lim, all_lim, next);
         }
     }
-    __syncthreads();                                      // the LDS is the next piece's
 }
 
-// The pieces of a workgroup: tiles [lo, hi) of the kind's, the segments s .. one after another.
+// The workgroup's piece.
 template <bool WIDE, class F>
-__device__ __forceinline__ void fs_pieces(const fs_args &a, F &&piece) {
-    const uint32_t l = threadIdx.x & 63u;
-    const fs_deal &dl = WIDE ? a.wide : a.narrow;
-    // neighbouring shares on one XCD: their units read the same tiles
-    uint32_t p = blockIdx.x;
-    if (dl.p % 8 == 0) p = (p & 7u) * (dl.p / 8) + (p >> 3);
-    const uint32_t lo = dl.first(p), hi = dl.first(p + 1);
-    uint32_t s = __popcll(__builtin_amdgcn_ballot_w64(l < a.n_seg && a.tile0[l < a.n_seg ? l : 0u] <= lo)) - 1;
-    if (a.n_seg > 64 && a.tile0[64] <= lo) s = 64;
-    s = __builtin_amdgcn_readfirstlane(s);
-    for (uint32_t at = lo; at < hi;) {
-        const fs_seg &sg = a.seg[s];
-        const uint32_t n_rt = fs_row_tiles(WIDE, sg.n_rows);
-        const uint32_t u = (at - a.tile0[s]) / sg.n_tiles, c0 = a.tile0[s] + u * sg.n_tiles, h = u / n_rt;
-        piece(sg, u - h * n_rt, h, a.slot0[s] + (p + u) * (WIDE ? 4u : 1u), at - c0, min(hi - c0, sg.n_tiles));
-        at = c0 + sg.n_tiles;
-        if (at >= a.tile0[s + 1]) ++s;
-    }
+__device__ __forceinline__ void fs_piece(const fs_args &a, F &&piece) {
+    // (loads that wait for no other)
+    const uint32_t piece0 = a.piece0[threadIdx.x & 63u], last0 = a.piece0[64], n_before = a.wide, n = WIDE ? n_before : a.narrow;
+    // neighbours on one XCD
+    const uint32_t each = (n + 7) / 8;
+    uint32_t p = n < 8 ? blockIdx.x : (blockIdx.x & 7u) * each + (blockIdx.x >> 3);
+    if (p >= n) return;
+    if (!WIDE) p += n_before;
+    const uint32_t s = __builtin_amdgcn_readfirstlane(last0 <= p ? 64u : (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(piece0 <= p)) - 1);
+    const fs_seg &sg = a.seg[s];
+    const uint32_t n_rt = fs_row_tiles(WIDE, sg.n_rows), x = p - a.piece0[s], y = x / n_rt, h = y / sg.pieces, j = y - h * sg.pieces;
+    const uint32_t i_lo = j * sg.per + min(j, sg.more);
+    piece(sg, x - y * n_rt, h, WIDE ? 4 * p : 4 * n_before + (p - n_before), i_lo, i_lo + sg.per + (j < sg.more ? 1u : 0u));
 }
 
 template <int D, bool QUANT>
 __global__ void __launch_bounds__(512) k_fs_wide(fs_args a) {
     __shared__ fs_lds_wide<D, QUANT> sm;
-    fs_pieces<true>(a, [&](const fs_seg &sg, uint32_t rt, uint32_t h, uint32_t slot, uint32_t i_lo, uint32_t i_hi) {
+    fs_piece<true>(a, [&](const fs_seg &sg, uint32_t rt, uint32_t h, uint32_t slot, uint32_t i_lo, uint32_t i_hi) {
         fs_wide_piece<D, QUANT>(a, sg, sm, rt, h, slot, i_lo, i_hi);
     });
 }
@@ -941,7 +927,7 @@ __global__ void __launch_bounds__(512) k_fs_wide(fs_args a) {
 template <int D>
 __global__ void __launch_bounds__(256, 2) k_fs_narrow(fs_args a) {
     __shared__ fs_lds_narrow<D> sm;
-    fs_pieces<false>(a, [&](const fs_seg &sg, uint32_t rt, uint32_t h, uint32_t slot, uint32_t i_lo, uint32_t i_hi) {
+    fs_piece<false>(a, [&](const fs_seg &sg, uint32_t rt, uint32_t h, uint32_t slot, uint32_t i_lo, uint32_t i_hi) {
         fs_narrow<D>(a, sg, sm, rt, h, slot, i_lo, i_hi);
     });
 }
@@ -957,46 +943,33 @@ __global__ void __launch_bounds__(256) k_fs_join(fs_join_args a) {
     __shared__ float s_m[4][64], s_l[4][64];
     const uint32_t l = threadIdx.x & 63u, w = threadIdx.x >> 6, m2 = l & 31u, h = blockIdx.z, row_b = 32 * blockIdx.x, row = row_b + m2;
     // lane x has conversation x's entries
-    const uint32_t t_row0 = a.row0[l], t_rows = a.rows[l], t_tile0 = a.tile0[l], t_tiles = a.tiles[l], t_slot0 = a.slot0[l];
+    const uint32_t t_row0 = a.row0[l], t_rows = a.rows[l], t_pieces = a.pieces[l], t_slot0 = a.slot0[l];
     // (as values: the compiler would load where each is used, one wait after another)
     auto pin = [](uint32_t x) {
         asm volatile("" : "+s"(x));
         return x;
     };
-    const uint32_t wb = pin(a.wide.base), wq = pin(a.wide.q), wr = pin(a.wide.r), nb = pin(a.narrow.base), nq = pin(a.narrow.q), nr = pin(a.narrow.r);
-    const uint32_t pre_tiles = pin(a.pre_tiles), pre_wide = pin(a.pre_wide), pre_slot0 = pin(a.pre_slot0), n_rows = pin(a.n_rows);
+    const uint32_t n_pre = pin(a.pre_pieces), pre_wide = pin(a.pre_wide), n_rows = pin(a.n_rows);
     const bool live = row < n_rows;
-    // the pieces of unit u (with `tiles` tiles, tile0 before the segment's) : n of them from p0 on
-    auto pieces = [&](bool wide, uint32_t tile0, uint32_t tiles, uint32_t u, uint32_t &n) {
-        fs_deal dl;
-        dl.base = wide ? wb : nb;
-        dl.q = wide ? wq : nq;
-        dl.r = wide ? wr : nr;
-        const uint32_t c0 = tile0 + u * tiles, p0 = dl.owner(c0);
-        n = dl.owner(c0 + tiles - 1) - p0 + 1;
-        return p0;
+    // the first slot of the segment's row r, and from one piece to the next
+    auto slots = [&](bool wide, uint32_t slot0, uint32_t pieces, uint32_t rows, uint32_t r, uint32_t &step) {
+        const uint32_t gr = wide ? 4u : 1u, rt = r >> (wide ? 7 : 5);
+        step = fs_row_tiles(wide, rows) * gr;
+        return slot0 + h * pieces * step + rt * gr + (wide ? r >> 5 & 3u : 0u);
     };
-    uint32_t n_pre = 0, step_pre = 0, slot_pre = 0, n_own = 0, step_own = 0, slot_own = 0, r_own = 0;
-    if (pre_tiles) {                                      // (its rows are all rows)
-        const uint32_t ur = fs_unit_rows(pre_wide), u = h * fs_row_tiles(pre_wide, n_rows) + row_b / ur;
-        const uint32_t p0 = pieces(pre_wide, 0, pre_tiles, u, n_pre);
-        step_pre = ur / 32;
-        slot_pre = pre_slot0 + (p0 + u) * step_pre + row_b % ur / 32;
-    }
+    uint32_t step_pre, n_own = 0, step_own = 0, slot_own = 0, r_own = 0;
+    const uint32_t slot_pre = slots(pre_wide, 0, n_pre, n_rows, row_b, step_pre);       // (the prefix's rows are all rows)
     // the conversation that the row is in: the last that begins at or before it
     const uint32_t c_lo = __popcll(__builtin_amdgcn_ballot_w64(t_row0 <= row_b)), c_hi = __popcll(__builtin_amdgcn_ballot_w64(t_row0 <= row_b + 31));
     uint32_t cv = c_lo;
     for (uint32_t x = c_lo; x < c_hi; ++x) cv += row >= (uint32_t)__builtin_amdgcn_readlane((int)t_row0, (int)x);
     if (c_hi) {
         auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_ds_bpermute((int)(4 * (cv ? cv - 1 : 0)), (int)v); };
-        const uint32_t row0 = of(t_row0), n = of(t_rows), tile0 = of(t_tile0), tiles = of(t_tiles), slot0 = of(t_slot0);
-        if (live && cv && row - row0 < n) {
-            const bool wide = tiles >> 31;
+        const uint32_t row0 = of(t_row0), rows = of(t_rows), pieces = of(t_pieces), slot0 = of(t_slot0);
+        if (live && cv && row - row0 < rows) {
             r_own = row - row0;
-            const uint32_t ur = fs_unit_rows(wide), u = h * fs_row_tiles(wide, n) + r_own / ur;
-            const uint32_t p0 = pieces(wide, tile0, tiles & 0x7fffffffu, u, n_own);
-            step_own = ur / 32;
-            slot_own = slot0 + (p0 + u) * step_own + r_own % ur / 32;
+            n_own = pieces & 0x7fffffffu;
+            slot_own = slots(pieces >> 31, slot0, n_own, rows, r_own, step_own);
         }
     }
     const uint32_t n = live ? n_pre + n_own : 0u, t = row / a.G;
@@ -1087,12 +1060,12 @@ static uint32_t fs_stride(uint32_t n) {
 }
 
 // The rows from which on a window's units are wide.  An f16 window has nothing to convert: all.
-// A CU's workgroup takes a tile of a wide unit of 256 dims in 2.0 us, its two narrow ones a tile
-// of theirs in 1.4: a wide unit pays from three narrow ones' rows on (two's: 48 rows over 32,768
-// cells with 8 x 6 over 2,048, all narrow 43 us, else 34 + 16).  Where some windows
-// stay narrow all the same, the wide ones are a launch more (10 us for its start and end) and
-// have to save that: 288 rows over 5,003 cells with 16 x 18 over 8,192, all narrow 73 us, else
-// 37 + 52; 768 rows over 32,768 with 32 x 24 over 2,048, 246 us and 136 + 37.
+// A CU takes a tile of a wide unit of 256 dims in 2.0 us, one of a narrow one in 1.05 (two
+// workgroups, 2.1 each): a wide unit pays from three narrow ones' rows on (two's: 48 rows over
+// 32,768 cells with 8 x 6 over 2,048, all narrow 33 us, else 28 + 16).  Where some windows stay
+// narrow all the same, the wide ones are a launch more (10 us for its start and end) and have to
+// save that: 288 rows over 5,003 cells with 16 x 18 over 8,192, all narrow 67 us, else 26 + 52;
+// 768 rows over 32,768 with 32 x 24 over 2,048, 251 us and 137 + 35.
 static uint32_t fs_wide_rows(const kvm_window *prefix, const kvm_window *const *windows, const uint32_t *n_tokens, uint32_t n_lanes, bool quant,
                              uint32_t n_cu, uint32_t H, uint32_t G, uint32_t n_rows) {
     if (!quant) return 1;
@@ -1101,35 +1074,59 @@ static uint32_t fs_wide_rows(const kvm_window *prefix, const kvm_window *const *
     auto add = [&](const kvm_window *w, uint32_t r) {
         if (!w || !r) return;
         if (r <= 64) narrow = true;
-        else saved += (double)(w->n_cells / KVM_TILE_CELLS) * H / n_cu * (1.4 * fs_row_tiles(false, r) - 2.0 * fs_row_tiles(true, r));
+        else saved += (double)(w->n_cells / KVM_TILE_CELLS) * H / n_cu * (1.05 * fs_row_tiles(false, r) - 2.0 * fs_row_tiles(true, r));
     };
     add(prefix, n_rows);
     for (uint32_t i = 0; i < n_lanes; ++i) add(windows ? windows[i] : nullptr, n_tokens[i] * G);
     return narrow && saved < 10.0 ? 0xffffffffu : 65;
 }
 
-// Fills the segments, their tiles and slots, and the numbers of workgroups.
+// Pieces of at most this many tiles: what `groups` workgroups at a time do in the least time,
+// in tiles, where a piece's start and end cost 4 tiles' time, and no piece is below `least`.
+static uint32_t fs_piece_tiles(const fs_seg *seg, uint32_t n, bool wide, uint32_t H, uint32_t groups, uint32_t least) {
+    uint64_t tiles = 0;
+    uint32_t most = 1;
+    for (uint32_t i = 0; i < n; ++i) {
+        tiles += (uint64_t)fs_row_tiles(wide, seg[i].n_rows) * H * seg[i].n_tiles;
+        most = std::max(most, seg[i].n_tiles);
+    }
+    auto pieces = [&](uint32_t t) {
+        uint64_t x = 0;
+        for (uint32_t i = 0; i < n; ++i) x += (uint64_t)fs_row_tiles(wide, seg[i].n_rows) * H * ((seg[i].n_tiles + t - 1) / t);
+        return x;
+    };
+    uint32_t best = most;
+    uint64_t best_time = ~0ull;
+    for (uint32_t rounds = 1; rounds <= 4; ++rounds) {
+        // the least number of tiles whose pieces are no more than the rounds' workgroups
+        uint32_t lo = (uint32_t)std::min<uint64_t>(most, std::max<uint64_t>(least, tiles / ((uint64_t)rounds * groups))), hi = most;
+        lo = std::max(lo, 1u);
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (pieces(mid) <= (uint64_t)rounds * groups) hi = mid;
+            else lo = mid + 1;
+        }
+        const uint64_t time = (pieces(lo) + groups - 1) / groups * (lo + 4);
+        if (time < best_time) {
+            best_time = time;
+            best = lo;
+        }
+        if (4 * tiles >= 3ull * groups * lo) break;       // (as even as it gets)
+    }
+    return best;
+}
+
+// Fills the segments, their pieces and slots.
 static int fs_shape(kvm_state *st, const char *what, const kvm_window *prefix, const kvm_window *const *windows,
                     const uint32_t *n_tokens, uint32_t n_lanes, bool quant, uint32_t n_cu, fs_args *a, fs_join_args *j, uint64_t *slots) {
     const uint32_t wide_rows = fs_wide_rows(prefix, windows, n_tokens, n_lanes, quant, n_cu, a->H, a->G, a->n_rows);
-    uint64_t tiles = 0, units = 0, wide = 0;
-    uint32_t n = 0;
+    uint32_t n = 0, nw = 0, lane_seg[FS_LANES], own = 0;
     auto add = [&](const kvm_window *w, uint32_t row0, uint32_t n_rows) {
         const uint32_t t = w->n_cells / KVM_TILE_CELLS;
-        const bool iw = n_rows >= wide_rows;
-        a->tile0[n] = (uint32_t)tiles;
-        a->seg[n++] = fs_seg{(const uint8_t *)w->k, (const uint8_t *)w->v, w->cell_pos, t, fs_stride(t), row0, n_rows};
-        const uint64_t u = (uint64_t)fs_row_tiles(iw, n_rows) * a->H;
-        units += u;
-        tiles += u * t;
-        if (iw) wide = tiles, a->n_wide = n;
+        a->seg[n++] = fs_seg{(const uint8_t *)w->k, (const uint8_t *)w->v, w->cell_pos, t, fs_stride(t), row0, n_rows, 1, t, 0};
+        if (n_rows >= wide_rows) nw = n;
     };
-    uint32_t lane_seg[FS_LANES], own = 0;
-    if (prefix) {                                          // (wide where a conversation is)
-        add(prefix, 0, a->n_rows);
-        j->pre_tiles = a->seg[0].n_tiles;
-        j->pre_wide = a->n_wide;
-    }
+    if (prefix) add(prefix, 0, a->n_rows);                 // (wide where a conversation is)
     for (int narrow = 0; narrow < 2; ++narrow) {
         uint32_t row = 0;
         own = 0;
@@ -1145,42 +1142,42 @@ static int fs_shape(kvm_state *st, const char *what, const kvm_window *prefix, c
             row += r;
         }
     }
-    if (tiles > 0x7fffffffu || units > (1u << 22))
-        return kvm_fail(st, KVM_ERANGE, "%s: %u rows over these windows are too many for one call", what, a->n_rows);
-    a->tile0[n] = (uint32_t)tiles;
-    a->n_seg = n;
-    // Workgroups: what the CUs hold at once, and a tile or more for each wave that has tiles of
-    // its own (8 rows over 1,024 + 2 x 256 f16 cells of 2 heads: 8.7 us, with 4 tiles a workgroup
-    // 15.6); eighths, one for each XCD
-    auto deal = [](uint32_t base, uint32_t of, uint32_t most, uint32_t least) {
-        uint32_t p = std::min(most, std::max(of / least, 1u));
-        if (p > 8) p &= ~7u;
-        return fs_deal{base, p, of / p, of % p};
-    };
-    a->wide = deal(0, (uint32_t)wide, n_cu, 1);
-    a->narrow = deal((uint32_t)wide, (uint32_t)(tiles - wide), 2 * n_cu, 2);
-    // A unit's pieces are those of the workgroups that its tiles reach over; from one piece
-    // of a segment to the next the workgroup, the unit or both go on by one.
-    uint64_t slot = 0;
+    // Workgroups: what the CUs hold at once.  A tile or more for each wave that has tiles of its
+    // own, or half a one where that leaves CUs idle (8 rows over 1,024 + 2 x 256 f16 cells of 2
+    // heads: 8.7 us, with 4 tiles a workgroup 15.6; 12 over 1,024 + 2 x 256 q8_0 cells of 4: 2
+    // tiles 12.1 us, 4 13.8); a second narrow workgroup a CU for pieces of 4 tiles or more (48 over
+    // 4,032 + 4 x 512: 320 workgroups of 2 tiles 19.0, 160 of 4 16.5).
+    const uint32_t tw = fs_piece_tiles(a->seg, nw, true, a->H, n_cu, 1);
+    uint32_t tn = fs_piece_tiles(a->seg + nw, n - nw, false, a->H, n_cu, 2);
+    if (tn > 4) tn = fs_piece_tiles(a->seg + nw, n - nw, false, a->H, 2 * n_cu, 4);
+    uint64_t piece = 0, wide = 0;
     for (uint32_t i = 0; i < n; ++i) {
-        const bool iw = i < a->n_wide;
-        const fs_deal &dl = iw ? a->wide : a->narrow;
-        const uint32_t gr = fs_unit_rows(iw) / 32, p0 = dl.owner(a->tile0[i]), p1 = dl.owner(a->tile0[i + 1] - 1);
-        a->slot0[i] = (uint32_t)slot - p0 * gr;
-        slot += (uint64_t)(p1 - p0 + fs_row_tiles(iw, a->seg[i].n_rows) * a->H) * gr;
+        fs_seg &sg = a->seg[i];
+        const uint32_t t = i < nw ? tw : tn;
+        sg.pieces = (sg.n_tiles + t - 1) / t;
+        sg.per = sg.n_tiles / sg.pieces;
+        sg.more = sg.n_tiles % sg.pieces;
+        a->piece0[i] = (uint32_t)piece;
+        piece += (uint64_t)fs_row_tiles(i < nw, sg.n_rows) * a->H * sg.pieces;
+        if (i + 1 == nw) wide = piece;
+        if (piece > (1u << 24))
+            return kvm_fail(st, KVM_ERANGE, "%s: %u rows over these windows are too many for one call", what, a->n_rows);
     }
-    *slots = slot;
-    j->wide = a->wide;
-    j->narrow = a->narrow;
-    if (prefix) j->pre_slot0 = a->slot0[0];
+    for (uint32_t i = n; i < FS_SEGS; ++i) a->piece0[i] = 0xffffffffu;
+    a->wide = (uint32_t)wide;
+    a->narrow = (uint32_t)(piece - wide);
+    *slots = 4 * wide + (piece - wide);
+    if (prefix) {
+        j->pre_pieces = a->seg[0].pieces;
+        j->pre_wide = nw > 0;
+    }
     for (uint32_t i = 0; i < FS_LANES; ++i) j->row0[i] = 0xffffffffu;
     for (uint32_t i = 0; i < own; ++i) {
         const uint32_t s = lane_seg[i];
         j->row0[i] = a->seg[s].row0;
         j->rows[i] = a->seg[s].n_rows;
-        j->tile0[i] = a->tile0[s];
-        j->tiles[i] = a->seg[s].n_tiles | (s < a->n_wide ? 0x80000000u : 0u);
-        j->slot0[i] = a->slot0[s];
+        j->pieces[i] = a->seg[s].pieces | (s < nw ? 0x80000000u : 0u);
+        j->slot0[i] = (uint32_t)(s < nw ? 4 * a->piece0[s] : 4 * wide + (a->piece0[s] - wide));
     }
     return KVM_OK;
 }
@@ -1259,8 +1256,9 @@ extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, con
     auto go = [&](auto d, auto qt) {
         constexpr int DD = decltype(d)::value;
         constexpr bool Q = decltype(qt)::value;
-        if (a.n_wide) hipLaunchKernelGGL((k_fs_wide<DD, Q>), dim3(a.wide.p), dim3(512), 0, st->stream, a);
-        if (Q && a.n_wide < a.n_seg) hipLaunchKernelGGL((k_fs_narrow<DD>), dim3(a.narrow.p), dim3(256), 0, st->stream, a);
+        auto grid = [](uint32_t n) { return dim3(n < 8 ? n : (n + 7) / 8 * 8); };       // (a grid of 8 for each XCD's)
+        if (a.wide) hipLaunchKernelGGL((k_fs_wide<DD, Q>), grid(a.wide), dim3(512), 0, st->stream, a);
+        if (Q && a.narrow) hipLaunchKernelGGL((k_fs_narrow<DD>), grid(a.narrow), dim3(256), 0, st->stream, a);
         hipLaunchKernelGGL((k_fs_join<DD>), dim3(kvm_cdiv(a.n_rows, 32), by, H), dim3(256), 0, st->stream, j);
     };
     auto go_d = [&](auto d) {

@@ -323,8 +323,8 @@ __device__ __forceinline__ void fs_copy4(const int32_t *src, uint32_t off, void 
 // A piece of a narrow unit (32 rows over a quantised window): tiles [i_lo, i_hi) in the
 // unit's order.  A tile of 256 dims is ~1,650 instructions of a wave, 930 of them its conversion,
 // and 64 MFMAs (2,048 cycles): the issue of two waves a SIMD bounds it (~2.1 us a tile and
-// workgroup; everything in the L2, a third less), next to the memory where no two units read the
-// same tiles, and for short pieces the start (8.6 us to the first half tile) and the sums' meeting
+// workgroup), next to the memory where no two units read the same tiles (all in the L2: 55 of 66
+// us), and for short pieces the start (8.6 us to the first half tile) and the sums' meeting
 // (2.2).  8 lanes x 6 rows of 4 heads over 32,768 + 2,048 cells of q8_0: 33 us for 74.5 MB, 2.3
 // TB/s; 16 x 18 over 5,003 + 8,192 of q4_0: 67 us, 154 MB.
 template <int D>
@@ -575,8 +575,8 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
 // A piece of a wide unit.  A tile of 256 dims is 64 MFMAs of an attention wave (2,048 cycles) in
 // ~4,600: its softmax and the other wave's conversion share the SIMD's issue, at the clock that
 // the power limit leaves.  768 rows of 4 heads over 32,768 cells of q8_0 (103 GFLOP): 137 us, 750
-// TFLOP/s.  Over an f16 window of few rows the memory: 36 tokens x 4 rows of 8 heads of 128 dims
-// over 8,192 + 12 x 1,024 cells, 24 us for 84 MB, the prefix read twice.
+// TFLOP/s.  36 tokens x 4 rows of 8 heads of 128 dims over 8,192 + 12 x 1,024 f16 cells: 24 us for
+// 84 MB, the prefix read twice (without the attention waves' work 17, without the copies 25).
 template <int D, bool QUANT>
 __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg, fs_lds_wide<D, QUANT> &sm, uint32_t rt, uint32_t h,
                                               uint32_t slot, uint32_t i_lo, uint32_t i_hi) {
