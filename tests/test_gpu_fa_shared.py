@@ -192,6 +192,31 @@ def test_many_tiles_a_workgroup(kvm_state):
         q_pos=rng.integers(n // 2, n, 40))
 
 
+@pytest.mark.parametrize("cache,H,G,tokens", [("q8_0", 8, 1, 1), ("f16", 4, 1, 1), ("q8_0", 4, 8, 9)])
+def test_pieces_longer_than_a_look(kvm_state, cache, H, G, tokens):
+    """As many units as the chip has workgroups, so that each is a piece of its own, of more tiles
+    than are looked at at a time: sixty-four conversations over the same window."""
+    st, rng, D, n = kvm_state, np.random.default_rng(21), 128, 64 * 301
+    p = rng.permutation(n)
+    p[rng.random(n) < 0.02] = -1
+    p[64 * 270:64 * 280] = -1
+    w = window(st, rng, n, H, D, cache, p)
+    counts = [tokens] * 64
+    q = torch.from_numpy(rng.standard_normal((64 * tokens, H * G, D)).astype(np.float32)).cuda()
+    qp = torch.from_numpy(rng.integers(-3, n, 64 * tokens).astype(np.int32)).cuda()
+    got = api.fa_decode_shared(st, None, [w[0]] * 64, counts, q, qp, H * G, D ** -0.5)
+    check(got, *expected(q, qp, counts, None, [w] * 64, H, D ** -0.5))
+
+
+@pytest.mark.parametrize("cache", ["q8_0", "f16"])
+@pytest.mark.parametrize("rows", [31, 32, 33, 63, 64, 65, 96, 97, 127, 128, 129, 257])
+def test_row_counts_at_the_units_edges(kvm_state, cache, rows):
+    """One conversation of that many rows of a kv head, over a prefix and its own cells."""
+    rng = np.random.default_rng(rows)
+    run(kvm_state, rng, 1, 1, 128, cache, 192, cells(192, 190, 0), [(320, cells(320, 320, 190))], [rows], torch.bfloat16,
+        torch.float32, q_pos=np.arange(510 - rows, 510))
+
+
 def test_workspace_under_capture(kvm_state):
     """A capture that needs a larger workspace is refused; one captured before another call
     grew it replays on the one it had."""
