@@ -47,6 +47,7 @@ struct fs_seg {
     const int32_t *cell_pos;
     uint32_t n_tiles, mult;      // tile i of a unit's order is (i mult) mod n_tiles
     uint32_t row0, n_rows;       // rows [row0, row0 + n_rows) of every kv head
+    uint32_t step;               // from tile i to tile i + 4 times the waves of a workgroup (mod n_tiles)
     uint32_t pieces, per, more;  // of a unit: pieces of `per` tiles, the first `more` of one more
 };
 
@@ -59,6 +60,7 @@ struct fs_args {
     uint32_t wide, narrow;       // pieces; the wide ones' segments come first
     float c, q_sign;             // |scale| log2(e); q times -1 for a negative scale, and 0 (c = 1) for none
     int q_type;
+    float inv_g;                 // 1 / G
     // Pieces of the segments before; a segment's: [head][piece of the unit][unit of the head],
     // so that neighbours read the same tiles.  A wide piece has 4 slots, a narrow one 1.
     uint32_t piece0[FS_SEGS];    // (past the last segment: ~0)
@@ -135,6 +137,17 @@ __device__ __forceinline__ uint32_t fs_opaque(uint32_t x) {
 // K row i of a half tile is this key: bits 2 and 3 swapped.
 __device__ __forceinline__ uint32_t fs_key(uint32_t i) { return (i & 0x13) | (i & 4) << 1 | (i & 8) >> 1; }
 
+// The token of a row (< 2^24), and its head of the group: a reciprocal, right to one, in a tenth of
+// the instructions of a division.
+__device__ __forceinline__ uint32_t fs_token(const fs_args &a, uint32_t row, uint32_t &g) {
+    uint32_t t = (uint32_t)((float)row * a.inv_g);
+    int32_t r = (int32_t)(row - t * a.G);
+    if (r < 0) --t, r += (int32_t)a.G;
+    if (r >= (int32_t)a.G) ++t, r -= (int32_t)a.G;
+    g = (uint32_t)r;
+    return t;
+}
+
 // Nothing moves over it.
 #define FS_FENCE() __builtin_amdgcn_sched_barrier(0)
 
@@ -149,8 +162,9 @@ struct fs_rows {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const uint32_t x = threadIdx.x + 64 * NW * i, b = x >> 6, r = b % (4 * RG) * 8 + (x & 63u) / 8, u = b / (4 * RG) * 8 + (x & 7u);
-            const uint32_t row = row_g + (r < rows ? r : 0u), t = row / a.G;
-            const uint64_t e = ((uint64_t)t * a.n_head + h * a.G + (row - t * a.G)) * D + 8 * u;
+            uint32_t g;
+            const uint32_t t = fs_token(a, row_g + (r < rows ? r : 0u), g);
+            const uint64_t e = ((uint64_t)t * a.n_head + h * a.G + g) * D + 8 * u;
             if (a.q_type == KVM_TYPE_F32) __builtin_memcpy(y[i], (const float *)a.q + e, 32);
             else __builtin_memcpy(y[i], (const uint16_t *)a.q + e, 16);
         }
@@ -172,23 +186,26 @@ struct fs_rows {
 
 // A row's limit: it sees the cells with (unsigned)position below it.
 __device__ __forceinline__ uint32_t fs_limit(const fs_args &a, uint32_t row_g, uint32_t rows, uint32_t r) {
-    const int32_t qp = r < rows ? a.q_pos[(row_g + r) / a.G] : -1;
+    uint32_t g;
+    const int32_t qp = r < rows ? a.q_pos[fs_token(a, row_g + r, g)] : -1;
     return qp >= 0 ? (uint32_t)qp + 1u : 0u;
 }
 
 // Tile i of a unit's order.
 __device__ __forceinline__ uint32_t fs_tile(const fs_seg &sg, uint32_t i) { return i * sg.mult % sg.n_tiles; }      // (n_tiles < 2^16)
 
-// Positions of the cells of tiles b0 + r0 .. of nb in the unit's order: 4 tiles a wave and load.
+// Positions of the cells of tiles b0 + r0 .. in the unit's order: 4 tiles a wave and load.
 template <int NW>
 struct fs_cells {
     kvm_u32x4 c[4];
     __device__ __forceinline__ static uint32_t at(uint32_t r0, int r) { return r0 + 4 * NW * r + 4 * (threadIdx.x >> 6) + ((threadIdx.x & 63u) >> 4); }
-    __device__ __forceinline__ void load(const fs_seg &sg, uint32_t b0, uint32_t nb, uint32_t r0) {
+    __device__ __forceinline__ void load(const fs_seg &sg, uint32_t b0, uint32_t r0) {
+        uint32_t t = fs_tile(sg, b0 + at(r0, 0));
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t i = at(r0, r);
-            c[r] = *(const kvm_u32x4 *)(sg.cell_pos + (uint64_t)fs_tile(sg, b0 + (i < nb ? i : 0u)) * 64 + 4 * (threadIdx.x & 15u));
+        for (int r = 0; r < 4; ++r) {                     // (past the last: another of the window's)
+            c[r] = *(const kvm_u32x4 *)(sg.cell_pos + (uint64_t)t * 64 + 4 * (threadIdx.x & 15u));
+            t += sg.step;
+            t -= t < sg.n_tiles ? 0u : sg.n_tiles;
         }
     }
 };
@@ -212,7 +229,7 @@ __device__ __forceinline__ uint32_t fs_tiles(const fs_seg &sg, fs_list<D, NW> &s
         }
         r0 += 16 * NW;
         if (r0 >= nb) break;
-        cells.load(sg, b0, nb, r0);
+        cells.load(sg, b0, r0);
     }
     __syncthreads();
     if (threadIdx.x == 0) sm.odd = 0;
@@ -339,7 +356,7 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
 
     // the loads of the start, all issued before any is used
     fs_cells<4> cells;
-    cells.load(sg, i_lo, min(FS_BATCH, i_hi - i_lo), 0);
+    cells.load(sg, i_lo, 0);
     const uint32_t qlim = fs_limit(a, row_g, rows, m2);
     {
         fs_rows<D, 1, 4> q;
@@ -361,7 +378,7 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
     const uint8_t *const k_head = sg.k + (uint64_t)h * sg.n_tiles * KB, *const v_head = sg.v + (uint64_t)h * sg.n_tiles * VB;
 
     for (uint32_t b0 = i_lo; b0 < i_hi; b0 += FS_BATCH) {
-        if (b0 != i_lo) cells.load(sg, b0, min(FS_BATCH, i_hi - b0), 0);
+        if (b0 != i_lo) cells.load(sg, b0, 0);
         const uint32_t n_t = fs_tiles<D, 4>(sg, sm, b0, min(FS_BATCH, i_hi - b0), some_lim, all_lim, cells);      // (its barriers: Q, too)
 
         // The wave's half tiles: half w & 1 of list entries w / 2, w / 2 + 2, ..  Their
@@ -589,7 +606,7 @@ __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg
 
     // the loads of the start, all issued before any is used
     fs_cells<8> cells;
-    cells.load(sg, i_lo, min(FS_BATCH, i_hi - i_lo), 0);
+    cells.load(sg, i_lo, 0);
     const uint32_t lim0 = fs_limit(a, row_g, rows, l), lim1 = fs_limit(a, row_g, rows, l + 64);
     {
         fs_rows<D, 4, 8> q;
@@ -742,7 +759,7 @@ __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg
             b0 += FS_BATCH;
             if (b0 >= i_hi) break;
             fs_cells<8> next;
-            next.load(sg, b0, min(FS_BATCH, i_hi - b0), 0);
+            next.load(sg, b0, 0);
             n_t = fs_tiles<D, 8>(sg, sm, b0, min(FS_BATCH, i_hi - b0), some_lim, all_lim, next);
         }
         if (active) {
@@ -893,7 +910,7 @@ __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg
             b0 += FS_BATCH;
             if (b0 >= i_hi) break;
             fs_cells<8> next;
-            next.load(sg, b0, min(FS_BATCH, i_hi - b0), 0);
+            next.load(sg, b0, 0);
             n_t = fs_tiles<D, 8>(sg, sm, b0, min(FS_BATCH, i_hi - b0), some_lim, all_lim, next);
         }
     }
@@ -1122,9 +1139,10 @@ static int fs_shape(kvm_state *st, const char *what, const kvm_window *prefix, c
     const uint32_t wide_rows = fs_wide_rows(prefix, windows, n_tokens, n_lanes, quant, n_cu, a->H, a->G, a->n_rows);
     uint32_t n = 0, nw = 0, lane_seg[FS_LANES], own = 0;
     auto add = [&](const kvm_window *w, uint32_t row0, uint32_t n_rows) {
-        const uint32_t t = w->n_cells / KVM_TILE_CELLS;
-        a->seg[n++] = fs_seg{(const uint8_t *)w->k, (const uint8_t *)w->v, w->cell_pos, t, fs_stride(t), row0, n_rows, 1, t, 0};
-        if (n_rows >= wide_rows) nw = n;
+        const uint32_t t = w->n_cells / KVM_TILE_CELLS, m = fs_stride(t);
+        const bool iw = n_rows >= wide_rows;
+        a->seg[n++] = fs_seg{(const uint8_t *)w->k, (const uint8_t *)w->v, w->cell_pos, t, m, row0, n_rows, (uint32_t)(4ull * (iw ? 8 : 4) * m % t), 1, t, 0};
+        if (iw) nw = n;
     };
     if (prefix) add(prefix, 0, a->n_rows);                 // (wide where a conversation is)
     for (int narrow = 0; narrow < 2; ++narrow) {
@@ -1221,6 +1239,7 @@ extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, con
     fs_join_args j{};
     a.H = H;
     a.G = n_head / H;
+    a.inv_g = 1.0f / (float)a.G;
     a.n_head = n_head;
     a.n_rows = (uint32_t)total * a.G;
     a.q = q;
