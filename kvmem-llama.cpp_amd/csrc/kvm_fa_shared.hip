@@ -341,9 +341,9 @@ __device__ __forceinline__ void fs_copy4(const int32_t *src, uint32_t off, void 
 // unit's order.  A tile of 256 dims is ~1,650 instructions of a wave, 930 of them its conversion,
 // and 64 MFMAs (2,048 cycles): the issue of two waves a SIMD bounds it (~2.1 us a tile and
 // workgroup), next to the memory where no two units read the same tiles (all in the L2: 55 of 66
-// us), and for short pieces the start (8.6 us to the first half tile) and the sums' meeting
-// (2.2).  8 lanes x 6 rows of 4 heads over 32,768 + 2,048 cells of q8_0: 33 us for 74.5 MB, 2.3
-// TB/s; 16 x 18 over 5,003 + 8,192 of q4_0: 67 us, 154 MB.
+// us), and for short pieces the start (5.6 us to the first half tile) and the sums' meeting
+// (2.2).  8 lanes x 6 rows of 4 heads over 32,768 + 2,048 cells of q8_0: 30 us for 74.5 MB, 2.5
+// TB/s; 16 x 18 over 5,003 + 8,192 of q4_0: 64 us, 154 MB.
 template <int D>
 __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs_lds_narrow<D> &sm, uint32_t rt, uint32_t h, uint32_t slot,
                                           uint32_t i_lo, uint32_t i_hi) {
@@ -1079,9 +1079,9 @@ static uint32_t fs_stride(uint32_t n) {
 // The rows from which on a window's units are wide.  An f16 window has nothing to convert: all.
 // A CU takes a tile of a wide unit of 256 dims in 2.0 us, one of a narrow one in 1.05 (two
 // workgroups, 2.1 each): a wide unit pays from three narrow ones' rows on (two's: 48 rows over
-// 32,768 cells with 8 x 6 over 2,048, all narrow 33 us, else 28 + 16).  Where some windows stay
+// 32,768 cells with 8 x 6 over 2,048, all narrow 30 us, else 28 + 16).  Where some windows stay
 // narrow all the same, the wide ones are a launch more (10 us for its start and end) and have to
-// save that: 288 rows over 5,003 cells with 16 x 18 over 8,192, all narrow 67 us, else 26 + 52;
+// save that: 288 rows over 5,003 cells with 16 x 18 over 8,192, all narrow 64 us, else 26 + 52;
 // 768 rows over 32,768 with 32 x 24 over 2,048, 251 us and 137 + 35.
 static uint32_t fs_wide_rows(const kvm_window *prefix, const kvm_window *const *windows, const uint32_t *n_tokens, uint32_t n_lanes, bool quant,
                              uint32_t n_cu, uint32_t H, uint32_t G, uint32_t n_rows) {
@@ -1098,18 +1098,20 @@ static uint32_t fs_wide_rows(const kvm_window *prefix, const kvm_window *const *
     return narrow && saved < 10.0 ? 0xffffffffu : 65;
 }
 
-// Pieces of at most this many tiles: what `groups` workgroups at a time do in the least time,
-// in tiles, where a piece's start and end cost 4 tiles' time, and no piece is below `least`.
-static uint32_t fs_piece_tiles(const fs_seg *seg, uint32_t n, bool wide, uint32_t H, uint32_t groups, uint32_t least) {
+// Cuts the units of n segments into pieces: of as many tiles at most as let `groups` workgroups at
+// a time end first, in tiles, where a piece's start and end cost 4 tiles' time, and no piece is
+// below `least`.  Returns that number of tiles.
+static uint32_t fs_cut(fs_seg *seg, uint32_t n, bool wide, uint32_t H, uint32_t groups, uint32_t least) {
     uint64_t tiles = 0;
     uint32_t most = 1;
+    auto units = [&](uint32_t i) { return (uint64_t)fs_row_tiles(wide, seg[i].n_rows) * H; };
     for (uint32_t i = 0; i < n; ++i) {
-        tiles += (uint64_t)fs_row_tiles(wide, seg[i].n_rows) * H * seg[i].n_tiles;
+        tiles += units(i) * seg[i].n_tiles;
         most = std::max(most, seg[i].n_tiles);
     }
     auto pieces = [&](uint32_t t) {
         uint64_t x = 0;
-        for (uint32_t i = 0; i < n; ++i) x += (uint64_t)fs_row_tiles(wide, seg[i].n_rows) * H * ((seg[i].n_tiles + t - 1) / t);
+        for (uint32_t i = 0; i < n; ++i) x += units(i) * ((seg[i].n_tiles + t - 1) / t);
         return x;
     };
     uint32_t best = most;
@@ -1129,6 +1131,27 @@ static uint32_t fs_piece_tiles(const fs_seg *seg, uint32_t n, bool wide, uint32_
             best = lo;
         }
         if (4 * tiles >= 3ull * groups * lo) break;       // (as even as it gets)
+    }
+    uint64_t left = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+        seg[i].pieces = (seg[i].n_tiles + best - 1) / best;
+        left += units(i) * seg[i].pieces;
+    }
+    // The workgroups that are left over shorten the longest pieces (8 lanes x 6 rows over 32,768 +
+    // 2,048 cells: 472 pieces of 11 tiles 32.7 us, 512 of 10 and 11 30.0).
+    left = (left + groups - 1) / groups * groups - left;
+    for (uint32_t x = 0; x < 64 && left; ++x) {
+        uint32_t at = n, longest = least;
+        for (uint32_t i = 0; i < n; ++i) {
+            const uint32_t t = (seg[i].n_tiles + seg[i].pieces - 1) / seg[i].pieces;
+            if (t > longest && units(i) <= left) at = i, longest = t;
+        }
+        if (at == n) break;
+        const uint32_t p = (seg[at].n_tiles + longest - 2) / (longest - 1);
+        const uint64_t more = units(at) * (p - seg[at].pieces);
+        if (more > left) break;
+        seg[at].pieces = p;
+        left -= more;
     }
     return best;
 }
@@ -1165,14 +1188,11 @@ static int fs_shape(kvm_state *st, const char *what, const kvm_window *prefix, c
     // heads: 8.7 us, with 4 tiles a workgroup 15.6; 12 over 1,024 + 2 x 256 q8_0 cells of 4: 2
     // tiles 12.1 us, 4 13.8); a second narrow workgroup a CU for pieces of 4 tiles or more (48 over
     // 4,032 + 4 x 512: 320 workgroups of 2 tiles 19.0, 160 of 4 16.5).
-    const uint32_t tw = fs_piece_tiles(a->seg, nw, true, a->H, n_cu, 1);
-    uint32_t tn = fs_piece_tiles(a->seg + nw, n - nw, false, a->H, n_cu, 2);
-    if (tn > 4) tn = fs_piece_tiles(a->seg + nw, n - nw, false, a->H, 2 * n_cu, 4);
+    fs_cut(a->seg, nw, true, a->H, n_cu, 1);
+    if (fs_cut(a->seg + nw, n - nw, false, a->H, n_cu, 2) > 4) fs_cut(a->seg + nw, n - nw, false, a->H, 2 * n_cu, 4);
     uint64_t piece = 0, wide = 0;
     for (uint32_t i = 0; i < n; ++i) {
         fs_seg &sg = a->seg[i];
-        const uint32_t t = i < nw ? tw : tn;
-        sg.pieces = (sg.n_tiles + t - 1) / t;
         sg.per = sg.n_tiles / sg.pieces;
         sg.more = sg.n_tiles % sg.pieces;
         a->piece0[i] = (uint32_t)piece;
