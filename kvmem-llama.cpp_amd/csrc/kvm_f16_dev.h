@@ -16,7 +16,8 @@ __device__ __forceinline__ void pf_pairs(uint32_t bytes, kvm_f16x2 &a, kvm_f16x2
 }
 // 8 int8 quants times one scale
 __device__ __forceinline__ kvm_f16x8 pf_q8(uint32_t w0, uint32_t w1, uint32_t dbits) {
-    const kvm_f16x2 off = {(_Float16)1152.0f, (_Float16)1152.0f}, d = pf_bits2(dbits * 0x10001u);
+    const _Float16 d1 = __builtin_bit_cast(_Float16, (uint16_t)dbits);
+    const kvm_f16x2 off = {(_Float16)1152.0f, (_Float16)1152.0f}, d = {d1, d1};
     kvm_f16x2 r[4];
     pf_pairs(w0 ^ 0x80808080u, r[0], r[1]);
     pf_pairs(w1 ^ 0x80808080u, r[2], r[3]);

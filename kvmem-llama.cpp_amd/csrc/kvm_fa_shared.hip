@@ -391,10 +391,10 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
             return __builtin_amdgcn_make_buffer_rsrc((void *)(head + (uint64_t)(e & 0x7fffffffu) * bytes), (short)0, more ? bytes : 0u, 0x00020000);
         };
         auto load_k = [&](__amdgpu_buffer_rsrc_t r, int set, int i) {
-            kr[set][i] = __builtin_amdgcn_raw_buffer_load_b128(r, fs_opaque(k_lane) + (i & 1) * 512, half * NB * 1024 + (i >> 1) * 1024, 0);
+            kr[set][i] = __builtin_amdgcn_raw_buffer_load_b128(r, k_lane + (i & 1) * 512, half * NB * 1024 + (i >> 1) * 1024, 0);
         };
         auto load_v = [&](__amdgpu_buffer_rsrc_t r, int set, int i) {
-            vq[set][i] = __builtin_amdgcn_raw_buffer_load_b32(r, fs_opaque(v_lane) + (i & 1) * 256, half * 4 + (i >> 1) * 1024, 0);
+            vq[set][i] = __builtin_amdgcn_raw_buffer_load_b32(r, v_lane + (i & 1) * 256, half * 4 + (i >> 1) * 1024, 0);
         };
         // lanes below 2 NB: the half's K scales, from 32 on its V scales (units of 8 keys of a block)
         auto copies = [&](uint32_t e, uint32_t buf) {
