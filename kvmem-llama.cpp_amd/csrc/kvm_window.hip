@@ -377,56 +377,65 @@ extern "C" int kvm_window_import_rows(kvm_state *st, const kvm_window *w, uint32
     for (uint64_t it = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; it < (total); it += (uint64_t)gridDim.x * blockDim.x)
 static dim3 win_grid(uint64_t items) { return dim3((uint32_t)std::min<uint64_t>((items + 255) / 256, 1u << 23)); }
 
-// Several threads a 32-value block, each 4 bytes of the row: they store side by side (2,047
-// rows of 4 x 256 in q8_0: 5.2 us; a block a thread, byte by byte, 10.3).
-__global__ void k_export_k_q8(win_geo g, uint32_t cell0, uint32_t n, uint8_t *rows) {
-    const uint32_t NB = g.D / 32;
-    WIN_ITEMS(x, (uint64_t)n * g.H * NB * 8) {
-        const uint64_t i = x / 8;
-        const uint32_t j = x % 8, b = i % NB, h = (i / NB) % g.H, t = (uint32_t)(i / ((uint64_t)NB * g.H));
-        const uint32_t cell = cell0 + t, tile = cell / 64, c = cell % 64;
-        uint8_t *dst = rows + i * 34;
-        const uint8_t *src = g.k + ((uint64_t)h * g.n_tiles + tile) * g.ktile;
-        if (j == 0) __builtin_memcpy(dst, src + kvm_kd_off(g.D, c, b), 2);
-        __builtin_memcpy(dst + 2 + 4 * j, src + kvm_kq_off(g.D, c, 32 * b + 8 * (j / 2)) + 4 * (j % 2), 4);
-    }
+// Block i of rows: its place in the row, its head, its row (64-bit divisions only where needed).
+__device__ __forceinline__ uint32_t win_block(const win_geo &g, uint64_t i, uint32_t &b, uint32_t &h) {
+    const uint32_t lb = g.D == 256 ? 3 : 2;               // (of 128 dims or 256)
+    b = (uint32_t)i & ((1u << lb) - 1);
+    const uint64_t r = i >> lb;
+    const uint32_t t = r >> 32 ? (uint32_t)(r / g.H) : (uint32_t)r / g.H;
+    h = (uint32_t)(r - (uint64_t)t * g.H);
+    return t;
 }
 
-// the q8_0-format tile of a q4_0 K window back to q4_0 rows (quant + 8)
-__global__ void k_export_k_q4(win_geo g, uint32_t cell0, uint32_t n, uint8_t *rows) {
+// K rows and V rows of a quantised window in one launch.  Several threads a 32-value block, each 4
+// bytes of a row: they store side by side.  A V word holds a dim of 8 cells, so a thread takes 4
+// bytes of all 8.  (2,047 rows of 4 x 256 in q8_0 / q4_0: 8.6 us; in two launches, a block a
+// thread, byte by byte, 10.3 + 6.6.)
+template <bool Q8>
+__global__ void k_export_quant(win_geo g, uint32_t cell0, uint32_t n, uint64_t n_k, uint64_t n_v, uint8_t *k_rows, uint8_t *v_rows) {
     const uint32_t NB = g.D / 32;
-    WIN_ITEMS(x, (uint64_t)n * g.H * NB * 4) {
-        const uint64_t i = x / 4;
-        const uint32_t j = x % 4, b = i % NB, h = (i / NB) % g.H, t = (uint32_t)(i / ((uint64_t)NB * g.H));
-        const uint32_t cell = cell0 + t, tile = cell / 64, c = cell % 64;
-        uint8_t *dst = rows + i * 18;
-        const uint8_t *src = g.k + ((uint64_t)h * g.n_tiles + tile) * g.ktile;
-        if (j == 0) __builtin_memcpy(dst, src + kvm_kd_off(g.D, c, b), 2);
-        uint32_t lo, hi;
-        __builtin_memcpy(&lo, src + kvm_kq_off(g.D, c, 32 * b + 8 * (j / 2)) + 4 * (j % 2), 4);
-        __builtin_memcpy(&hi, src + kvm_kq_off(g.D, c, 32 * b + 16 + 8 * (j / 2)) + 4 * (j % 2), 4);
-        // quants of -8 .. 7: adding 8 to the low nibble is flipping its high bit
-        const uint32_t out = ((lo ^ 0x08080808u) & 0x0f0f0f0fu) | ((hi ^ 0x08080808u) & 0x0f0f0f0fu) << 4;
-        __builtin_memcpy(dst + 2 + 4 * j, &out, 4);
-    }
-}
-
-__global__ void k_export_v_q4(win_geo g, uint32_t cell0, uint32_t n, uint8_t *rows) {
-    const uint32_t NB = g.D / 32;
-    const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= (uint64_t)n * g.H * NB) return;
-    const uint32_t b = i % NB, h = (i / NB) % g.H, t = (uint32_t)(i / ((uint64_t)NB * g.H));
-    const uint32_t cell = cell0 + t, tile = cell / 64, c = cell % 64;
-    uint8_t *dst = rows + ((uint64_t)t * g.H + h) * NB * 18 + (uint64_t)b * 18;
-    const uint8_t *src = g.v + ((uint64_t)h * g.n_tiles + tile) * g.vtile;
-    const uint8_t *sd = src + kvm_vd_off(g.D, c, b);
-    dst[0] = sd[0];
-    dst[1] = sd[1];
-    const uint32_t sh = kvm_vq_shift(c);
-    for (uint32_t e = 0; e < 16; ++e) {
-        const uint8_t n0 = (src[kvm_vq_byte(c, 32 * b + e)] >> sh) & 15;
-        const uint8_t n1 = (src[kvm_vq_byte(c, 32 * b + e + 16)] >> sh) & 15;
-        dst[2 + e] = (uint8_t)(n0 | (n1 << 4));
+    constexpr uint32_t KT = Q8 ? 8 : 4, KR = Q8 ? 34 : 18;         // threads, bytes of a K block
+    WIN_ITEMS(x, n_k + n_v) {
+        if (x < n_k) {
+            const uint64_t i = x / KT;
+            uint32_t b, h;
+            const uint32_t j = x % KT, cell = cell0 + win_block(g, i, b, h), c = cell % 64;
+            uint8_t *dst = k_rows + i * KR;
+            const uint8_t *src = g.k + ((uint64_t)h * g.n_tiles + cell / 64) * g.ktile;
+            if (j == 0) __builtin_memcpy(dst, src + kvm_kd_off(g.D, c, b), 2);
+            uint32_t lo, hi;
+            __builtin_memcpy(&lo, src + kvm_kq_off(g.D, c, 32 * b + 8 * (j / 2)) + 4 * (j % 2), 4);
+            if constexpr (!Q8) {
+                // the q8_0-format tile of a q4_0 K window back to nibbles: quants of -8 .. 7, to which
+                // 8 is added by flipping the high bit
+                __builtin_memcpy(&hi, src + kvm_kq_off(g.D, c, 32 * b + 16 + 8 * (j / 2)) + 4 * (j % 2), 4);
+                lo = ((lo ^ 0x08080808u) & 0x0f0f0f0fu) | ((hi ^ 0x08080808u) & 0x0f0f0f0fu) << 4;
+            }
+            __builtin_memcpy(dst + 2 + 4 * j, &lo, 4);
+            continue;
+        }
+        const uint64_t i = (x - n_k) / 4;
+        uint32_t b, h;
+        const uint32_t j = (x - n_k) % 4, grp = cell0 / 8 + win_block(g, i, b, h), c = 8 * grp % 64;
+        const uint8_t *src = g.v + ((uint64_t)h * g.n_tiles + grp / 8) * g.vtile;
+        uint32_t w[2][4];
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e)
+            __builtin_memcpy(&w[e / 4][e % 4], src + kvm_vq_word(32 * b + 16 * (e / 4) + 4 * j + e % 4, (c & 31u) >> 3, c >> 5), 4);
+        uint16_t d[8];
+        __builtin_memcpy(d, src + kvm_vd_off(g.D, c, b), 16);
+#pragma unroll
+        for (uint32_t q = 0; q < 8; ++q) {
+            const uint32_t t = 8 * grp + q - cell0;                // (wraps below cell0)
+            uint32_t out = 0;
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+                out |= ((w[0][e] >> kvm_vq_nib_shift(q) & 15u) | (w[1][e] >> kvm_vq_nib_shift(q) & 15u) << 4) << (8 * e);
+            if (t >= n) continue;
+            uint8_t *dst = v_rows + (((uint64_t)t * g.H + h) * NB + b) * 18;
+            if (j == 0) __builtin_memcpy(dst, &d[q], 2);
+            __builtin_memcpy(dst + 2 + 4 * j, &out, 4);
+        }
     }
 }
 
@@ -456,16 +465,17 @@ extern "C" int kvm_window_export_rows(kvm_state *st, const kvm_window *w, uint32
     const win_geo g = geo_of(w);
     const uint32_t NB = g.D / 32;
     if (kvm_k_quant(w->k_type)) {
-        const uint64_t nt = (uint64_t)n * g.H * NB;
-        if (k_rows && w->k_type == KVM_TYPE_Q8_0)
-            hipLaunchKernelGGL(k_export_k_q8, win_grid(nt * 8), dim3(256), 0, st->stream, g, cell0, n,
-                               (uint8_t *)k_rows);
-        if (k_rows && w->k_type == KVM_TYPE_Q4_0)
-            hipLaunchKernelGGL(k_export_k_q4, win_grid(nt * 4), dim3(256), 0, st->stream, g, cell0, n,
-                               (uint8_t *)k_rows);
-        if (v_rows)
-            hipLaunchKernelGGL(k_export_v_q4, dim3(kvm_cdiv(nt, 256)), dim3(256), 0, st->stream, g, cell0, n,
-                               (uint8_t *)v_rows);
+        const bool q8 = w->k_type == KVM_TYPE_Q8_0;
+        const uint64_t per = (uint64_t)g.H * NB, n_k = k_rows ? n * per * (q8 ? 8 : 4) : 0;
+        const uint64_t n_v = v_rows ? ((uint64_t)(cell0 + n - 1) / 8 - cell0 / 8 + 1) * per * 4 : 0;
+        auto go = [&](auto kt) {
+            hipLaunchKernelGGL((k_export_quant<decltype(kt)::value>), win_grid(n_k + n_v), dim3(256), 0, st->stream, g, cell0, n, n_k, n_v,
+                               (uint8_t *)k_rows, (uint8_t *)v_rows);
+        };
+        if (n_k + n_v) {
+            if (q8) go(std::true_type{});
+            else go(std::false_type{});
+        }
     } else {
         const uint64_t nt = (uint64_t)n * g.H * g.D;
         hipLaunchKernelGGL(k_export_f16, dim3(kvm_cdiv(nt, 256)), dim3(256), 0, st->stream, g, cell0, n,
@@ -516,7 +526,7 @@ __global__ void k_quant_f16(const float *x, uint16_t *y, uint64_t n) {
 }
 
 // several threads a block, so that they store side by side (65,504 blocks of q8_0 and q4_0:
-// 3.8 and 6.0 us; a block a thread 14.6 and 14.7)
+// 4.0 and 3.7 us; a block a thread 14.6 and 14.7)
 __global__ void k_dequant_q8(const uint8_t *x, float *y, uint64_t nblk) {
     WIN_ITEMS(t, nblk * 8) {
         const uint64_t i = t / 8;
@@ -535,19 +545,20 @@ __global__ void k_dequant_q8(const uint8_t *x, float *y, uint64_t nblk) {
 }
 
 __global__ void k_dequant_q4(const uint8_t *x, float *y, uint64_t nblk) {
-    WIN_ITEMS(t, nblk * 8) {
-        const uint64_t i = t / 8;
-        const uint32_t j = t % 8;                             // values 4 j .. + 3: low nibbles, then high ones
+    WIN_ITEMS(t, nblk * 4) {
+        const uint64_t i = t / 4;
+        const uint32_t j = t % 4;                             // values 4 j .. + 3 (low nibbles) and 16 more on
         const uint8_t *b = x + i * 18;
         uint16_t dbits;
         uint32_t q;
         __builtin_memcpy(&dbits, b, 2);
-        __builtin_memcpy(&q, b + 2 + 4 * (j % 4), 4);
+        __builtin_memcpy(&q, b + 2 + 4 * j, 4);
         const float d = kvm_h2f(dbits);
-        float v[4];
+        float v[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (float)((int)(q >> (8 * e + (j / 4) * 4) & 15u) - 8) * d;
+        for (int e = 0; e < 8; ++e) v[e] = (float)((int)(q >> (8 * (e % 4) + 4 * (e / 4)) & 15u) - 8) * d;
         __builtin_memcpy(y + i * 32 + 4 * j, v, 16);
+        __builtin_memcpy(y + i * 32 + 16 + 4 * j, v + 4, 16);
     }
 }
 
@@ -590,7 +601,7 @@ extern "C" int kvm_dequantize_rows(kvm_state *st, int type, const void *src, flo
         if (type == KVM_TYPE_Q8_0)
             hipLaunchKernelGGL(k_dequant_q8, win_grid(nb * 8), dim3(256), 0, st->stream, (const uint8_t *)src, dst, nb);
         else
-            hipLaunchKernelGGL(k_dequant_q4, win_grid(nb * 8), dim3(256), 0, st->stream, (const uint8_t *)src, dst, nb);
+            hipLaunchKernelGGL(k_dequant_q4, win_grid(nb * 4), dim3(256), 0, st->stream, (const uint8_t *)src, dst, nb);
     } else if (type == KVM_TYPE_F16) {
         hipLaunchKernelGGL(k_dequant_f16, dim3(kvm_cdiv(n, 256)), dim3(256), 0, st->stream, (const uint16_t *)src, dst, n);
     } else {

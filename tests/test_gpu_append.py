@@ -272,6 +272,31 @@ def test_append_writes_the_stage_in_bytes(kvm_state, kt, D, n_rot):
 
 
 @pytest.mark.parametrize("cache", ["q8_0", "q4_0", "f16"])
+@pytest.mark.parametrize("D", [128, 256])
+def test_rows_come_back_from_any_cells(kvm_state, cache, D):
+    """Rows imported into a window come back byte for byte from any run of its cells, K or V
+    alone too, and nothing beside them is written."""
+    st, rng, H, n = kvm_state, np.random.default_rng(D + 1), 3, 192
+    kt, vt = TYPES[cache]
+    rows = [api.quantize_rows(st, t, rand(rng, (n, H * D))).view(n, -1) for t in (kt, vt)]
+    w = api.KVWindow(st, n, H, D, 64, kt, vt)
+    w.import_rows(0, *rows, torch.arange(n, dtype=torch.int32).cuda())
+    for cell0, m in ((0, n), (0, 1), (3, 1), (5, 8), (61, 7), (63, 2), (64, 64), (7, 130), (191, 1)):
+        k, v = w.export_rows(cell0, m)
+        assert torch.equal(k.view(m, -1), rows[0][cell0:cell0 + m]) and torch.equal(v.view(m, -1), rows[1][cell0:cell0 + m])
+        one = [torch.full((m + 2, r.shape[1]), 0x5a, dtype=torch.uint8, device="cuda") if r.dtype == torch.uint8 else
+               torch.full((m + 2, r.shape[1]), 7, dtype=r.dtype, device="cuda") for r in rows]
+        for which in (0, 1):
+            pair = [None, None]
+            pair[which] = one[which][1:].data_ptr()
+            assert st.lib.kvm_window_export_rows(st.h, C.byref(w.c), cell0, m, *pair) == L.KVM_OK
+        torch.cuda.synchronize()
+        for r, got in zip(rows, one):
+            assert torch.equal(got[1:-1], r[cell0:cell0 + m])
+            assert torch.equal(got[0], got[-1]) and bool((got[0] == got[0, 0]).all()) and got[0, 0].item() in (0x5a, 7)
+
+
+@pytest.mark.parametrize("cache", ["q8_0", "q4_0", "f16"])
 def test_append_runs(kvm_state, cache):
     """Runs of many windows and of one: empty ones, neighbours in one 8-cell group or one
     slot, the same cells twice (the later run's rows stay), more runs than a launch has."""
