@@ -530,6 +530,7 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
     // ---- the waves' sums: one maximum, then each wave's quarter of the dims from the others,
     // two waves' and the third's
     const float lr = kvm_add_xor32(lp);
+    if (lr != lr) ms = 0.0f;                              // (scores that are no numbers have no maximum; the sums are not empty)
     if (g2 == 0) {
         sm.ml[w][0][m2] = ms;
         sm.ml[w][1][m2] = lr;
@@ -765,6 +766,7 @@ __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg
         if (active) {
             // quad i of O: dims 8 i + 4 g2 .. + 3 of the lane's row
             const float lr = kvm_add_xor32(lp);
+            if (lr != lr) ms = 0.0f;                      // (scores that are no numbers have no maximum; the sums are not empty)
             const uint32_t le = fs_opaque(l);
             float *o = a.ws_o + (uint64_t)(slot + rg) * 32 * D + 4 * le;
             if (__builtin_amdgcn_ballot_w64(ms != -INFINITY) != 0) {

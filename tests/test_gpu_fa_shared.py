@@ -390,6 +390,34 @@ def test_infinite_values_that_are_seen(kvm_state):
     assert bool(got.isfinite().all())
 
 
+@pytest.mark.parametrize("cache", ["q8_0", "f16"])
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_what_is_no_number_is_not_hidden(kvm_state, cache, tokens):
+    """A query that holds a NaN gives NaN, in its own head and token alone; a key that does gives
+    NaN to every row that sees it, also where it is all that the row sees."""
+    st, rng, H, G, D = kvm_state, np.random.default_rng(22), 2, 3, 128
+    pre, own = window(st, rng, 256, H, D, cache, cells(256, 256, 10)), window(st, rng, 64, H, D, cache, cells(64, 50, 266))
+    q = torch.from_numpy(rng.standard_normal((tokens + 2, H * G, D)).astype(np.float32)).cuda()
+    qp = torch.full((tokens + 2,), 315, dtype=torch.int32, device="cuda")
+    qp[-1] = 10                                         # one cell of the prefix
+    args = (st, pre[0], [own[0], None], [tokens, 2], q, qp, H * G, D ** -0.5)
+    clean = api.fa_decode_shared(*args)
+    assert bool(clean.isfinite().all())
+    q[0, 4, 77] = float("nan")
+    got = api.fa_decode_shared(*args)
+    assert bool(got[0, 4].isnan().all())
+    got[0, 4] = clean[0, 4]
+    assert torch.equal(got, clean)
+    q[0, 4, 77] = 0.0
+    k = pre[0].k.view(torch.float16).view(H, -1, 64 * D if cache == "f16" else (64 * D + 128 * (D // 32)) // 2)
+    if cache == "f16":
+        k[0, 0].view(4, D // 32, 4, 16, 8)[0, 1, 2, 0, 3] = float("nan")       # cell 0, kv head 0
+    else:
+        k[0, 0][32 * D:].view(4, D // 32, 16)[0, 1, 0] = float("nan")
+    got = api.fa_decode_shared(*args).view(tokens + 2, H, G, D)
+    assert bool(got[:, 0].isnan().all()) and bool(got[:, 1].isfinite().all())
+
+
 def test_same_as_one_window(kvm_state):
     """A prefix and an own window give what one window with all the cells gives (kvm_fa_prefill),
     to the roundings of both."""
