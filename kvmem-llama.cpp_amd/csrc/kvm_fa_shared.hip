@@ -100,7 +100,7 @@ struct fs_geo {
 template <int D, int NW>
 struct fs_list {
     alignas(16) float odd_v[4][D];
-    uint32_t odd;                // the batch has values that are no finite numbers where not all rows see them
+    uint32_t odd;                // the batch has values that fs_clear took out where some rows see them
     uint32_t list[FS_BATCH];
     uint8_t flag[FS_BATCH];
 };
@@ -258,29 +258,56 @@ __device__ __forceinline__ void fs_mask(kvm_f32x16 &S, const int32_t *cp, uint32
     }
 }
 
+// Values that an f16 operand cannot hold as finite numbers, by these bits of the f16 that is stored:
+// infinities and NaN, and of scales also those from 8,192 on, which times -8 are infinite.
+template <bool QUANT>
+__device__ constexpr uint32_t fs_odd_bits = QUANT ? 0x7000u : 0x7c00u;
+
 // Halves of v (values, or scales of values) whose keys, base .. base + 7, no row sees become
-// 0, and so do those that are no finite numbers where not all rows see the key (0 times them
-// would not be 0): whether there are such.
+// 0, and so do odd ones where not all rows see the key (0 times them would not be 0): whether there
+// are such.
+template <bool QUANT>
 __device__ __forceinline__ bool fs_clear(kvm_u32x4 &v, uint32_t base, uint64_t seen, uint64_t part) {
     const uint32_t on = (uint32_t)(seen >> base) & 0xffu, pt = (uint32_t)(part >> base) & 0xffu;
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const uint32_t sh = 16 * (i & 1), x = v[i >> 1] >> sh & 0xffffu;
-        const bool no = (pt >> i & 1u) && (x & 0x7c00u) == 0x7c00u;
+        const bool no = (pt >> i & 1u) && (x & fs_odd_bits<QUANT>) == fs_odd_bits<QUANT>;
         odd |= no;
         if (!(on >> i & 1u) || no) v[i >> 1] &= ~(0xffffu << sh);
     }
     return odd;
 }
 
-// What fs_clear took out of keys k0 .. k0 + n_k - 1 of the list's tiles j0, j0 + step, ..: values that are no finite
-// numbers are added to the rows that see them (a positive p times one is itself).  sx: the
-// wave's own.
+// p of a row's score with key k of a quantised tile, by the row's two lanes (half a 16-dim step
+// each; one dim after the other, so that the rare path asks for few registers).
+template <int D>
+__device__ __forceinline__ float fs_p_again(const fs_args &a, const uint8_t *k_tile, uint32_t k, uint32_t h, uint32_t row, uint32_t g2, float ms) {
+    uint32_t g;
+    const uint32_t t = fs_token(a, row, g);
+    const uint64_t q0 = ((uint64_t)t * a.n_head + h * a.G + g) * D;
+    float s = 0.0f;
+#pragma unroll 1
+    for (uint32_t i = 0; i < D / 2; ++i) {
+        const uint32_t d = 16 * (i >> 3) + 8 * g2 + (i & 7u);
+        const float q = a.q_type == KVM_TYPE_F32 ? ((const float *)a.q)[q0 + d] : kvm_bf2f(((const uint16_t *)a.q)[q0 + d]);
+        const float x = (float)(int8_t)k_tile[kvm_kq_off(D, k, d)] * kvm_h2f(*(const uint16_t *)(k_tile + kvm_kd_off(D, k, d / 32)));
+        s = fmaf((float)(_Float16)x, (float)(_Float16)(q * a.q_sign), s);
+    }
+    return __builtin_amdgcn_exp2f(fmaf(kvm_add_xor32(s), a.c, ms == -INFINITY ? 0.0f : -ms));
+}
+
+// What fs_clear took out of keys k0 .. k0 + n_k - 1 of the list's tiles j0, j0 + step, .. is added to the rows
+// that see them, in fp32: times the p of the row's score, formed again from the same operands where
+// a value is finite (of a large scale).  The wave has `rows` (or 32) rows from row_g on; ms: what O is
+// relative to; sx: the wave's own.
 template <int D, bool QUANT>
-__device__ __forceinline__ void fs_add_odd(kvm_f32x16 (&O)[D / 32], const fs_seg &sg, const uint8_t *v_head, const uint32_t *list, uint32_t j0,
-                                           uint32_t step, uint32_t n_t, uint32_t k0, uint32_t n_k, uint32_t some_lim, uint32_t all_lim, uint32_t qlim, float *sx) {
-    const uint32_t l = threadIdx.x & 63u;
+__device__ __forceinline__ void fs_add_odd(kvm_f32x16 (&O)[D / 32], const fs_args &a, const fs_seg &sg, const uint8_t *k_head,
+                                           const uint8_t *v_head, const uint32_t *list, uint32_t j0, uint32_t step, uint32_t n_t, uint32_t k0,
+                                           uint32_t n_k, uint32_t some_lim, uint32_t all_lim, uint32_t qlim, uint32_t h, uint32_t row_g,
+                                           uint32_t rows, float ms, float *sx) {
+    const uint32_t l = fs_opaque(threadIdx.x & 63u);
     for (uint32_t j = j0; j < n_t; j += step) {
         const uint32_t e = list[j], t = e & 0x7fffffffu;
         if (e >> 31) continue;
@@ -288,31 +315,36 @@ __device__ __forceinline__ void fs_add_odd(kvm_f32x16 (&O)[D / 32], const fs_seg
         for (uint32_t k = k0; k < k0 + n_k; ++k) {
             const uint32_t cp = (uint32_t)sg.cell_pos[(uint64_t)t * 64 + k];
             if (!(cp < some_lim) || cp < all_lim) continue;
-            bool any = false;
+            bool any = false, finite = false;
             for (uint32_t d = l; d < D; d += 64) {
-                bool bad;
-                float v;
-                if constexpr (QUANT) {
-                    const float sc = kvm_h2f(*(const uint16_t *)(v_tile + kvm_vd_off(D, k, d / 32)));
-                    bad = !(sc - sc == 0.0f);
-                    v = (float)((int)(v_tile[kvm_vq_byte(k, d)] >> kvm_vq_shift(k) & 15u) - 8) * sc;
-                } else {
-                    v = kvm_h2f(((const uint16_t *)v_tile)[kvm_vh_idx(k, d)]);
-                    bad = !(v - v == 0.0f);
-                }
-                sx[d] = bad ? v : 0.0f;
-                any |= bad;
+                const uint32_t x = *(const uint16_t *)(QUANT ? v_tile + kvm_vd_off(D, k, d / 32) : v_tile + 2 * kvm_vh_idx(k, d));
+                const bool odd = (x & fs_odd_bits<QUANT>) == fs_odd_bits<QUANT>;
+                float v = kvm_h2f((uint16_t)x);
+                if constexpr (QUANT) v *= (float)((int)(v_tile[kvm_vq_byte(k, d)] >> kvm_vq_shift(k) & 15u) - 8);
+                sx[d] = odd ? v : 0.0f;
+                any |= odd;
+                finite |= odd && v - v == 0.0f;
             }
             if (__builtin_amdgcn_ballot_w64(any) == 0) continue;
+            // (at least the smallest number: infinite values under a p that underflows stay infinite;
+            // rows past the last: some row's)
+            float p = 1.0f;
+            if (QUANT && __builtin_amdgcn_ballot_w64(finite) != 0)
+                p = fmaxf(fs_p_again<D>(a, k_head + (uint64_t)t * fs_geo<D, true>::KB, k, h, row_g + ((l & 31u) < rows ? l & 31u : 0u), l >> 5, ms),
+                          0x1p-126f);
             __builtin_amdgcn_wave_barrier();
+            if (cp < qlim) {
 #pragma unroll
-            for (int dt = 0; dt < D / 32; ++dt)
+                for (int dt = 0; dt < D / 32; ++dt) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const kvm_f32x4 v = *(const kvm_f32x4 *)(sx + 32 * dt + 8 * x + 4 * (l >> 5));
+                    for (int x = 0; x < 4; ++x) {
+                        const kvm_f32x4 v = *(const kvm_f32x4 *)(sx + 32 * dt + 8 * x + 4 * (l >> 5));
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) O[dt][4 * x + r] += cp < qlim ? v[r] : 0.0f;
+                        for (int r = 0; r < 4; ++r) O[dt][4 * x + r] = fmaf(v[r], p, O[dt][4 * x + r]);
+                    }
+                    FS_FENCE();
                 }
+            }
             __builtin_amdgcn_wave_barrier();
         }
     }
@@ -434,7 +466,7 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
                 if (lo < 4u * NB) {
                     kvm_u32x4 *const at = (kvm_u32x4 *)(sm.sc[w][buf] + 512 + 16 * lo);
                     kvm_u32x4 scv = *at;
-                    if (fs_clear(scv, 32 * half + 8 * (lo & 3u), seen, part)) sm.odd = 1;
+                    if (fs_clear<true>(scv, 32 * half + 8 * (lo & 3u), seen, part)) sm.odd = 1;
                     *at = scv;
                 }
             }
@@ -524,7 +556,9 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
             }
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the last items' copies, which nobody reads)
-        if (__builtin_amdgcn_readfirstlane(sm.odd)) fs_add_odd<D, true>(O, sg, v_head, sm.list, j0, 2, n_t, 32 * half, 32, some_lim, all_lim, qlim, sm.odd_v[w]);
+        if (__builtin_amdgcn_readfirstlane(sm.odd))
+            fs_add_odd<D, true>(O, a, sg, k_head, v_head, sm.list, j0, 2, n_t, 32 * half, 32, some_lim, all_lim, qlim, h, row_g, rows, ms,
+                                sm.odd_v[w]);
     }
 
     // ---- the waves' sums: one maximum, then each wave's quarter of the dims from the others,
@@ -756,7 +790,9 @@ __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg
                 accumulate(R0, sv + TB / 2, pb1, nothing);
                 KVM_LDS_BARRIER();
             }
-            if (__builtin_amdgcn_readfirstlane(sm.odd)) fs_add_odd<D, QUANT>(O, sg, v_head, sm.list, 0, 1, n_t, 0, 64, some_lim, all_lim, qlim, sm.odd_v[w]);
+            if (active && __builtin_amdgcn_readfirstlane(sm.odd))
+                fs_add_odd<D, QUANT>(O, a, sg, k_head, v_head, sm.list, 0, 1, n_t, 0, 64, some_lim, all_lim, qlim, h, row_g + 32 * rg,
+                                     rows - 32 * rg, ms, sm.odd_v[w]);
             b0 += FS_BATCH;
             if (b0 >= i_hi) break;
             fs_cells<8> next;
@@ -834,7 +870,7 @@ __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg
 #pragma unroll
                         for (int b = 0; b < VB2; ++b)
 #pragma unroll
-                            for (int ks = 0; ks < 2; ++ks) odd |= fs_clear(r.vs[b][ks], 32 * ks + 8 * (fs_opaque(l) >> 4), seen, part);
+                            for (int ks = 0; ks < 2; ++ks) odd |= fs_clear<true>(r.vs[b][ks], 32 * ks + 8 * (fs_opaque(l) >> 4), seen, part);
                         if (odd) sm.odd = 1;
                     }
                     uint8_t *dk = sm.ring[buf] + 16 * fs_opaque(l), *dv = dk + TB;
@@ -896,7 +932,7 @@ __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg
                             const uint32_t x = pw * NC + i;
                             kvm_u32x4 *const u = (kvm_u32x4 *)(dst + TB + x * 1024u + 16 * ln);
                             kvm_u32x4 v = *u;
-                            odd |= fs_clear(v, 32 * (x / (D / 16)) + 8 * (ln >> 4), seen, part);
+                            odd |= fs_clear<false>(v, 32 * (x / (D / 16)) + 8 * (ln >> 4), seen, part);
                             *u = v;
                         }
                         if (odd) sm.odd = 1;

@@ -418,6 +418,40 @@ def test_what_is_no_number_is_not_hidden(kvm_state, cache, tokens):
     assert bool(got[:, 0].isnan().all()) and bool(got[:, 1].isfinite().all())
 
 
+def _held(st, w, pos):
+    """(window, K, V, positions) in 64 bits from what the window's cells hold now."""
+    rows = w.export_rows(0, w.n_cells)
+    k, v = (api.dequantize_rows(st, t, r, w.n_head_kv * w.head_dim).double().view(w.n_cells, w.n_head_kv, w.head_dim)
+            for t, r in zip((w.k_type, w.v_type), rows))
+    return w, k, v, pos
+
+
+@pytest.mark.parametrize("cache", ["q8_0", "q4_0"])
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("counts", [[4, 3], [30, 21]])
+@pytest.mark.parametrize("what", [8192.0, 20000.0, -65504.0])
+def test_large_values_that_are_not_seen_are_not_used(kvm_state, cache, D, counts, what):
+    """Scales that are finite but whose values are beyond f16, in empty cells and in cells that
+    some rows of a unit see: the others' outputs are as if they were small, bit for bit, and
+    those that see them have the finite result."""
+    st, H, G = kvm_state, 2, 7
+    fills, n = [100, 64], sum(counts)
+    qp = np.concatenate([256 + f - c + np.arange(c) for f, c in zip(fills, counts)])
+    clean, prefix, owns, q, qpos = run(st, np.random.default_rng(23), H, G, D, cache, 320, cells(320, 256, 0),
+                                       [(128, cells(128, f, 256)) for f in fills], counts, torch.float32, torch.float32, q_pos=qp)
+    _poison(prefix[0], cache, 300, 0, what)             # empty
+    _poison(owns[0][0], cache, 120, 1, what)
+    _poison(owns[0][0], cache, 99, 1, what)             # lane 0's last token
+    for c in (62, 63):
+        _poison(owns[1][0], cache, c, 0, what)          # lane 1's last two tokens see the first, its last both
+    got = api.fa_decode_shared(st, prefix[0], [x[0] for x in owns], counts, q, qpos, H * G, D ** -0.5)
+    same = torch.ones((n, H), dtype=torch.bool)
+    same[counts[0] - 1, 1] = same[n - 2:, 0] = False
+    assert torch.equal(got.view(n, H, G, D)[same], clean.view(n, H, G, D)[same])
+    assert not bool((got == clean).view(n, H, G, D)[~same].flatten(1).all(1).any())
+    check(got, *expected(q, qpos, counts, prefix, [_held(st, x[0], x[3]) for x in owns], H, D ** -0.5))
+
+
 def test_same_as_one_window(kvm_state):
     """A prefix and an own window give what one window with all the cells gives (kvm_fa_prefill),
     to the roundings of both."""
