@@ -613,9 +613,10 @@ int kvm_fa_decode_lanes(kvm_state *st, const kvm_lane *lanes, uint32_t n_lanes, 
  * prefix NULL: none.  At most 64 lanes; any number of tokens a lane; all
  * windows have the same kv heads and head_dim and are all quantised or all f16.
  * Arithmetic as kvm_fa_prefill's: f16 operands (q, the cells' values, the
- * probabilities), fp32 sums, one rounding to out_type.  A token that sees no
- * cell outputs zeros; what cells hold that a token does not see does not reach
- * its output, be it infinite or no number.  Windows' k, v and cell_pos: 16-byte
+ * probabilities), fp32 sums, one rounding to out_type.  Queries and keys beyond
+ * 65,504 count as infinite there; q4_0 values may be as large as the cells hold
+ * (524,032).  A token that sees no cell outputs zeros; what cells hold that a
+ * token does not see does not reach its output, be it infinite or no number.  Windows' k, v and cell_pos: 16-byte
  * aligned.  Partial sums go through the state's workspace: calls of one state, and
  * replays of graphs captured from it, follow one another.  A capture cannot grow
  * it (KVM_ENOMEM): call once before with as many tokens and cells. */

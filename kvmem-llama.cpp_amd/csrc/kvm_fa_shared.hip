@@ -23,6 +23,11 @@
 //   wide units: workgroups of 8 waves, one a CU.  Waves 0 - 3 have 32 rows each and take every
 //     key; waves 4 - 7 bring the next tile into one of two LDS buffers, converted, while the
 //     other is worked on.
+// A value that f16 does not hold as a finite number is taken out of tiles that some row does not see
+// (fs_clear) and added in fp32 to the rows that do (fs_add_odd).  In other tiles nothing looks for one:
+// where a piece's sums come out as no finite numbers, it is formed again with every tile treated so
+// (CAREFUL), which finite values, and infinite ones under a p that f16 rounds to 0, then come out of right.
+// (Looking costs 0.2 us of 8.3 and 0.4 of 24.5 over f16 windows, nothing measurable over others.)
 // A workgroup has one piece: the units of a window are cut into equal numbers of pieces, and
 // longer ones into more.  The tiles are taken in an order that steps through a window in
 // strides: a part-filled window's live tiles are spread evenly over its pieces.
@@ -101,6 +106,7 @@ template <int D, int NW>
 struct fs_list {
     alignas(16) float odd_v[4][D];
     uint32_t odd;                // the batch has values that fs_clear took out where some rows see them
+    uint32_t wild;               // an output of the piece is no finite number
     uint32_t list[FS_BATCH];
     uint8_t flag[FS_BATCH];
 };
@@ -151,6 +157,12 @@ __device__ __forceinline__ uint32_t fs_token(const fs_args &a, uint32_t row, uin
 // Nothing moves over it.
 #define FS_FENCE() __builtin_amdgcn_sched_barrier(0)
 
+// Value j of the 8 queries of y, as operands have it.
+__device__ __forceinline__ _Float16 fs_q(const fs_args &a, const kvm_u32x4 (&y)[2], int j) {
+    const uint32_t v = a.q_type == KVM_TYPE_F32 ? y[j >> 2][j & 3] : j & 1 ? y[0][j >> 1] & 0xffff0000u : y[0][j >> 1] << 16;
+    return (_Float16)(__uint_as_float(v) * a.q_sign);
+}
+
 // Q rows [row_g, row_g + rows) of head h, RG groups of 32: loaded, then as f16 operands into
 // LDS (rows past the last: zeros).  8 rows x 8 units of 8 dims an instruction.
 template <int D, int RG, int NW>
@@ -158,10 +170,12 @@ struct fs_rows {
     static constexpr uint32_t KS = D / 16, QU = 528;
     static constexpr int N = 32 * RG * 2 * KS / (64 * NW);
     kvm_u32x4 y[N][2];
+    uint32_t x0;
     __device__ __forceinline__ void load(const fs_args &a, uint32_t h, uint32_t row_g, uint32_t rows) {
+        x0 = fs_opaque(threadIdx.x);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const uint32_t x = threadIdx.x + 64 * NW * i, b = x >> 6, r = b % (4 * RG) * 8 + (x & 63u) / 8, u = b / (4 * RG) * 8 + (x & 7u);
+            const uint32_t x = x0 + 64 * NW * i, b = x >> 6, r = b % (4 * RG) * 8 + (x & 63u) / 8, u = b / (4 * RG) * 8 + (x & 7u);
             uint32_t g;
             const uint32_t t = fs_token(a, row_g + (r < rows ? r : 0u), g);
             const uint64_t e = ((uint64_t)t * a.n_head + h * a.G + g) * D + 8 * u;
@@ -172,13 +186,10 @@ struct fs_rows {
     __device__ __forceinline__ void store(const fs_args &a, uint32_t rows, uint8_t *dst) const {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const uint32_t x = threadIdx.x + 64 * NW * i, b = x >> 6, r = b % (4 * RG) * 8 + (x & 63u) / 8, u = b / (4 * RG) * 8 + (x & 7u);
+            const uint32_t x = x0 + 64 * NW * i, b = x >> 6, r = b % (4 * RG) * 8 + (x & 63u) / 8, u = b / (4 * RG) * 8 + (x & 7u);
             kvm_f16x8 o;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t v = a.q_type == KVM_TYPE_F32 ? y[i][j >> 2][j & 3] : j & 1 ? y[i][0][j >> 1] & 0xffff0000u : y[i][0][j >> 1] << 16;
-                o[j] = r < rows ? (_Float16)(__uint_as_float(v) * a.q_sign) : (_Float16)0.0f;
-            }
+            for (int j = 0; j < 8; ++j) o[j] = r < rows ? fs_q(a, y[i], j) : (_Float16)0.0f;
             *(kvm_f16x8 *)(dst + (r >> 5) * (2 * KS * QU) + u * QU + (r & 31u) * 16) = o;
         }
     }
@@ -198,12 +209,14 @@ __device__ __forceinline__ uint32_t fs_tile(const fs_seg &sg, uint32_t i) { retu
 template <int NW>
 struct fs_cells {
     kvm_u32x4 c[4];
-    __device__ __forceinline__ static uint32_t at(uint32_t r0, int r) { return r0 + 4 * NW * r + 4 * (threadIdx.x >> 6) + ((threadIdx.x & 63u) >> 4); }
+    uint32_t x0;
+    __device__ __forceinline__ uint32_t at(uint32_t r0, int r) const { return r0 + 4 * NW * r + (x0 >> 4); }
     __device__ __forceinline__ void load(const fs_seg &sg, uint32_t b0, uint32_t r0) {
+        x0 = fs_opaque(threadIdx.x);
         uint32_t t = fs_tile(sg, b0 + at(r0, 0));
 #pragma unroll
         for (int r = 0; r < 4; ++r) {                     // (past the last: another of the window's)
-            c[r] = *(const kvm_u32x4 *)(sg.cell_pos + (uint64_t)t * 64 + 4 * (threadIdx.x & 15u));
+            c[r] = *(const kvm_u32x4 *)(sg.cell_pos + (uint64_t)t * 64 + 4 * (x0 & 15u));
             t += sg.step;
             t -= t < sg.n_tiles ? 0u : sg.n_tiles;
         }
@@ -281,19 +294,26 @@ __device__ __forceinline__ bool fs_clear(kvm_u32x4 &v, uint32_t base, uint64_t s
 }
 
 // p of a row's score with key k of a quantised tile, by the row's two lanes (half a 16-dim step
-// each; one dim after the other, so that the rare path asks for few registers).
+// each; one step after the other, so that the rare path asks for few registers).
 template <int D>
 __device__ __forceinline__ float fs_p_again(const fs_args &a, const uint8_t *k_tile, uint32_t k, uint32_t h, uint32_t row, uint32_t g2, float ms) {
     uint32_t g;
     const uint32_t t = fs_token(a, row, g);
-    const uint64_t q0 = ((uint64_t)t * a.n_head + h * a.G + g) * D;
+    const uint64_t q0 = ((uint64_t)t * a.n_head + h * a.G + g) * D + 8 * g2;
     float s = 0.0f;
 #pragma unroll 1
-    for (uint32_t i = 0; i < D / 2; ++i) {
-        const uint32_t d = 16 * (i >> 3) + 8 * g2 + (i & 7u);
-        const float q = a.q_type == KVM_TYPE_F32 ? ((const float *)a.q)[q0 + d] : kvm_bf2f(((const uint16_t *)a.q)[q0 + d]);
-        const float x = (float)(int8_t)k_tile[kvm_kq_off(D, k, d)] * kvm_h2f(*(const uint16_t *)(k_tile + kvm_kd_off(D, k, d / 32)));
-        s = fmaf((float)(_Float16)x, (float)(_Float16)(q * a.q_sign), s);
+    for (uint32_t d = 0; d < D; d += 16) {
+        kvm_u32x4 y[2];
+        uint32_t kq[2];
+        if (a.q_type == KVM_TYPE_F32) __builtin_memcpy(y, (const float *)a.q + q0 + d, 32);
+        else __builtin_memcpy(y, (const uint16_t *)a.q + q0 + d, 16);
+        __builtin_memcpy(kq, k_tile + kvm_kq_off(D, k, d + 8 * g2), 8);
+        const float sc = kvm_h2f(*(const uint16_t *)(k_tile + kvm_kd_off(D, k, d / 32)));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float x = (float)(int8_t)(kq[j >> 2] >> 8 * (j & 3)) * sc;
+            s = fmaf((float)(_Float16)x, (float)fs_q(a, y, j), s);
+        }
     }
     return __builtin_amdgcn_exp2f(fmaf(kvm_add_xor32(s), a.c, ms == -INFINITY ? 0.0f : -ms));
 }
@@ -350,6 +370,15 @@ __device__ __forceinline__ void fs_add_odd(kvm_f32x16 (&O)[D / 32], const fs_arg
     }
 }
 
+// Whether a lane of the workgroup has a z that is no number.  (The flag is cleared at the start of the
+// first time through a piece only: whoever is first to begin again writes none that others still read.)
+template <int D, int NW>
+__device__ __forceinline__ bool fs_wild(fs_list<D, NW> &sm, float z) {
+    if (z != z) sm.wild = 1;
+    KVM_LDS_BARRIER();
+    return __builtin_amdgcn_readfirstlane(sm.wild) != 0;
+}
+
 // Direct copies to LDS (lane l writes 16 or 4 bytes at M0 + 16 l or 4 l), issued from asm, so
 // that the compiler adds no wait for them; the asm restores M0, which the compiler reserves.
 // Whoever reads waits by vmcnt first.
@@ -376,8 +405,8 @@ __device__ __forceinline__ void fs_copy4(const int32_t *src, uint32_t off, void 
 // us), and for short pieces the start (5.6 us to the first half tile) and the sums' meeting
 // (2.2).  8 lanes x 6 rows of 4 heads over 32,768 + 2,048 cells of q8_0: 30 us for 74.5 MB, 2.5
 // TB/s; 16 x 18 over 5,003 + 8,192 of q4_0: 64 us, 154 MB.
-template <int D>
-__device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs_lds_narrow<D> &sm, uint32_t rt, uint32_t h, uint32_t slot,
+template <int D, bool CAREFUL>
+__device__ __forceinline__ bool fs_narrow(const fs_args &a, const fs_seg &sg, fs_lds_narrow<D> &sm, uint32_t rt, uint32_t h, uint32_t slot,
                                           uint32_t i_lo, uint32_t i_hi) {
     using G = fs_geo<D, true>;
     constexpr int KS = G::KS, NB = G::NB, DT = G::DT, NQ = G::NQ, SETS = G::SETS;
@@ -386,6 +415,7 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t rows = min(32u, sg.n_rows - 32 * rt), row_g = sg.row0 + 32 * rt;
 
+    if (!CAREFUL && threadIdx.x == 0) sm.wild = 0;
     // the loads of the start, all issued before any is used
     fs_cells<4> cells;
     cells.load(sg, i_lo, 0);
@@ -395,7 +425,7 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
         q.load(a, h, row_g, rows);
         q.store(a, rows, sm.q);
     }
-    const uint32_t all_lim = kvm_wave_min_u32(m2 < rows ? qlim : 0xffffffffu), some_lim = ~kvm_wave_min_u32(~qlim);
+    const uint32_t all_lim = CAREFUL ? 0u : kvm_wave_min_u32(m2 < rows ? qlim : 0xffffffffu), some_lim = ~kvm_wave_min_u32(~qlim);
 
     kvm_f32x16 O[DT];
     float ms = -INFINITY, lp = 0.0f;     // the row's reference maximum (times c), the lane's share of its sum
@@ -606,7 +636,7 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
 #pragma unroll
             for (int x = 0; x < NQ; ++x) acc[x] += *(const kvm_f32x4 *)(sm.x[w][k] + 256 * x + 4 * l);
         }
-        __syncthreads();
+        if (round == 0) __syncthreads();
     }
 #pragma unroll
     for (int x = 0; x < NQ; ++x) *(kvm_f32x4 *)(a.ws_o + ((uint64_t)slot * (D / 8) + w * NQ + x) * 256 + 4 * l) = acc[x];
@@ -615,6 +645,11 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
         ml[0] = M;
         ml[1] = L;
     }
+    if (CAREFUL) return false;
+    float z = 0.0f;
+#pragma unroll
+    for (int x = 0; x < 4 * NQ; ++x) z = fmaf(acc[x >> 2][x & 3], 0.0f, z);
+    return fs_wild(sm, z);
 }
 
 // x stays where it is: nothing moves over it, the MFMA that wrote it included.
@@ -629,8 +664,8 @@ __device__ __forceinline__ void fs_narrow(const fs_args &a, const fs_seg &sg, fs
 // the power limit leaves.  768 rows of 4 heads over 32,768 cells of q8_0 (103 GFLOP): 137 us, 750
 // TFLOP/s.  36 tokens x 4 rows of 8 heads of 128 dims over 8,192 + 12 x 1,024 f16 cells: 24 us for
 // 84 MB, the prefix read twice (without the attention waves' work 17, without the copies 25).
-template <int D, bool QUANT>
-__device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg, fs_lds_wide<D, QUANT> &sm, uint32_t rt, uint32_t h,
+template <int D, bool QUANT, bool CAREFUL>
+__device__ __forceinline__ bool fs_wide_piece(const fs_args &a, const fs_seg &sg, fs_lds_wide<D, QUANT> &sm, uint32_t rt, uint32_t h,
                                               uint32_t slot, uint32_t i_lo, uint32_t i_hi) {
     using G = fs_geo<D, QUANT>;
     constexpr int KS = G::KS, NB = G::NB, DT = G::DT;     // (2 DT = KS)
@@ -639,6 +674,7 @@ __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = w & 3;
     const uint32_t rows = min(128u, sg.n_rows - 128 * rt), row_g = sg.row0 + 128 * rt;
 
+    if (!CAREFUL && threadIdx.x == 0) sm.wild = 0;
     // the loads of the start, all issued before any is used
     fs_cells<8> cells;
     cells.load(sg, i_lo, 0);
@@ -648,11 +684,12 @@ __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg
         q.load(a, h, row_g, rows);
         q.store(a, rows, sm.q4[0]);
     }
-    const uint32_t all_lim = kvm_wave_min_u32(min(l < rows ? lim0 : 0xffffffffu, l + 64 < rows ? lim1 : 0xffffffffu));
+    const uint32_t all_lim = CAREFUL ? 0u : kvm_wave_min_u32(min(l < rows ? lim0 : 0xffffffffu, l + 64 < rows ? lim1 : 0xffffffffu));
     const uint32_t some_lim = ~kvm_wave_min_u32(~max(lim0, lim1));
     const uint8_t *const k_head = sg.k + (uint64_t)h * sg.n_tiles * KB, *const v_head = sg.v + (uint64_t)h * sg.n_tiles * VB;
     uint32_t n_t = fs_tiles<D, 8>(sg, sm, i_lo, min(FS_BATCH, i_hi - i_lo), some_lim, all_lim, cells);   // (its barriers: Q, too)
 
+    float z = 0.0f;
     // Both roles take the same barriers: one when Q is in registers, and for a batch of tiles
     // one when the first is in LDS, one a tile, and those of the next batch's list.
     if (w < 4) {
@@ -815,6 +852,12 @@ __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg
                 ml[0] = ms;
                 ml[1] = lr;
             }
+            float zs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) zs[r & 3] = fmaf(O[dt][r], 0.0f, zs[r & 3]);
+            z = (zs[0] + zs[1]) + (zs[2] + zs[3]);
         }
     } else {
         // ======== tile k + 1 into one buffer while the others work on tile k
@@ -952,7 +995,12 @@ __device__ __forceinline__ void fs_wide_piece(const fs_args &a, const fs_seg &sg
             n_t = fs_tiles<D, 8>(sg, sm, b0, min(FS_BATCH, i_hi - b0), some_lim, all_lim, next);
         }
     }
+    return !CAREFUL && fs_wild(sm, z);
 }
+
+// The second (rare) time through a piece starts from what the compiler takes for other values: formed
+// from the same ones, what both need is kept from the first and takes its registers.
+#define FS_AGAIN(rt, h, slot, i_lo, i_hi) asm volatile("" : "+s"(rt), "+s"(h), "+s"(slot), "+s"(i_lo), "+s"(i_hi) : : "memory")
 
 // The workgroup's piece.
 template <bool WIDE, class F>
@@ -975,7 +1023,10 @@ template <int D, bool QUANT>
 __global__ void __launch_bounds__(512) k_fs_wide(fs_args a) {
     __shared__ fs_lds_wide<D, QUANT> sm;
     fs_piece<true>(a, [&](const fs_seg &sg, uint32_t rt, uint32_t h, uint32_t slot, uint32_t i_lo, uint32_t i_hi) {
-        fs_wide_piece<D, QUANT>(a, sg, sm, rt, h, slot, i_lo, i_hi);
+        if (fs_wide_piece<D, QUANT, false>(a, sg, sm, rt, h, slot, i_lo, i_hi)) {
+            FS_AGAIN(rt, h, slot, i_lo, i_hi);
+            fs_wide_piece<D, QUANT, true>(a, sg, sm, rt, h, slot, i_lo, i_hi);
+        }
     });
 }
 
@@ -983,7 +1034,10 @@ template <int D>
 __global__ void __launch_bounds__(256, 2) k_fs_narrow(fs_args a) {
     __shared__ fs_lds_narrow<D> sm;
     fs_piece<false>(a, [&](const fs_seg &sg, uint32_t rt, uint32_t h, uint32_t slot, uint32_t i_lo, uint32_t i_hi) {
-        fs_narrow<D>(a, sg, sm, rt, h, slot, i_lo, i_hi);
+        if (fs_narrow<D, false>(a, sg, sm, rt, h, slot, i_lo, i_hi)) {
+            FS_AGAIN(rt, h, slot, i_lo, i_hi);
+            fs_narrow<D, true>(a, sg, sm, rt, h, slot, i_lo, i_hi);
+        }
     });
 }
 

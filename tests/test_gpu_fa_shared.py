@@ -452,6 +452,41 @@ def test_large_values_that_are_not_seen_are_not_used(kvm_state, cache, D, counts
     check(got, *expected(q, qpos, counts, prefix, [_held(st, x[0], x[3]) for x in owns], H, D ** -0.5))
 
 
+@pytest.mark.parametrize("cache", ["q8_0", "q4_0"])
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("tokens,sharp", [(2, 1.0), (2, 5.0), (40, 1.0), (40, 5.0)])
+def test_large_values_that_every_row_sees(kvm_state, cache, D, tokens, sharp):
+    """The same in tiles whose every cell every row sees, also under probabilities too small for
+    f16: finite values give finite outputs."""
+    st, rng, H, G = kvm_state, np.random.default_rng(24), 2, 3
+    w, k, v, pos = window(st, rng, 512, H, D, cache, cells(512, 512, 0))
+    for c, h, what in ((77, 1, 20000.0), (200, 0, -9000.0), (450, 1, 65504.0), (451, 1, 8192.0)):
+        _poison(w, cache, c, h, what)
+    q = torch.from_numpy(rng.standard_normal((tokens, H * G, D)).astype(np.float32) * np.float32(sharp)).cuda()
+    qp = torch.full((tokens,), 600, dtype=torch.int32, device="cuda")
+    got = api.fa_decode_shared(st, w, [None], [tokens], q, qp, H * G, D ** -0.5)
+    check(got, *expected(q, qp, [tokens], _held(st, w, pos), [None], H, D ** -0.5))
+
+
+@pytest.mark.parametrize("cache", ["q8_0", "f16"])
+@pytest.mark.parametrize("tokens", [2, 40])
+def test_infinite_values_under_small_probabilities(kvm_state, cache, tokens):
+    """An infinite value that every row sees is infinite in every row, however small its (positive)
+    probability: some 28 nats below the row's largest here, and f16 ends at 17."""
+    st, rng, H, G, D = kvm_state, np.random.default_rng(25), 2, 3, 128
+    w, k, v, pos = window(st, rng, 256, H, D, cache, cells(256, 256, 0))
+    q = (-2.0 * k[100].float())[None, :, None].expand(tokens, H, G, D).reshape(tokens, H * G, D).contiguous()
+    qp = torch.full((tokens,), 600, dtype=torch.int32, device="cuda")
+    args = (st, w, [None], [tokens], q, qp, H * G, D ** -0.5)
+    clean = api.fa_decode_shared(*args)
+    _poison(w, cache, 100, 1, float("inf"))
+    got = api.fa_decode_shared(*args).view(tokens, H, G, D)
+    want = _held(st, w, pos)[2][100, 1].float()         # +-inf, NaN (0 times inf)
+    assert torch.equal(got[:, 0], clean.view(tokens, H, G, D)[:, 0])
+    assert not bool(want.isfinite().any()) and bool((want == float("inf")).any())
+    assert torch.equal(got[:, 1].nan_to_num(7.0), want.nan_to_num(7.0).expand(tokens, G, D))
+
+
 def test_same_as_one_window(kvm_state):
     """A prefix and an own window give what one window with all the cells gives (kvm_fa_prefill),
     to the roundings of both."""
