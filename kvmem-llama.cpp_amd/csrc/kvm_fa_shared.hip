@@ -1312,6 +1312,20 @@ static int fs_shape(kvm_state *st, const char *what, const kvm_window *prefix, c
     return KVM_OK;
 }
 
+// The most slots of any call of no more tokens and tiles (of all windows), however they are spread
+// over conversations.  The slots of a call go up and down with how its units divide into the
+// workgroups: 96 tokens over 32,768 f16 cells of 8 heads take 960, 64 tokens and 1 take 1,024.  fs_cut
+// makes no more pieces than units, tiles or four rounds of workgroups ask for, in whole rounds.
+static uint64_t fs_most_slots(bool quant, uint32_t n_cu, uint32_t H, uint32_t G, uint64_t tokens, uint64_t tiles) {
+    const uint64_t rows = tokens * G, lanes = std::min<uint64_t>(tokens, FS_LANES);
+    auto pieces = [&](bool wide, uint64_t groups) {
+        const uint64_t rt = (rows + fs_unit_rows(wide) - 1) / fs_unit_rows(wide);
+        const uint64_t units = (rt + rows / fs_unit_rows(wide) + lanes) * H;       // the prefix's, the conversations'
+        return std::min(rt * H * tiles, std::max(4 * groups, (units + groups - 1) / groups * groups));
+    };
+    return (!quant || rows > 64 ? 4 * pieces(true, n_cu) : 0) + (quant ? pieces(false, 2 * n_cu) : 0);
+}
+
 extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, const kvm_window *const *windows,
                                     const uint32_t *n_tokens, uint32_t n_lanes, const void *q, int q_type,
                                     const int32_t *q_pos, uint32_t n_head, float scale, int out_type, void *out) {
@@ -1323,7 +1337,7 @@ extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, con
     if (out_type != KVM_TYPE_F32 && out_type != KVM_TYPE_BF16 && out_type != KVM_TYPE_F16)
         return kvm_fail(st, KVM_EUNSUPPORTED, "%s: output type %d", what, out_type);
     const kvm_window *w0 = prefix;
-    uint64_t total = 0;
+    uint64_t total = 0, tiles = 0;
     for (uint32_t i = 0; i < n_lanes; ++i) {
         total += n_tokens[i];
         if (!w0 && windows) w0 = windows[i];
@@ -1339,6 +1353,7 @@ extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, con
         if (((uintptr_t)w->k | (uintptr_t)w->v | (uintptr_t)w->cell_pos) & 15)
             return kvm_fail(st, KVM_EINVAL, "%s: lane %u: a window that is not aligned to 16 bytes", what, i);
         if (w->n_cells / KVM_TILE_CELLS > 65535) return kvm_fail(st, KVM_ERANGE, "%s: lane %u: %u cells", what, i, w->n_cells);
+        tiles += w->n_cells / KVM_TILE_CELLS;
     }
     const uint32_t H = w0->n_head_kv, D = w0->head_dim;
     if (n_head == 0 || n_head % H) return kvm_fail(st, KVM_EINVAL, "%s: %u heads on %u", what, n_head, H);
@@ -1369,11 +1384,12 @@ extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, con
     const int rc = fs_shape(st, what, prefix, windows, n_tokens, n_lanes, quant, st ? st->n_cu : 256u, &a, &j, &slots);
     if (rc) return rc;
     if (!st) return KVM_EINVAL;
-    const size_t bytes_o = (size_t)slots * 32 * D * 4, bytes = bytes_o + (size_t)slots * 32 * 8;
+    const size_t slot_bytes = 32 * (D * 4 + 8), bytes_o = (size_t)slots * 32 * D * 4;
     KVM_HIP(st, hipSetDevice(st->device));
     if (slots) {
         void *ws = nullptr;
-        if (const int bad = kvm_shared_workspace(st, what, bytes, &ws)) return bad;
+        const uint64_t most = fs_most_slots(quant, st->n_cu, H, a.G, total, tiles);
+        if (const int bad = kvm_shared_workspace(st, what, slots * slot_bytes, most * slot_bytes, &ws)) return bad;
         a.ws_o = (float *)ws;
         a.ws_ml = (float *)((uint8_t *)a.ws_o + bytes_o);
         j.ws_o = a.ws_o;

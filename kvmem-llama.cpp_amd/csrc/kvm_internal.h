@@ -127,9 +127,10 @@ size_t kvm_fa_sync_bytes();
 void *kvm_workspace(kvm_state *st, size_t bytes);
 // The same for the attention workspace (kvm_state::fa_ws).
 void *kvm_fa_workspace(kvm_state *st, size_t bytes);
-// The pieces of the shared-prefix attention (kvm_state::fs_ws): never freed before the
-// state, and not grown while the stream is captured (*buf; KVM_ENOMEM).
-int kvm_shared_workspace(kvm_state *st, const char *what, size_t bytes, void **buf);
+// The pieces of the shared-prefix attention (kvm_state::fs_ws): `bytes` for this call, `most` for
+// any that may follow under a capture; never freed before the state, and not grown while the stream
+// is captured (*buf; KVM_ENOMEM).
+int kvm_shared_workspace(kvm_state *st, const char *what, size_t bytes, size_t most, void **buf);
 // The same for the stage-in move staging (kvm_state::mv_ws).
 void *kvm_move_workspace(kvm_state *st, size_t bytes);
 // Workgroups of `threads` threads and `lds` bytes of dynamic LDS of kernel fn

@@ -157,17 +157,20 @@ void *kvm_fa_workspace(kvm_state *st, size_t bytes) { return grow(st, &st->fa_ws
 
 void *kvm_move_workspace(kvm_state *st, size_t bytes) { return grow(st, &st->mv_ws, &st->mv_ws_bytes, bytes); }
 
-int kvm_shared_workspace(kvm_state *st, const char *what, size_t bytes, void **buf) {
+int kvm_shared_workspace(kvm_state *st, const char *what, size_t bytes, size_t most, void **buf) {
     *buf = st->fs_ws;
-    if (bytes <= st->fs_ws_bytes) return KVM_OK;
+    if (most <= st->fs_ws_bytes) return KVM_OK;
     hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
     KVM_HIP(st, hipStreamIsCapturing(st->stream, &capturing));
-    if (capturing != hipStreamCaptureStatusNone)
+    if (capturing != hipStreamCaptureStatusNone) {
+        if (bytes <= st->fs_ws_bytes) return KVM_OK;
         return kvm_fail(st, KVM_ENOMEM, "%s: the workspace has to grow to %zu bytes: call it once before the capture", what, bytes);
-    const size_t twice = 2 * st->fs_ws_bytes, least = bytes < (4u << 20) ? (4u << 20) : bytes, want = twice > least ? twice : least;
+    }
+    const size_t twice = 2 * st->fs_ws_bytes, least = most < (4u << 20) ? (4u << 20) : most, want = twice > least ? twice : least;
     void *p = nullptr;
     if (st->n_fs_old == sizeof(st->fs_old) / sizeof(st->fs_old[0]) || hipMalloc(&p, want) != hipSuccess) {
         (void)hipGetLastError();
+        if (bytes <= st->fs_ws_bytes) return KVM_OK;
         return kvm_fail(st, KVM_ENOMEM, "%s: workspace of %zu bytes", what, want);
     }
     if (st->fs_ws) st->fs_old[st->n_fs_old++] = st->fs_ws;

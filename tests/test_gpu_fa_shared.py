@@ -251,6 +251,37 @@ def test_workspace_under_capture(kvm_state):
         st.close()
 
 
+@pytest.mark.parametrize("cache,D", [("f16", 256), ("q8_0", 128)])
+def test_captures_of_smaller_calls(kvm_state, cache, D):
+    """After one call on a fresh state, calls of no more tokens and cells can be captured, however
+    many tokens they have (fewer can ask for more pieces) and however these are spread over lanes."""
+    st, H, G, n = api.State(0), 8, 8, 32768
+    try:
+        torch.manual_seed(26)
+        w = api.KVWindow(st, n, H, D, 64, *TYPES[cache])
+        w.import_rows(0, *(api.quantize_rows(st, t, torch.randn(n, H * D, device="cuda")) for t in TYPES[cache]),
+                      torch.arange(n, dtype=torch.int32, device="cuda"))
+        q = torch.randn(96, H * G, D, device="cuda")
+        pos = torch.full((96,), n, dtype=torch.int32, device="cuda")
+        full = api.prepare_fa_decode_shared(st, w, [None], [96], q, pos, H * G, D ** -0.5)
+        full()
+        for counts in ([64], [16], [1], [1] * 64, [40, 56], [5]):
+            m = sum(counts)
+            p = api.prepare_fa_decode_shared(st, w, [None] * len(counts), counts, q[:m], pos[:m], H * G, D ** -0.5)
+            g = st.capture(p)
+            for _ in range(2):
+                p.out.zero_()
+                torch.cuda.synchronize()
+                g.replay()
+                full()
+                torch.cuda.synchronize()
+                rel = float((p.out - full.out[:m]).norm() / full.out[:m].norm())
+                assert rel <= 1e-3, (counts, rel)        # (two forms of 3e-4 each)
+    finally:
+        torch.cuda.synchronize()
+        st.close()
+
+
 def test_rows_that_see_little_or_nothing(kvm_state):
     """Rows whose positions lie before every cell give zeros; others see a single cell, a part
     of the prefix and none of their own, or cells in no order with holes and whole empty tiles."""
