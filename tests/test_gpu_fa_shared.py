@@ -299,6 +299,25 @@ def test_rows_that_see_little_or_nothing(kvm_state):
             assert torch.equal(got[1].view(H, G, D)[:, 0], prefix[2][first].float())
 
 
+@pytest.mark.parametrize("cache", ["q8_0", "q4_0", "f16"])
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_rows_that_see_one_cell(kvm_state, cache, tokens):
+    """A row that sees a single cell, of the prefix or of its own window, gives that cell's values as
+    the f16 operands hold them."""
+    st, rng, H, G, D = kvm_state, np.random.default_rng(27), 2, 3, 128
+    pre, own = rng.permutation(640) + 10, np.full(128, -1)
+    own[[3, 77]] = 500, 5
+    prefix, mine = window(st, rng, 640, H, D, cache, pre), window(st, rng, 128, H, D, cache, own)
+    counts, at = [tokens, tokens], [(prefix, int(np.flatnonzero(pre == 10)[0])), (mine, 77)]
+    q = torch.from_numpy(rng.standard_normal((2 * tokens, H * G, D)).astype(np.float32)).cuda()
+    qp = torch.tensor([10] * tokens + [9] * tokens, dtype=torch.int32, device="cuda")
+    assert int(((pre >= 0) & (pre <= 10)).sum()) == 1 and not ((pre >= 0) & (pre <= 9)).any()
+    assert int(((own >= 0) & (own <= 9)).sum()) == 1
+    got = api.fa_decode_shared(st, prefix[0], [None, mine[0]], counts, q, qp, H * G, D ** -0.5).view(2, tokens, H, G, D)
+    for i, (w, c) in enumerate(at):
+        assert torch.equal(got[i], w[2][c].half().float()[None, :, None].expand(tokens, H, G, D))
+
+
 def test_empty_windows(kvm_state):
     """Nothing anywhere: zeros, whatever was there; no tokens: nothing is written."""
     st, rng = kvm_state, np.random.default_rng(4)
