@@ -792,7 +792,8 @@ def prepare_window_append(st, windows, cell0, n_tokens, k, v, pos, n_rot, freq_b
     if k is None or v is None:
         raise L.KvmError(L.KVM_EINVAL, "window_append: no keys or no values")
     _on_device(st, torch.int32, (k.shape[0],), pos=pos)
-    _on_device(st, torch.float32, (k.shape[2],), k_weight=k_weight, q_weight=q_weight)
+    if windows:                                          # (the views' rows may hold several heads)
+        _on_device(st, torch.float32, (windows[0].head_dim,), k_weight=k_weight, q_weight=q_weight)
     q_out = None if q is None else _out_of(st, q, q_out, q_out_dtype, "q_out")
     n = len(windows)
     arr, c0, nt = _window_ptrs(st, windows), (L._u32 * max(n, 1))(*map(int, cell0)), (L._u32 * max(n, 1))(*map(int, n_tokens))

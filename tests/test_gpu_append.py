@@ -368,6 +368,27 @@ def test_append_long_rows_as_views(kvm_state):
     same(a, b)
 
 
+def test_append_weights_of_long_rows(kvm_state):
+    """Weights have head_dim values whatever the rows of the views hold: the same with several
+    heads in a row, and one value for each of a row's is refused."""
+    st, rng, H, D, n = kvm_state, np.random.default_rng(28), 4, 128, 6
+    k, v, q = rand(rng, (n, H, D)), rand(rng, (n, H, D)), rand(rng, (n, 2 * H, D))
+    kw, qw = rand(rng, (D,)) + 1.0, rand(rng, (D,)) + 1.0
+    pos = torch.arange(n, dtype=torch.int32).cuda()
+    a, b = (api.KVWindow(st, 64, H, D, 64) for _ in range(2))
+    want = api.window_append(st, [a], [1], [n], k, v, pos, 64, BASE, eps=1e-6, k_weight=kw, q=q, q_weight=qw)
+    long = (k.view(n, 1, H * D), v.view(n, 2, H * D // 2))
+    got = api.window_append(st, [b], [1], [n], *long, pos, 64, BASE, eps=1e-6, k_weight=kw, q=q.view(n, 1, 2 * H * D), q_weight=qw)
+    same(a, b)
+    assert torch.equal(got.view(n, 2 * H, D), want)
+    for bad in ({"k_weight": torch.ones(H * D, device="cuda")}, {"q": q, "q_weight": torch.ones(H * D, device="cuda")},
+                {"k_weight": torch.ones(D - 1, device="cuda")}):
+        with pytest.raises(L.KvmError) as e:
+            api.window_append(st, [b], [1], [n], *long, pos, 64, BASE, eps=1e-6, **bad)
+        assert e.value.code == L.KVM_EINVAL
+    same(a, b)
+
+
 def test_append_on_another_stream_and_replayed(kvm_state):
     """On a stream of its own, and captured: every replay appends the rows that its inputs
     then hold, beside eager calls between the replays."""
