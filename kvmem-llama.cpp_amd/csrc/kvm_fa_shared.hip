@@ -1358,7 +1358,7 @@ extern "C" int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, con
     const uint32_t H = w0->n_head_kv, D = w0->head_dim;
     if (n_head == 0 || n_head % H) return kvm_fail(st, KVM_EINVAL, "%s: %u heads on %u", what, n_head, H);
     if (!std::isfinite(scale * 1.4426950408889634f)) return kvm_fail(st, KVM_EINVAL, "%s: scale %g", what, (double)scale);
-    if (total * (n_head / H) > (1u << 24)) return kvm_fail(st, KVM_ERANGE, "%s: %llu tokens", what, (unsigned long long)total);
+    if (total > (1u << 24) / (n_head / H)) return kvm_fail(st, KVM_ERANGE, "%s: %llu tokens", what, (unsigned long long)total);
     if (H > 65535) return kvm_fail(st, KVM_ERANGE, "%s: %u kv heads", what, H);
     if (total == 0) return KVM_OK;
     if (!q || !q_pos || !out) return kvm_fail(st, KVM_EINVAL, "%s: null argument", what);

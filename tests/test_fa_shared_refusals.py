@@ -48,3 +48,9 @@ def _call(prefix, windows, counts, heads=8, q_type=L.T_F32, out_type=L.T_F32, sc
 ])
 def test_refusals(code, call):
     assert call() == code
+
+
+@pytest.mark.parametrize("counts,heads", [([2 ** 31] * 4, 2 ** 31), ([2 ** 30] * 16 + [1], 2 ** 30), ([2 ** 31], 2 ** 31)])
+def test_products_past_64_bits(counts, heads):
+    """Tokens times heads of a group are compared without their product, which wraps to little."""
+    assert _call(_window(H=1), [None] * len(counts), counts, heads=heads) == L.KVM_ERANGE
