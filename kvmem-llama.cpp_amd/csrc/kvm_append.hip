@@ -726,7 +726,11 @@ extern "C" int kvm_window_append(kvm_state *st, const kvm_window *const *windows
                                  const float *k_weight, float eps, const kvm_rope_params *rope, const int32_t *pos,
                                  const kvm_view *q, const float *q_weight, int q_out_type, void *q_out) {
     const char *what = "window_append";
-    if (n_runs == 0) return KVM_OK;
+    if (n_runs == 0) {
+        for (const kvm_view *x : {k, v, q})
+            if (x && x->ne2 != 0) return kvm_fail(st, KVM_EINVAL, "%s: no runs, views of %lld tokens", what, (long long)x->ne2);
+        return KVM_OK;
+    }
     if (!windows || !cell0 || !n_tokens || !k || !v) return kvm_fail(st, KVM_EINVAL, "%s: null argument", what);
     if (q && !float_type(q_out_type)) return kvm_fail(st, KVM_EUNSUPPORTED, "%s: output type %d", what, q_out_type);
     uint64_t total = 0;

@@ -65,3 +65,18 @@ def _append(windows, cell0, counts, k, v, q=None, had=-1, q_type=L.T_F32):
 ])
 def test_append(code, call):
     assert call() == code
+
+
+def test_tokens_without_a_run():
+    """No run holds no tokens: views that have some are refused, as where the runs hold too few."""
+    r = L.RopeParams(64, 1e6, 1.0, -1)
+
+    def call(k, v, q):
+        refs = [None if x is None else C.byref(x) for x in (k, v, q)]
+        return L.load().kvm_window_append(None, None, None, None, 0, refs[0], refs[1], None, 1e-6, C.byref(r), 1 << 23, refs[2], None,
+                                          L.T_F32, 1 << 24)
+
+    none, some = _view(0, 2, 128), _view(4, 2, 128)
+    assert call(none, none, none) == call(None, None, None) == call(none, none, None) == L.KVM_OK
+    for views in ((some, none, None), (none, some, None), (none, none, _view(4, 8, 128)), (some, some, _view(4, 8, 128))):
+        assert call(*views) == L.KVM_EINVAL
