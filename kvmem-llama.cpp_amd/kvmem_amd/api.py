@@ -802,7 +802,7 @@ def prepare_window_append(st, windows, cell0, n_tokens, k, v, pos, n_rot, freq_b
                  (st.h, arr, c0, nt, n, C.byref(kv), C.byref(vv), _ptr(k_weight), -1.0 if eps is None else float(eps),
                   C.byref(r), _ptr(pos), None if q is None else C.byref(qv), _ptr(q_weight),
                   L.T_F32 if q is None else _VIEW_TYPES[q_out.dtype], _ptr(q_out)),
-                 (windows, arr, c0, nt, k, v, kv, vv, k_weight, r, pos, q, qv, q_weight))
+                 (tuple(windows), arr, c0, nt, k, v, kv, vv, k_weight, r, pos, q, qv, q_weight))
     p.q_out = q_out
     return p
 
@@ -838,7 +838,7 @@ def prepare_fa_decode_shared(st, prefix, windows, n_tokens, q, q_pos, n_head, sc
     p = Prepared(st, st.lib.kvm_fa_decode_shared,
                  (st.h, pre[0] if prefix is not None else None, arr, nt, n, _ptr(q), _VIEW_TYPES[q.dtype], _ptr(q_pos), n_head,
                   float(scale), _VIEW_TYPES[out.dtype], _ptr(out)),
-                 (prefix, windows, arr, nt, pre, q, q_pos))
+                 (prefix, tuple(windows), arr, nt, pre, q, q_pos))
     p.out = out
     return p
 

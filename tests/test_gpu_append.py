@@ -3,7 +3,9 @@ window bytes against kvm_quantize_rows + kvm_window_import_rows of the same rows
 against the oracle's stage-in chain, runs that share words or cells, strides, streams,
 graphs and refusals."""
 import ctypes as C
+import gc
 import math
+import weakref
 
 import numpy as np
 import pytest
@@ -387,6 +389,26 @@ def test_append_weights_of_long_rows(kvm_state):
             api.window_append(st, [b], [1], [n], *long, pos, 64, BASE, eps=1e-6, **bad)
         assert e.value.code == L.KVM_EINVAL
     same(a, b)
+
+
+def test_prepared_calls_keep_their_windows(kvm_state):
+    """A prepared append or attention holds its windows, whatever becomes of the caller's list."""
+    st, rng, H, D = kvm_state, np.random.default_rng(29), 2, 128
+    k, v, q = rand(rng, (1, H, D)), rand(rng, (1, H, D)), rand(rng, (1, 4, D))
+    pos = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for prepare in (lambda ws: api.prepare_window_append(st, ws, [0], [1], k, v, pos, 64, BASE),
+                    lambda ws: api.prepare_fa_decode_shared(st, None, ws, [1], q, pos, 4, 0.1)):
+        ws = [api.KVWindow(st, 64, H, D, 64)]
+        held = weakref.ref(ws[0])
+        p = prepare(ws)
+        ws.clear()
+        gc.collect()
+        assert held() is not None
+        p()
+        st.sync()
+        del p
+        gc.collect()
+        assert held() is None
 
 
 def test_append_on_another_stream_and_replayed(kvm_state):
