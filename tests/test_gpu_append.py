@@ -411,6 +411,43 @@ def test_prepared_calls_keep_their_windows(kvm_state):
         assert held() is None
 
 
+@pytest.mark.parametrize("tq,tk", [(torch.bfloat16, torch.float16), (torch.float32, torch.bfloat16), (torch.float16, torch.float32)])
+@pytest.mark.parametrize("how", [("packed", "packed"), ("odd", "heads_first"), ("dims_first", "packed")])
+def test_queries_and_keys_of_different_types(kvm_state, tq, tk, how):
+    """Queries and keys (and values) of unlike types and strides are rows like any others."""
+    st, rng, D, n = kvm_state, np.random.default_rng(30), 128, 300
+    q, k, v = layout(rand(rng, (n, 7, D), tq), how[0]), layout(rand(rng, (n, 2, D), tk), how[1]), layout(rand(rng, (n, 2, D), tq), how[0])
+    pos = torch.arange(n, dtype=torch.int32).cuda()
+    got = api.qk_norm_rope(st, q, k, pos, 64, BASE, eps=1e-6, out_dtype=torch.float32)
+    for x, y in zip((q, k), got):
+        close(y, *formula(x, None, 1e-6, pos, 64, 0))
+    w, o = (api.KVWindow(st, 512, 2, D, 64) for _ in range(2))
+    qo = api.window_append(st, [w], [3], [n], k, v, pos, 64, BASE, eps=1e-6, q=q, q_out_dtype=torch.float32)
+    by_parts(st, o, 3, k, v, pos, 64, -1, 1e-6, None)
+    same(w, o)
+    assert torch.equal(qo, api.qk_norm_rope(st, q, None, pos, 64, BASE, hadamard_nrot=D, eps=1e-6, out_dtype=torch.float32)[0])
+
+
+@pytest.mark.parametrize("cache", ["q8_0", "f16"])
+def test_append_far_cells(kvm_state, cache):
+    """Cells whose offsets pass 32 bits end as an import of the same rows leaves them."""
+    st, rng, H, D, n = kvm_state, np.random.default_rng(31), 8, 256, 37
+    N = 64 * 65535 if cache == "q8_0" else 2 ** 20
+    w = api.KVWindow(st, N, H, D, 64, *TYPES[cache])
+    k, v = rand(rng, (n, H, D)), rand(rng, (n, H, D))
+    pos = torch.arange(n, dtype=torch.int32).cuda()
+    at = (0, N // 2 + 5, N - n)
+    for c in at:
+        by_parts(st, w, c, k, v, pos, 64, -1, 1e-6, None)
+    want = [w.export_rows(c, n) for c in at]
+    for c in at:
+        api.window_append(st, [w], [c], [n], v, k, pos, 64, BASE, eps=1e-6)
+    api.window_append(st, [w] * 3, at, [n] * 3, k.repeat(3, 1, 1), v.repeat(3, 1, 1), pos.repeat(3), 64, BASE, eps=1e-6)
+    for c, rows in zip(at, want):
+        assert all(torch.equal(a, b) for a, b in zip(w.export_rows(c, n), rows))
+        assert torch.equal(w.cell_pos[c:c + n], pos)
+
+
 def test_append_on_another_stream_and_replayed(kvm_state):
     """On a stream of its own, and captured: every replay appends the rows that its inputs
     then hold, beside eager calls between the replays."""

@@ -542,6 +542,95 @@ def test_infinite_values_under_small_probabilities(kvm_state, cache, tokens):
     assert torch.equal(got[:, 1].nan_to_num(7.0), want.nan_to_num(7.0).expand(tokens, G, D))
 
 
+@pytest.mark.parametrize("cache", ["q8_0", "f16"])
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_largest_window(kvm_state, cache, tokens):
+    """Windows whose tiles' offsets pass 32 bits (of the most cells there can be where quantised), almost
+    all of them empty: the few rows that they hold, at both ends and between."""
+    st, rng, H, G, D, n = kvm_state, np.random.default_rng(32), 8, 2, 256, 70
+    N = 64 * 65535 if cache == "q8_0" else 2 ** 20
+    w = api.KVWindow(st, N, H, D, 64, *TYPES[cache])
+    w.cell_pos.fill_(-1)
+    held, at = [], (0, 64 * 12345 + 9, N - n)
+    for i, c in enumerate(at):
+        rows = [api.quantize_rows(st, t, torch.from_numpy(rng.standard_normal((n, H * D)).astype(np.float32)).cuda()) for t in TYPES[cache]]
+        p = torch.arange(1000 * i, 1000 * i + n, dtype=torch.int32).cuda()
+        w.import_rows(c, *rows, p)
+        held.append((*(api.dequantize_rows(st, t, r, H * D).double().view(n, H, D) for t, r in zip(TYPES[cache], rows)), p))
+    part = (w, *(torch.cat([x[i] for x in held]) for i in range(3)))
+    q = torch.from_numpy(rng.standard_normal((tokens, H * G, D)).astype(np.float32)).cuda()
+    qp = torch.from_numpy(rng.integers(0, 3000, tokens).astype(np.int32)).cuda()
+    got = api.fa_decode_shared(st, w, [None], [tokens], q, qp, H * G, D ** -0.5)
+    check(got, *expected(q, qp, [tokens], part, [None], H, D ** -0.5))
+
+
+def test_two_states_at_once():
+    """Calls of two states on streams of their own, over the same prefix, side by side: each has its own
+    pieces, and gives what it gives alone."""
+    rng, H, G, D = np.random.default_rng(33), 4, 4, 128
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    sts = [api.State(0, stream=s.cuda_stream) for s in streams]
+    try:
+        with torch.cuda.stream(streams[0]):
+            pre = window(sts[0], rng, 8192, H, D, "q8_0", cells(8192, 8192, 0))[0]
+            qs = [torch.from_numpy(rng.standard_normal((m, H * G, D)).astype(np.float32)).cuda() for m in (3, 40)]
+            ps = [torch.full((x.shape[0],), 9000, dtype=torch.int32, device="cuda") for x in qs]
+        torch.cuda.synchronize()
+        calls = [api.prepare_fa_decode_shared(st, pre, [None], [q.shape[0]], q, p, H * G, D ** -0.5) for st, q, p in zip(sts, qs, ps)]
+        want = []
+        for c in calls:
+            c()
+            torch.cuda.synchronize()
+            want.append(c.out.clone())
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for c in calls:
+                c()
+        torch.cuda.synchronize()
+        assert all(torch.equal(c.out, x) for c, x in zip(calls, want))
+    finally:
+        torch.cuda.synchronize()
+        for st in sts:
+            st.close()
+
+
+def test_two_graphs_of_one_state(kvm_state):
+    """Graphs captured from one state, of many rows and of few, replayed in turn with eager calls
+    between: they follow one another in its workspace."""
+    rng, H, G, D = np.random.default_rng(34), 4, 6, 256
+    s = torch.cuda.Stream()
+    st = api.State(0, stream=s.cuda_stream)
+    try:
+        with torch.cuda.stream(s):
+            pre, own = (window(st, rng, n, H, D, "q8_0", cells(n, n, p))[0] for n, p in ((2048, 0), (128, 2048)))
+            calls = []
+            for m in (40, 2, 7):
+                q = torch.from_numpy(rng.standard_normal((m, H * G, D)).astype(np.float32)).cuda()
+                qp = torch.full((m,), 2100, dtype=torch.int32, device="cuda")
+                calls.append(api.prepare_fa_decode_shared(st, pre, [own], [m], q, qp, H * G, D ** -0.5))
+            want = []
+            for c in calls:
+                c()
+                torch.cuda.synchronize()
+                want.append(c.out.clone())
+        torch.cuda.synchronize()
+        graphs = [st.capture(c) for c in calls[:2]]
+        for _ in range(3):
+            for c in calls:
+                c.out.fill_(3.0)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(s):
+                graphs[0].replay()
+                calls[2]()
+                graphs[1].replay()
+                graphs[0].replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(c.out, x) for c, x in zip(calls, want))
+    finally:
+        torch.cuda.synchronize()
+        st.close()
+
+
 def test_same_as_one_window(kvm_state):
     """A prefix and an own window give what one window with all the cells gives (kvm_fa_prefill),
     to the roundings of both."""
