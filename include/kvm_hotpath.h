@@ -566,7 +566,9 @@ int kvm_qk_norm_rope(kvm_state *st, const kvm_view *q, const kvm_view *k, const 
  * the runs' tokens exactly.  rope = NULL and eps < 0: the keys as they come.
  * With q != NULL the tokens' queries are normed, rotated and transformed like
  * the keys (q_weight; the transform of both leaves the scores as they are) into
- * q_out, [tokens][heads][head_dim] of q_out_type: what the attention takes. */
+ * q_out, [tokens][heads][head_dim] of q_out_type (F32, F16, BF16; the attentions
+ * take F32 and BF16).  cell0 and n_tokens are read at the call: a captured call
+ * writes the same cells at every replay, with what k, v and pos then hold. */
 int kvm_window_append(kvm_state *st, const kvm_window *const *windows, const uint32_t *cell0,
                       const uint32_t *n_tokens, uint32_t n_runs, const kvm_view *k, const kvm_view *v,
                       const float *k_weight, float eps, const kvm_rope_params *rope, const int32_t *pos,
@@ -610,8 +612,9 @@ int kvm_fa_decode_lanes(kvm_state *st, const kvm_lane *lanes, uint32_t n_lanes, 
  * hold the lanes' tokens after each other: q [tokens][n_head][head_dim] (F32 or
  * BF16), out the same shape of out_type (F32, BF16 or F16).  windows: host
  * [n_lanes], NULL entries = a lane without cells of its own (windows NULL: all);
- * prefix NULL: none.  At most 64 lanes; any number of tokens a lane; all
- * windows have the same kv heads and head_dim and are all quantised or all f16.
+ * prefix NULL: none.  At most 64 lanes; any number of tokens a lane, 2^24 query
+ * rows of a kv head in all; windows of 65,535 tiles of 64 cells at most, all of
+ * the same kv heads and head_dim and all quantised or all f16.
  * Arithmetic as kvm_fa_prefill's: f16 operands (q, the cells' values, the
  * probabilities), fp32 sums, one rounding to out_type.  Queries and keys beyond
  * 65,504 count as infinite there; q4_0 values may be as large as the cells hold

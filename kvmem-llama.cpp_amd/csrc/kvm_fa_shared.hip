@@ -13,8 +13,9 @@
 // k_fs_wide and k_fs_narrow form the pieces, k_fs_join joins those of each row.
 //
 // S^T = K Q^T and O^T += V^T P^T on 32x32x16 f16 MFMAs, 32 rows a wave.  Quantised tiles
-// become f16 on the way: K and V as (f16)(q d); Q and P are rounded to f16, everything else
-// is fp32.  Key order: score row i of a half tile is key i with bits 2 and 3 swapped, so that
+// become f16 on the way: K and V as (f16)(q d); Q and P are rounded to f16, as the products take
+// them, everything else is fp32.  (fp32 outputs are 1.8e-4 - 3.9e-4 from the 64-bit ones, 2-norm; bf16
+// ones 1.7e-3, their own rounding.)  Key order: score row i of a half tile is key i with bits 2 and 3 swapped, so that
 // a lane's scores are 8 consecutive keys of each 16, what the P V operand wants.
 //   narrow units (quantised windows of few rows): workgroups of 4 waves, two a CU.
 //     Each wave takes every fourth half of the piece's tiles.  Nothing is shared in the loop and no
@@ -404,7 +405,9 @@ __device__ __forceinline__ void fs_copy4(const int32_t *src, uint32_t off, void 
 // workgroup), next to the memory where no two units read the same tiles (all in the L2: 55 of 66
 // us), and for short pieces the start (5.6 us to the first half tile) and the sums' meeting
 // (2.2).  8 lanes x 6 rows of 4 heads over 32,768 + 2,048 cells of q8_0: 30 us for 74.5 MB, 2.5
-// TB/s; 16 x 18 over 5,003 + 8,192 of q4_0: 64 us, 154 MB.
+// TB/s; 16 x 18 over 5,003 + 8,192 of q4_0: 64 us, 154 MB.  (256 dims take all 256 registers and one
+// more, spilled before the loop and read back after it.)
+// True: an output is no finite number, and the piece is to be formed again with CAREFUL.
 template <int D, bool CAREFUL>
 __device__ __forceinline__ bool fs_narrow(const fs_args &a, const fs_seg &sg, fs_lds_narrow<D> &sm, uint32_t rt, uint32_t h, uint32_t slot,
                                           uint32_t i_lo, uint32_t i_hi) {
@@ -458,7 +461,8 @@ __device__ __forceinline__ bool fs_narrow(const fs_args &a, const fs_seg &sg, fs
         auto load_v = [&](__amdgpu_buffer_rsrc_t r, int set, int i) {
             vq[set][i] = __builtin_amdgcn_raw_buffer_load_b32(r, v_lane + (i & 1) * 256, half * 4 + (i >> 1) * 1024, 0);
         };
-        // lanes below 2 NB: the half's K scales, from 32 on its V scales (units of 8 keys of a block)
+        // lanes below 4 NB: the half's K scales, 32 .. 32 + 4 NB - 1: its V scales (units of 8 keys of a
+        // block); of 128 dims the other lanes copy the same again, which nobody reads
         auto copies = [&](uint32_t e, uint32_t buf) {
             const uint32_t t = e & 0x7fffffffu, ln = fs_opaque(l), x = ln & (4u * NB - 1);
             const uint8_t *const src = ln < 32 ? k_head + (uint64_t)t * KB + 64 * D + half * (64u * NB) + 16 * x
@@ -1169,6 +1173,7 @@ static uint32_t fs_stride(uint32_t n) {
 }
 
 // The rows from which on a window's units are wide.  An f16 window has nothing to convert: all.
+// All figures are of 256 dims; at 128 the rule is the same one, not measured by itself.
 // A CU takes a tile of a wide unit of 256 dims in 2.0 us, one of a narrow one in 1.05 (two
 // workgroups, 2.1 each): a wide unit pays from three narrow ones' rows on (two's: 48 rows over
 // 32,768 cells with 8 x 6 over 2,048, all narrow 30 us, else 28 + 16).  Where some windows stay

@@ -782,8 +782,10 @@ def prepare_window_append(st, windows, cell0, n_tokens, k, v, pos, n_rot, freq_b
     """kvm_window_append: run i takes the next n_tokens[i] tokens of k and v
     ([tokens][kv heads][dims], any strides) into cells cell0[i] .. of windows[i]; keys
     normed (eps = None: not), rotated and transformed on the way (hadamard_nrot = -1: the
-    window type's width).  With q, the call's q_out holds the tokens' queries treated
-    the same."""
+    window type's width).  Weights: [head_dim].  With q, the call's q_out holds the tokens'
+    queries treated the same (of q's type unless q_out_dtype says another: the attentions
+    take fp32 and bf16).  The prepared call, and a graph captured from it, writes the same
+    cells every time."""
     if not (len(windows) == len(cell0) == len(n_tokens)):
         raise L.KvmError(L.KVM_EINVAL, f"window_append: {len(windows)} windows, {len(cell0)} cells, {len(n_tokens)} counts")
     if any(w is None for w in windows) or any(int(x) < 0 for x in (*cell0, *n_tokens)):
