@@ -523,6 +523,37 @@ def test_large_values_that_every_row_sees(kvm_state, cache, D, tokens, sharp):
     check(got, *expected(q, qp, [tokens], _held(st, w, pos), [None], H, D ** -0.5))
 
 
+@pytest.mark.parametrize("cache,H,G,tokens", [("q8_0", 8, 1, 1), ("q4_0", 4, 8, 9)])
+def test_large_values_in_long_pieces(kvm_state, cache, H, G, tokens):
+    """The same where a piece has more tiles than are looked at at a time: in the first of them, the
+    last and between, some seen by every row and some by few."""
+    st, rng, D, n = kvm_state, np.random.default_rng(35), 128, 64 * 301
+    p = np.arange(n)
+    w, k, v, pos = window(st, rng, n, H, D, cache, p)
+    for c in (3, 64 * 255 + 1, 64 * 256, 64 * 280 + 17, n - 900, n - 5):
+        _poison(w, cache, c, int(rng.integers(0, H)), float(rng.choice([8192.0, -30000.0])))
+    counts = [tokens] * 64
+    q = torch.from_numpy(rng.standard_normal((64 * tokens, H * G, D)).astype(np.float32)).cuda()
+    qp = torch.from_numpy(rng.integers(n - 1200, n, 64 * tokens).astype(np.int32)).cuda()
+    got = api.fa_decode_shared(st, None, [w] * 64, counts, q, qp, H * G, D ** -0.5)
+    check(got, *expected(q, qp, counts, None, [_held(st, w, pos)] * 64, H, D ** -0.5))
+
+
+@pytest.mark.parametrize("cache", ["q8_0", "q4_0"])
+@pytest.mark.parametrize("tokens", [1, 30])
+def test_large_values_everywhere(kvm_state, cache, tokens):
+    """Windows of nothing but values that f16 does not hold."""
+    st, rng, H, G, D = kvm_state, np.random.default_rng(36), 2, 5, 256
+    w, k, v, pos = window(st, rng, 256, H, D, cache, cells(256, 250, 0))
+    for c in range(256):
+        for h in range(H):
+            _poison(w, cache, c, h, 60000.0 * (1 if c % 3 else -1))
+    q = torch.from_numpy(rng.standard_normal((tokens, H * G, D)).astype(np.float32)).cuda()
+    qp = torch.from_numpy(rng.integers(100, 300, tokens).astype(np.int32)).cuda()
+    got = api.fa_decode_shared(st, w, [None], [tokens], q, qp, H * G, D ** -0.5)
+    check(got, *expected(q, qp, [tokens], _held(st, w, pos), [None], H, D ** -0.5))
+
+
 @pytest.mark.parametrize("cache", ["q8_0", "f16"])
 @pytest.mark.parametrize("tokens", [2, 40])
 def test_infinite_values_under_small_probabilities(kvm_state, cache, tokens):
