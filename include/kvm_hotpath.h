@@ -619,12 +619,12 @@ int kvm_fa_decode_lanes(kvm_state *st, const kvm_lane *lanes, uint32_t n_lanes, 
  * probabilities), fp32 sums, one rounding to out_type.  Queries and keys beyond
  * 65,504 count as infinite there; q4_0 values may be as large as the cells hold
  * (524,032).  A token that sees no cell outputs zeros; what cells hold that a
- * token does not see does not reach its output, be it infinite or no number.  Windows' k, v and cell_pos: 16-byte
- * aligned.  Partial sums go through the state's workspace: calls of one state, and
- * replays of graphs captured from it, follow one another.  A capture cannot grow
- * it (KVM_ENOMEM): call once before with as many tokens and cells in all, of
- * the same heads and types; calls of fewer then fit, however they are spread
- * over lanes. */
+ * token does not see does not reach its output, be it infinite or no number.
+ * Windows' k, v and cell_pos: 16-byte aligned.  Partial sums go through the
+ * state's workspace: calls of one state, and replays of graphs captured from it,
+ * follow one another.  A capture cannot grow it (KVM_ENOMEM): call once before
+ * with as many tokens and cells in all, of the same heads and types; calls of
+ * fewer then fit, however they are spread over lanes. */
 int kvm_fa_decode_shared(kvm_state *st, const kvm_window *prefix, const kvm_window *const *windows,
                          const uint32_t *n_tokens, uint32_t n_lanes, const void *q, int q_type,
                          const int32_t *q_pos, uint32_t n_head, float scale, int out_type, void *out);
