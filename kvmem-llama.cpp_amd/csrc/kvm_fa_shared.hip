@@ -15,8 +15,8 @@
 // S^T = K Q^T and O^T += V^T P^T on 32x32x16 f16 MFMAs, 32 rows a wave.  Quantised tiles
 // become f16 on the way: K and V as (f16)(q d); Q and P are rounded to f16, as the products take
 // them, everything else is fp32.  (fp32 outputs are 1.8e-4 - 3.9e-4 from the 64-bit ones, 2-norm; bf16
-// ones 1.7e-3, their own rounding.)  Key order: score row i of a half tile is key i with bits 2 and 3 swapped, so that
-// a lane's scores are 8 consecutive keys of each 16, what the P V operand wants.
+// ones 1.7e-3, their own rounding.)  Key order: score row i of a half tile is key i with bits 2 and 3
+// swapped, so that a lane's scores are 8 consecutive keys of each 16, what the P V operand wants.
 //   narrow units (quantised windows of few rows): workgroups of 4 waves, two a CU.
 //     Each wave takes every fourth half of the piece's tiles.  Nothing is shared in the loop and no
 //     barrier is in it: tiles go from memory into registers (the tile layout is the matrix

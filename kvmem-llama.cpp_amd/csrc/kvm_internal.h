@@ -79,11 +79,13 @@ struct kvm_state {
     void *fa_ws = nullptr;
     size_t fa_ws_bytes = 0;
     // pieces of the shared-prefix attention; the buffers that it outgrew stay until the
-    // state is freed, since captured graphs may use them (each at least twice the last)
+    // state is freed, since captured graphs may use them (each at least twice the last, or
+    // what a call needs where there is no memory for that)
     void *fs_ws = nullptr;
     size_t fs_ws_bytes = 0;
     void *fs_old[48] = {};
     uint32_t n_fs_old = 0;
+    size_t fs_refused = SIZE_MAX;        // a size that could not be allocated
     // staging of the blocks a stage-in plan moves within the window (their
     // shadow K rows and V rows, gathered before any slot is written)
     void *mv_ws = nullptr;

@@ -166,12 +166,19 @@ int kvm_shared_workspace(kvm_state *st, const char *what, size_t bytes, size_t m
         if (bytes <= st->fs_ws_bytes) return KVM_OK;
         return kvm_fail(st, KVM_ENOMEM, "%s: the workspace has to grow to %zu bytes: call it once before the capture", what, bytes);
     }
-    const size_t twice = 2 * st->fs_ws_bytes, least = most < (4u << 20) ? (4u << 20) : most, want = twice > least ? twice : least;
+    const size_t twice = 2 * st->fs_ws_bytes, least = most < (4u << 20) ? (4u << 20) : most;
+    size_t want = twice > least ? twice : least;
     void *p = nullptr;
-    if (st->n_fs_old == sizeof(st->fs_old) / sizeof(st->fs_old[0]) || hipMalloc(&p, want) != hipSuccess) {
-        (void)hipGetLastError();
+    auto got = [&]() {
+        const bool ok = st->n_fs_old < sizeof(st->fs_old) / sizeof(st->fs_old[0]) && hipMalloc(&p, want) == hipSuccess;
+        if (!ok) (void)hipGetLastError();
+        return ok;
+    };
+    if (want >= st->fs_refused || !got()) {              // (what did not fit is not asked for again)
+        if (want < st->fs_refused) st->fs_refused = want;
         if (bytes <= st->fs_ws_bytes) return KVM_OK;
-        return kvm_fail(st, KVM_ENOMEM, "%s: workspace of %zu bytes", what, want);
+        want = bytes;
+        if (!got()) return kvm_fail(st, KVM_ENOMEM, "%s: workspace of %zu bytes", what, want);
     }
     if (st->fs_ws) st->fs_old[st->n_fs_old++] = st->fs_ws;
     st->fs_ws = *buf = p;
